@@ -38,15 +38,13 @@
 #include <algorithm>
 #include <mutex>
 
-#include "common.hpp"
+#include "token_attention.hpp"
 
 namespace amd {
 
-constexpr float kLog2eTA = 1.4426950408889634f;
 constexpr int kTaWaves = 4;
 constexpr int kTaUnroll = 2;
 constexpr int kTaChunk = 512;  // tokens of one sequence handled by one workgroup (grows for very long sequences)
-constexpr int kTaMaxSplit = 256;  // decodeMergeWideKernel holds four splits' weights per lane
 // Splits that a wave of decodeMergeKernel requests at once and merges: eight, or sixteen where there are many (sequence,
 // head) pairs. More take a workgroup per pair, whose waves request up to 32 at once: 28 splits of 32 heads (1 x 1777 tokens,
 // with the kernel before it) 13.3 -> 12.1 us, 250 splits (1 x 32000) 97.9 -> 91.1; with a workgroup from five splits on
@@ -55,31 +53,6 @@ constexpr int kTaNarrowSplits = 8, kTaNarrowSplitsMany = 16, kTaManyPairs = 1024
 constexpr int kTaMinChunk = 128;  // shorter chunks cost more in prologues, partial results and merging than they gain ...
 constexpr int kTaTinyChunk = 64;  // ... unless even those leave CUs without a workgroup
 constexpr int kTaWgsPerCu = 8;    // workgroups per CU the chunk length aims for
-
-__device__ __forceinline__ int64_t ldIndex(const void* p, int64_t i, bool is64) {
-  return is64 ? reinterpret_cast<const int64_t*>(p)[i] : static_cast<int64_t>(reinterpret_cast<const int32_t*>(p)[i]);
-}
-
-struct TaArgs {
-  const void* q;
-  const void* k;
-  const void* v;
-  const void* bLoc;
-  const void* bStart;
-  const void* bLen;
-  bool loc64, start64, len64;
-  bool generic;  // head rows the vector kernels do not take: the generic kernels run
-  int64_t locRowStride;  // elements
-  int64_t kSlotStride, kHeadStride, vSlotStride, vHeadStride;  // elements
-  int64_t qBatchStride, qHeadStride;
-  int64_t slots;
-  int heads, kvHeads, d, maxLen, nsplit, chunk;
-  float scaleLog2e;  // log2(e) / sqrt(d)
-  const void* logits;  // two-call form: scores [heads, total_tokens], row h at logits + h * logitsHeadStride (elements)
-  int64_t logitsHeadStride;
-  int qGroups;  // grouped-query layouts: workgroups that share the query heads of one K/V head between them
-  int batch;    // sequences (the grouped-query kernels decode a one-dimensional grid)
-};
 
 // Merge (m, l, acc) of another online-softmax stream into this one.
 template <int E>
@@ -972,26 +945,6 @@ __global__ __launch_bounds__(256) void decodeMergeWideKernel(T* __restrict__ out
 }
 
 // ------------------------------------------------ any head size: generic kernels --
-constexpr int kTaGenericMaxD = 1024;  // four elements of the head row per thread
-
-// max / sum of one value per thread over the workgroup of 256 (red: 4 floats of LDS; two barriers)
-__device__ __forceinline__ float blockMax256(float v, float* red) {
-  v = waveMax(v);
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  __syncthreads();
-  return v;
-}
-__device__ __forceinline__ float blockSum256(float v, float* red) {
-  v = waveSum(v);
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = red[0] + red[1] + red[2] + red[3];
-  __syncthreads();
-  return v;
-}
-
 // Fused decode attention, one workgroup per (sequence, head) (ext_ops.py:100-133). Tokens whose slot lies outside the
 // pool are skipped, as in the vector kernels; a sequence of length 0 gives zeros.
 template <typename T>
@@ -1123,10 +1076,6 @@ __global__ __launch_bounds__(256) void softmaxReduceVGenericKernel(TaArgs a, T* 
 }
 
 // ---------------------------------------------------------------- host side --
-struct TaViews {
-  TensorView q, k, v, loc, start, len;
-};
-
 static diopiError_t checkIndex(const TensorView& t, const char* name) {
   AMD_CHECK(t.defined(), "token attention: %s is null", name);
   AMD_CHECK(t.dtype == diopi_dtype_int32 || t.dtype == diopi_dtype_int64, "token attention: %s must be int32/int64, got %s",
@@ -1135,7 +1084,44 @@ static diopiError_t checkIndex(const TensorView& t, const char* name) {
   return diopiSuccess;
 }
 
-static diopiError_t fillArgs(const TaViews& t, bool needK, bool needV, int maxLen, TaArgs* a) {
+// q, the slot table, the starts and the lengths.
+diopiError_t tableArgs(const TaViews& t, int maxLen, TaArgs* a) {
+  const TensorView& q = t.q;
+  AMD_CHECK(q.defined() && q.ndim == 3, "token attention: q must be [batch, heads, head_dim]");
+  AMD_CHECK(q.stride[2] == 1 || q.shape[2] == 1, "token attention: q head_dim must be contiguous");
+  AMD_TRY(checkIndex(t.loc, "b_loc"));
+  AMD_TRY(checkIndex(t.start, "b_start_loc"));
+  AMD_TRY(checkIndex(t.len, "b_seq_len"));
+  const int64_t batch = q.shape[0];
+  AMD_CHECK(t.loc.ndim == 2 && t.loc.shape[0] == batch && (t.loc.stride[1] == 1 || t.loc.shape[1] == 1),
+            "token attention: b_loc must be [batch, n] with a contiguous last dim");
+  AMD_CHECK(maxLen >= 0 && t.loc.shape[1] >= maxLen, "token attention: b_loc has %ld columns, max_input_len is %d",
+            (long)t.loc.shape[1], maxLen);
+  AMD_CHECK(t.start.numel == batch && t.len.numel == batch, "token attention: b_start_loc/b_seq_len must have %ld entries",
+            (long)batch);
+  AMD_CHECK(q.dtype == diopi_dtype_bfloat16 || q.dtype == diopi_dtype_float16 || q.dtype == diopi_dtype_float32,
+            "token attention: unsupported dtype %s", dtypeName(q.dtype));
+  *a = TaArgs{};
+  a->q = q.data;
+  a->bLoc = t.loc.data;
+  a->bStart = t.start.data;
+  a->bLen = t.len.data;
+  a->loc64 = t.loc.dtype == diopi_dtype_int64;
+  a->start64 = t.start.dtype == diopi_dtype_int64;
+  a->len64 = t.len.dtype == diopi_dtype_int64;
+  a->locRowStride = t.loc.stride[0];
+  a->qBatchStride = q.stride[0];
+  a->qHeadStride = q.stride[1];
+  a->heads = (int)q.shape[1];
+  a->d = (int)q.shape[2];
+  a->maxLen = maxLen;
+  a->nsplit = 1;
+  a->qGroups = 1, a->batch = (int)batch;
+  a->scaleLog2e = kLog2eTA / sqrtf((float)q.shape[2]);
+  return diopiSuccess;
+}
+
+diopiError_t fillArgs(const TaViews& t, bool needK, bool needV, int maxLen, TaArgs* a) {
   const TensorView& q = t.q;
   AMD_CHECK(q.defined() && q.ndim == 3, "token attention: q must be [batch, heads, head_dim]");
   AMD_CHECK(q.stride[2] == 1 || q.shape[2] == 1, "token attention: q head_dim must be contiguous");
@@ -1153,18 +1139,7 @@ static diopiError_t fillArgs(const TaViews& t, bool needK, bool needV, int maxLe
     AMD_CHECK(t.v.defined() && t.v.ndim == 3 && t.v.dtype == q.dtype && t.v.stride[2] == 1, "token attention: bad v");
     for (int d = 0; d < 3; ++d) AMD_CHECK(t.v.shape[d] == t.k.shape[d], "token attention: k and v shapes differ");
   }
-  AMD_TRY(checkIndex(t.loc, "b_loc"));
-  AMD_TRY(checkIndex(t.start, "b_start_loc"));
-  AMD_TRY(checkIndex(t.len, "b_seq_len"));
-  const int64_t batch = q.shape[0];
-  AMD_CHECK(t.loc.ndim == 2 && t.loc.shape[0] == batch && (t.loc.stride[1] == 1 || t.loc.shape[1] == 1),
-            "token attention: b_loc must be [batch, n] with a contiguous last dim");
-  AMD_CHECK(maxLen >= 0 && t.loc.shape[1] >= maxLen, "token attention: b_loc has %ld columns, max_input_len is %d",
-            (long)t.loc.shape[1], maxLen);
-  AMD_CHECK(t.start.numel == batch && t.len.numel == batch, "token attention: b_start_loc/b_seq_len must have %ld entries",
-            (long)batch);
-  AMD_CHECK(q.dtype == diopi_dtype_bfloat16 || q.dtype == diopi_dtype_float16 || q.dtype == diopi_dtype_float32,
-            "token attention: unsupported dtype %s", dtypeName(q.dtype));
+  AMD_TRY(tableArgs(t, maxLen, a));
   const int64_t bytes = q.shape[2] * q.itemsize;
   // head rows of whole 16-byte pieces up to 512 bytes: the streaming kernels span them with 8, 16 or 32 lanes
   bool vector = bytes % 16 == 0 && bytes >= 16 && bytes <= 512 && q.aligned16() && kv.aligned16() &&
@@ -1174,33 +1149,17 @@ static diopiError_t fillArgs(const TaViews& t, bool needK, bool needV, int maxLe
     vector = vector && t.v.aligned16() && (t.v.stride[0] * q.itemsize) % 16 == 0 && (t.v.stride[1] * q.itemsize) % 16 == 0;
   a->generic = !vector;
   AMD_CHECK(!a->generic || q.shape[2] <= kTaGenericMaxD, "token attention: head_dim %ld exceeds %d", (long)q.shape[2], kTaGenericMaxD);
-  a->q = q.data;
   a->k = needK ? t.k.data : nullptr;
   a->v = needV ? t.v.data : nullptr;
-  a->bLoc = t.loc.data;
-  a->bStart = t.start.data;
-  a->bLen = t.len.data;
-  a->loc64 = t.loc.dtype == diopi_dtype_int64;
-  a->start64 = t.start.dtype == diopi_dtype_int64;
-  a->len64 = t.len.dtype == diopi_dtype_int64;
-  a->locRowStride = t.loc.stride[0];
   a->kSlotStride = needK ? t.k.stride[0] : 0;
   a->kHeadStride = needK ? t.k.stride[1] : 0;
   a->vSlotStride = needV ? t.v.stride[0] : 0;
   a->vHeadStride = needV ? t.v.stride[1] : 0;
-  a->qBatchStride = q.stride[0];
-  a->qHeadStride = q.stride[1];
   a->slots = kv.shape[0];
-  a->heads = (int)q.shape[1];
   a->kvHeads = (int)kv.shape[1];
-  a->d = (int)q.shape[2];
-  a->maxLen = maxLen;
-  a->nsplit = 1;
-  a->logits = nullptr, a->logitsHeadStride = 0, a->qGroups = 1, a->batch = (int)q.shape[0];
   // at most kTaMaxSplit chunks per sequence; chunks stay a multiple of 64 tokens
   a->chunk = kTaChunk;
   if ((int64_t)maxLen > (int64_t)kTaChunk * kTaMaxSplit) a->chunk = (int)(ceilDiv(ceilDiv(maxLen, kTaMaxSplit), 64) * 64);
-  a->scaleLog2e = kLog2eTA / sqrtf((float)q.shape[2]);
   return diopiSuccess;
 }
 
@@ -1254,6 +1213,31 @@ static void chooseChunk(TaArgs* a, int64_t groupsPerSeq, int64_t batch, int maxI
     else if (DTYPE == diopi_dtype_float16) { CALL(half_t); }            \
     else { CALL(float); }                                               \
   } while (0)
+
+diopiError_t mergeChunks(hipStream_t stream, diopiDtype_t dtype, void* out, const float* partial, const TaArgs& a, int64_t batch) {
+  const int64_t pairs = batch * a.heads;
+  if (a.nsplit > (pairs >= kTaManyPairs ? kTaNarrowSplitsMany : kTaNarrowSplits)) {
+    AMD_CHECK(a.nsplit <= kTaMaxSplit && a.d <= 256, "token attention: %d splits of head size %d cannot be merged", a.nsplit, a.d);
+#define MERGE_WIDE_CALL(T)                                                                                                       \
+  hipLaunchKernelGGL((decodeMergeWideKernel<T>), dim3((unsigned)pairs), dim3(256), 0, stream, static_cast<T*>(out), partial, a.bLen, \
+                     a.len64, a.heads, a.d, a.nsplit, a.chunk)
+    TA_GENERIC_DISPATCH(dtype, MERGE_WIDE_CALL);
+#undef MERGE_WIDE_CALL
+  } else {
+    dim3 mgrid((unsigned)ceilDiv(pairs, 4)), mblock(256);
+#define MERGE_CALL(T)                                                                                                               \
+  if (a.nsplit <= kTaNarrowSplits)                                                                                                  \
+    hipLaunchKernelGGL((decodeMergeKernel<T, kTaNarrowSplits>), mgrid, mblock, 0, stream, static_cast<T*>(out), partial, a.bLen,     \
+                       a.len64, pairs, a.heads, a.d, a.nsplit, a.chunk);                                                            \
+  else                                                                                                                              \
+    hipLaunchKernelGGL((decodeMergeKernel<T, kTaNarrowSplitsMany>), mgrid, mblock, 0, stream, static_cast<T*>(out), partial, a.bLen, \
+                       a.len64, pairs, a.heads, a.d, a.nsplit, a.chunk)
+    TA_GENERIC_DISPATCH(dtype, MERGE_CALL);
+#undef MERGE_CALL
+  }
+  AMD_LAUNCH_CHECK();
+  return diopiSuccess;
+}
 
 // Split-KV partial results for the entry point that allocates nothing. Every device the library's code object is
 // loaded on holds its own copy of this array, at its own address, until the process ends.
@@ -1434,29 +1418,7 @@ static diopiError_t streamChunks(diopiContextHandle_t ctx, hipStream_t stream, T
   }
   AMD_LAUNCH_CHECK();
   if (MODE == kTaLogitsOut) return diopiSuccess;
-  const int64_t pairs = batch * a.heads;
-  if (a.nsplit > (pairs >= kTaManyPairs ? kTaNarrowSplitsMany : kTaNarrowSplits)) {
-    AMD_CHECK(a.nsplit <= kTaMaxSplit && a.d <= 256, "token attention: %d splits of head size %d cannot be merged", a.nsplit, a.d);
-#define MERGE_WIDE_CALL(T, LPT)                                                                                                      \
-  hipLaunchKernelGGL((decodeMergeWideKernel<T>), dim3((unsigned)pairs), dim3(256), 0, stream, static_cast<T*>(outPtr), partial, a.bLen, \
-                     a.len64, a.heads, a.d, a.nsplit, a.chunk)
-    TA_DISPATCH(dtype, bytes, MERGE_WIDE_CALL);
-#undef MERGE_WIDE_CALL
-    AMD_LAUNCH_CHECK();
-  } else if (a.nsplit > 1) {
-    dim3 mgrid((unsigned)ceilDiv(pairs, 4)), mblock(256);
-#define MERGE_CALL(T, LPT)                                                                                                              \
-  if (a.nsplit <= kTaNarrowSplits)                                                                                                      \
-    hipLaunchKernelGGL((decodeMergeKernel<T, kTaNarrowSplits>), mgrid, mblock, 0, stream, static_cast<T*>(outPtr), partial, a.bLen,      \
-                       a.len64, pairs, a.heads, a.d, a.nsplit, a.chunk);                                                                \
-  else                                                                                                                                  \
-    hipLaunchKernelGGL((decodeMergeKernel<T, kTaNarrowSplitsMany>), mgrid, mblock, 0, stream, static_cast<T*>(outPtr), partial, a.bLen,  \
-                       a.len64, pairs, a.heads, a.d, a.nsplit, a.chunk)
-    TA_DISPATCH(dtype, bytes, MERGE_CALL);
-#undef MERGE_CALL
-    AMD_LAUNCH_CHECK();
-  }
-  return diopiSuccess;
+  return a.nsplit > 1 ? mergeChunks(stream, dtype, outPtr, partial, a, batch) : diopiSuccess;
 }
 
 static diopiError_t decodeAttention(diopiContextHandle_t ctx, diopiTensorHandle_t outH, diopiConstTensorHandle_t qH,

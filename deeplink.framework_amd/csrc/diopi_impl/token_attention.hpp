@@ -1,0 +1,70 @@
+// What the decode attentions share: the arguments and checks of a paged pool, and the launch that merges the shares of a
+// sequence. Kernels: token_attention.hip (float pools), token_attention_int8.hip, token_attention_prefix.hip.
+#pragma once
+
+#include "common.hpp"
+
+namespace amd {
+
+constexpr float kLog2eTA = 1.4426950408889634f;
+constexpr int kTaMaxSplit = 256;  // decodeMergeWideKernel holds four splits' weights per lane
+constexpr int kTaGenericMaxD = 1024;  // four elements of the head row per thread
+
+__device__ __forceinline__ int64_t ldIndex(const void* p, int64_t i, bool is64) {
+  return is64 ? reinterpret_cast<const int64_t*>(p)[i] : static_cast<int64_t>(reinterpret_cast<const int32_t*>(p)[i]);
+}
+
+struct TaArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  const void* bLoc;
+  const void* bStart;
+  const void* bLen;
+  bool loc64, start64, len64;
+  bool generic;  // head rows the vector kernels do not take: the generic kernels run
+  int64_t locRowStride;  // elements
+  int64_t kSlotStride, kHeadStride, vSlotStride, vHeadStride;  // elements
+  int64_t qBatchStride, qHeadStride;
+  int64_t slots;
+  int heads, kvHeads, d, maxLen, nsplit, chunk;
+  float scaleLog2e;  // log2(e) / sqrt(d)
+  const void* logits;  // two-call form: scores [heads, total_tokens], row h at logits + h * logitsHeadStride (elements)
+  int64_t logitsHeadStride;
+  int qGroups;  // grouped-query layouts: workgroups that share the query heads of one K/V head between them
+  int batch;    // sequences (the grouped-query kernels decode a one-dimensional grid)
+};
+
+// max / sum of one value per thread over the workgroup of 256 (red: 4 floats of LDS; two barriers)
+__device__ __forceinline__ float blockMax256(float v, float* red) {
+  v = waveMax(v);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  __syncthreads();
+  return v;
+}
+__device__ __forceinline__ float blockSum256(float v, float* red) {
+  v = waveSum(v);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = red[0] + red[1] + red[2] + red[3];
+  __syncthreads();
+  return v;
+}
+
+// ---------------------------------------------------------------- host side --
+struct TaViews {
+  TensorView q, k, v, loc, start, len;
+};
+
+// q, the slot table, the starts and the lengths alone: checked, and in `a` (the rest of it zero).
+diopiError_t tableArgs(const TaViews& t, int maxLen, TaArgs* a);
+// q, k, v (those needed), the slot table, the starts and the lengths: checked, and their strides and types in `a`.
+diopiError_t fillArgs(const TaViews& t, bool needK, bool needV, int maxLen, TaArgs* a);
+
+// out[b, h, :] (dense, `dtype`) from the partial results [batch, heads, nsplit, 2 + d] of chunks of `a.chunk` tokens: maximum (in
+// units of log2), sum and weighted sum of V, chunk i written where i = 0 or a sequence has more than i * chunk tokens.
+diopiError_t mergeChunks(hipStream_t stream, diopiDtype_t dtype, void* out, const float* partial, const TaArgs& a, int64_t batch);
+
+}  // namespace amd

@@ -289,7 +289,8 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
   X(diopiAddmm) X(diopiBaddbmm) X(diopiLinear) X(diopiRMSNorm) X(diopiRotaryEmbedding) X(diopiDestIndexCopyKV)                \
   X(diopiDestIndexCopyKVPair) X(diopiTokenAttentionInference) X(diopiTokenSoftmaxReduceVInference)                            \
   X(diopiContextAttentionInference) X(diopiTokenDecodeAttentionInference) X(diopiTokenDecodeAttentionInferenceNoAlloc)        \
-  X(diopiWeightOnlyInt8Linear) X(diopiSiluMul) X(diopiLinearSiluMul) X(diopiLinearRotary)
+  X(diopiWeightOnlyInt8Linear) X(diopiSiluMul) X(diopiLinearSiluMul) X(diopiLinearRotary) X(diopiDestIndexCopyKVPairInt8)      \
+  X(diopiIndexSelectKVPairInt8) X(diopiTokenDecodeAttentionInt8Inference) X(diopiTokenDecodeAttentionSharedPrefixInference)
 
 #define X(f)                                        \
   struct Tag_##f {                                  \

@@ -286,6 +286,10 @@ SIGNATURES = {
     "diopiContextAttentionInference": [_T, _T, _T, _T, _T, _T, c_int],
     "diopiTokenDecodeAttentionInference": [_T, _T, _T, _T, _T, _T, _T, c_int],
     "diopiTokenDecodeAttentionInferenceNoAlloc": [_T, _T, _T, _T, _T, _T, _T, c_int],
+    "diopiDestIndexCopyKVPairInt8": [_T, _T, _T, _T, _T, _T, _T],
+    "diopiIndexSelectKVPairInt8": [_T, _T, _T, _T, _T, _T, _T],
+    "diopiTokenDecodeAttentionInt8Inference": [_T, _T, _T, _T, _T, _T, _T, _T, _T, c_int],
+    "diopiTokenDecodeAttentionSharedPrefixInference": [_T, _T, _T, _T, _T, _T, _T, _T, c_int],
     "diopiWeightOnlyInt8Linear": [_T, _T, _T, _T, _T],
     "diopiSiluMul": [_T, _T, _T],
     "diopiLinearSiluMul": [_T, _T, _T],

@@ -504,6 +504,26 @@ def dest_index_copy_kv_pair(k, v, dest_loc, out_k, out_v):
     return out_k, out_v
 
 
+def dest_index_copy_kv_pair_int8(k, v, dest_loc, out_k, out_k_scale, out_v, out_v_scale):
+    """k[i] and v[i] quantised to int8 with a scale per token and head, into slot dest_loc[i] of two pools, in one launch
+    (backend extension, functions_ext.h). Pools [slots, kv_heads, d] int8, scales [slots, kv_heads] float32."""
+    _host.diopiDestIndexCopyKVPairInt8(_ctx, out_k, out_k_scale, k, out_v, out_v_scale, v, dest_loc)
+    return out_k, out_k_scale, out_v, out_v_scale
+
+
+def index_select_kv_pair_int8(k, k_scale, v, v_scale, index, *, dtype=None, out_k=None, out_v=None):
+    """k[index] * k_scale[index] and v[index] * v_scale[index] of an int8 cache in `dtype` (by default that of out_k, or
+    torch's default type), in one launch (backend extension, functions_ext.h)."""
+    if out_k is None or out_v is None:
+        if dtype is None:
+            dtype = next((o.dtype for o in (out_k, out_v) if o is not None), torch.get_default_dtype())
+        shape = (index.shape[0], *k.shape[1:])
+        out_k = torch.empty(shape, dtype=dtype, device=k.device) if out_k is None else out_k
+        out_v = torch.empty(shape, dtype=dtype, device=k.device) if out_v is None else out_v
+    _host.diopiIndexSelectKVPairInt8(_ctx, out_k, out_v, k, k_scale, v, v_scale, index)
+    return out_k, out_v
+
+
 def token_attention(q, k, attention_out, b_loc, b_start_loc, b_seq_len, max_input_len):
     _host.diopiTokenAttentionInference(_ctx, attention_out, q, k, b_loc, b_start_loc, b_seq_len, int(max_input_len))
     return attention_out
@@ -521,6 +541,23 @@ def token_decode_attention(q, k, v, b_loc, b_start_loc, b_seq_len, max_input_len
         out = torch.empty_like(q)
     decode = _host.diopiTokenDecodeAttentionInferenceNoAlloc if no_alloc else _host.diopiTokenDecodeAttentionInference
     decode(_ctx, out, q, k, v, b_loc, b_start_loc, b_seq_len, int(max_input_len))
+    return out
+
+
+def token_decode_attention_int8(q, k, k_scale, v, v_scale, b_loc, b_start_loc, b_seq_len, max_input_len, *, out=None):
+    """token_decode_attention over an int8 cache (backend extension, functions_ext.h)."""
+    if out is None:
+        out = _host.like(q)
+    _host.diopiTokenDecodeAttentionInt8Inference(_ctx, out, q, k, k_scale, v, v_scale, b_loc, b_start_loc, b_seq_len, int(max_input_len))
+    return out
+
+
+def token_decode_attention_shared_prefix(q, k, v, prefix_loc, b_loc, b_start_loc, b_seq_len, max_input_len, *, out=None):
+    """token_decode_attention where every sequence begins with the tokens in slots prefix_loc, read for many sequences at
+    a time; b_loc, b_seq_len and max_input_len are about the tokens behind them (backend extension, functions_ext.h)."""
+    if out is None:
+        out = _host.like(q)
+    _host.diopiTokenDecodeAttentionSharedPrefixInference(_ctx, out, q, k, v, prefix_loc, b_loc, b_start_loc, b_seq_len, int(max_input_len))
     return out
 
 

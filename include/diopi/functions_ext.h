@@ -113,6 +113,54 @@ DIOPI_API diopiError_t diopiTokenDecodeAttentionInferenceNoAlloc(diopiContextHan
                                                                  diopiConstTensorHandle_t b_start_loc,
                                                                  diopiConstTensorHandle_t b_seq_len, int max_input_len);
 
+/* The int8 KV cache: a pool [slots, kv_heads, d] of int8 with a float32 scale for each row, [slots, kv_heads].
+ * diopiDestIndexCopyKVPairInt8 quantises the K row and the V row of every new token as it writes them, in one launch:
+ *   scale[dest_loc[i], h] = max |x[i, h, :]| / 127 in float32,  out[dest_loc[i], h, :] = x[i, h, :] / scale to the nearest
+ *   whole number, ties to the even one, within [-127, 127].
+ * k, v [tokens, kv_heads, d] are float16, bfloat16 or float32, dest_loc [tokens] int32 or int64. As in
+ * diopiDestIndexCopyKV a negative destination counts from the end and one outside the pool is dropped; of several tokens
+ * with one destination the last is kept. A row of zeros has scale 0; a row that holds an infinity or NaN has scale NaN and
+ * reads back as NaN. Heads, tokens and slots may lie at any strides, head_dim is contiguous. (More than 16384 tokens take a workspace of 4
+ * bytes per slot.) No counterpart in the reference, whose cache holds the activations' type. */
+DIOPI_API diopiError_t diopiDestIndexCopyKVPairInt8(diopiContextHandle_t ctx, diopiTensorHandle_t out_k,
+                                                    diopiTensorHandle_t out_k_scale, diopiConstTensorHandle_t k,
+                                                    diopiTensorHandle_t out_v, diopiTensorHandle_t out_v_scale,
+                                                    diopiConstTensorHandle_t v, diopiConstTensorHandle_t dest_loc);
+
+/* Rows of an int8 cache read back: out_k[i] = k[index[i]] * k_scale[index[i]] (in float32, then rounded to the type of
+ * out_k: float16, bfloat16 or float32), out_v likewise; out_k, out_v [n, kv_heads, d], index [n] int32 or int64. As in
+ * diopiIndexSelect an index outside [0, slots) is never dereferenced and gives zeros. No counterpart in the reference. */
+DIOPI_API diopiError_t diopiIndexSelectKVPairInt8(diopiContextHandle_t ctx, diopiTensorHandle_t out_k,
+                                                  diopiTensorHandle_t out_v, diopiConstTensorHandle_t k,
+                                                  diopiConstTensorHandle_t k_scale, diopiConstTensorHandle_t v,
+                                                  diopiConstTensorHandle_t v_scale, diopiConstTensorHandle_t index);
+
+/* diopiTokenDecodeAttentionInference over an int8 cache (k, v int8 with k_scale, v_scale as above): the same table, lengths
+ * and rules; q and out are float32, float16 or bfloat16. Rows are multiplied as the whole numbers they are and scaled in
+ * float32, nothing is rounded to the type of q on the way. head_dim is contiguous and at most 1024. */
+DIOPI_API diopiError_t diopiTokenDecodeAttentionInt8Inference(diopiContextHandle_t ctx, diopiTensorHandle_t out,
+                                                              diopiConstTensorHandle_t q, diopiConstTensorHandle_t k,
+                                                              diopiConstTensorHandle_t k_scale, diopiConstTensorHandle_t v,
+                                                              diopiConstTensorHandle_t v_scale,
+                                                              diopiConstTensorHandle_t b_loc,
+                                                              diopiConstTensorHandle_t b_start_loc,
+                                                              diopiConstTensorHandle_t b_seq_len, int max_input_len);
+
+/* diopiTokenDecodeAttentionInference for a batch whose sequences all begin with the same tokens, which the pool holds once:
+ * sequence b attends to the tokens in slots prefix_loc[0 .. n) (int32 or int64, every one of them for every sequence) and to
+ * its own b_seq_len[b] tokens behind them, which b_loc, b_seq_len and max_input_len describe as they do there (none of them
+ * count the prefix). The shared rows are read for many sequences at a time. Slots outside the pool are skipped; a sequence without any token
+ * gives zeros. The same types and head sizes. */
+DIOPI_API diopiError_t diopiTokenDecodeAttentionSharedPrefixInference(diopiContextHandle_t ctx, diopiTensorHandle_t out,
+                                                                      diopiConstTensorHandle_t q,
+                                                                      diopiConstTensorHandle_t k,
+                                                                      diopiConstTensorHandle_t v,
+                                                                      diopiConstTensorHandle_t prefix_loc,
+                                                                      diopiConstTensorHandle_t b_loc,
+                                                                      diopiConstTensorHandle_t b_start_loc,
+                                                                      diopiConstTensorHandle_t b_seq_len,
+                                                                      int max_input_len);
+
 /* out[M,N] = input[M,K] @ (weight[N,K] (int8) * scale[N])^T + bias[N].
  * input/out bf16 or fp16; scale fp16/bf16/fp32 per output channel; bias nullable.
  * The int8 -> bf16/fp16 conversion happens while the MFMA operand tile is loaded; the
