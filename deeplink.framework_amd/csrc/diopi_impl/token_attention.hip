@@ -1322,13 +1322,14 @@ static bool lanesPay(int64_t perKv, int64_t kvHeads, bool wholeLoads, bool partR
   return wide && perKv > 6 && (many(256, 0, 32) || many(512, 16, 64));
 }
 
-// staticScratch: partial results go to the library's own device array instead of workspace from the context.
+// staticScratch: partial results go to the library's own device array instead of workspace from the context. keep: the partial
+// results are not merged but left to the caller.
 // Launches decodeSplitKernel or decodeGroupedKernel in one mode over (head groups, chunks, sequences) and, for the modes that produce
 // the attention output, merges the chunks. scoresF32: the stored scores of the two-call modes are float32 (else T).
 template <int MODE>
 static diopiError_t streamChunks(diopiContextHandle_t ctx, hipStream_t stream, TaArgs a, diopiDtype_t dtype, int64_t bytes,
                                  int64_t batch, int maxInputLen, void* outPtr, bool scoresF32, bool staticScratch,
-                                 float* ownScratch) {
+                                 float* ownScratch, TaPartials* keep = nullptr) {
   // a head row is spanned by 8, 16 or 32 lanes of 16 bytes: the next of 128 / 256 / 512 bytes (the kernel masks the rest)
   const bool partRows = bytes != 128 && bytes != 256 && bytes != 512;
   bytes = bytes <= 128 ? 128 : bytes <= 256 ? 256 : 512;
@@ -1347,6 +1348,7 @@ static diopiError_t streamChunks(diopiContextHandle_t ctx, hipStream_t stream, T
   const int groupsPerSeq = qpk > 1 ? a.kvHeads * a.qGroups : (hiw ? a.heads / tpw : a.heads);
   chooseChunk(&a, groupsPerSeq, batch, maxInputLen, grouped, MODE == kTaFused && bytes == 256, MODE != kTaLogitsOut);
   a.nsplit = (int)std::max<int64_t>(1, ceilDiv(maxInputLen, a.chunk));
+  if (keep) a.nsplit = std::max(a.nsplit, 2);  // (one share is written as the result: a second one, without tokens, makes it a partial result)
   AMD_CHECK(batch <= 65535 && a.nsplit <= 65535, "token attention: batch %ld / splits %d exceed the grid limits", (long)batch,
             a.nsplit);
   float* partial = nullptr;
@@ -1418,7 +1420,15 @@ static diopiError_t streamChunks(diopiContextHandle_t ctx, hipStream_t stream, T
   }
   AMD_LAUNCH_CHECK();
   if (MODE == kTaLogitsOut) return diopiSuccess;
+  if (keep) {
+    *keep = TaPartials{partial, a.nsplit, a.chunk, grouped && dtype == diopi_dtype_float16 ? GqMfma<half_t>::kRaise : 0.f};
+    return diopiSuccess;
+  }
   return a.nsplit > 1 ? mergeChunks(stream, dtype, outPtr, partial, a, batch) : diopiSuccess;
+}
+
+diopiError_t amd::decodePartials(diopiContextHandle_t ctx, hipStream_t stream, const TaArgs& a, diopiDtype_t dtype, int maxInputLen, TaPartials* keep) {
+  return streamChunks<kTaFused>(ctx, stream, a, dtype, a.d * dtypeSize(dtype), a.batch, maxInputLen, nullptr, true, false, nullptr, keep);
 }
 
 static diopiError_t decodeAttention(diopiContextHandle_t ctx, diopiTensorHandle_t outH, diopiConstTensorHandle_t qH,

@@ -67,4 +67,13 @@ diopiError_t fillArgs(const TaViews& t, bool needK, bool needV, int maxLen, TaAr
 // units of log2), sum and weighted sum of V, chunk i written where i = 0 or a sequence has more than i * chunk tokens.
 diopiError_t mergeChunks(hipStream_t stream, diopiDtype_t dtype, void* out, const float* partial, const TaArgs& a, int64_t batch);
 
+// The partial results that mergeChunks merges, of diopiTokenDecodeAttentionInference's kernels (not of generic arguments), in
+// workspace of the context: at least two chunks.
+struct TaPartials {
+  const float* partial;
+  int nsplit, chunk;
+  float raise;  // sums are against the maximum less this (in units of log2)
+};
+diopiError_t decodePartials(diopiContextHandle_t ctx, hipStream_t stream, const TaArgs& a, diopiDtype_t dtype, int maxInputLen, TaPartials* keep);
+
 }  // namespace amd

@@ -17,6 +17,8 @@ struct TaPrefixArgs {
   const void* loc;  // slots of the shared tokens
   bool loc64;
   int len;
+  int chunk, nsplit;          // of the shared tokens
+  unsigned kStride, vStride;  // slot strides of the pools in bytes, as decodePrefixKernel takes them
 };
 
 // Any head size up to 1024: one workgroup per (sequence, head) walks the shared tokens and then its own, 256 at a time, one
@@ -76,6 +78,574 @@ __global__ __launch_bounds__(256) void decodePrefixAnyKernel(TaPrefixArgs x, T* 
   }
 }
 
+// ------------------------------------------------ head rows of whole 16-byte pieces up to 512 bytes: the matrix pipe --
+// The shared tokens see the same K and V from every sequence, so a K/V head's columns are the query heads that share it of ALL
+// sequences: S^T = K . Q^T and O^T += V^T . P^T with up to 64 columns for one read of a row. Partial results (maximum, sum, weighted
+// sum of V) of each chunk of the prefix go to workspace; those of the sequences' own tokens come from the kernels of
+// diopiTokenDecodeAttentionInference, and a last launch merges both. Few columns: bound by memory, every shared row once; many
+// (192 columns, 16 001 tokens): by the matrix pipe, 24 products of 16 cycles for 32 tokens and 16 columns (fp16 32), and the softmax
+// between them.
+//   * rows go from the pool into the registers that the products read, whole 128-byte lines of 8 rows in a load: K as in
+//     token_attention_int8.hip (a piece of 16 bytes is an operand, two lanes swap one); of V a lane takes 16 bytes of each of its
+//     eight tokens, which are eight places of the head, and v_perm puts pairs of tokens side by side, so V is turned round in registers.
+//   * a probability is cut into parts of 8 bits, two of them for bf16 (off by at most 2^-16 relative). fp16 has no room for the
+//     small ones: there V is cut into two bf16 parts too (exact: 8 bits and 3), and three of the four products are added up (the
+//     fourth is below 2^-16). fp32 rows are multiplied as they are (16x16x4).
+//   * the running maximum is followed at once, so a probability is at most one.
+//   * the first walk multiplies V as it is: infinities and NaN in it, or in slot 0 for a slot outside the pool, against parts
+//     that are zero or negative, leave sums that are not finite, and the wave then walks again with care: rows that do not count
+//     are zeros, what is not finite meets a one for each probability that is not zero.
+// Four waves share a chunk's tokens and meet in LDS, a lane always adding to what is its own.
+constexpr int kPxWaves = 4;
+constexpr int kPxBlock = 2048;    // tokens whose slots a workgroup holds in LDS at once
+constexpr int kPxMaxSplit = 256;  // chunks of the prefix
+
+template <typename T, int D>
+struct PxShape {
+  static constexpr bool kWide = sizeof(T) == 4;
+  static constexpr int TOKENS = kWide ? 16 : 32;             // of a wave's step
+  static constexpr int TILES = TOKENS / 16;
+  static constexpr int ROWB = D * (int)sizeof(T);
+  static constexpr int KP = ROWB / 64;                        // 16-byte pieces of K per lane and tile
+  static constexpr int EP = 16 / (int)sizeof(T);              // elements of a piece
+  static constexpr int RUN = D / 16;                          // places of V per lane
+  static constexpr bool PAIRS = ROWB / 16 < 16;               // 8 bytes of V per token: two tokens in a load
+  static constexpr int VP = PAIRS ? 1 : ROWB / 256;           // 16-byte pieces of V per lane and token
+  static constexpr int VTOK = 4 * TILES, VLOADS = PAIRS ? VTOK / 2 : VTOK;
+  // place t of lane c's places of V in the head
+  static __device__ __forceinline__ int place(int c, int t) {
+    return PAIRS ? (c & 7) * 2 * RUN + (c >> 3) * RUN + t : t / EP * (256 / (int)sizeof(T)) + c * EP + t % EP;
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ bf16x8 pxPart(float (&x)[8]) {  // the next 8 bits of eight numbers, and what they leave
+  bf16x8 part;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    part[i] = static_cast<bf16_t>(x[i]);
+    x[i] -= static_cast<float>(part[i]);
+  }
+  return part;
+}
+
+// D: head size the rows are laid out for; a.d is any whole number of 16-byte pieces up to it. NC: column tiles of 16.
+template <typename T, int D, int NC>
+__global__ __launch_bounds__(kPxWaves * 64, 1) void decodePrefixKernel(TaPrefixArgs x, float* __restrict__ partial) {
+  using S = PxShape<T, D>;
+  constexpr int TOKENS = S::TOKENS, TILES = S::TILES, KP = S::KP, RUN = S::RUN, VP = S::VP, VTOK = S::VTOK;
+  constexpr bool WIDE = S::kWide, HALF = std::is_same<T, half_t>::value;
+  const TaArgs& a = x.a;
+  extern __shared__ __attribute__((aligned(16))) f32x4 pxLds[];  // sums on their way to the waves that add them up
+  __shared__ __attribute__((aligned(16))) int slots[kPxBlock];  // of a block's tokens; negative: does not count
+  __shared__ int badBuf[kPxWaves];
+  __shared__ float stateBuf[kPxWaves][NC][2][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 15, quad = lane >> 4, upperHalf = (lane >> 3) & 1;
+
+  // Workgroup ids go round the 8 XCDs. A unit is a (chunk, K/V head); its groups of columns read the same rows and run next to
+  // each other on one XCD.
+  const int f = blockIdx.x, idx = f >> 3;
+  const int perKv = a.heads / a.kvHeads, columns = a.batch * perKv, groups = (columns + 16 * NC - 1) / (16 * NC);
+  const int group = idx % groups, u = (idx / groups) * 8 + (f & 7);
+  if (u >= a.kvHeads * x.nsplit) return;  // the grid is rounded up to whole rounds of the XCDs
+  const int kvh = u % a.kvHeads, split = u / a.kvHeads;
+  const int begin = split * x.chunk, end = min(x.len, begin + x.chunk);
+
+  // q of the columns: column c of the K/V head is its query head c % perKv in sequence c / perKv. Piece p holds EP places from
+  // the byte 128 (p / 2) + 32 quad + 16 (p % 2) of the row on.
+  u32x4 qf[NC][KP];
+  int pairOf[NC];  // row of the partial results of this lane's column, or -1
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const int column = (group * NC + c) * 16 + col;
+    const bool have = column < columns;
+    const int b = have ? column / perKv : 0, h = kvh * perKv + (have ? column % perKv : 0);
+    pairOf[c] = have ? b * a.heads + h : -1;
+    const T* src = reinterpret_cast<const T*>(a.q) + b * a.qBatchStride + h * a.qHeadStride;
+#pragma unroll
+    for (int p = 0; p < KP; ++p) {
+      const int e = (128 * (p >> 1) + 32 * quad + 16 * (p & 1)) / (int)sizeof(T);
+      qf[c][p] = *reinterpret_cast<const u32x4*>(src + (e < a.d ? e : 0));
+      if (!have || e >= a.d) qf[c][p] = u32x4{0, 0, 0, 0};
+    }
+  }
+
+  int kOff[KP], vOff[VP];  // bytes; pieces past the row's end repeat its first one
+  const int rowBytes = a.d * (int)sizeof(T);
+#pragma unroll
+  for (int p = 0; p < KP; ++p) {
+    const int e = 128 * (p >> 1) + 32 * quad + 16 * upperHalf;
+    kOff[p] = e < rowBytes ? e : 0;
+  }
+#pragma unroll
+  for (int p = 0; p < VP; ++p) {
+    const int e = S::PAIRS ? 16 * (lane & 7) : 256 * p + 16 * col;
+    vOff[p] = e < rowBytes ? e : 0;
+  }
+  const char* const kBase = reinterpret_cast<const char*>(reinterpret_cast<const T*>(a.k) + kvh * a.kHeadStride);
+  const char* const vBase = reinterpret_cast<const char*>(reinterpret_cast<const T*>(a.v) + kvh * a.vHeadStride);
+
+  struct Step {
+    u32x4 k[TILES][KP];
+    u32x4 v[S::VLOADS][VP];
+  };
+  auto request = [&](Step& s, int at) {
+#pragma unroll
+    for (int t = 0; t < TILES; ++t)
+#pragma unroll
+      for (int p = 0; p < KP; ++p) {
+        const int token = at + 16 * t + (lane & 7) + 8 * (p & 1);
+        s.k[t][p] = *reinterpret_cast<const u32x4*>(kBase + (uint64_t)((unsigned)slots[token] & 0x7fffffffu) * x.kStride + kOff[p]);
+      }
+#pragma unroll
+    for (int i = 0; i < S::VLOADS; ++i) {
+      const int token = at + (S::PAIRS ? 16 * (i >> 1) + 4 * quad + 2 * (i & 1) + upperHalf : 16 * (i >> 2) + 4 * quad + (i & 3));
+      const char* row = vBase + (uint64_t)((unsigned)slots[token] & 0x7fffffffu) * x.vStride;
+#pragma unroll
+      for (int p = 0; p < VP; ++p) s.v[i][p] = *reinterpret_cast<const u32x4*>(row + vOff[p]);
+    }
+    __builtin_amdgcn_sched_barrier(0);  // nothing of the step before is touched (and waited for) ahead of these loads
+  };
+  // `own` in the lanes of `banks` (0xc: 8 .. 15 of each 16, 0x3: 0 .. 7) replaced by what the lane 8 aside has in `other`
+  auto swapped = [](uint32_t own, uint32_t other, auto banks) {
+    return (uint32_t)__builtin_amdgcn_update_dpp((int)own, (int)other, 0x128 /* rotate 16 lanes by 8 */, 0xf, decltype(banks)::value, false);
+  };
+  constexpr std::integral_constant<int, 0xc> kUpper{};
+  constexpr std::integral_constant<int, 0x3> kLower{};
+
+  f32x4 acc[NC][RUN];
+  float most[NC], m[NC], mRef[NC], l[NC];  // the largest score, the same in units of log2, what scores are taken against, the sum
+  auto clear = [&] {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      most[c] = m[c] = -INFINITY, mRef[c] = l[c] = 0.f;
+#pragma unroll
+      for (int t = 0; t < RUN; ++t) acc[c][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+  };
+  auto multiply = [&](Step& s, int at, bool all, auto withCare) {  // all: every one of the tokens counts
+    constexpr bool CAREFUL = decltype(withCare)::value;
+    u32x4 kf[TILES][KP];
+#pragma unroll
+    for (int t = 0; t < TILES; ++t)
+#pragma unroll
+      for (int p = 0; p < KP; ++p) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+          kf[t][p][w] = p & 1 ? swapped(s.k[t][p][w], s.k[t][p - 1][w], kLower) : swapped(s.k[t][p][w], s.k[t][p + 1][w], kUpper);
+        if (CAREFUL && 128 * (p >> 1) + 32 * quad + 16 * (p & 1) >= rowBytes) kf[t][p] = u32x4{0, 0, 0, 0};
+      }
+    // V of the lane's tokens at its places
+    constexpr int WORDS = RUN * (int)sizeof(T) / 4;
+    uint32_t v[VTOK][WORDS];
+#pragma unroll
+    for (int i = 0; i < S::VLOADS; ++i)
+#pragma unroll
+      for (int w = 0; w < WORDS; ++w) {
+        if constexpr (S::PAIRS) {
+          v[2 * i][w] = swapped(s.v[i][0][w], s.v[i][0][WORDS + w], kUpper);
+          v[2 * i + 1][w] = swapped(s.v[i][0][WORDS + w], s.v[i][0][w], kLower);
+        } else {
+          v[i][w] = s.v[i][w / 4][w % 4];
+        }
+      }
+    bool counts[VTOK];
+#pragma unroll
+    for (int i = 0; i < VTOK; ++i) counts[i] = true;
+    if (CAREFUL || !all) {
+#pragma unroll
+      for (int t = 0; t < TILES; ++t) {
+        const int4 m4 = *reinterpret_cast<const int4*>(slots + at + 16 * t + 4 * quad);
+        counts[4 * t] = m4.x >= 0, counts[4 * t + 1] = m4.y >= 0, counts[4 * t + 2] = m4.z >= 0, counts[4 * t + 3] = m4.w >= 0;
+      }
+      if constexpr (CAREFUL) {
+#pragma unroll
+        for (int i = 0; i < VTOK; ++i)
+#pragma unroll
+          for (int w = 0; w < WORDS; ++w) v[i][w] = counts[i] ? v[i][w] : 0u;
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      f32x4 s4[TILES];
+#pragma unroll
+      for (int t = 0; t < TILES; ++t) {
+        s4[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int p = 0; p < KP; ++p) {
+          if constexpr (WIDE) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              s4[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kf[t][p][e]), __uint_as_float(qf[c][p][e]), s4[t], 0, 0, 0);
+          } else if constexpr (HALF) {
+            s4[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, kf[t][p]), __builtin_bit_cast(f16x8, qf[c][p]), s4[t], 0, 0, 0);
+          } else {
+            s4[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kf[t][p]), __builtin_bit_cast(bf16x8, qf[c][p]), s4[t], 0, 0, 0);
+          }
+        }
+      }
+      float w[8];
+      float mt = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < VTOK; ++i) w[i] = s4[i >> 2][i & 3];
+      if (CAREFUL || !all) {
+#pragma unroll
+        for (int i = 0; i < VTOK; ++i) w[i] = counts[i] ? w[i] : -INFINITY;
+      }
+#pragma unroll
+      for (int i = 0; i < VTOK; ++i) mt = fmaxf(mt, w[i]);
+      if (__builtin_amdgcn_ballot_w64(mt > most[c]) != 0) {
+        auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mt), __float_as_uint(mt), false, false);
+        mt = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+        sw = __builtin_amdgcn_permlane16_swap(__float_as_uint(mt), __float_as_uint(mt), false, false);
+        mt = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+        if (mt > most[c]) {
+          most[c] = mt;
+          const float mNew = mt * a.scaleLog2e;
+          const float corr = m[c] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[c] - mNew);  // (no maximum yet: the sums are 0, or NaN)
+          m[c] = mRef[c] = mNew;
+          l[c] *= corr;
+#pragma unroll
+          for (int t = 0; t < RUN; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[c][t][i] *= corr;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < VTOK; ++i) {
+        w[i] = __builtin_amdgcn_exp2f(fmaf(w[i], a.scaleLog2e, -mRef[c]));
+        l[c] += w[i];
+      }
+      if constexpr (WIDE) {
+#pragma unroll
+        for (int t = 0; t < RUN; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float vi = __uint_as_float(v[i][t]);
+            if constexpr (CAREFUL) {
+              const bool finite = (v[i][t] & 0x7f800000u) != 0x7f800000u;
+              acc[c][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(finite ? 0.f : vi, w[i] > 0.f ? 1.f : w[i], acc[c][t], 0, 0, 0);
+              vi = finite ? vi : 0.f;
+            }
+            acc[c][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(vi, w[i], acc[c][t], 0, 0, 0);
+          }
+      } else {
+        bf16x8 some;
+        if constexpr (CAREFUL) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) some[i] = static_cast<bf16_t>(w[i] > 0.f ? 1.f : w[i]);
+        }
+        const bf16x8 hi = pxPart<T>(w), lo = pxPart<T>(w);
+        staticFor<RUN>([&](auto t) {
+          constexpr int W = t.value / 2;
+          constexpr unsigned kPick = t.value % 2 ? 0x07060302u : 0x05040100u;
+          u32x4 o;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[j] = __builtin_amdgcn_perm(v[2 * j + 1][W], v[2 * j][W], kPick);
+          u32x4 first, second;  // bf16 parts of V
+          if constexpr (HALF) {
+            const f16x8 oh = __builtin_bit_cast(f16x8, o);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float f0 = static_cast<float>(oh[2 * j]), f1 = static_cast<float>(oh[2 * j + 1]);
+              const uint32_t u0 = __float_as_uint(f0), u1 = __float_as_uint(f1);
+              first[j] = __builtin_amdgcn_perm(u1, u0, 0x07060302u);  // the upper 8 bits, cut: what is left has 3
+              const float r0 = f0 - __uint_as_float(u0 & 0xffff0000u), r1 = f1 - __uint_as_float(u1 & 0xffff0000u);
+              second[j] = __builtin_amdgcn_perm(__float_as_uint(r1), __float_as_uint(r0), 0x07060302u);
+            }
+          } else {
+            first = o;
+          }
+          if constexpr (CAREFUL) {
+            u32x4 odd;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const uint32_t bad = ((first[j] & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((first[j] & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
+              odd[j] = first[j] & bad, first[j] &= ~bad;
+              if constexpr (HALF) second[j] &= ~bad;
+            }
+            acc[c][t.value] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, odd), some, acc[c][t.value], 0, 0, 0);
+          }
+          acc[c][t.value] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, first), hi, acc[c][t.value], 0, 0, 0);
+          acc[c][t.value] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, first), lo, acc[c][t.value], 0, 0, 0);
+          if constexpr (HALF) acc[c][t.value] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, second), hi, acc[c][t.value], 0, 0, 0);
+        });
+      }
+    }
+  };
+  // the wave's share of a block, after the block's slots have been published
+  auto walk = [&](int n, bool clean, auto withCare) {
+    const int share = ((n + kPxWaves - 1) / kPxWaves + TOKENS - 1) / TOKENS * TOKENS;  // whole steps
+    const int from = min(wave * share, kPxBlock - TOKENS), to = min(n, wave * share + share);
+    const int last = from + (to - from - 1) / TOKENS * TOKENS;
+    Step s0;
+    request(s0, from);  // (also where the wave has no step: all of the block's slots can be read)
+    if constexpr (decltype(withCare)::value) {
+      for (int at = from; at < to; at += TOKENS) {
+        multiply(s0, at, false, withCare);
+        request(s0, min(at + TOKENS, last));
+      }
+    } else {
+      Step s1;
+      int at = from;
+      for (; at + TOKENS < to; at += 2 * TOKENS) {
+        request(s1, at + TOKENS);
+        multiply(s0, at, clean, withCare);
+        request(s0, min(at + 2 * TOKENS, last));  // (after the last step its rows again: a branch around the loads would make every wait one for all of them)
+        multiply(s1, at + TOKENS, clean && at + 2 * TOKENS <= n, withCare);
+      }
+      if (at < to) multiply(s0, at, clean && at + TOKENS <= n, withCare);
+    }
+  };
+  // Publishes the slots of [block, block + n): a thread looks up every 256th (past the last: that one again).
+  auto publish = [&](int block, int n) {
+    __syncthreads();  // every wave is done with the block before
+    bool bad = false;
+    for (int i = threadIdx.x; i < kPxBlock; i += kPxWaves * 64) {
+      if (i >= n + kPxWaves * TOKENS) break;  // (no step reaches further)
+      const int64_t slot = ldIndex(x.loc, block + min(i, n - 1), x.loc64);
+      const bool in = slot >= 0 && slot < a.slots;  // slots outside the pool are skipped, never dereferenced
+      slots[i] = in && i < n ? (int)slot : (int)((in ? (unsigned)slot : 0u) | 0x80000000u);
+      bad |= !in;
+    }
+    const bool waveBad = __builtin_amdgcn_ballot_w64(bad) != 0;
+    if (lane == 0) badBuf[wave] = waveBad;
+    __syncthreads();
+    return !(badBuf[0] | badBuf[1] | badBuf[2] | badBuf[3]);
+  };
+
+  clear();
+  for (int block = begin; block < end; block += kPxBlock) {
+    const int n = min(kPxBlock, end - block);
+    const bool clean = publish(block, n);
+    walk(n, clean, std::false_type{});
+  }
+  uint32_t largest = 0;
+#pragma unroll
+  for (int c = 0; c < NC; ++c)
+#pragma unroll
+    for (int t = 0; t < RUN; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) largest = max(largest, pairOf[c] >= 0 ? __float_as_uint(acc[c][t][i]) & 0x7fffffffu : 0u);
+  if (__syncthreads_or(largest >= 0x7f800000u)) {
+    clear();
+    for (int block = begin; block < end; block += kPxBlock) {
+      const int n = min(kPxBlock, end - block);
+      publish(block, n);
+      walk(n, false, std::true_type{});
+    }
+  }
+
+  // every lane group holds its own share of l; then waves 2 and 3 hand their sums to 0 and 1, and 1 its to 0
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(l[c]), __float_as_uint(l[c]), false, false);
+    l[c] = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
+    sw = __builtin_amdgcn_permlane16_swap(__float_as_uint(l[c]), __float_as_uint(l[c]), false, false);
+    l[c] = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
+    if (l[c] != l[c] && m[c] == -INFINITY) m[c] = 0.f;  // scores that are not numbers alone: as a maximum of minus infinity they would be left out
+  }
+#pragma unroll
+  for (int givers = kPxWaves / 2; givers >= 1; givers >>= 1) {
+    __syncthreads();
+    if (wave >= givers && wave < 2 * givers) {
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        stateBuf[wave - givers][c][0][lane] = m[c], stateBuf[wave - givers][c][1][lane] = l[c];
+#pragma unroll
+        for (int t = 0; t < RUN; ++t) pxLds[((wave - givers) * NC * RUN + c * RUN + t) * 64 + lane] = acc[c][t];
+      }
+    }
+    __syncthreads();
+    if (wave < givers) {
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const float m2 = stateBuf[wave][c][0][lane], l2 = stateBuf[wave][c][1][lane], mNew = fmaxf(m[c], m2);
+        const float w1 = m[c] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[c] - mNew), w2 = m2 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m2 - mNew);
+        m[c] = mNew, l[c] = l[c] * w1 + l2 * w2;
+#pragma unroll
+        for (int t = 0; t < RUN; ++t) {
+          const f32x4 o = pxLds[(wave * NC * RUN + c * RUN + t) * 64 + lane];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[c][t][i] = acc[c][t][i] * w1 + o[i] * w2;
+        }
+      }
+    }
+  }
+  if (wave != 0) return;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    if (pairOf[c] < 0) continue;
+    float* dst = partial + ((int64_t)pairOf[c] * x.nsplit + split) * (2 + a.d);
+    if (quad == 0) dst[0] = m[c], dst[1] = l[c];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int t = 0; t < RUN; ++t) {
+        const int e = S::place(4 * quad + i, t);
+        if (e < a.d) dst[2 + e] = acc[c][t][i];
+      }
+  }
+}
+
+// out[b, h, :] from the partial results of the prefix's chunks and of the sequence's own (see mergeChunks), WAVES to a (sequence,
+// head): every wave works out the weights of all shares, lane s those of shares s, s + 64, ..., then takes every WAVES-th share. The
+// length, the (maximum, sum) pairs and the first shares' elements are asked for before any of them is waited for; rows of shares
+// without tokens were never written, and what is read from them is discarded by a select.
+template <typename T, int WAVES>
+__global__ __launch_bounds__(256) void decodePrefixMergeKernel(T* __restrict__ out, const float* __restrict__ shared, int nShared, const float* __restrict__ own,
+                                                               int nOwn, int chunk, float raise, const void* bLen, bool len64, int maxLen, int64_t pairs, int heads, int d) {
+  constexpr int kBatch = 8, kMaxPerLane = 4, kPerLane = 8;  // d <= 256, at most 512 shares
+  __shared__ float red[4][64 * kMaxPerLane];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, part = wave % WAVES;
+  const int64_t pair = (int64_t)blockIdx.x * (4 / WAVES) + wave / WAVES;
+  if (WAVES == 1 && pair >= pairs) return;
+  const int row = 2 + d, all = nShared + nOwn;
+  const float* const sharedRows = shared + pair * nShared * row;
+  const float* const ownRows = own + pair * nOwn * row;
+  auto rowOf = [&](int s) { return s < nShared ? sharedRows + (int64_t)s * row : ownRows + (int64_t)(s - nShared) * row; };
+  float ms[kPerLane], ls[kPerLane], v[kBatch][kMaxPerLane];
+#pragma unroll
+  for (int k = 0; k < kPerLane; ++k) {
+    if (64 * k >= all) break;
+    const float* r = rowOf(min(lane + 64 * k, all - 1));
+    ms[k] = r[0] - (lane + 64 * k < nShared ? 0.f : raise), ls[k] = r[1];
+  }
+  auto loadBatch = [&](int s0) {
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const float* r = rowOf(min(s0 + WAVES * u, all - 1)) + 2;
+#pragma unroll
+      for (int k = 0; k < kMaxPerLane; ++k) {
+        const int e = lane + 64 * k;
+        v[u][k] = e < d ? r[e] : 0.f;
+      }
+    }
+  };
+  loadBatch(part);
+  const int64_t len = min(ldIndex(bLen, pair / heads, len64), (int64_t)maxLen);
+  const int used = nShared + (nOwn == 0 ? 0 : len <= 0 ? 1 : (int)((len + chunk - 1) / chunk));
+  float m = -INFINITY;
+#pragma unroll
+  for (int k = 0; k < kPerLane; ++k) {
+    if (64 * k >= all) break;
+    if (lane + 64 * k >= used) ms[k] = -INFINITY, ls[k] = 0.f;
+    m = fmaxf(m, ms[k]);
+  }
+  m = waveMax(m);
+  float sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < kPerLane; ++k) {
+    if (64 * k >= all) break;
+    ms[k] = ms[k] == -INFINITY ? 0.f : exp2f(ms[k] - m);  // the weight
+    sum += ls[k] * ms[k];
+  }
+  const float total = waveSum(sum), inv = total == 0.f ? 0.f : 1.f / total;
+  float acc[kMaxPerLane] = {0.f, 0.f, 0.f, 0.f};
+  for (int s0 = part; s0 < used; s0 += WAVES * kBatch) {
+    if (s0 != part) loadBatch(s0);
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int s = s0 + WAVES * u, owner = min(s, all - 1) >> 6;  // wave-uniform
+      float w = 0.f;
+#pragma unroll
+      for (int k = 0; k < kPerLane; ++k) {
+        if (64 * k >= all) break;
+        w = owner == k ? ms[k] : w;
+      }
+      w = __shfl(w, s & 63, 64) * inv;
+#pragma unroll
+      for (int k = 0; k < kMaxPerLane; ++k) acc[k] += s < used ? w * v[u][k] : 0.f;
+    }
+  }
+  if (WAVES == 1) {
+#pragma unroll
+    for (int k = 0; k < kMaxPerLane; ++k) {
+      const int e = lane + 64 * k;
+      if (e < d) out[pair * d + e] = static_cast<T>(acc[k]);
+    }
+    return;
+  }
+#pragma unroll
+  for (int k = 0; k < kMaxPerLane; ++k) red[wave][lane + 64 * k] = acc[k];
+  __syncthreads();
+  if (wave == 0) {
+#pragma unroll
+    for (int k = 0; k < kMaxPerLane; ++k) {
+      const int e = lane + 64 * k;
+      if (e < d) out[pair * d + e] = static_cast<T>(red[0][e] + red[1][e] + red[2][e] + red[3][e]);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- host side --
+template <typename T, int D, int NC>
+static diopiError_t launchPrefix(hipStream_t stream, const TaPrefixArgs& x, int64_t wgs, float* partial) {
+  const int lds = kPxWaves / 2 * NC * PxShape<T, D>::RUN * 64 * (int)sizeof(f32x4);
+  AMD_HIP(allowDynamicLds(reinterpret_cast<const void*>(decodePrefixKernel<T, D, NC>), lds));
+  hipLaunchKernelGGL((decodePrefixKernel<T, D, NC>), dim3((unsigned)wgs), dim3(kPxWaves * 64), lds, stream, x, partial);
+  AMD_LAUNCH_CHECK();
+  return diopiSuccess;
+}
+
+static diopiError_t decodeSharedPrefix(diopiContextHandle_t ctx, hipStream_t stream, TaPrefixArgs x, diopiDtype_t dtype, void* out) {
+  TaArgs& a = x.a;
+  const int64_t perKv = a.heads / a.kvHeads, columns = a.batch * perKv, cus = computeUnits(), itemsize = dtypeSize(dtype);
+  const int D = a.d <= 64 ? 64 : a.d <= 128 ? 128 : 256;
+  x.kStride = (unsigned)(a.kSlotStride * itemsize), x.vStride = (unsigned)(a.vSlotStride * itemsize);
+  const int64_t rowBytes = D * itemsize;
+  const int nc = columns <= 32 || rowBytes > 256 ? 1 : 2;
+  const int64_t groups = ceilDiv(columns, 16 * nc), step = kPxWaves * (itemsize == 4 ? 16 : 32);
+  const int64_t chunk = std::max<int64_t>(256, ceilDiv(x.len * a.kvHeads * groups, cus));
+  x.chunk = (int)(ceilDiv(std::max(chunk, ceilDiv(x.len, kPxMaxSplit)), step) * step);
+  x.nsplit = (int)ceilDiv(x.len, x.chunk);
+  const int64_t pairs = (int64_t)a.batch * a.heads, wgs = ceilDiv((int64_t)a.kvHeads * x.nsplit, 8) * 8 * groups;
+  AMD_CHECK(wgs < ((int64_t)1 << 31) && pairs < ((int64_t)1 << 31), "shared prefix attention: %ld workgroups exceed the grid limits", (long)wgs);
+  void* ws = nullptr;
+  AMD_TRY(requireWorkspace(ctx, pairs * x.nsplit * (2 + a.d) * (int64_t)sizeof(float), &ws));
+  float* partial = static_cast<float*>(ws);
+#define PREFIX_CALL(T, SIZE, N) AMD_TRY((launchPrefix<T, SIZE, N>(stream, x, wgs, partial)))
+#define PREFIX_COLUMNS(T, SIZE) \
+  do { if (nc == 1) PREFIX_CALL(T, SIZE, 1); else PREFIX_CALL(T, SIZE, 2); } while (0)
+#define PREFIX_SIZES(T)                       \
+  do {                                        \
+    if (D == 64) PREFIX_COLUMNS(T, 64);       \
+    else if (D == 128) PREFIX_COLUMNS(T, 128); \
+    else PREFIX_CALL(T, 256, 1);              \
+  } while (0)
+  if (dtype == diopi_dtype_bfloat16) {
+    PREFIX_SIZES(bf16_t);
+  } else if (dtype == diopi_dtype_float16) {
+    PREFIX_SIZES(half_t);
+  } else if (D == 64) {
+    PREFIX_COLUMNS(float, 64);
+  } else {
+    PREFIX_CALL(float, 128, 1);
+  }
+#undef PREFIX_SIZES
+#undef PREFIX_COLUMNS
+#undef PREFIX_CALL
+  TaPartials own{nullptr, 0, 1, 0.f};
+  if (a.maxLen > 0) AMD_TRY(decodePartials(ctx, stream, a, dtype, a.maxLen, &own));
+  const bool narrow = x.nsplit + own.nsplit <= 16;
+#define PREFIX_MERGE(T)                                                                                                                          \
+  do {                                                                                                                                           \
+    if (narrow)                                                                                                                                  \
+      hipLaunchKernelGGL((decodePrefixMergeKernel<T, 1>), dim3((unsigned)ceilDiv(pairs, 4)), dim3(256), 0, stream, static_cast<T*>(out), partial, \
+                         x.nsplit, own.partial, own.nsplit, own.chunk, own.raise, a.bLen, a.len64, a.maxLen, pairs, a.heads, a.d);                                    \
+    else                                                                                                                                         \
+      hipLaunchKernelGGL((decodePrefixMergeKernel<T, 4>), dim3((unsigned)pairs), dim3(256), 0, stream, static_cast<T*>(out), partial, x.nsplit,   \
+                         own.partial, own.nsplit, own.chunk, own.raise, a.bLen, a.len64, a.maxLen, pairs, a.heads, a.d);                                              \
+  } while (0)
+  if (dtype == diopi_dtype_bfloat16) PREFIX_MERGE(bf16_t);
+  else if (dtype == diopi_dtype_float16) PREFIX_MERGE(half_t);
+  else PREFIX_MERGE(float);
+#undef PREFIX_MERGE
+  AMD_LAUNCH_CHECK();
+  return diopiSuccess;
+}
+
 }  // namespace amd
 
 using namespace amd;
@@ -111,6 +681,9 @@ extern "C" __attribute__((visibility("default"))) diopiError_t diopiTokenDecodeA
   AMD_CHECK(t.q.shape[2] <= kTaGenericMaxD, "shared prefix attention: head_dim %ld exceeds %d", (long)t.q.shape[2], kTaGenericMaxD);
   AMD_TRY(makeContiguous(ctx, stream, prefix, &densePrefix));
   x.loc = densePrefix.data, x.loc64 = prefix.dtype == diopi_dtype_int64, x.len = (int)prefix.shape[0];
+  // (slot numbers in 31 bits; a prefix of nothing shares nothing, and is no case of its own)
+  if (!a.generic && x.len > 0 && a.slots <= 0x7fffffff && std::max(a.kSlotStride, a.vSlotStride) * t.q.itemsize <= 0xffffffffll)
+    return decodeSharedPrefix(ctx, stream, x, t.q.dtype, out.data);
   const dim3 grid(a.heads, a.batch);
   if (t.q.dtype == diopi_dtype_bfloat16) hipLaunchKernelGGL((decodePrefixAnyKernel<bf16_t>), grid, dim3(256), 0, stream, x, out.ptr<bf16_t>());
   else if (t.q.dtype == diopi_dtype_float16) hipLaunchKernelGGL((decodePrefixAnyKernel<half_t>), grid, dim3(256), 0, stream, x, out.ptr<half_t>());
