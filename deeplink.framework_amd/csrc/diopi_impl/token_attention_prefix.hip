@@ -489,6 +489,488 @@ __global__ __launch_bounds__(kPxWaves * 64, 1) void decodePrefixKernel(TaPrefixA
   }
 }
 
+// ------------------------------------------------ many columns: rows shared by the waves through LDS --
+// With more than two tiles of columns every wave would read the rows for itself, turn V round for itself, and, one wave to a SIMD, let
+// the matrix pipe wait for the softmax (16 001 tokens, 192 columns: 99 us). Here eight waves share a stage of 64 tokens: four
+// groups of NC column tiles times two halves of the tokens, so a workgroup takes up to 192 columns from one read of a row, and of
+// the two waves of a SIMD one multiplies while the other takes exponentials. Rows go straight into a ring of stages in LDS
+// (global_load_lds, 16 bytes to a lane, pieces XOR-swizzled by row), K is read as it lies, V through the transposing read; one
+// barrier per stage.
+// Probabilities in fp16 are taken times 2^15 (at most 2^15) and cut into two fp16 parts, all bits down to 2^-17 of the
+// largest, 16 down to 2^-24; a step that has smaller ones multiplies what is left of them times 2^24, 2^48 ... too, until
+// nothing is left.
+constexpr int kPtWaves = 8;
+constexpr float kPtRescaleStep = 8.f;  // log2 domain
+constexpr float kPtTwoParts = 16.f;    // two fp16 parts hold 16 bits of what is at least 2^-this
+template <typename T, int D>
+struct PtShape {
+  static constexpr int HALVES = D == 256 ? 1 : 2;                              // shares of a stage's tokens, 32 each
+  static constexpr int TOKENS = 32 * HALVES, COLUMN_WAVES = kPtWaves / HALVES;
+  static constexpr int ROWB = D * 2, CPR = ROWB / 16, RPL = 64 / CPR;         // pieces of a row, rows of a wave's load
+  static constexpr int LOADS = TOKENS / RPL / kPtWaves;                        // of a wave, per matrix and stage
+  static constexpr int STAGEB = 2 * TOKENS * ROWB, STAGES = 4;
+  static constexpr int KS = D / 32, DT = D / 16;
+  // XOR on the 16-byte piece index of row r: 16 rows' pieces of one index of K fall on 16 different bank groups, the 8 rows x 32
+  // bytes of half a transposing read of V on 8
+  static __device__ __forceinline__ int swizzleK(int r) { return D >= 128 ? (r & 15) : ((r >> 1) & 7); }
+  static __device__ __forceinline__ int swizzleV(int r) { return D >= 128 ? 2 * (r & 7) : 2 * ((r >> 1) & 3); }
+};
+template <typename T>
+struct PtMfma;
+template <>
+struct PtMfma<bf16_t> {
+  typedef bf16x8 Frag;
+  static __device__ __forceinline__ f32x4 run(u32x4 a, Frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), b, c, 0, 0, 0); }
+  static constexpr float kRaise = 0.f;  // log2 of what probabilities are multiplied by
+  static constexpr uint32_t kExponent = 0x7f80u;
+};
+template <>
+struct PtMfma<half_t> {
+  typedef f16x8 Frag;
+  static __device__ __forceinline__ f32x4 run(u32x4 a, Frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), b, c, 0, 0, 0); }
+  static constexpr float kRaise = 7.f;
+  static constexpr uint32_t kExponent = 0x7c00u;
+};
+// The next part of eight numbers, and what it leaves. fp16: cut, not rounded, and subtracted in one mixed instruction each (half the
+// instructions; what is left is then a number of up to 13 bits more, of which the second part, rounded, has 11).
+template <typename T>
+__device__ __forceinline__ typename PtMfma<T>::Frag ptPart(float (&x)[8]) {
+  typename PtMfma<T>::Frag part;
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    if constexpr (std::is_same<T, half_t>::value) {
+      typedef __fp16 Cut __attribute__((ext_vector_type(2)));
+      typedef half_t Pair __attribute__((ext_vector_type(2)));
+      const Cut cut = __builtin_amdgcn_cvt_pkrtz(x[i], x[i + 1]);
+      const Pair pair = __builtin_bit_cast(Pair, cut);
+      part[i] = pair[0], part[i + 1] = pair[1];
+      x[i] = fmaf(static_cast<float>(pair[0]), -1.f, x[i]), x[i + 1] = fmaf(static_cast<float>(pair[1]), -1.f, x[i + 1]);
+    } else {
+      part[i] = static_cast<T>(x[i]), part[i + 1] = static_cast<T>(x[i + 1]);
+      x[i] -= static_cast<float>(part[i]), x[i + 1] -= static_cast<float>(part[i + 1]);
+    }
+  }
+  return part;
+}
+template <typename T>
+__device__ __forceinline__ typename PtMfma<T>::Frag ptLast(const float (&x)[8]) {  // eight numbers rounded
+  typename PtMfma<T>::Frag part;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) part[i] = static_cast<T>(x[i]);
+  return part;
+}
+
+template <typename T, int D, int NC>
+__global__ __launch_bounds__(kPtWaves * 64, 2) void decodePrefixTiledKernel(TaPrefixArgs x, float* __restrict__ partial) {
+  using S = PtShape<T, D>;
+  using M = PtMfma<T>;
+  using Frag = typename M::Frag;
+  constexpr int ROWB = S::ROWB, KS = S::KS, DT = S::DT, STAGES = S::STAGES, TOKENS = S::TOKENS, COLUMN_WAVES = S::COLUMN_WAVES;
+  constexpr bool HALF = std::is_same<T, half_t>::value;
+  const TaArgs& a = x.a;
+  extern __shared__ __attribute__((aligned(16))) f32x4 ptLds[];  // the ring; at the end, sums on their way to the waves that add them up
+  __shared__ __attribute__((aligned(16))) int slots[kPxBlock];  // of a block's tokens; negative: does not count
+  __shared__ int badBuf[kPtWaves];
+  __shared__ float stateBuf[S::HALVES == 2 ? COLUMN_WAVES : 1][NC][2][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 15, quad = lane >> 4;
+  const int columnWave = wave % COLUMN_WAVES, half = wave / COLUMN_WAVES;
+
+  // grid as in decodePrefixKernel
+  const int f = blockIdx.x, idx = f >> 3;
+  const int perKv = a.heads / a.kvHeads, columns = a.batch * perKv, groups = (columns + 16 * COLUMN_WAVES * NC - 1) / (16 * COLUMN_WAVES * NC);
+  const int group = idx % groups, u = (idx / groups) * 8 + (f & 7);
+  if (u >= a.kvHeads * x.nsplit) return;  // the grid is rounded up to whole rounds of the XCDs
+  const int kvh = u % a.kvHeads, split = u / a.kvHeads;
+  const int begin = split * x.chunk, end = min(x.len, begin + x.chunk);
+  const int firstColumn = (group * COLUMN_WAVES + columnWave) * NC * 16;
+  const bool active = firstColumn < columns;  // (a wave without columns only copies)
+
+  Frag qf[NC][KS];
+  int pairOf[NC];  // row of the partial results of this lane's column, or -1
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const int column = firstColumn + c * 16 + col;
+    const bool have = column < columns;
+    const int b = have ? column / perKv : 0, h = kvh * perKv + (have ? column % perKv : 0);
+    pairOf[c] = have ? b * a.heads + h : -1;
+    const T* src = reinterpret_cast<const T*>(a.q) + b * a.qBatchStride + h * a.qHeadStride;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const int e = 32 * s + 8 * quad;
+      u32x4 v = *reinterpret_cast<const u32x4*>(src + (e < a.d ? e : 0));
+      if (!have || e >= a.d) v = u32x4{0, 0, 0, 0};
+      qf[c][s] = __builtin_bit_cast(Frag, v);
+    }
+  }
+
+  // copies: load i of this wave fills the KiB i * 8 + wave of a matrix; lane l owns the place (row l / CPR, piece l % CPR) of it and
+  // fetches the piece that the swizzle puts there (pieces past the row's end repeat its first one)
+  const unsigned ring = (unsigned)(uintptr_t)ptLds;
+  const char* kSrc[S::LOADS];
+  const char* vSrc[S::LOADS];
+  int rowOf[S::LOADS];
+#pragma unroll
+  for (int i = 0; i < S::LOADS; ++i) {
+    rowOf[i] = (i * kPtWaves + wave) * S::RPL + lane / S::CPR;
+    const int p = lane % S::CPR, kc = (p ^ S::swizzleK(rowOf[i])) * 8, vc = (p ^ S::swizzleV(rowOf[i])) * 8;
+    kSrc[i] = reinterpret_cast<const char*>(reinterpret_cast<const T*>(a.k) + kvh * a.kHeadStride + (kc < a.d ? kc : 0));
+    vSrc[i] = reinterpret_cast<const char*>(reinterpret_cast<const T*>(a.v) + kvh * a.vHeadStride + (vc < a.d ? vc : 0));
+  }
+  auto copy = [&](int at, int stage) {
+    const unsigned to = ring + (unsigned)(stage * S::STAGEB + wave * 1024);
+#pragma unroll
+    for (int i = 0; i < S::LOADS; ++i) {
+      const uint64_t n = (unsigned)slots[at + rowOf[i]] & 0x7fffffffu;
+      globalLoadToLds16(kSrc[i] + n * x.kStride, to + i * kPtWaves * 1024u);
+      globalLoadToLds16(vSrc[i] + n * x.vStride, to + TOKENS * ROWB + i * kPtWaves * 1024u);
+    }
+  };
+
+  f32x4 acc[NC][DT];
+  float most[NC], m[NC], mRef[NC], l[NC];  // the largest score, the same in units of log2, what scores are taken against, the sum
+  auto clear = [&] {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      most[c] = m[c] = -INFINITY, mRef[c] = l[c] = 0.f;
+#pragma unroll
+      for (int t = 0; t < DT; ++t) acc[c][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+  };
+  // What a stage goes through. Rows of K and of V are asked for ahead of what is done with those before them: the first products of
+  // a stage find K in registers, those with V the first kAhead places.
+  constexpr int kAhead = HALF && D == 128 && NC == 2 ? 2 : 4;  // (four would not fit the registers there)
+  constexpr bool kAheadK = D < 256;  // (rows of 512 bytes: the registers for it are not there)
+  typedef __attribute__((address_space(3))) const u32x4* LdsPiece;
+  typedef __attribute__((address_space(3))) s16x4* LdsTr;
+  auto readK = [&](u32x4 (&kf)[2][KS], int stage) {
+    const unsigned at = ring + (unsigned)(stage * S::STAGEB + half * 32 * ROWB);
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const int row = 16 * t + col;
+        kf[t][s] = *(LdsPiece)(uintptr_t)(at + (unsigned)(row * ROWB + (((4 * s + quad) ^ S::swizzleK(row)) << 4)));
+      }
+  };
+  auto scoresOf = [&](const u32x4 (&kf)[2][KS], f32x4 (&s4)[NC][2], auto withCare) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+      for (int c = 0; c < NC; ++c) s4[c][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        u32x4 k = kf[t][s];
+        if (decltype(withCare)::value && 32 * s + 8 * quad >= a.d) k = u32x4{0, 0, 0, 0};  // (an infinity against q's zeros would be NaN)
+#pragma unroll
+        for (int c = 0; c < NC; ++c) s4[c][t] = M::run(k, qf[c][s], s4[c][t]);
+      }
+  };
+  struct Counts {  // which of the lane's eight tokens count
+    bool of[8];
+  };
+  auto countsOf = [&](int at, bool all) {
+    Counts n;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) n.of[i] = true;
+    if (!all) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int4 m4 = *reinterpret_cast<const int4*>(slots + at + 32 * half + 16 * t + 4 * quad);
+        n.of[4 * t] = m4.x >= 0, n.of[4 * t + 1] = m4.y >= 0, n.of[4 * t + 2] = m4.z >= 0, n.of[4 * t + 3] = m4.w >= 0;
+      }
+    }
+    return n;
+  };
+  // the scores of column tile c: its maximum followed (and all that was summed against the old one), as powers of two
+  auto powersOf = [&](int c, const f32x4 (&s4)[2], const Counts& n, bool all, float (&arg)[8], bool follow, float step) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) arg[i] = s4[i >> 2][i & 3];
+    if (!all) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) arg[i] = n.of[i] ? arg[i] : -INFINITY;
+    }
+    if (follow) {
+      float mt = arg[0];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) mt = fmaxf(mt, arg[i]);
+      if (__builtin_amdgcn_ballot_w64(mt * a.scaleLog2e > m[c] + step) != 0) {
+        auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mt), __float_as_uint(mt), false, false);
+        mt = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+        sw = __builtin_amdgcn_permlane16_swap(__float_as_uint(mt), __float_as_uint(mt), false, false);
+        mt = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+        if (mt > most[c]) {
+          most[c] = mt;
+          const float mNew = mt * a.scaleLog2e;
+          const float corr = m[c] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[c] - mNew);  // (no maximum yet: the sums are 0, or NaN)
+          m[c] = mRef[c] = mNew;
+          l[c] *= corr;
+#pragma unroll
+          for (int t = 0; t < DT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[c][t][i] *= corr;
+        }
+      }
+    }
+    const float ref = mRef[c] - M::kRaise;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) arg[i] = fmaf(arg[i], a.scaleLog2e, -ref);
+  };
+  auto readV = [&](int d, int stage) {  // eight tokens at the lane's place of the head
+    const unsigned at = ring + (unsigned)(stage * S::STAGEB + (TOKENS + half * 32) * ROWB);
+    const int vRow = 4 * quad + ((lane & 15) >> 2);
+    u32x2 v[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int row = 16 * t + vRow;
+      const unsigned piece = (unsigned)((2 * d + ((lane & 3) >> 1)) ^ S::swizzleV(row)) << 4;
+      v[t] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsTr)(uintptr_t)(at + (unsigned)(row * ROWB + (lane & 1) * 8) + piece)));
+    }
+    return u32x4{v[0][0], v[0][1], v[1][0], v[1][1]};
+  };
+  auto infinite = [](u32x4 v) {  // ones where V is not finite
+    u32x4 bad;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      bad[j] = ((v[j] & M::kExponent) == M::kExponent ? 0xffffu : 0u) | ((v[j] & (M::kExponent << 16)) == (M::kExponent << 16) ? 0xffff0000u : 0u);
+    return bad;
+  };
+  auto keepOf = [&](const Counts& n) {  // ones where a token counts
+    u32x4 keep = {~0u, ~0u, ~0u, ~0u};
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (!n.of[i]) keep[i >> 1] &= i & 1 ? 0xffffu : 0xffff0000u;
+    return keep;
+  };
+  // What two parts leave of probabilities below 2^-24 of the largest, times 2^24, 2^48 ... (the scores once more: keeping them for
+  // this would cost the registers of a column tile).
+  auto addRest = [&](int stage, int at, bool all, auto withCare) {
+    constexpr bool CAREFUL = decltype(withCare)::value;
+    const Counts n = countsOf(at, all);
+    const u32x4 keep = keepOf(n);
+    u32x4 kf[2][KS];
+    readK(kf, stage);
+    f32x4 s4[NC][2];
+    scoresOf(kf, s4, withCare);
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      float w[8];
+      powersOf(c, s4[c], n, all, w, false, 0.f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        w[i] = __builtin_amdgcn_exp2f(w[i]);
+        w[i] = w[i] == w[i] ? w[i] : 0.f;  // (NaN is in the first part)
+      }
+      auto leave = [&] {  // the first part, and the second
+        const Frag first = ptPart<T>(w), second = ptLast<T>(w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] -= static_cast<float>(second[i]);
+        return std::pair<Frag, Frag>{first, second};
+      };
+      leave();
+      float back = 1.f;
+      for (int round = 0; round < 6; ++round) {  // (2^-169 is all that could be left after them)
+        bool any = false;
+        back *= 0x1p-24f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          w[i] *= 0x1p24f;
+          any |= w[i] != 0.f;
+        }
+        if (__builtin_amdgcn_ballot_w64(any) == 0) break;
+        const auto [hi, lo] = leave();
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          u32x4 v = readV(d, stage);
+          if constexpr (CAREFUL) v &= keep & ~infinite(v);
+          f32x4 rest = M::run(v, hi, f32x4{0.f, 0.f, 0.f, 0.f});
+          rest = M::run(v, lo, rest);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[c][d][i] += rest[i] * back;
+        }
+      }
+    }
+  };
+  // the stages of a block, after its slots have been published; clean: all of its slots lie in the pool
+  auto walk = [&](int n, bool clean, auto withCare) {
+    constexpr bool CAREFUL = decltype(withCare)::value;
+    const int stages = (n + TOKENS - 1) / TOKENS;
+    // this wave's copies of a stage have landed (loads end in order; `behind` stages are on their way) and then everybody's have
+    auto landed = [&](bool behind) {
+      constexpr int kBehind = 2 * S::LOADS * (STAGES - 3);
+      if (behind) __builtin_amdgcn_s_waitcnt(0x0f70 | (kBehind & 15) | (kBehind >> 4) << 14);
+      else __builtin_amdgcn_s_waitcnt(0x0f70);
+      asm volatile("" : : : "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" : : : "memory");
+    };
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; ++s)
+      if (s < stages) copy(s * TOKENS, s);
+    __builtin_amdgcn_s_waitcnt(0x0f70);
+    asm volatile("" : : : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" : : : "memory");
+    u32x4 kf[2][KS];
+    if (kAheadK && active) readK(kf, 0);
+    int stage = 0;
+    for (int s = 0; s < stages; ++s) {
+      const bool all = !CAREFUL && clean && (s + 1) * TOKENS <= n;
+      const int next = stage + 1 == STAGES ? 0 : stage + 1;
+      Frag hi[NC], lo[NC], some[CAREFUL ? NC : 1];
+      u32x4 v[kAhead], keep = {~0u, ~0u, ~0u, ~0u};
+      bool small = false;  // of a probability some bits may be left
+      if (active) {
+        f32x4 s4[NC][2];
+        if (!kAheadK) readK(kf, stage);
+        scoresOf(kf, s4, withCare);
+        const Counts counts = countsOf(s * TOKENS, all);
+        if constexpr (CAREFUL) keep = keepOf(counts);
+#pragma unroll
+        for (int d = 0; d < kAhead; ++d) v[d] = readV(d, stage);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          float w[8], lowest = 0.f;
+          powersOf(c, s4[c], counts, all, w, true, CAREFUL ? 0.f : kPtRescaleStep);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            if (HALF) lowest = fminf(lowest, w[i]);
+            w[i] = __builtin_amdgcn_exp2f(w[i]);
+            l[c] += w[i];
+          }
+          small |= lowest < M::kRaise - kPtTwoParts;
+          if constexpr (CAREFUL) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) some[c][i] = static_cast<T>(w[i] > 0.f ? 1.f : w[i]);
+          }
+          hi[c] = ptPart<T>(w), lo[c] = ptLast<T>(w);
+        }
+      }
+      if (s + 1 < stages) {
+        landed(s + STAGES - 2 < stages);
+        // (everybody has read the stage before this one: its place is free)
+        if (s + STAGES - 1 < stages) copy((s + STAGES - 1) * TOKENS, stage == 0 ? STAGES - 1 : stage - 1);
+        if (kAheadK && active) readK(kf, next);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if (active) {
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          u32x4 now = v[d % kAhead];
+          if (d + kAhead < DT) v[d % kAhead] = readV(d + kAhead, stage);
+          if constexpr (CAREFUL) {
+            now &= keep;
+            const u32x4 bad = infinite(now), odd = now & bad;
+            now &= ~bad;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) acc[c][d] = M::run(odd, some[c], acc[c][d]);
+          }
+#pragma unroll
+          for (int c = 0; c < NC; ++c) acc[c][d] = M::run(now, hi[c], acc[c][d]);
+#pragma unroll
+          for (int c = 0; c < NC; ++c) acc[c][d] = M::run(now, lo[c], acc[c][d]);
+        }
+        if constexpr (HALF) {
+          if (__builtin_amdgcn_ballot_w64(small) != 0) addRest(stage, s * TOKENS, all, withCare);
+        }
+      }
+      stage = next;
+    }
+  };
+  // Publishes the slots of [block, block + n) (up to a whole stage: that of the last token again).
+  auto publish = [&](int block, int n) {
+    __syncthreads();  // every wave is done with the block before
+    bool bad = false;
+    for (int i = threadIdx.x; i < (n + TOKENS - 1) / TOKENS * TOKENS; i += kPtWaves * 64) {
+      const int64_t slot = ldIndex(x.loc, block + min(i, n - 1), x.loc64);
+      const bool in = slot >= 0 && slot < a.slots;  // slots outside the pool are skipped, never dereferenced
+      slots[i] = in && i < n ? (int)slot : (int)((in ? (unsigned)slot : 0u) | 0x80000000u);
+      bad |= !in;
+    }
+    const bool waveBad = __builtin_amdgcn_ballot_w64(bad) != 0;
+    if (lane == 0) badBuf[wave] = waveBad;
+    __syncthreads();
+    bool any = false;
+#pragma unroll
+    for (int w = 0; w < kPtWaves; ++w) any |= badBuf[w] != 0;
+    return !any;
+  };
+
+  clear();
+  for (int block = begin; block < end; block += kPxBlock) {
+    const int n = min(kPxBlock, end - block);
+    const bool clean = publish(block, n);
+    walk(n, clean, std::false_type{});
+  }
+  uint32_t largest = 0;
+#pragma unroll
+  for (int c = 0; c < NC; ++c)
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) largest = max(largest, pairOf[c] >= 0 ? __float_as_uint(acc[c][t][i]) & 0x7fffffffu : 0u);
+  if (__syncthreads_or(largest >= 0x7f800000u)) {
+    clear();
+    for (int block = begin; block < end; block += kPxBlock) {
+      const int n = min(kPxBlock, end - block);
+      publish(block, n);
+      walk(n, false, std::true_type{});
+    }
+  }
+
+  // every lane group holds its own share of l; the waves of the second half hand their sums to those of the first
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(l[c]), __float_as_uint(l[c]), false, false);
+    l[c] = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
+    sw = __builtin_amdgcn_permlane16_swap(__float_as_uint(l[c]), __float_as_uint(l[c]), false, false);
+    l[c] = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
+    if (l[c] != l[c] && m[c] == -INFINITY) m[c] = 0.f;  // scores that are not numbers alone: as a maximum of minus infinity they would be left out
+  }
+  if constexpr (S::HALVES == 2) __syncthreads();
+  if (half == 1) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      stateBuf[columnWave][c][0][lane] = m[c], stateBuf[columnWave][c][1][lane] = l[c];
+#pragma unroll
+      for (int t = 0; t < DT; ++t) ptLds[((columnWave * NC + c) * DT + t) * 64 + lane] = acc[c][t];
+    }
+  }
+  if constexpr (S::HALVES == 2) __syncthreads();
+  if (half == 1) return;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    float mNew = m[c], w1 = 1.f, w2 = 0.f, sum = l[c];
+    if constexpr (S::HALVES == 2) {
+      const float m2 = stateBuf[columnWave][c][0][lane];
+      mNew = fmaxf(m[c], m2);
+      w1 = m[c] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[c] - mNew), w2 = m2 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m2 - mNew);
+      sum = l[c] * w1 + stateBuf[columnWave][c][1][lane] * w2;
+    }
+    float* dst = partial + ((int64_t)pairOf[c] * x.nsplit + split) * (2 + a.d);
+    if (pairOf[c] < 0) continue;
+    // (sums are against the maximum less the raise)
+    if (quad == 0) *reinterpret_cast<float2*>(dst) = float2{mNew - M::kRaise, sum};
+#pragma unroll
+    for (int t = 0; t < DT; ++t) {
+      const int e = 16 * t + 4 * quad;
+      if (e >= a.d) continue;
+      f32x4 r = acc[c][t];
+      if constexpr (S::HALVES == 2) {
+        const f32x4 o = ptLds[((columnWave * NC + c) * DT + t) * 64 + lane];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = r[i] * w1 + o[i] * w2;
+      }
+      *reinterpret_cast<float2*>(dst + 2 + e) = float2{r[0], r[1]};
+      *reinterpret_cast<float2*>(dst + 4 + e) = float2{r[2], r[3]};
+    }
+  }
+}
+
 // out[b, h, :] from the partial results of the prefix's chunks and of the sequence's own (see mergeChunks), WAVES to a (sequence,
 // head): every wave works out the weights of all shares, lane s those of shares s, s + 64, ..., then takes every WAVES-th share. The
 // length, the (maximum, sum) pairs and the first shares' elements are asked for before any of them is waited for; rows of shares
@@ -581,6 +1063,16 @@ __global__ __launch_bounds__(256) void decodePrefixMergeKernel(T* __restrict__ o
 
 // ---------------------------------------------------------------- host side --
 template <typename T, int D, int NC>
+static diopiError_t launchTiled(hipStream_t stream, const TaPrefixArgs& x, int64_t wgs, float* partial) {
+  const int lds = PtShape<T, D>::STAGES * PtShape<T, D>::STAGEB;
+  static_assert(PtShape<T, D>::HALVES == 1 || PtShape<T, D>::STAGES * PtShape<T, D>::STAGEB >= PtShape<T, D>::COLUMN_WAVES * NC * PtShape<T, D>::DT * 64 * (int)sizeof(f32x4), "the sums of half the waves take the place of the ring");
+  AMD_HIP(allowDynamicLds(reinterpret_cast<const void*>(decodePrefixTiledKernel<T, D, NC>), lds));
+  hipLaunchKernelGGL((decodePrefixTiledKernel<T, D, NC>), dim3((unsigned)wgs), dim3(kPtWaves * 64), lds, stream, x, partial);
+  AMD_LAUNCH_CHECK();
+  return diopiSuccess;
+}
+
+template <typename T, int D, int NC>
 static diopiError_t launchPrefix(hipStream_t stream, const TaPrefixArgs& x, int64_t wgs, float* partial) {
   const int lds = kPxWaves / 2 * NC * PxShape<T, D>::RUN * 64 * (int)sizeof(f32x4);
   AMD_HIP(allowDynamicLds(reinterpret_cast<const void*>(decodePrefixKernel<T, D, NC>), lds));
@@ -595,8 +1087,12 @@ static diopiError_t decodeSharedPrefix(diopiContextHandle_t ctx, hipStream_t str
   const int D = a.d <= 64 ? 64 : a.d <= 128 ? 128 : 256;
   x.kStride = (unsigned)(a.kSlotStride * itemsize), x.vStride = (unsigned)(a.vSlotStride * itemsize);
   const int64_t rowBytes = D * itemsize;
-  const int nc = columns <= 32 || rowBytes > 256 ? 1 : 2;
-  const int64_t groups = ceilDiv(columns, 16 * nc), step = kPxWaves * (itemsize == 4 ? 16 : 32);
+  const bool tiled = itemsize == 2 && columns > 32;
+  const int64_t tiles = ceilDiv(columns, 16), columnWaves = D == 256 ? PtShape<half_t, 256>::COLUMN_WAVES : PtShape<half_t, 128>::COLUMN_WAVES;
+  int nc = columns <= 32 || rowBytes > 256 ? 1 : 2;
+  const int ncMost = D == 256 ? 1 : D == 128 ? 2 : 3;  // (more spill registers)
+  if (tiled) nc = std::min(ncMost, tiles <= 4 ? 1 : tiles <= 8 ? 2 : 3);
+  const int64_t groups = ceilDiv(tiles, tiled ? columnWaves * nc : nc), step = tiled ? (D == 256 ? 32 : 64) : kPxWaves * (itemsize == 4 ? 16 : 32);
   const int64_t chunk = std::max<int64_t>(256, ceilDiv(x.len * a.kvHeads * groups, cus));
   x.chunk = (int)(ceilDiv(std::max(chunk, ceilDiv(x.len, kPxMaxSplit)), step) * step);
   x.nsplit = (int)ceilDiv(x.len, x.chunk);
@@ -610,11 +1106,24 @@ static diopiError_t decodeSharedPrefix(diopiContextHandle_t ctx, hipStream_t str
   do { if (nc == 1) PREFIX_CALL(T, SIZE, 1); else PREFIX_CALL(T, SIZE, 2); } while (0)
 #define PREFIX_SIZES(T)                       \
   do {                                        \
-    if (D == 64) PREFIX_COLUMNS(T, 64);       \
-    else if (D == 128) PREFIX_COLUMNS(T, 128); \
+    if (D == 64) PREFIX_CALL(T, 64, 1);       \
+    else if (D == 128) PREFIX_CALL(T, 128, 1); \
     else PREFIX_CALL(T, 256, 1);              \
   } while (0)
-  if (dtype == diopi_dtype_bfloat16) {
+#define TILED_CALL(T, SIZE, N) AMD_TRY((launchTiled<T, SIZE, N>(stream, x, wgs, partial)))
+#define TILED_COLUMNS(T, SIZE) \
+  do { if (nc == 1) TILED_CALL(T, SIZE, 1); else TILED_CALL(T, SIZE, 2); } while (0)
+#define TILED_SIZES(T)                        \
+  do {                                        \
+    if (D == 64 && nc == 3) TILED_CALL(T, 64, 3); \
+    else if (D == 64) TILED_COLUMNS(T, 64);       \
+    else if (D == 128) TILED_COLUMNS(T, 128);     \
+    else TILED_CALL(T, 256, 1);               \
+  } while (0)
+  if (tiled) {
+    if (dtype == diopi_dtype_bfloat16) TILED_SIZES(bf16_t);
+    else TILED_SIZES(half_t);
+  } else if (dtype == diopi_dtype_bfloat16) {
     PREFIX_SIZES(bf16_t);
   } else if (dtype == diopi_dtype_float16) {
     PREFIX_SIZES(half_t);
@@ -623,6 +1132,9 @@ static diopiError_t decodeSharedPrefix(diopiContextHandle_t ctx, hipStream_t str
   } else {
     PREFIX_CALL(float, 128, 1);
   }
+#undef TILED_SIZES
+#undef TILED_COLUMNS
+#undef TILED_CALL
 #undef PREFIX_SIZES
 #undef PREFIX_COLUMNS
 #undef PREFIX_CALL
