@@ -5,18 +5,22 @@
 //
 // A row (one token, one head) x is kept as whole numbers q and a scale s:
 //   s = max |x| / 127 rounded to fp32,  q = the whole number nearest to x / s, ties to the even one
-// so q lies in [-127, 127] (it is cut to that where s has lost its last places below 2^-126). q is that of the EXACT quotient: a quotient rounded to fp32 falls on a half for one element in
-// 10^5 that does not, and which neighbour it goes to would depend on how the division is done. Rows of zeros have s = 0. A row
-// that holds an infinity or NaN has s = NaN and q = 0: all of it reads back as NaN, none of it as a plausible number.
-// Read back: q * s rounded to fp32, and once more to a 16-bit type.
+// so q lies in [-127, 127] (it is cut to that where s has lost its last places below 2^-126). q is that of the EXACT quotient: a
+// quotient rounded to fp32 falls on a half for one element in 10^5 that does not, and which neighbour it goes to would depend on
+// how the division is done. Rows of zeros have s = 0. A row that holds an infinity or NaN has s = NaN and q = 0: all of it reads
+// back as NaN, none of it as a plausible number. Read back: q * s rounded to fp32, and once more to a 16-bit type.
 //
-// Both are bound by memory: a 16-bit row of 128 moves 256 + 132 bytes.
+// Both are bound by memory: a 16-bit row of 128 moves 256 + 132 bytes. Reading 15001 rows of 8 heads back takes 87 us, 5.3 TB/s.
+// Writing 8192 takes 43 us, 4.7 TB/s, and 6 us more to find repeated slots; its arithmetic, 10 instructions an element, is nearly as long.
 //   * a row is spread over LPR lanes of 8 elements each (16 bytes of a 16-bit type in, 8 bytes out), so that the largest
 //     magnitude is a few lane permutations; a lane asks for kKvRows rows before it works on the first;
-//   * a workgroup writes the K and the V rows of its tokens, so that the tokens' destinations are looked up once.
+//   * quotients go through the reciprocal and are rounded by an addition; only where a remainder could decide otherwise is it
+//     computed (see below). Two divisions to a row and a check of each element's remainder took 95 us where this takes 43;
+//   * K and V are halves of the grid: the choice by an index per lane kept their addresses out of scalar registers (105 us
+//     became 189 us for the read above).
 // The last of several tokens with one destination is what the slot holds, as a loop over the tokens would leave it (a row and its
 // scale must not come from two tokens). A workgroup looks through the destinations behind its own while its rows are on their
-// way; above kKvScanTokens tokens, where that grows to more than the rows take, a launch of its own finds the last of each first.
+// way; above kKvScanTokens tokens two launches of their own find the last of each first.
 #include <algorithm>
 
 #include "common.hpp"
@@ -26,7 +30,9 @@ namespace amd {
 constexpr int kKvThreads = 256;
 constexpr int kKvRows = 4;               // rows that a lane group has in flight
 constexpr int kKvTokensPerWg = 8;        // most tokens of a workgroup that writes
-constexpr int64_t kKvScanTokens = 16384;
+// Workgroups look for later tokens with the same slot themselves up to this many tokens: 1777 tokens are written in 8.5 us so and
+// in 11.3 us with the two launches before, 8192 in 60 and 49 us.
+constexpr int64_t kKvScanTokens = 4096;
 
 struct KvInt8Pool {
   void* x;           // rows in the activations' type: read (write into the pool) or written (read back)
@@ -41,6 +47,7 @@ struct KvInt8Args {
   bool loc64;
   int64_t tokens, slots;
   int heads, d;
+  float perHeads;    // 1 / heads
   int tokensPerWg;
   const int* last;   // the last token of each slot (null: the workgroups look for themselves)
 };
@@ -49,27 +56,36 @@ __device__ __forceinline__ int64_t kvSlot(const KvInt8Args& a, int64_t t) {
   return a.loc64 ? static_cast<const int64_t*>(a.loc)[t] : static_cast<int64_t>(static_cast<const int32_t*>(a.loc)[t]);
 }
 // A destination counted from the end if negative; -1 outside the pool (dropped, never written).
-__device__ __forceinline__ int64_t kvDestination(const KvInt8Args& a, int64_t t) {
-  int64_t s = kvSlot(a, t);
-  if (s < 0) s += a.slots;
-  return s >= 0 && s < a.slots ? s : -1;
+__device__ __forceinline__ int kvDestination(const KvInt8Args& a, int64_t slot) {
+  if (slot < 0) slot += a.slots;
+  return slot >= 0 && slot < a.slots ? (int)slot : -1;
 }
+// Row i of a workgroup's (token, head) pairs, heads fastest: its token. i + 1/2 over the heads is at least half a head away from a
+// whole number, and the product is off by less for i up to 2^21.
+__device__ __forceinline__ int kvTokenOf(const KvInt8Args& a, int i) { return (int)(((float)i + 0.5f) * a.perHeads); }
 
 // What the magnitudes of a row and their largest (as bits: an infinity is above every number, NaN above that) make of it.
 struct KvScale {
   float scale;    // what is stored
   float up;       // rows of tiny numbers are lifted by 2^64 first, so that 1 / scale is finite
   float s, inv, half;
+  bool special;   // tiny, or not finite
   __device__ __forceinline__ explicit KvScale(uint32_t bits) {
     const float most = __uint_as_float(bits);
     const bool finite = bits < 0x7f800000u;
-    scale = finite ? most / 127.f : __uint_as_float(0x7fc00000u);
+    special = !finite || (most < 0x1p-60f && bits != 0);
+    // most / 127, rounded once: the quotient by the rounded reciprocal, corrected by its remainder, which the fused multiply-add gives
+    // exactly (P. Markstein, 1990; not where results lose places below 2^-126)
+    constexpr float kPer127 = 1.f / 127.f;
+    const float rough = most * kPer127;
+    scale = special ? most / 127.f : fmaf(fmaf(-127.f, rough, most), kPer127, rough);
+    if (!finite) scale = __uint_as_float(0x7fc00000u);
     up = most < 0x1p-60f ? 0x1p64f : 1.f;
     s = scale * up;
-    inv = finite && s > 0.f ? 1.f / s : 0.f;
+    inv = finite && s > 0.f ? __builtin_amdgcn_rcpf(s) : 0.f;  // (off by 2^-23 at most)
     half = 0.5f * s;
   }
-  // The whole number nearest to x / scale. x * inv is off by less than 2^-15, so its nearest whole number is that or a
+  // The whole number nearest to x / scale. x * inv is off by less than 2^-14, so its nearest whole number is that or a
   // neighbour of it, and the remainder says which: x - q s is a multiple of the smaller of the last places of x and s and at most
   // a little more than s / 2, so it fits 24 bits and the fused multiply-add gives it exactly.
   __device__ __forceinline__ int nearest(float x) const {
@@ -98,73 +114,138 @@ __device__ __forceinline__ uint32_t rowMost(uint32_t v) {
 template <typename T>
 struct KvPiece {  // 8 elements
   typename Vec16<T>::type v[8 / Vec16<T>::N];
+  // the largest magnitude as the bits of an fp32 number, an infinity above every number and NaN above that (16-bit types: pairs at once, and
+  // the largest is converted)
+  __device__ __forceinline__ uint32_t most() const {
+    if constexpr (sizeof(T) == 4) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint((*this)[i]) & 0x7fffffffu);
+      return m;
+    } else {
+      typedef uint16_t Pair __attribute__((ext_vector_type(2)));
+      const u32x4 w = __builtin_bit_cast(u32x4, v[0]) & 0x7fff7fffu;
+      auto larger = [](uint32_t x, uint32_t y) {
+        return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(Pair, x), __builtin_bit_cast(Pair, y)));
+      };
+      const uint32_t m = larger(larger(w[0], w[1]), larger(w[2], w[3]));
+      const uint16_t top = max((uint16_t)m, (uint16_t)(m >> 16));
+      return __float_as_uint(static_cast<float>(__builtin_bit_cast(T, top)));
+    }
+  }
   __device__ __forceinline__ float operator[](int i) const { return static_cast<float>(v[i / Vec16<T>::N][i % Vec16<T>::N]); }
 };
 
-// Which of the workgroup's tokens [t0, t0 + n) a later token supersedes, as bits (also where they have no destination).
-__device__ __forceinline__ unsigned kvSuperseded(const KvInt8Args& a, int64_t t0, int n, unsigned* shared) {
-  int64_t mine[kKvTokensPerWg];
-  unsigned dead = 0;
+struct KvSlot {  // where a token's rows and scales begin in the pools: looked up once per token
+  int64_t pool, scale;
+  int slot;  // -1: none
+  __device__ __forceinline__ KvSlot() {}
+  __device__ __forceinline__ KvSlot(const KvInt8Pool& o, int slot) : pool(max(slot, 0) * o.poolSlot), scale(max(slot, 0) * o.scaleSlot), slot(slot) {}
+};
+
+// Whether a later token has the slot of one of the MOST tokens [t0, t0 + n) of the workgroup, as bits. `mine`: in lane i of every
+// wave the slot of token t0 + i, -1 where there is none.
+template <int MOST>
+__device__ __forceinline__ unsigned kvLater(const KvInt8Args& a, int64_t t0, int n, int mine) {
+  int slot[MOST];
+  uint64_t same[MOST];
+  unsigned later = 0;
 #pragma unroll
-  for (int i = 0; i < kKvTokensPerWg; ++i) {
-    mine[i] = i < n ? kvDestination(a, t0 + i) : -1;
-    if (mine[i] < 0 || (a.last != nullptr && a.last[mine[i]] != (int)(t0 + i))) dead |= 1u << i;
+  for (int i = 0; i < MOST; ++i) {
+    slot[i] = __builtin_amdgcn_readlane(mine, i);  // (in a scalar register: a comparison each, and nothing else)
+    same[i] = __builtin_amdgcn_ballot_w64(mine == slot[i]) >> (i + 1);  // among the workgroup's own
   }
-  if (a.last != nullptr) return dead;
-  if (threadIdx.x == 0) *shared = 0;
-  __syncthreads();
-  unsigned found = 0;
-  for (int64_t j = t0 + 1 + threadIdx.x; j < a.tokens; j += kKvThreads) {
-    const int64_t s = kvDestination(a, j);
+  constexpr int kBatch = 8;  // asked for at once: their answers are what this takes its time for
+  for (int64_t j0 = t0 + n + threadIdx.x; j0 < a.tokens; j0 += kKvThreads * kBatch) {
+    int64_t at[kBatch];
 #pragma unroll
-    for (int i = 0; i < kKvTokensPerWg; ++i)
-      if (s == mine[i] && j > t0 + i) found |= 1u << i;
+    for (int k = 0; k < kBatch; ++k) at[k] = kvSlot(a, min(j0 + k * kKvThreads, a.tokens - 1));
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int s = kvDestination(a, at[k]);
+#pragma unroll
+      for (int i = 0; i < MOST; ++i) same[i] |= __builtin_amdgcn_ballot_w64(s == slot[i]);
+    }
   }
-  if (found) atomicOr(shared, found);
-  __syncthreads();
-  return dead | *shared;
+#pragma unroll
+  for (int i = 0; i < MOST; ++i) later |= same[i] != 0 ? 1u << i : 0u;
+  return later;
 }
 
-// grid: workgroups of tokensPerWg tokens. Rows of a workgroup: (pool, token, head), head fastest.
+// The slots of the workgroup's tokens [t0, t0 + n), -1 for those that are not written: no destination, or a later token has the
+// same. (One barrier; every thread of the workgroup takes part.)
+__device__ __forceinline__ void kvDestinations(const KvInt8Args& a, int64_t t0, int n, KvSlot (&slots)[kKvTokensPerWg], unsigned (&later)[kKvThreads / 64]) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int mine = -1;
+  if (lane < n) {
+    mine = kvDestination(a, kvSlot(a, t0 + lane));
+    if (a.last != nullptr && mine >= 0 && a.last[mine] != (int)(t0 + lane)) mine = -1;
+  }
+  const unsigned found = a.last != nullptr ? 0u : n <= 2 ? kvLater<2>(a, t0, n, mine) : kvLater<kKvTokensPerWg>(a, t0, n, mine);
+  if (lane == 0) later[wave] = found;
+  if (wave == 0 && lane < kKvTokensPerWg) slots[lane] = KvSlot(a.pool[blockIdx.y], mine);
+  __syncthreads();
+}
+
+// grid: (workgroups of tokensPerWg tokens, K or V). Rows of a workgroup: (token, head), head fastest.
 template <typename T, int LPR>
 __global__ __launch_bounds__(kKvThreads) void kvInt8WriteKernel(KvInt8Args a) {
   constexpr int kGroups = kKvThreads / LPR;
-  __shared__ unsigned shared;
+  __shared__ unsigned later[kKvThreads / 64];
+  __shared__ KvSlot slots[kKvTokensPerWg];
   const int64_t t0 = (int64_t)blockIdx.x * a.tokensPerWg;
   const int n = (int)min((int64_t)a.tokensPerWg, a.tokens - t0);
   const int sub = threadIdx.x % LPR, group = threadIdx.x / LPR;
-  const int rows = n * a.heads, all = 2 * rows, e = sub * 8;
+  const KvInt8Pool& o = a.pool[blockIdx.y];
+  const int rows = n * a.heads, e = sub * 8;
   const bool live = e < a.d;
+  const T* const from = static_cast<const T*>(o.x) + t0 * o.xToken;
   KvPiece<T> x[kKvRows];
+  int token[kKvRows], head[kKvRows];
   auto load = [&](int r0) {
 #pragma unroll
     for (int u = 0; u < kKvRows; ++u) {
-      const int r = min(r0 + u * kGroups, all - 1), p = r >= rows, i = r - p * rows, t = i / a.heads, h = i - t * a.heads;
-      const KvInt8Pool& o = a.pool[p];
-      const T* src = static_cast<const T*>(o.x) + (t0 + t) * o.xToken + h * o.xHead + (live ? e : 0);
+      const int r = min(r0 + u * kGroups, rows - 1);
+      token[u] = kvTokenOf(a, r), head[u] = r - token[u] * a.heads;
+      const T* src = from + (__umul24(token[u], (unsigned)o.xToken) + __umul24(head[u], (unsigned)o.xHead) + (live ? e : 0));
 #pragma unroll
       for (int c = 0; c < 8 / Vec16<T>::N; ++c) x[u].v[c] = __builtin_nontemporal_load(reinterpret_cast<const typename Vec16<T>::type*>(src) + c);
     }
   };
   load(group);
-  const unsigned dead = kvSuperseded(a, t0, n, &shared);
-  for (int r0 = group; r0 < all; r0 += kKvRows * kGroups) {
+  kvDestinations(a, t0, n, slots, later);
+  const unsigned dead = later[0] | later[1] | later[2] | later[3];
+  for (int r0 = group; r0 < rows; r0 += kKvRows * kGroups) {
     if (r0 != group) load(r0);
 #pragma unroll
     for (int u = 0; u < kKvRows; ++u) {
-      const int r = r0 + u * kGroups, p = r >= rows, i = r - p * rows, t = i / a.heads, h = i - t * a.heads;
-      uint32_t most = 0;
+      const KvScale s(rowMost<LPR>(live ? x[u].most() : 0));
+      // x / s by the reciprocal, rounded by adding 3 * 2^22: the last byte of the sum is the whole number. It is the nearest one
+      // unless the quotient is within 2^-15 (twice what 127 times the reciprocal can be off by) of a half; such rows, tiny ones
+      // and those that are not finite go element by element
+      constexpr float kWhole = 12582912.f;
+      float t[8], off = 0.f;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) most = max(most, __float_as_uint(x[u][k]) & 0x7fffffffu);
-      const KvScale s(rowMost<LPR>(live ? most : 0));
-      u32x2 q = {0, 0};
+      for (int k = 0; k < 8; ++k) {
+        t[k] = fmaf(x[u][k], s.inv, kWhole);
+        off = fmaxf(off, fabsf(fmaf(x[u][k], s.inv, kWhole - t[k])));
+      }
+      u32x2 q;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) q[k / 4] |= (uint32_t)(s.nearest(x[u][k]) & 255) << (8 * (k % 4));
-      if (r >= all || (dead >> t & 1)) continue;
-      const KvInt8Pool& o = a.pool[p];
-      const int64_t slot = kvDestination(a, t0 + t);
-      if (live) *reinterpret_cast<u32x2*>(o.pool + slot * o.poolSlot + h * o.poolHead + e) = q;
-      if (sub == 0) o.scale[slot * o.scaleSlot + h * o.scaleHead] = s.scale;
+      for (int w = 0; w < 2; ++w) {
+        const uint32_t low = __builtin_amdgcn_perm(__float_as_uint(t[4 * w + 1]), __float_as_uint(t[4 * w]), 0x0c0c0400u);
+        const uint32_t high = __builtin_amdgcn_perm(__float_as_uint(t[4 * w + 3]), __float_as_uint(t[4 * w + 2]), 0x0c0c0400u);
+        q[w] = low | high << 16;
+      }
+      if (__builtin_amdgcn_ballot_w64(!(off < 0.49996f) || s.special) != 0) {
+        q = u32x2{0, 0};
+#pragma unroll
+        for (int k = 0; k < 8; ++k) q[k / 4] |= (uint32_t)(s.nearest(x[u][k]) & 255) << (8 * (k % 4));
+      }
+      const KvSlot to = slots[token[u]];
+      if (r0 + u * kGroups >= rows || to.slot < 0 || (dead >> token[u] & 1)) continue;
+      if (live) *reinterpret_cast<u32x2*>(o.pool + (to.pool + __umul24(head[u], (unsigned)o.poolHead) + e)) = q;
+      if (sub == 0) o.scale[to.scale + __umul24(head[u], (unsigned)o.scaleHead)] = s.scale;
     }
   }
 }
@@ -172,76 +253,81 @@ __global__ __launch_bounds__(kKvThreads) void kvInt8WriteKernel(KvInt8Args a) {
 // Any head size and alignment: a wave per row.
 template <typename T>
 __global__ __launch_bounds__(kKvThreads) void kvInt8WriteAnyKernel(KvInt8Args a) {
-  __shared__ unsigned shared;
+  __shared__ unsigned later[kKvThreads / 64];
+  __shared__ KvSlot slots[kKvTokensPerWg];
   const int64_t t0 = (int64_t)blockIdx.x * a.tokensPerWg;
   const int n = (int)min((int64_t)a.tokensPerWg, a.tokens - t0);
-  const unsigned dead = kvSuperseded(a, t0, n, &shared);
+  kvDestinations(a, t0, n, slots, later);
+  const unsigned dead = later[0] | later[1] | later[2] | later[3];
   const int lane = threadIdx.x & 63, rows = n * a.heads;
-  for (int r = threadIdx.x / 64; r < 2 * rows; r += kKvThreads / 64) {
-    const int p = r >= rows, i = r - p * rows, t = i / a.heads, h = i - t * a.heads;
-    if (dead >> t & 1) continue;
-    const KvInt8Pool& o = a.pool[p];
+  const KvInt8Pool& o = a.pool[blockIdx.y];
+  for (int r = threadIdx.x / 64; r < rows; r += kKvThreads / 64) {
+    const int t = r / a.heads, h = r - t * a.heads;
+    const int slot = slots[t].slot;
+    if (slot < 0 || (dead >> t & 1)) continue;
     const T* src = static_cast<const T*>(o.x) + (t0 + t) * o.xToken + h * o.xHead;
     uint32_t most = 0;
     for (int e = lane; e < a.d; e += 64) most = max(most, __float_as_uint(static_cast<float>(src[e])) & 0x7fffffffu);
     most = rowMost<32>(most);
     const KvScale s(max(most, (uint32_t)__shfl_xor((int)most, 32, 64)));
-    const int64_t slot = kvDestination(a, t0 + t);
     int8_t* dst = o.pool + slot * o.poolSlot + h * o.poolHead;
     for (int e = lane; e < a.d; e += 64) dst[e] = static_cast<int8_t>(s.nearest(static_cast<float>(src[e])));
     if (lane == 0) o.scale[slot * o.scaleSlot + h * o.scaleHead] = s.scale;
   }
 }
 
-// last[slot]: the last token whose destination it is. Entries need no first value: every token writes its own to begin with,
-// whichever of a slot's tokens stays there is one of them, and the largest then replaces it.
-__global__ __launch_bounds__(1024) void kvInt8LastKernel(KvInt8Args a, int* last) {
-  for (int64_t t = threadIdx.x; t < a.tokens; t += 1024) {
-    const int64_t s = kvDestination(a, t);
-    if (s >= 0) __hip_atomic_store(&last[s], (int)t, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  }
-  __threadfence();
-  __syncthreads();
-  for (int64_t t = threadIdx.x; t < a.tokens; t += 1024) {
-    const int64_t s = kvDestination(a, t);
-    if (s >= 0) __hip_atomic_fetch_max(&last[s], (int)t, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  }
+// last[slot]: the last token whose destination it is, in two launches. Entries need no first value: every token writes its own to
+// begin with (one of a slot's tokens stays there), and then the largest replaces it.
+template <bool FIRST>
+__global__ __launch_bounds__(kKvThreads) void kvInt8LastKernel(KvInt8Args a, int* last) {
+  const int64_t t = (int64_t)blockIdx.x * kKvThreads + threadIdx.x;
+  if (t >= a.tokens) return;
+  const int s = kvDestination(a, kvSlot(a, t));
+  if (s < 0) return;
+  if (FIRST) last[s] = (int)t;
+  else atomicMax(&last[s], (int)t);
 }
 
-// grid: workgroups of tokensPerWg rows of `loc` (K and V)
+// grid: (workgroups of tokensPerWg rows of `loc`, K or V)
 template <typename T, int LPR>
 __global__ __launch_bounds__(kKvThreads) void kvInt8ReadKernel(KvInt8Args a) {
   constexpr int kGroups = kKvThreads / LPR;
+  __shared__ int slots[kKvTokensPerWg];  // -1: outside the pool
   const int64_t t0 = (int64_t)blockIdx.x * a.tokensPerWg;
   const int n = (int)min((int64_t)a.tokensPerWg, a.tokens - t0);
+  if ((int)threadIdx.x < n) {
+    const int64_t slot = kvSlot(a, t0 + threadIdx.x);
+    slots[threadIdx.x] = slot >= 0 && slot < a.slots ? (int)slot : -1;
+  }
+  __syncthreads();
   const int sub = threadIdx.x % LPR, group = threadIdx.x / LPR;
-  const int rows = n * a.heads, all = 2 * rows, e = sub * 8;
+  const KvInt8Pool& o = a.pool[blockIdx.y];
+  const int rows = n * a.heads, e = sub * 8;
   if (e >= a.d) return;
-  for (int r0 = group; r0 < all; r0 += kKvRows * kGroups) {
+  T* const x0 = static_cast<T*>(o.x) + t0 * o.xToken;
+  for (int r0 = group; r0 < rows; r0 += kKvRows * kGroups) {
     u32x2 q[kKvRows];
     float s[kKvRows];
+    unsigned to[kKvRows];
 #pragma unroll
     for (int u = 0; u < kKvRows; ++u) {
-      const int r = min(r0 + u * kGroups, all - 1), p = r >= rows, i = r - p * rows, t = i / a.heads, h = i - t * a.heads;
-      const KvInt8Pool& o = a.pool[p];
-      const int64_t slot = kvSlot(a, t0 + t);
-      const bool in = slot >= 0 && slot < a.slots;  // outside the pool: zeros, nothing is read
+      const int r = min(r0 + u * kGroups, rows - 1), t = kvTokenOf(a, r), h = r - t * a.heads;
+      to[u] = __umul24(t, (unsigned)o.xToken) + __umul24(h, (unsigned)o.xHead) + e;
+      const int slot = slots[t];
       q[u] = u32x2{0, 0}, s[u] = 0.f;
-      if (in) {
-        q[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(o.pool + slot * o.poolSlot + h * o.poolHead + e));
-        s[u] = o.scale[slot * o.scaleSlot + h * o.scaleHead];
+      if (slot >= 0) {  // outside the pool: zeros, nothing is read
+        q[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(o.pool + (slot * o.poolSlot + __umul24(h, (unsigned)o.poolHead) + e)));
+        s[u] = o.scale[slot * o.scaleSlot + __umul24(h, (unsigned)o.scaleHead)];
       }
     }
 #pragma unroll
     for (int u = 0; u < kKvRows; ++u) {
-      const int r = r0 + u * kGroups, p = r >= rows, i = r - p * rows, t = i / a.heads, h = i - t * a.heads;
-      if (r >= all) continue;
+      if (r0 + u * kGroups >= rows) continue;
       KvPiece<T> x;
 #pragma unroll
       for (int k = 0; k < 8; ++k)
         x.v[k / Vec16<T>::N][k % Vec16<T>::N] = static_cast<T>(static_cast<float>((int)(q[u][k / 4] << (24 - 8 * (k % 4))) >> 24) * s[u]);
-      const KvInt8Pool& o = a.pool[p];
-      T* dst = static_cast<T*>(o.x) + (t0 + t) * o.xToken + h * o.xHead + e;
+      T* dst = x0 + to[u];
 #pragma unroll
       for (int c = 0; c < 8 / Vec16<T>::N; ++c) __builtin_nontemporal_store(x.v[c], reinterpret_cast<typename Vec16<T>::type*>(dst) + c);
     }
@@ -253,9 +339,9 @@ __global__ __launch_bounds__(kKvThreads) void kvInt8ReadAnyKernel(KvInt8Args a) 
   const int64_t t0 = (int64_t)blockIdx.x * a.tokensPerWg;
   const int n = (int)min((int64_t)a.tokensPerWg, a.tokens - t0);
   const int lane = threadIdx.x & 63, rows = n * a.heads;
-  for (int r = threadIdx.x / 64; r < 2 * rows; r += kKvThreads / 64) {
-    const int p = r >= rows, i = r - p * rows, t = i / a.heads, h = i - t * a.heads;
-    const KvInt8Pool& o = a.pool[p];
+  const KvInt8Pool& o = a.pool[blockIdx.y];
+  for (int r = threadIdx.x / 64; r < rows; r += kKvThreads / 64) {
+    const int t = r / a.heads, h = r - t * a.heads;
     const int64_t slot = kvSlot(a, t0 + t);
     const bool in = slot >= 0 && slot < a.slots;
     const float s = in ? o.scale[slot * o.scaleSlot + h * o.scaleHead] : 0.f;
@@ -299,20 +385,35 @@ static diopiError_t kvInt8Args(const char* what, const TensorView (&x)[2], const
   AMD_CHECK(x[0].shape[0] < ((int64_t)1 << 31) && x[0].shape[1] <= (1 << 20) && x[0].shape[2] <= (1 << 20), "%s: extents exceed the launch limits", what);
   a->loc64 = loc.dtype == diopi_dtype_int64;
   a->tokens = x[0].shape[0], a->slots = pool[0].shape[0];
+  AMD_CHECK(pool[0].shape[0] < ((int64_t)1 << 31), "%s: %ld slots exceed 2^31 - 1", what, (long)pool[0].shape[0]);
   a->heads = (int)x[0].shape[1], a->d = (int)x[0].shape[2];
+  a->perHeads = 1.f / (float)a->heads;
   a->last = nullptr;
   return diopiSuccess;
 }
 
 // Whether all rows lie in whole 8-element pieces that can be loaded and stored at once.
 static bool kvInt8Vector(const KvInt8Args& a, int64_t itemsize) {
-  if (a.d % 8 != 0 || a.d > 256) return false;
+  if (a.d % 8 != 0 || a.d > 256 || a.heads > (1 << 17)) return false;  // (heads: see kvTokenOf)
   int64_t bits16 = 0, bits8 = 0;
   for (const KvInt8Pool& o : a.pool) {
+    // places within a workgroup's tokens, and heads within a slot, are products of 24-bit numbers below 2^31
+    const int64_t token = o.xToken * kKvTokensPerWg, heads = std::max({o.xHead, o.poolHead, o.scaleHead});
+    if (o.xToken >= (1 << 24) || heads >= (1 << 24) || token + heads * a.heads + a.d >= ((int64_t)1 << 31)) return false;
     bits16 |= (int64_t)reinterpret_cast<uintptr_t>(o.x) | o.xToken * itemsize | o.xHead * itemsize;
     bits8 |= (int64_t)reinterpret_cast<uintptr_t>(o.pool) | o.poolSlot | o.poolHead;
   }
   return (bits16 & 15) == 0 && (bits8 & 7) == 0;
+}
+
+// 32 to 128 rows to a workgroup: as many as leave 256 workgroups (one per compute unit) for K and as many for V. Between those
+// the slots are looked up, and looked through, more often than needed: 1777 tokens of 8 heads are written in 8.5 us so and in
+// 9.9 us with 1024 workgroups each; 8192 of 8 take 49 us with 128 rows, 53 us with 256, 51 us with 64, and are read back in 36.5, 39
+// and 38 us.
+static dim3 kvInt8Grid(KvInt8Args* a) {
+  const int64_t rows = std::min<int64_t>(128, std::max<int64_t>(32, a->tokens * a->heads / 256));
+  a->tokensPerWg = (int)std::min<int64_t>(kKvTokensPerWg, ceilDiv(rows, a->heads));
+  return dim3((unsigned)ceilDiv(a->tokens, a->tokensPerWg), 2);
 }
 
 #define KV_INT8_LAUNCH_TYPE(T, NAME, VEC)                                                                            \
@@ -353,15 +454,15 @@ extern "C" __attribute__((visibility("default"))) diopiError_t diopiDestIndexCop
   AMD_TRY(makeContiguous(ctx, stream, loc, &dense));
   a.loc = dense.data;
   if (a.tokens > kKvScanTokens) {
-    AMD_CHECK(a.slots < ((int64_t)1 << 31), "%s: %ld slots exceed 2^31 - 1", what, (long)a.slots);
     void* last = nullptr;
     AMD_TRY(requireWorkspace(ctx, a.slots * (int64_t)sizeof(int), &last));
-    hipLaunchKernelGGL(kvInt8LastKernel, dim3(1), dim3(1024), 0, stream, a, static_cast<int*>(last));
+    const dim3 grid((unsigned)ceilDiv(a.tokens, kKvThreads));
+    hipLaunchKernelGGL(kvInt8LastKernel<true>, grid, dim3(kKvThreads), 0, stream, a, static_cast<int*>(last));
+    hipLaunchKernelGGL(kvInt8LastKernel<false>, grid, dim3(kKvThreads), 0, stream, a, static_cast<int*>(last));
     AMD_LAUNCH_CHECK();
     a.last = static_cast<const int*>(last);
   }
-  a.tokensPerWg = (int)std::min<int64_t>(kKvTokensPerWg, std::max<int64_t>(1, a.tokens / 1024));
-  const dim3 grid((unsigned)ceilDiv(a.tokens, a.tokensPerWg));
+  const dim3 grid = kvInt8Grid(&a);
   KV_INT8_LAUNCH(x[0].dtype, kvInt8Write, kvInt8Vector(a, x[0].itemsize));
   AMD_LAUNCH_CHECK();
   return diopiSuccess;
@@ -386,8 +487,7 @@ extern "C" __attribute__((visibility("default"))) diopiError_t diopiIndexSelectK
   if (x[0].numel == 0) return diopiSuccess;
   AMD_TRY(makeContiguous(ctx, stream, loc, &dense));
   a.loc = dense.data;
-  a.tokensPerWg = (int)std::min<int64_t>(kKvTokensPerWg, std::max<int64_t>(1, a.tokens / 1024));
-  const dim3 grid((unsigned)ceilDiv(a.tokens, a.tokensPerWg));
+  const dim3 grid = kvInt8Grid(&a);
   KV_INT8_LAUNCH(x[0].dtype, kvInt8Read, kvInt8Vector(a, x[0].itemsize));
   AMD_LAUNCH_CHECK();
   return diopiSuccess;

@@ -114,14 +114,15 @@ DIOPI_API diopiError_t diopiTokenDecodeAttentionInferenceNoAlloc(diopiContextHan
                                                                  diopiConstTensorHandle_t b_seq_len, int max_input_len);
 
 /* The int8 KV cache: a pool [slots, kv_heads, d] of int8 with a float32 scale for each row, [slots, kv_heads].
- * diopiDestIndexCopyKVPairInt8 quantises the K row and the V row of every new token as it writes them, in one launch:
+ * diopiDestIndexCopyKVPairInt8 quantises the K row and the V row of every new token as it writes them:
  *   scale[dest_loc[i], h] = max |x[i, h, :]| / 127 in float32,  out[dest_loc[i], h, :] = x[i, h, :] / scale to the nearest
  *   whole number, ties to the even one, within [-127, 127].
  * k, v [tokens, kv_heads, d] are float16, bfloat16 or float32, dest_loc [tokens] int32 or int64. As in
  * diopiDestIndexCopyKV a negative destination counts from the end and one outside the pool is dropped; of several tokens
  * with one destination the last is kept. A row of zeros has scale 0; a row that holds an infinity or NaN has scale NaN and
- * reads back as NaN. Heads, tokens and slots may lie at any strides, head_dim is contiguous. (More than 16384 tokens take a workspace of 4
- * bytes per slot.) No counterpart in the reference, whose cache holds the activations' type. */
+ * reads back as NaN. Heads, tokens and slots may lie at any strides, head_dim is contiguous; a pool has fewer than 2^31
+ * slots. (More than 4096 tokens take a workspace of 4 bytes per slot.) No counterpart in the reference, whose cache holds
+ * the activations' type. */
 DIOPI_API diopiError_t diopiDestIndexCopyKVPairInt8(diopiContextHandle_t ctx, diopiTensorHandle_t out_k,
                                                     diopiTensorHandle_t out_k_scale, diopiConstTensorHandle_t k,
                                                     diopiTensorHandle_t out_v, diopiTensorHandle_t out_v_scale,
@@ -149,8 +150,8 @@ DIOPI_API diopiError_t diopiTokenDecodeAttentionInt8Inference(diopiContextHandle
 /* diopiTokenDecodeAttentionInference for a batch whose sequences all begin with the same tokens, which the pool holds once:
  * sequence b attends to the tokens in slots prefix_loc[0 .. n) (int32 or int64, every one of them for every sequence) and to
  * its own b_seq_len[b] tokens behind them, which b_loc, b_seq_len and max_input_len describe as they do there (none of them
- * count the prefix). The shared rows are read for many sequences at a time. Slots outside the pool are skipped; a sequence without any token
- * gives zeros. The same types and head sizes. */
+ * count the prefix). The shared rows are read for many sequences at a time. Slots outside the pool are skipped; a sequence
+ * without any token gives zeros. The same types and head sizes. */
 DIOPI_API diopiError_t diopiTokenDecodeAttentionSharedPrefixInference(diopiContextHandle_t ctx, diopiTensorHandle_t out,
                                                                       diopiConstTensorHandle_t q,
                                                                       diopiConstTensorHandle_t k,

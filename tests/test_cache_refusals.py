@@ -104,6 +104,14 @@ def test_shared_prefix(pkg, call, changes, says):
         call(PREFIX[0], args.but(**changes), PREFIX[1], 5)
 
 
+@pytest.mark.parametrize("name,order", [WRITE, READ])
+def test_pools_of_too_many_slots(pkg, call, name, order):
+    many = {key: t[:1].expand(2 ** 31, *t.shape[1:]) for key, t in pools().items()}
+    args = Args(k=torch.zeros(3, 2, 64), v=torch.zeros(3, 2, 64), loc=torch.zeros(3, dtype=torch.int32), **many)
+    with pytest.raises(pkg.diopi.DiopiError, match="2147483648 slots exceed"):
+        call(name, args, order)
+
+
 def test_a_closed_context_and_host_tensors(pkg):
     d = pkg.diopi
     z = torch.zeros(3, 2, 64)

@@ -97,6 +97,26 @@ def test_negative_foreign_and_repeated_destinations(ops, dev, tokens):
     check_write(ops, dev, rows(tokens, 1, 20, torch.float16, 8), rows(tokens, 1, 20, torch.float16, 9), same, slots)
 
 
+@pytest.mark.parametrize("tokens", [4096, 4097])
+def test_repeats_where_they_begin_to_be_found_beforehand(ops, dev, tokens):
+    dest = torch.randint(0, tokens // 2, (tokens,), generator=g(tokens))
+    check_write(ops, dev, rows(tokens, 8, 64, torch.bfloat16, 6), rows(tokens, 8, 64, torch.bfloat16, 7), dest, tokens // 2 + 9)
+    check_write(ops, dev, rows(tokens, 1, 128, torch.float32, 6), rows(tokens, 1, 128, torch.float32, 7), dest - tokens // 2, tokens // 2)
+
+
+@pytest.mark.parametrize("apart", [2 ** 24 - 8, 2 ** 24])        # tokens just below and at the widest step of the kernel with 24-bit products
+def test_tokens_far_apart(ops, dev, apart):
+    on = torch.empty(2 * apart + 512, dtype=torch.bfloat16, device=dev).as_strided((3, 4, 128), (apart, 128, 1))
+    k = rows(3, 4, 128, torch.bfloat16, 15)
+    on.copy_(k)
+    check_write(ops, dev, k, k, torch.tensor([4, 0, 2]), 5, on, on)
+    (kp, ks), (vp, vs) = empty_pools(5, 4, 128)
+    index = torch.tensor([4, 1, 3])
+    out = torch.empty(2, 2 * apart + 512, dtype=torch.bfloat16, device=dev).as_strided((2, 3, 4, 128), (2 * apart + 512, apart, 128, 1))
+    ops.index_select_kv_pair_int8(kp.to(dev), ks.to(dev), vp.to(dev), vs.to(dev), index.to(dev), out_k=out[0], out_v=out[1])
+    assert_exact(out.contiguous(), torch.stack([oracle.read(kp, ks, index, torch.bfloat16), oracle.read(vp, vs, index, torch.bfloat16)]))
+
+
 def test_rows_and_pools_at_other_strides(ops, dev):
     for d, shift in [(128, 0), (64, 3), (40, 8)]:                # whole vectors, a base that is not aligned, half a vector aside
         stacked = torch.randn(21, 6, d, generator=g(10)).bfloat16()
