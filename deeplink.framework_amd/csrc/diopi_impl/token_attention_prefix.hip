@@ -18,6 +18,7 @@ struct TaPrefixArgs {
   bool loc64;
   int len;
   int chunk, nsplit;          // of the shared tokens
+  int groups;                 // of columns, decodePrefixTiledKernel
   unsigned kStride, vStride;  // slot strides of the pools in bytes, as decodePrefixKernel takes them
 };
 
@@ -80,11 +81,11 @@ __global__ __launch_bounds__(256) void decodePrefixAnyKernel(TaPrefixArgs x, T* 
 
 // ------------------------------------------------ head rows of whole 16-byte pieces up to 512 bytes: the matrix pipe --
 // The shared tokens see the same K and V from every sequence, so a K/V head's columns are the query heads that share it of ALL
-// sequences: S^T = K . Q^T and O^T += V^T . P^T with up to 64 columns for one read of a row. Partial results (maximum, sum, weighted
+// sequences: S^T = K . Q^T and O^T += V^T . P^T with many columns for one read of a row. Partial results (maximum, sum, weighted
 // sum of V) of each chunk of the prefix go to workspace; those of the sequences' own tokens come from the kernels of
-// diopiTokenDecodeAttentionInference, and a last launch merges both. Few columns: bound by memory, every shared row once; many
-// (192 columns, 16 001 tokens): by the matrix pipe, 24 products of 16 cycles for 32 tokens and 16 columns (fp16 32), and the softmax
-// between them.
+// diopiTokenDecodeAttentionInference, and a last launch merges both.
+// With up to 32 columns, or fp32: bound by memory, every shared row read once (fp32 with more columns: once for every 32 of them),
+// and for short prefixes by the three launches and the latency of slots, then rows.
 //   * rows go from the pool into the registers that the products read, whole 128-byte lines of 8 rows in a load: K as in
 //     token_attention_int8.hip (a piece of 16 bytes is an operand, two lanes swap one); of V a lane takes 16 bytes of each of its
 //     eight tokens, which are eight places of the head, and v_perm puts pairs of tokens side by side, so V is turned round in registers.
@@ -574,24 +575,28 @@ __global__ __launch_bounds__(kPtWaves * 64, 2) void decodePrefixTiledKernel(TaPr
   __shared__ float stateBuf[S::HALVES == 2 ? COLUMN_WAVES : 1][NC][2][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, quad = lane >> 4;
-  const int columnWave = wave % COLUMN_WAVES, half = wave / COLUMN_WAVES;
+  // (the second half's waves in the opposite order: waves i and i + 4 share a SIMD, and one of them may have a tile less)
+  const int half = wave / COLUMN_WAVES, columnWave = half == 0 ? wave % COLUMN_WAVES : COLUMN_WAVES - 1 - wave % COLUMN_WAVES;
 
-  // grid as in decodePrefixKernel
+  // grid as in decodePrefixKernel; tiles of columns are dealt out evenly, to the groups and to the waves of one: NC to a wave, or one
+  // less (16 001 tokens, 192 columns: 36 us with two groups of 6 tiles, 40 us with full groups, one of 8 and one of 4)
   const int f = blockIdx.x, idx = f >> 3;
-  const int perKv = a.heads / a.kvHeads, columns = a.batch * perKv, groups = (columns + 16 * COLUMN_WAVES * NC - 1) / (16 * COLUMN_WAVES * NC);
+  const int perKv = a.heads / a.kvHeads, columns = a.batch * perKv, tiles = (columns + 15) / 16, groups = x.groups;
   const int group = idx % groups, u = (idx / groups) * 8 + (f & 7);
   if (u >= a.kvHeads * x.nsplit) return;  // the grid is rounded up to whole rounds of the XCDs
   const int kvh = u % a.kvHeads, split = u / a.kvHeads;
   const int begin = split * x.chunk, end = min(x.len, begin + x.chunk);
-  const int firstColumn = (group * COLUMN_WAVES + columnWave) * NC * 16;
-  const bool active = firstColumn < columns;  // (a wave without columns only copies)
+  const int groupTile = group * tiles / groups, groupTiles = (group + 1) * tiles / groups - groupTile;
+  const int firstTile = columnWave * groupTiles / COLUMN_WAVES, mine = (columnWave + 1) * groupTiles / COLUMN_WAVES - firstTile;
+  const int firstColumn = (groupTile + firstTile) * 16;
+  const bool active = NC > 1 || mine > 0;  // (a wave without columns only copies)
 
   Frag qf[NC][KS];
   int pairOf[NC];  // row of the partial results of this lane's column, or -1
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
     const int column = firstColumn + c * 16 + col;
-    const bool have = column < columns;
+    const bool have = c < mine && column < columns;
     const int b = have ? column / perKv : 0, h = kvh * perKv + (have ? column % perKv : 0);
     pairOf[c] = have ? b * a.heads + h : -1;
     const T* src = reinterpret_cast<const T*>(a.q) + b * a.qBatchStride + h * a.qHeadStride;
@@ -653,11 +658,12 @@ __global__ __launch_bounds__(kPtWaves * 64, 2) void decodePrefixTiledKernel(TaPr
         kf[t][s] = *(LdsPiece)(uintptr_t)(at + (unsigned)(row * ROWB + (((4 * s + quad) ^ S::swizzleK(row)) << 4)));
       }
   };
-  auto scoresOf = [&](const u32x4 (&kf)[2][KS], f32x4 (&s4)[NC][2], auto withCare) {
+  auto scoresOf = [&](const u32x4 (&kf)[2][KS], f32x4 (&s4)[NC][2], auto columnTiles, auto withCare) {
+    constexpr int N = decltype(columnTiles)::value;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
 #pragma unroll
-      for (int c = 0; c < NC; ++c) s4[c][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int c = 0; c < N; ++c) s4[c][t] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
 #pragma unroll
     for (int s = 0; s < KS; ++s)
@@ -666,7 +672,7 @@ __global__ __launch_bounds__(kPtWaves * 64, 2) void decodePrefixTiledKernel(TaPr
         u32x4 k = kf[t][s];
         if (decltype(withCare)::value && 32 * s + 8 * quad >= a.d) k = u32x4{0, 0, 0, 0};  // (an infinity against q's zeros would be NaN)
 #pragma unroll
-        for (int c = 0; c < NC; ++c) s4[c][t] = M::run(k, qf[c][s], s4[c][t]);
+        for (int c = 0; c < N; ++c) s4[c][t] = M::run(k, qf[c][s], s4[c][t]);
       }
   };
   struct Counts {  // which of the lane's eight tokens count
@@ -747,16 +753,17 @@ __global__ __launch_bounds__(kPtWaves * 64, 2) void decodePrefixTiledKernel(TaPr
   };
   // What two parts leave of probabilities below 2^-24 of the largest, times 2^24, 2^48 ... (the scores once more: keeping them for
   // this would cost the registers of a column tile).
-  auto addRest = [&](int stage, int at, bool all, auto withCare) {
+  auto addRest = [&](int stage, int at, bool all, auto columnTiles, auto withCare) {
     constexpr bool CAREFUL = decltype(withCare)::value;
+    constexpr int N = decltype(columnTiles)::value;
     const Counts n = countsOf(at, all);
     const u32x4 keep = keepOf(n);
     u32x4 kf[2][KS];
     readK(kf, stage);
     f32x4 s4[NC][2];
-    scoresOf(kf, s4, withCare);
+    scoresOf(kf, s4, columnTiles, withCare);
 #pragma unroll
-    for (int c = 0; c < NC; ++c) {
+    for (int c = 0; c < N; ++c) {
       float w[8];
       powersOf(c, s4[c], n, all, w, false, 0.f);
 #pragma unroll
@@ -795,8 +802,9 @@ __global__ __launch_bounds__(kPtWaves * 64, 2) void decodePrefixTiledKernel(TaPr
     }
   };
   // the stages of a block, after its slots have been published; clean: all of its slots lie in the pool
-  auto walk = [&](int n, bool clean, auto withCare) {
+  auto walk = [&](int n, bool clean, auto columnTiles, auto withCare) {
     constexpr bool CAREFUL = decltype(withCare)::value;
+    constexpr int N = decltype(columnTiles)::value;
     const int stages = (n + TOKENS - 1) / TOKENS;
     // this wave's copies of a stage have landed (loads end in order; `behind` stages are on their way) and then everybody's have
     auto landed = [&](bool behind) {
@@ -826,14 +834,14 @@ __global__ __launch_bounds__(kPtWaves * 64, 2) void decodePrefixTiledKernel(TaPr
       if (active) {
         f32x4 s4[NC][2];
         if (!kAheadK) readK(kf, stage);
-        scoresOf(kf, s4, withCare);
+        scoresOf(kf, s4, columnTiles, withCare);
         const Counts counts = countsOf(s * TOKENS, all);
         if constexpr (CAREFUL) keep = keepOf(counts);
 #pragma unroll
         for (int d = 0; d < kAhead; ++d) v[d] = readV(d, stage);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
+        for (int c = 0; c < N; ++c) {
           float w[8], lowest = 0.f;
           powersOf(c, s4[c], counts, all, w, true, CAREFUL ? 0.f : kPtRescaleStep);
 #pragma unroll
@@ -867,15 +875,15 @@ __global__ __launch_bounds__(kPtWaves * 64, 2) void decodePrefixTiledKernel(TaPr
             const u32x4 bad = infinite(now), odd = now & bad;
             now &= ~bad;
 #pragma unroll
-            for (int c = 0; c < NC; ++c) acc[c][d] = M::run(odd, some[c], acc[c][d]);
+            for (int c = 0; c < N; ++c) acc[c][d] = M::run(odd, some[c], acc[c][d]);
           }
 #pragma unroll
-          for (int c = 0; c < NC; ++c) acc[c][d] = M::run(now, hi[c], acc[c][d]);
+          for (int c = 0; c < N; ++c) acc[c][d] = M::run(now, hi[c], acc[c][d]);
 #pragma unroll
-          for (int c = 0; c < NC; ++c) acc[c][d] = M::run(now, lo[c], acc[c][d]);
+          for (int c = 0; c < N; ++c) acc[c][d] = M::run(now, lo[c], acc[c][d]);
         }
         if constexpr (HALF) {
-          if (__builtin_amdgcn_ballot_w64(small) != 0) addRest(stage, s * TOKENS, all, withCare);
+          if (__builtin_amdgcn_ballot_w64(small) != 0) addRest(stage, s * TOKENS, all, columnTiles, withCare);
         }
       }
       stage = next;
@@ -904,7 +912,8 @@ __global__ __launch_bounds__(kPtWaves * 64, 2) void decodePrefixTiledKernel(TaPr
   for (int block = begin; block < end; block += kPxBlock) {
     const int n = min(kPxBlock, end - block);
     const bool clean = publish(block, n);
-    walk(n, clean, std::false_type{});
+    if (NC == 1 || mine == NC) walk(n, clean, std::integral_constant<int, NC>{}, std::false_type{});
+    else walk(n, clean, std::integral_constant<int, NC == 1 ? 1 : NC - 1>{}, std::false_type{});
   }
   uint32_t largest = 0;
 #pragma unroll
@@ -918,7 +927,7 @@ __global__ __launch_bounds__(kPtWaves * 64, 2) void decodePrefixTiledKernel(TaPr
     for (int block = begin; block < end; block += kPxBlock) {
       const int n = min(kPxBlock, end - block);
       publish(block, n);
-      walk(n, false, std::true_type{});
+      walk(n, false, std::integral_constant<int, NC>{}, std::true_type{});
     }
   }
 
@@ -1089,11 +1098,18 @@ static diopiError_t decodeSharedPrefix(diopiContextHandle_t ctx, hipStream_t str
   const int64_t rowBytes = D * itemsize;
   const bool tiled = itemsize == 2 && columns > 32;
   const int64_t tiles = ceilDiv(columns, 16), columnWaves = D == 256 ? PtShape<half_t, 256>::COLUMN_WAVES : PtShape<half_t, 128>::COLUMN_WAVES;
-  int nc = columns <= 32 || rowBytes > 256 ? 1 : 2;
-  const int ncMost = D == 256 ? 1 : D == 128 ? 2 : 3;  // (more spill registers)
-  if (tiled) nc = std::min(ncMost, tiles <= 4 ? 1 : tiles <= 8 ? 2 : 3);
-  const int64_t groups = ceilDiv(tiles, tiled ? columnWaves * nc : nc), step = tiled ? (D == 256 ? 32 : 64) : kPxWaves * (itemsize == 4 ? 16 : 32);
-  const int64_t chunk = std::max<int64_t>(256, ceilDiv(x.len * a.kvHeads * groups, cus));
+  const int ncMost = tiled ? (D == 256 ? 1 : D == 128 ? 2 : 3) : columns <= 32 || rowBytes > 256 ? 1 : 2;  // (more spill registers)
+  // Few groups of columns read a row least often, but where they and chunks as short as pays leave compute units without work, more
+  // take it (8 K/V heads of 64, 192 columns each: 700 tokens 17.0 us, with the fewest groups 22.5; 4096 tokens 24 and 28 us).
+  const int64_t shortest = tiled ? 256 : 128, fewest = ceilDiv(tiles, tiled ? columnWaves * ncMost : ncMost);
+  const int64_t groups = tiled ? std::max(fewest, std::min(ceilDiv(tiles, columnWaves), cus / (a.kvHeads * ceilDiv(x.len, shortest)))) : fewest;
+  const int nc = tiled ? (int)ceilDiv(ceilDiv(tiles, groups), columnWaves) : ncMost;
+  x.groups = (int)groups;
+  const int64_t step = tiled ? (D == 256 ? 32 : 64) : kPxWaves * (itemsize == 4 ? 16 : 32);
+  // Chunks below the share of a compute unit end where a workgroup's few steps no longer pay for its start and its partial results:
+  // 777 tokens, 8 heads of 64, batch 5 take 17.0 us with 128 and with 64, 18.8 us with 256; 4096 tokens, 8 K/V heads with 64 columns each,
+  // where a step of all waves is 64 tokens, take 22 us with 256, 25 us with 128.
+  const int64_t chunk = std::max<int64_t>(shortest, ceilDiv(x.len * a.kvHeads * groups, cus));
   x.chunk = (int)(ceilDiv(std::max(chunk, ceilDiv(x.len, kPxMaxSplit)), step) * step);
   x.nsplit = (int)ceilDiv(x.len, x.chunk);
   const int64_t pairs = (int64_t)a.batch * a.heads, wgs = ceilDiv((int64_t)a.kvHeads * x.nsplit, 8) * 8 * groups;

@@ -57,6 +57,13 @@ def test_prefixes_and_lengths_from_nothing_to_several_shares(ops, dev, dtype, he
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_any_number_of_columns(ops, dev, dtype, d):
+    for batch in (8, 9, 12, 13, 17, 20, 21, 25, 29, 33, 37, 41, 49, 53, 57, 65, 69, 97, 101):   # of 4 columns each: 2 to 26 tiles of 16
+        check(ops, dev, *batch_of(70 + batch, [batch % 3] * (batch - 1) + [9], 4, 1, d, dtype, 200 + batch))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_a_long_prefix_and_long_sequences(ops, dev, dtype):
     check(ops, dev, *batch_of(6001, [1, 700, 30], 4, 2, 128, dtype, 30))
     check(ops, dev, *batch_of(2049, [2600, 1], 2, 2, 64, dtype, 31))
