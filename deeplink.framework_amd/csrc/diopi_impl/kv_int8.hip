@@ -410,10 +410,13 @@ static bool kvInt8Vector(const KvInt8Args& a, int64_t itemsize) {
 // the slots are looked up, and looked through, more often than needed: 1777 tokens of 8 heads are written in 8.5 us so and in
 // 9.9 us with 1024 workgroups each; 8192 of 8 take 49 us with 128 rows, 53 us with 256, 51 us with 64, and are read back in 36.5, 39
 // and 38 us.
-static dim3 kvInt8Grid(KvInt8Args* a) {
+static diopiError_t kvInt8Grid(const char* what, KvInt8Args* a, dim3* grid) {
   const int64_t rows = std::min<int64_t>(128, std::max<int64_t>(32, a->tokens * a->heads / 256));
   a->tokensPerWg = (int)std::min<int64_t>(kKvTokensPerWg, ceilDiv(rows, a->heads));
-  return dim3((unsigned)ceilDiv(a->tokens, a->tokensPerWg), 2);
+  const int64_t wgs = ceilDiv(a->tokens, a->tokensPerWg);
+  AMD_CHECK(wgs < 1 << 24, "%s: %ld rows of %d heads exceed the launch limits", what, (long)a->tokens, a->heads);  // (2^32 threads)
+  *grid = dim3((unsigned)wgs, 2);
+  return diopiSuccess;
 }
 
 #define KV_INT8_LAUNCH_TYPE(T, NAME, VEC)                                                                            \
@@ -451,18 +454,19 @@ extern "C" __attribute__((visibility("default"))) diopiError_t diopiDestIndexCop
   KvInt8Args a;
   AMD_TRY(kvInt8Args(what, x, pool, scale, loc, &a));
   if (x[0].numel == 0) return diopiSuccess;
+  dim3 grid;
+  AMD_TRY(kvInt8Grid(what, &a, &grid));
   AMD_TRY(makeContiguous(ctx, stream, loc, &dense));
   a.loc = dense.data;
   if (a.tokens > kKvScanTokens) {
     void* last = nullptr;
     AMD_TRY(requireWorkspace(ctx, a.slots * (int64_t)sizeof(int), &last));
-    const dim3 grid((unsigned)ceilDiv(a.tokens, kKvThreads));
-    hipLaunchKernelGGL(kvInt8LastKernel<true>, grid, dim3(kKvThreads), 0, stream, a, static_cast<int*>(last));
-    hipLaunchKernelGGL(kvInt8LastKernel<false>, grid, dim3(kKvThreads), 0, stream, a, static_cast<int*>(last));
+    const dim3 perToken((unsigned)ceilDiv(a.tokens, kKvThreads));
+    hipLaunchKernelGGL(kvInt8LastKernel<true>, perToken, dim3(kKvThreads), 0, stream, a, static_cast<int*>(last));
+    hipLaunchKernelGGL(kvInt8LastKernel<false>, perToken, dim3(kKvThreads), 0, stream, a, static_cast<int*>(last));
     AMD_LAUNCH_CHECK();
     a.last = static_cast<const int*>(last);
   }
-  const dim3 grid = kvInt8Grid(&a);
   KV_INT8_LAUNCH(x[0].dtype, kvInt8Write, kvInt8Vector(a, x[0].itemsize));
   AMD_LAUNCH_CHECK();
   return diopiSuccess;
@@ -485,9 +489,10 @@ extern "C" __attribute__((visibility("default"))) diopiError_t diopiIndexSelectK
   KvInt8Args a;
   AMD_TRY(kvInt8Args(what, x, pool, scale, loc, &a));
   if (x[0].numel == 0) return diopiSuccess;
+  dim3 grid;
+  AMD_TRY(kvInt8Grid(what, &a, &grid));
   AMD_TRY(makeContiguous(ctx, stream, loc, &dense));
   a.loc = dense.data;
-  const dim3 grid = kvInt8Grid(&a);
   KV_INT8_LAUNCH(x[0].dtype, kvInt8Read, kvInt8Vector(a, x[0].itemsize));
   AMD_LAUNCH_CHECK();
   return diopiSuccess;

@@ -535,7 +535,7 @@ static diopiError_t decodeInt8(diopiContextHandle_t ctx, hipStream_t stream, TaI
     partial = static_cast<float*>(ws);
   }
   const int64_t wgs = ceilDiv((int64_t)a.batch * a.nsplit, 8) * 8 * headGroups;
-  AMD_CHECK(wgs < ((int64_t)1 << 31), "int8 token attention: %ld workgroups exceed the grid limits", (long)wgs);
+  AMD_CHECK(wgs < 1 << 24, "int8 token attention: %ld workgroups exceed the grid limits", (long)wgs);  // (2^32 threads)
   const int lds = 2 * kI8Waves * kI8Block * (int)sizeof(float) + (x.headsPerWg == kI8Waves ? 0 : kI8Waves * (int)std::min<int64_t>(perKv, kI8Heads) * (D + 4) * (int)sizeof(float));
 #define INT8_CALL(T, SIZE)                                                                                              \
   do {                                                                                                                  \

@@ -586,7 +586,7 @@ __global__ __launch_bounds__(kPtWaves * 64, 2) void decodePrefixTiledKernel(TaPr
   if (u >= a.kvHeads * x.nsplit) return;  // the grid is rounded up to whole rounds of the XCDs
   const int kvh = u % a.kvHeads, split = u / a.kvHeads;
   const int begin = split * x.chunk, end = min(x.len, begin + x.chunk);
-  const int groupTile = group * tiles / groups, groupTiles = (group + 1) * tiles / groups - groupTile;
+  const int groupTile = (int)((int64_t)group * tiles / groups), groupTiles = (int)((int64_t)(group + 1) * tiles / groups) - groupTile;
   const int firstTile = columnWave * groupTiles / COLUMN_WAVES, mine = (columnWave + 1) * groupTiles / COLUMN_WAVES - firstTile;
   const int firstColumn = (groupTile + firstTile) * 16;
   const bool active = NC > 1 || mine > 0;  // (a wave without columns only copies)
@@ -1113,7 +1113,8 @@ static diopiError_t decodeSharedPrefix(diopiContextHandle_t ctx, hipStream_t str
   x.chunk = (int)(ceilDiv(std::max(chunk, ceilDiv(x.len, kPxMaxSplit)), step) * step);
   x.nsplit = (int)ceilDiv(x.len, x.chunk);
   const int64_t pairs = (int64_t)a.batch * a.heads, wgs = ceilDiv((int64_t)a.kvHeads * x.nsplit, 8) * 8 * groups;
-  AMD_CHECK(wgs < ((int64_t)1 << 31) && pairs < ((int64_t)1 << 31), "shared prefix attention: %ld workgroups exceed the grid limits", (long)wgs);
+  // (fewer than 2^32 threads to a launch)
+  AMD_CHECK(wgs < 1 << 23 && pairs < 1 << 24, "shared prefix attention: %d sequences of %d heads exceed the grid limits", a.batch, a.heads);
   void* ws = nullptr;
   AMD_TRY(requireWorkspace(ctx, pairs * x.nsplit * (2 + a.d) * (int64_t)sizeof(float), &ws));
   float* partial = static_cast<float*>(ws);
@@ -1200,17 +1201,18 @@ extern "C" __attribute__((visibility("default"))) diopiError_t diopiTokenDecodeA
   AMD_CHECK(prefix.defined() && prefix.ndim == 1, "shared prefix attention: prefix_loc must be a tensor of one dim");
   AMD_CHECK(prefix.dtype == diopi_dtype_int32 || prefix.dtype == diopi_dtype_int64, "shared prefix attention: prefix_loc must be int32 or int64, got %s",
             dtypeName(prefix.dtype));
-  AMD_CHECK(prefix.shape[0] + (int64_t)maxInputLen < ((int64_t)1 << 31) - 256, "shared prefix attention: %ld shared tokens and %d own ones exceed 2^31",
+  AMD_CHECK(prefix.shape[0] + (int64_t)maxInputLen <= 1 << 30, "shared prefix attention: %ld shared tokens and %d own ones exceed 2^30",
             (long)prefix.shape[0], maxInputLen);
   AMD_CHECK(out.defined() && out.dtype == t.q.dtype && out.ndim == 3 && out.isContiguous(), "shared prefix attention: out must be a dense tensor shaped like q");
   for (int d = 0; d < 3; ++d) AMD_CHECK(out.shape[d] == t.q.shape[d], "shared prefix attention: out must be shaped like q");
   if (t.q.numel == 0) return diopiSuccess;
   AMD_CHECK(a.batch <= 65535, "shared prefix attention: batch %d exceeds the grid limits", a.batch);
   AMD_CHECK(t.q.shape[2] <= kTaGenericMaxD, "shared prefix attention: head_dim %ld exceeds %d", (long)t.q.shape[2], kTaGenericMaxD);
+  if (prefix.shape[0] == 0) return diopiTokenDecodeAttentionInference(ctx, outH, qH, kH, vH, locH, startH, lenH, maxInputLen);  // nothing is shared
   AMD_TRY(makeContiguous(ctx, stream, prefix, &densePrefix));
   x.loc = densePrefix.data, x.loc64 = prefix.dtype == diopi_dtype_int64, x.len = (int)prefix.shape[0];
-  // (slot numbers in 31 bits; a prefix of nothing shares nothing, and is no case of its own)
-  if (!a.generic && x.len > 0 && a.slots <= 0x7fffffff && std::max(a.kSlotStride, a.vSlotStride) * t.q.itemsize <= 0xffffffffll)
+  // (slot numbers in 31 bits)
+  if (!a.generic && a.slots <= 0x7fffffff && std::max(a.kSlotStride, a.vSlotStride) * t.q.itemsize <= 0xffffffffll)
     return decodeSharedPrefix(ctx, stream, x, t.q.dtype, out.data);
   const dim3 grid(a.heads, a.batch);
   if (t.q.dtype == diopi_dtype_bfloat16) hipLaunchKernelGGL((decodePrefixAnyKernel<bf16_t>), grid, dim3(256), 0, stream, x, out.ptr<bf16_t>());

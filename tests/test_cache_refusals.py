@@ -93,7 +93,7 @@ def test_int8_attention(pkg, call, changes, says):
     (dict(k=torch.zeros(6, 3, 64), v=torch.zeros(6, 3, 64)), "multiple"),
     (dict(k=torch.zeros(0, 2, 64), v=torch.zeros(0, 2, 64)), "no slots"),
     (dict(b_loc=torch.zeros(2, 4, dtype=torch.int32)), "columns"), (dict(lens=torch.zeros(1, dtype=torch.int32)), "entries"),
-    (dict(prefix=torch.zeros(1, dtype=torch.int32).expand(2 ** 31)), "exceed 2"),
+    (dict(prefix=torch.zeros(1, dtype=torch.int32).expand(2 ** 31)), "exceed 2"), (dict(prefix=torch.zeros(1, dtype=torch.int32).expand(2 ** 30 - 4)), "exceed 2"),
     (dict(q=torch.zeros(2, 4, 1040), out=torch.zeros(2, 4, 1040), k=torch.zeros(6, 2, 1040), v=torch.zeros(6, 2, 1040)), "exceeds 1024"),
 ])
 def test_shared_prefix(pkg, call, changes, says):
@@ -110,6 +110,26 @@ def test_pools_of_too_many_slots(pkg, call, name, order):
     args = Args(k=torch.zeros(3, 2, 64), v=torch.zeros(3, 2, 64), loc=torch.zeros(3, dtype=torch.int32), **many)
     with pytest.raises(pkg.diopi.DiopiError, match="2147483648 slots exceed"):
         call(name, args, order)
+
+
+@pytest.mark.parametrize("name,order", [WRITE, READ])
+def test_more_rows_than_a_launch_holds(pkg, call, name, order):
+    rows = torch.zeros(1, 128, 1).expand(2 ** 24, 128, 1)
+    with pytest.raises(pkg.diopi.DiopiError, match="16777216 rows of 128 heads exceed"):
+        call(name, Args(k=rows, v=rows, loc=torch.zeros(1, dtype=torch.int32).expand(2 ** 24), **pools(6, 128, 1)), order)
+
+
+def test_more_heads_than_a_launch_holds(pkg, call):
+    one, batch = torch.ones(65535, dtype=torch.int32), 65535
+    table = dict(b_loc=torch.zeros(batch, 1, dtype=torch.int32), start=one, lens=one)
+    q = torch.zeros(1, 1, 16).bfloat16()
+    args = Args(q=q.expand(batch, 1024, 16), out=torch.empty(batch, 1024, 16, dtype=torch.bfloat16), **table, **pools(6, 1024, 16))
+    with pytest.raises(pkg.diopi.DiopiError, match="workgroups exceed"):
+        call(INT8[0], args, INT8[1], 1)
+    k = torch.zeros(6, 1, 16).bfloat16()
+    args = Args(q=q.expand(batch, 300, 16), out=torch.empty(batch, 300, 16, dtype=torch.bfloat16), k=k, v=k, prefix=torch.zeros(3, dtype=torch.int32), **table)
+    with pytest.raises(pkg.diopi.DiopiError, match="65535 sequences of 300 heads exceed"):
+        call(PREFIX[0], args, PREFIX[1], 1)
 
 
 def test_a_closed_context_and_host_tensors(pkg):

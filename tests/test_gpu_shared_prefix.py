@@ -162,6 +162,20 @@ def test_a_pool_past_2_to_the_31_elements(ops, dev):
     oracle.assert_within(out, *oracle.attend(q, kk, vv, [torch.arange(5), torch.tensor([0, 1, 2, 4])], PART[torch.bfloat16]))
 
 
+def test_the_largest_batch_on_one_head(ops, dev):
+    """2.6 million columns: (groups of columns) x (their tiles) pass 2^31."""
+    batch, heads, d = 65535, 40, 64
+    q, k, v, prefix, b_loc, lens, max_len = batch_of(6, [1] * 2 + [0] + [1] * 3, heads, 1, d, torch.bfloat16, 90)
+    at = torch.randint(0, len(lens), (batch,), generator=g(91))
+    got = run(ops, dev, q.to(dev)[at.to(dev)], k, v, prefix, b_loc[at], lens[at], max_len)
+    want = run(ops, dev, q, k, v, prefix, b_loc, lens, max_len)
+    full, bound = oracle.attend(q, k, v, own_and_shared(prefix, b_loc, lens, max_len), PART[q.dtype])
+    oracle.assert_within(want, full, bound)
+    for first in range(0, batch, 8192):
+        some = at[first:first + 8192]
+        oracle.assert_within(got[first:first + 8192], full[some], bound[some])
+
+
 def test_no_sequences(ops, dev):
     k, none = torch.ones(4, 2, 64, device=dev), torch.zeros(0, dtype=torch.int32, device=dev)
     out = ops.token_decode_attention_shared_prefix(torch.zeros(0, 2, 64, device=dev), k, k, none, torch.zeros(0, 5, dtype=torch.int32, device=dev), none, none, 5)
