@@ -381,7 +381,6 @@ __global__ __launch_bounds__(kI8Waves * 64, D == 256 ? 1 : 2) void decodeInt8Ker
     }
     const int perShare = ((n + shares - 1) / shares + kI8Tile - 1) / kI8Tile * kI8Tile;  // whole steps
     const int from = share * perShare, to = mine ? min(n, from + perShare) : from;
-    const int last = from + (to - from - 1) / kI8Tile * kI8Tile;  // the last step
     Step s0, s1;
     request(s0, from);  // (also where the wave has no step: all of the block's slots can be read, and a branch would cost as below)
 #pragma unroll
@@ -392,16 +391,21 @@ __global__ __launch_bounds__(kI8Waves * 64, D == 256 ? 1 : 2) void decodeInt8Ker
         scaleBuf[(kI8Waves + w) * kI8Block + threadIdx.x + 256 * i] = vsv[i][w];
       }
     __syncthreads();
-    // (after the last step its rows are asked for again, which costs nothing to speak of: a branch around the loads would make
-    // every wait one for all of them)
+    // (the last one or two steps stand by themselves: a branch around the loads of the loop would make every wait one for all of them)
     int at = from;
-    for (; at + kI8Tile < to; at += 2 * kI8Tile) {
+    for (; at + 2 * kI8Tile < to; at += 2 * kI8Tile) {
       request(s1, at + kI8Tile);
       multiply(s0, at, clean);
-      request(s0, min(at + 2 * kI8Tile, last));
-      multiply(s1, at + kI8Tile, clean && at + 2 * kI8Tile <= n);
+      request(s0, at + 2 * kI8Tile);
+      multiply(s1, at + kI8Tile, clean);
     }
-    if (at < to) multiply(s0, at, clean && at + kI8Tile <= n);
+    if (at + kI8Tile < to) {
+      request(s1, at + kI8Tile);
+      multiply(s0, at, clean);
+      multiply(s1, at + kI8Tile, clean && at + 2 * kI8Tile <= n);
+    } else if (at < to) {
+      multiply(s0, at, clean && at + kI8Tile <= n);
+    }
   }
 
   // every lane group holds its own share of l; O^T lies in the lanes as (head = column, places runOf(4 quad + i) + t)
