@@ -18,8 +18,8 @@ struct TaPrefixArgs {
   bool loc64;
   int len;
   int chunk, nsplit;          // of the shared tokens
-  int groups;                 // of columns, decodePrefixTiledKernel
-  unsigned kStride, vStride;  // slot strides of the pools in bytes, as decodePrefixKernel takes them
+  int groups;                 // of columns
+  unsigned kStride, vStride;  // slot strides of the pools in bytes
 };
 
 // Any head size up to 1024: one workgroup per (sequence, head) walks the shared tokens and then its own, 256 at a time, one
@@ -84,58 +84,37 @@ __global__ __launch_bounds__(256) void decodePrefixAnyKernel(TaPrefixArgs x, T* 
 // sequences: S^T = K . Q^T and O^T += V^T . P^T with many columns for one read of a row. Partial results (maximum, sum, weighted
 // sum of V) of each chunk of the prefix go to workspace; those of the sequences' own tokens come from the kernels of
 // diopiTokenDecodeAttentionInference, and a last launch merges both.
-// With up to 32 columns, or fp32: bound by memory, every shared row read once (fp32 with more columns: once for every 32 of them),
-// and for short prefixes by the three launches and the latency of slots, then rows.
-//   * rows go from the pool into the registers that the products read, whole 128-byte lines of 8 rows in a load: K as in
-//     token_attention_int8.hip (a piece of 16 bytes is an operand, two lanes swap one); of V a lane takes 16 bytes of each of its
-//     eight tokens, which are eight places of the head, and v_perm puts pairs of tokens side by side, so V is turned round in registers.
-//   * a probability is cut into parts of 8 bits, two of them for bf16 (off by at most 2^-16 relative). fp16 has no room for the
-//     small ones: there V is cut into two bf16 parts too (exact: 8 bits and 3), and three of the four products are added up (the
-//     fourth is below 2^-16). fp32 rows are multiplied as they are (16x16x4).
+//
+// Long prefixes are bound by memory, every shared row read once (for each group of columns), and, with many columns, by the matrix
+// pipe and the exponentials; short ones by the three launches and the latency of slots, then rows.
+//
+// ------------------------------------------------ fp32 --
+// Rows go from the pool into the registers that the products (16x16x4) read, whole 128-byte lines of 8 rows in a load: K as in
+// token_attention_int8.hip (two lanes swap a piece of 16 bytes), of V a lane takes 16 adjacent bytes of each of its four tokens.
 //   * the running maximum is followed at once, so a probability is at most one.
-//   * the first walk multiplies V as it is: infinities and NaN in it, or in slot 0 for a slot outside the pool, against parts
-//     that are zero or negative, leave sums that are not finite, and the wave then walks again with care: rows that do not count
+//   * the first walk multiplies V as it is: infinities and NaN in it, or in slot 0 for a slot outside the pool, against
+//     probabilities that are zero leave sums that are not finite, and the wave then walks again with care: rows that do not count
 //     are zeros, what is not finite meets a one for each probability that is not zero.
-// Four waves share a chunk's tokens and meet in LDS, a lane always adding to what is its own.
+// Four waves share a chunk's tokens and meet in LDS, a lane always adding to what is its own. 16 000 tokens, 32 heads of 128, 24
+// sequences: 136 us, 3.9 TB/s; two tiles of columns share a read with heads of 64 (with 128 that takes more registers than there are).
 constexpr int kPxWaves = 4;
 constexpr int kPxBlock = 2048;    // tokens whose slots a workgroup holds in LDS at once
 constexpr int kPxMaxSplit = 256;  // chunks of the prefix
 
-template <typename T, int D>
+template <int D>
 struct PxShape {
-  static constexpr bool kWide = sizeof(T) == 4;
-  static constexpr int TOKENS = kWide ? 16 : 32;             // of a wave's step
-  static constexpr int TILES = TOKENS / 16;
-  static constexpr int ROWB = D * (int)sizeof(T);
-  static constexpr int KP = ROWB / 64;                        // 16-byte pieces of K per lane and tile
-  static constexpr int EP = 16 / (int)sizeof(T);              // elements of a piece
-  static constexpr int RUN = D / 16;                          // places of V per lane
-  static constexpr bool PAIRS = ROWB / 16 < 16;               // 8 bytes of V per token: two tokens in a load
-  static constexpr int VP = PAIRS ? 1 : ROWB / 256;           // 16-byte pieces of V per lane and token
-  static constexpr int VTOK = 4 * TILES, VLOADS = PAIRS ? VTOK / 2 : VTOK;
+  static constexpr int KP = D / 16;   // 16-byte pieces of K per lane
+  static constexpr int RUN = D / 16;  // places of V per lane
+  static constexpr int VP = D / 64;   // 16-byte pieces of V per lane and token
   // place t of lane c's places of V in the head
-  static __device__ __forceinline__ int place(int c, int t) {
-    return PAIRS ? (c & 7) * 2 * RUN + (c >> 3) * RUN + t : t / EP * (256 / (int)sizeof(T)) + c * EP + t % EP;
-  }
+  static __device__ __forceinline__ int place(int c, int t) { return t / 4 * 64 + c * 4 + t % 4; }
 };
 
-template <typename T>
-__device__ __forceinline__ bf16x8 pxPart(float (&x)[8]) {  // the next 8 bits of eight numbers, and what they leave
-  bf16x8 part;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    part[i] = static_cast<bf16_t>(x[i]);
-    x[i] -= static_cast<float>(part[i]);
-  }
-  return part;
-}
-
 // D: head size the rows are laid out for; a.d is any whole number of 16-byte pieces up to it. NC: column tiles of 16.
-template <typename T, int D, int NC>
-__global__ __launch_bounds__(kPxWaves * 64, 1) void decodePrefixKernel(TaPrefixArgs x, float* __restrict__ partial) {
-  using S = PxShape<T, D>;
-  constexpr int TOKENS = S::TOKENS, TILES = S::TILES, KP = S::KP, RUN = S::RUN, VP = S::VP, VTOK = S::VTOK;
-  constexpr bool WIDE = S::kWide, HALF = std::is_same<T, half_t>::value;
+template <int D, int NC>
+__global__ __launch_bounds__(kPxWaves * 64, 1) void decodePrefixFloatKernel(TaPrefixArgs x, float* __restrict__ partial) {
+  using S = PxShape<D>;
+  constexpr int TOKENS = 16, KP = S::KP, RUN = S::RUN, VP = S::VP;  // TOKENS: of a wave's step
   const TaArgs& a = x.a;
   extern __shared__ __attribute__((aligned(16))) f32x4 pxLds[];  // sums on their way to the waves that add them up
   __shared__ __attribute__((aligned(16))) int slots[kPxBlock];  // of a block's tokens; negative: does not count
@@ -147,33 +126,36 @@ __global__ __launch_bounds__(kPxWaves * 64, 1) void decodePrefixKernel(TaPrefixA
   // Workgroup ids go round the 8 XCDs. A unit is a (chunk, K/V head); its groups of columns read the same rows and run next to
   // each other on one XCD.
   const int f = blockIdx.x, idx = f >> 3;
-  const int perKv = a.heads / a.kvHeads, columns = a.batch * perKv, groups = (columns + 16 * NC - 1) / (16 * NC);
+  const int perKv = a.heads / a.kvHeads, columns = a.batch * perKv, tiles = (columns + 15) / 16, groups = x.groups;
   const int group = idx % groups, u = (idx / groups) * 8 + (f & 7);
   if (u >= a.kvHeads * x.nsplit) return;  // the grid is rounded up to whole rounds of the XCDs
   const int kvh = u % a.kvHeads, split = u / a.kvHeads;
   const int begin = split * x.chunk, end = min(x.len, begin + x.chunk);
 
-  // q of the columns: column c of the K/V head is its query head c % perKv in sequence c / perKv. Piece p holds EP places from
+  // tiles of columns are dealt out evenly to the groups: up to NC to one
+  const int firstTile = (int)((int64_t)group * tiles / groups), lastTile = (int)((int64_t)(group + 1) * tiles / groups);
+
+  // q of the columns: column c of the K/V head is its query head c % perKv in sequence c / perKv. Piece p holds four places from
   // the byte 128 (p / 2) + 32 quad + 16 (p % 2) of the row on.
-  u32x4 qf[NC][KP];
+  f32x4 qf[NC][KP];
   int pairOf[NC];  // row of the partial results of this lane's column, or -1
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
-    const int column = (group * NC + c) * 16 + col;
-    const bool have = column < columns;
+    const int column = (firstTile + c) * 16 + col;
+    const bool have = firstTile + c < lastTile && column < columns;
     const int b = have ? column / perKv : 0, h = kvh * perKv + (have ? column % perKv : 0);
     pairOf[c] = have ? b * a.heads + h : -1;
-    const T* src = reinterpret_cast<const T*>(a.q) + b * a.qBatchStride + h * a.qHeadStride;
+    const float* src = reinterpret_cast<const float*>(a.q) + b * a.qBatchStride + h * a.qHeadStride;
 #pragma unroll
     for (int p = 0; p < KP; ++p) {
-      const int e = (128 * (p >> 1) + 32 * quad + 16 * (p & 1)) / (int)sizeof(T);
-      qf[c][p] = *reinterpret_cast<const u32x4*>(src + (e < a.d ? e : 0));
-      if (!have || e >= a.d) qf[c][p] = u32x4{0, 0, 0, 0};
+      const int e = 32 * (p >> 1) + 8 * quad + 4 * (p & 1);
+      qf[c][p] = *reinterpret_cast<const f32x4*>(src + (e < a.d ? e : 0));
+      if (!have || e >= a.d) qf[c][p] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
   }
 
   int kOff[KP], vOff[VP];  // bytes; pieces past the row's end repeat its first one
-  const int rowBytes = a.d * (int)sizeof(T);
+  const int rowBytes = a.d * (int)sizeof(float);
 #pragma unroll
   for (int p = 0; p < KP; ++p) {
     const int e = 128 * (p >> 1) + 32 * quad + 16 * upperHalf;
@@ -181,30 +163,27 @@ __global__ __launch_bounds__(kPxWaves * 64, 1) void decodePrefixKernel(TaPrefixA
   }
 #pragma unroll
   for (int p = 0; p < VP; ++p) {
-    const int e = S::PAIRS ? 16 * (lane & 7) : 256 * p + 16 * col;
+    const int e = 256 * p + 16 * col;
     vOff[p] = e < rowBytes ? e : 0;
   }
-  const char* const kBase = reinterpret_cast<const char*>(reinterpret_cast<const T*>(a.k) + kvh * a.kHeadStride);
-  const char* const vBase = reinterpret_cast<const char*>(reinterpret_cast<const T*>(a.v) + kvh * a.vHeadStride);
+  const char* const kBase = reinterpret_cast<const char*>(reinterpret_cast<const float*>(a.k) + kvh * a.kHeadStride);
+  const char* const vBase = reinterpret_cast<const char*>(reinterpret_cast<const float*>(a.v) + kvh * a.vHeadStride);
 
   struct Step {
-    u32x4 k[TILES][KP];
-    u32x4 v[S::VLOADS][VP];
+    u32x4 k[KP];
+    f32x4 v[4][VP];
   };
   auto request = [&](Step& s, int at) {
 #pragma unroll
-    for (int t = 0; t < TILES; ++t)
+    for (int p = 0; p < KP; ++p) {
+      const char* row = kBase + (uint64_t)((unsigned)slots[at + (lane & 7) + 8 * (p & 1)] & 0x7fffffffu) * x.kStride;
+      s.k[p] = *reinterpret_cast<const u32x4*>(row + kOff[p]);
+    }
 #pragma unroll
-      for (int p = 0; p < KP; ++p) {
-        const int token = at + 16 * t + (lane & 7) + 8 * (p & 1);
-        s.k[t][p] = *reinterpret_cast<const u32x4*>(kBase + (uint64_t)((unsigned)slots[token] & 0x7fffffffu) * x.kStride + kOff[p]);
-      }
+    for (int i = 0; i < 4; ++i) {
+      const char* row = vBase + (uint64_t)((unsigned)slots[at + 4 * quad + i] & 0x7fffffffu) * x.vStride;
 #pragma unroll
-    for (int i = 0; i < S::VLOADS; ++i) {
-      const int token = at + (S::PAIRS ? 16 * (i >> 1) + 4 * quad + 2 * (i & 1) + upperHalf : 16 * (i >> 2) + 4 * quad + (i & 3));
-      const char* row = vBase + (uint64_t)((unsigned)slots[token] & 0x7fffffffu) * x.vStride;
-#pragma unroll
-      for (int p = 0; p < VP; ++p) s.v[i][p] = *reinterpret_cast<const u32x4*>(row + vOff[p]);
+      for (int p = 0; p < VP; ++p) s.v[i][p] = *reinterpret_cast<const f32x4*>(row + vOff[p]);
     }
     __builtin_amdgcn_sched_barrier(0);  // nothing of the step before is touched (and waited for) ahead of these loads
   };
@@ -227,75 +206,30 @@ __global__ __launch_bounds__(kPxWaves * 64, 1) void decodePrefixKernel(TaPrefixA
   };
   auto multiply = [&](Step& s, int at, bool all, auto withCare) {  // all: every one of the tokens counts
     constexpr bool CAREFUL = decltype(withCare)::value;
-    u32x4 kf[TILES][KP];
+    u32x4 kf[KP];
 #pragma unroll
-    for (int t = 0; t < TILES; ++t)
+    for (int p = 0; p < KP; ++p) {
 #pragma unroll
-      for (int p = 0; p < KP; ++p) {
-#pragma unroll
-        for (int w = 0; w < 4; ++w)
-          kf[t][p][w] = p & 1 ? swapped(s.k[t][p][w], s.k[t][p - 1][w], kLower) : swapped(s.k[t][p][w], s.k[t][p + 1][w], kUpper);
-        if (CAREFUL && 128 * (p >> 1) + 32 * quad + 16 * (p & 1) >= rowBytes) kf[t][p] = u32x4{0, 0, 0, 0};
-      }
-    // V of the lane's tokens at its places
-    constexpr int WORDS = RUN * (int)sizeof(T) / 4;
-    uint32_t v[VTOK][WORDS];
-#pragma unroll
-    for (int i = 0; i < S::VLOADS; ++i)
-#pragma unroll
-      for (int w = 0; w < WORDS; ++w) {
-        if constexpr (S::PAIRS) {
-          v[2 * i][w] = swapped(s.v[i][0][w], s.v[i][0][WORDS + w], kUpper);
-          v[2 * i + 1][w] = swapped(s.v[i][0][WORDS + w], s.v[i][0][w], kLower);
-        } else {
-          v[i][w] = s.v[i][w / 4][w % 4];
-        }
-      }
-    bool counts[VTOK];
-#pragma unroll
-    for (int i = 0; i < VTOK; ++i) counts[i] = true;
+      for (int w = 0; w < 4; ++w) kf[p][w] = p & 1 ? swapped(s.k[p][w], s.k[p - 1][w], kLower) : swapped(s.k[p][w], s.k[p + 1][w], kUpper);
+      if (CAREFUL && 128 * (p >> 1) + 32 * quad + 16 * (p & 1) >= rowBytes) kf[p] = u32x4{0, 0, 0, 0};
+    }
+    bool counts[4] = {true, true, true, true};
     if (CAREFUL || !all) {
-#pragma unroll
-      for (int t = 0; t < TILES; ++t) {
-        const int4 m4 = *reinterpret_cast<const int4*>(slots + at + 16 * t + 4 * quad);
-        counts[4 * t] = m4.x >= 0, counts[4 * t + 1] = m4.y >= 0, counts[4 * t + 2] = m4.z >= 0, counts[4 * t + 3] = m4.w >= 0;
-      }
-      if constexpr (CAREFUL) {
-#pragma unroll
-        for (int i = 0; i < VTOK; ++i)
-#pragma unroll
-          for (int w = 0; w < WORDS; ++w) v[i][w] = counts[i] ? v[i][w] : 0u;
-      }
+      const int4 m4 = *reinterpret_cast<const int4*>(slots + at + 4 * quad);
+      counts[0] = m4.x >= 0, counts[1] = m4.y >= 0, counts[2] = m4.z >= 0, counts[3] = m4.w >= 0;
     }
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      f32x4 s4[TILES];
+      f32x4 w = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int t = 0; t < TILES; ++t) {
-        s4[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int p = 0; p < KP; ++p)
 #pragma unroll
-        for (int p = 0; p < KP; ++p) {
-          if constexpr (WIDE) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              s4[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kf[t][p][e]), __uint_as_float(qf[c][p][e]), s4[t], 0, 0, 0);
-          } else if constexpr (HALF) {
-            s4[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, kf[t][p]), __builtin_bit_cast(f16x8, qf[c][p]), s4[t], 0, 0, 0);
-          } else {
-            s4[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kf[t][p]), __builtin_bit_cast(bf16x8, qf[c][p]), s4[t], 0, 0, 0);
-          }
-        }
-      }
-      float w[8];
-      float mt = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < VTOK; ++i) w[i] = s4[i >> 2][i & 3];
+        for (int e = 0; e < 4; ++e) w = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kf[p][e]), qf[c][p][e], w, 0, 0, 0);
       if (CAREFUL || !all) {
 #pragma unroll
-        for (int i = 0; i < VTOK; ++i) w[i] = counts[i] ? w[i] : -INFINITY;
+        for (int i = 0; i < 4; ++i) w[i] = counts[i] ? w[i] : -INFINITY;
       }
-#pragma unroll
-      for (int i = 0; i < VTOK; ++i) mt = fmaxf(mt, w[i]);
+      float mt = fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3]));
       if (__builtin_amdgcn_ballot_w64(mt > most[c]) != 0) {
         auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mt), __float_as_uint(mt), false, false);
         mt = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
@@ -314,65 +248,23 @@ __global__ __launch_bounds__(kPxWaves * 64, 1) void decodePrefixKernel(TaPrefixA
         }
       }
 #pragma unroll
-      for (int i = 0; i < VTOK; ++i) {
+      for (int i = 0; i < 4; ++i) {
         w[i] = __builtin_amdgcn_exp2f(fmaf(w[i], a.scaleLog2e, -mRef[c]));
         l[c] += w[i];
       }
-      if constexpr (WIDE) {
 #pragma unroll
-        for (int t = 0; t < RUN; ++t)
+      for (int t = 0; t < RUN; ++t)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float vi = __uint_as_float(v[i][t]);
-            if constexpr (CAREFUL) {
-              const bool finite = (v[i][t] & 0x7f800000u) != 0x7f800000u;
-              acc[c][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(finite ? 0.f : vi, w[i] > 0.f ? 1.f : w[i], acc[c][t], 0, 0, 0);
-              vi = finite ? vi : 0.f;
-            }
-            acc[c][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(vi, w[i], acc[c][t], 0, 0, 0);
-          }
-      } else {
-        bf16x8 some;
-        if constexpr (CAREFUL) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) some[i] = static_cast<bf16_t>(w[i] > 0.f ? 1.f : w[i]);
-        }
-        const bf16x8 hi = pxPart<T>(w), lo = pxPart<T>(w);
-        staticFor<RUN>([&](auto t) {
-          constexpr int W = t.value / 2;
-          constexpr unsigned kPick = t.value % 2 ? 0x07060302u : 0x05040100u;
-          u32x4 o;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) o[j] = __builtin_amdgcn_perm(v[2 * j + 1][W], v[2 * j][W], kPick);
-          u32x4 first, second;  // bf16 parts of V
-          if constexpr (HALF) {
-            const f16x8 oh = __builtin_bit_cast(f16x8, o);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const float f0 = static_cast<float>(oh[2 * j]), f1 = static_cast<float>(oh[2 * j + 1]);
-              const uint32_t u0 = __float_as_uint(f0), u1 = __float_as_uint(f1);
-              first[j] = __builtin_amdgcn_perm(u1, u0, 0x07060302u);  // the upper 8 bits, cut: what is left has 3
-              const float r0 = f0 - __uint_as_float(u0 & 0xffff0000u), r1 = f1 - __uint_as_float(u1 & 0xffff0000u);
-              second[j] = __builtin_amdgcn_perm(__float_as_uint(r1), __float_as_uint(r0), 0x07060302u);
-            }
-          } else {
-            first = o;
-          }
+        for (int i = 0; i < 4; ++i) {
+          float vi = s.v[i][t / 4][t % 4];
           if constexpr (CAREFUL) {
-            u32x4 odd;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const uint32_t bad = ((first[j] & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((first[j] & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
-              odd[j] = first[j] & bad, first[j] &= ~bad;
-              if constexpr (HALF) second[j] &= ~bad;
-            }
-            acc[c][t.value] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, odd), some, acc[c][t.value], 0, 0, 0);
+            vi = counts[i] ? vi : 0.f;
+            const bool finite = (__float_as_uint(vi) & 0x7f800000u) != 0x7f800000u;
+            acc[c][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(finite ? 0.f : vi, w[i] > 0.f ? 1.f : w[i], acc[c][t], 0, 0, 0);
+            vi = finite ? vi : 0.f;
           }
-          acc[c][t.value] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, first), hi, acc[c][t.value], 0, 0, 0);
-          acc[c][t.value] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, first), lo, acc[c][t.value], 0, 0, 0);
-          if constexpr (HALF) acc[c][t.value] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, second), hi, acc[c][t.value], 0, 0, 0);
-        });
-      }
+          acc[c][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(vi, w[i], acc[c][t], 0, 0, 0);
+        }
     }
   };
   // the wave's share of a block, after the block's slots have been published
@@ -390,13 +282,20 @@ __global__ __launch_bounds__(kPxWaves * 64, 1) void decodePrefixKernel(TaPrefixA
     } else {
       Step s1;
       int at = from;
-      for (; at + TOKENS < to; at += 2 * TOKENS) {
+      // (the last one or two steps stand by themselves: a branch around the loads of the loop would make every wait one for all of them)
+      for (; at + 2 * TOKENS < to; at += 2 * TOKENS) {
         request(s1, at + TOKENS);
         multiply(s0, at, clean, withCare);
-        request(s0, min(at + 2 * TOKENS, last));  // (after the last step its rows again: a branch around the loads would make every wait one for all of them)
-        multiply(s1, at + TOKENS, clean && at + 2 * TOKENS <= n, withCare);
+        request(s0, at + 2 * TOKENS);
+        multiply(s1, at + TOKENS, clean, withCare);
       }
-      if (at < to) multiply(s0, at, clean && at + TOKENS <= n, withCare);
+      if (at + TOKENS < to) {
+        request(s1, at + TOKENS);
+        multiply(s0, at, clean, withCare);
+        multiply(s1, at + TOKENS, clean && at + 2 * TOKENS <= n, withCare);
+      } else if (at < to) {
+        multiply(s0, at, clean && at + TOKENS <= n, withCare);
+      }
     }
   };
   // Publishes the slots of [block, block + n): a thread looks up every 256th (past the last: that one again).
@@ -490,16 +389,18 @@ __global__ __launch_bounds__(kPxWaves * 64, 1) void decodePrefixKernel(TaPrefixA
   }
 }
 
-// ------------------------------------------------ many columns: rows shared by the waves through LDS --
-// With more than two tiles of columns every wave would read the rows for itself, turn V round for itself, and, one wave to a SIMD, let
-// the matrix pipe wait for the softmax (16 001 tokens, 192 columns: 99 us). Here eight waves share a stage of 64 tokens: four
-// groups of NC column tiles times two halves of the tokens, so a workgroup takes up to 192 columns from one read of a row, and of
-// the two waves of a SIMD one multiplies while the other takes exponentials. Rows go straight into a ring of stages in LDS
-// (global_load_lds, 16 bytes to a lane, pieces XOR-swizzled by row), K is read as it lies, V through the transposing read; one
-// barrier per stage.
-// Probabilities in fp16 are taken times 2^15 (at most 2^15) and cut into two fp16 parts, all bits down to 2^-17 of the
-// largest, 16 down to 2^-24; a step that has smaller ones multiplies what is left of them times 2^24, 2^48 ... too, until
-// nothing is left.
+// ------------------------------------------------ 16-bit rows: shared by the waves through LDS --
+// Eight waves share a stage of 64 tokens (32 of 512-byte rows): four groups of NC column tiles times two halves of the tokens, so a
+// workgroup takes up to 192 columns from one read of a row. Rows go straight into a ring of stages in LDS (global_load_lds, 16 bytes
+// to a lane, pieces XOR-swizzled by row), K is read as it lies, V through the transposing read; one barrier per stage. Against
+// rows that each wave loads into its own registers, where V has to be turned round by lane permutations and a wave has a SIMD
+// to itself (us, 16 000 tokens, bf16): 8 K/V heads of 128 with 192 columns each 99 -> 45, with 32 30.5 -> 27.9; 32 with 32 81.6 -> 65.7, with
+// 12 66.5 -> 64.9. Of the 36 us that 192 columns take, the matrix pipe is busy for 7.5 and the vector ALUs issue for 11; the rest is the
+// start (slots, then rows) and the end (12.8 MB of partial results), and the waits at the barriers. Half the waves a
+// phase behind the other half, so that one multiplies while the other takes exponentials, was no faster (45 us).
+// The maximum is followed when a score exceeds it by more than 2^8. bf16 probabilities are cut into two bf16 parts (off by at most
+// 2^-16 relative). fp16 ones, times 2^7 (so at most 2^15), into two fp16 parts: 22 bits of those down to 2^-10 of the largest, 16 down
+// to 2^-16; a step that has smaller ones multiplies what is left of them times 2^24, 2^48 ... too, until nothing is left.
 constexpr int kPtWaves = 8;
 constexpr float kPtRescaleStep = 8.f;  // log2 domain
 constexpr float kPtTwoParts = 16.f;    // two fp16 parts hold 16 bits of what is at least 2^-this
@@ -578,7 +479,7 @@ __global__ __launch_bounds__(kPtWaves * 64, 2) void decodePrefixTiledKernel(TaPr
   // (the second half's waves in the opposite order: waves i and i + 4 share a SIMD, and one of them may have a tile less)
   const int half = wave / COLUMN_WAVES, columnWave = half == 0 ? wave % COLUMN_WAVES : COLUMN_WAVES - 1 - wave % COLUMN_WAVES;
 
-  // grid as in decodePrefixKernel; tiles of columns are dealt out evenly, to the groups and to the waves of one: NC to a wave, or one
+  // grid as in decodePrefixFloatKernel; tiles of columns are dealt out evenly, to the groups and to the waves of one: NC to a wave, or one
   // less (16 001 tokens, 192 columns: 36 us with two groups of 6 tiles, 40 us with full groups, one of 8 and one of 4)
   const int f = blockIdx.x, idx = f >> 3;
   const int perKv = a.heads / a.kvHeads, columns = a.batch * perKv, tiles = (columns + 15) / 16, groups = x.groups;
@@ -751,7 +652,7 @@ __global__ __launch_bounds__(kPtWaves * 64, 2) void decodePrefixTiledKernel(TaPr
       if (!n.of[i]) keep[i >> 1] &= i & 1 ? 0xffffu : 0xffff0000u;
     return keep;
   };
-  // What two parts leave of probabilities below 2^-24 of the largest, times 2^24, 2^48 ... (the scores once more: keeping them for
+  // What two parts leave of probabilities, times 2^24, 2^48 ... (the scores once more: keeping them for
   // this would cost the registers of a column tile).
   auto addRest = [&](int stage, int at, bool all, auto columnTiles, auto withCare) {
     constexpr bool CAREFUL = decltype(withCare)::value;
@@ -987,7 +888,7 @@ __global__ __launch_bounds__(kPtWaves * 64, 2) void decodePrefixTiledKernel(TaPr
 template <typename T, int WAVES>
 __global__ __launch_bounds__(256) void decodePrefixMergeKernel(T* __restrict__ out, const float* __restrict__ shared, int nShared, const float* __restrict__ own,
                                                                int nOwn, int chunk, float raise, const void* bLen, bool len64, int maxLen, int64_t pairs, int heads, int d) {
-  constexpr int kBatch = 8, kMaxPerLane = 4, kPerLane = 8;  // d <= 256, at most 512 shares
+  constexpr int kBatch = 9, kMaxPerLane = 4, kPerLane = 8;  // d <= 256, at most 512 shares
   __shared__ float red[4][64 * kMaxPerLane];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, part = wave % WAVES;
   const int64_t pair = (int64_t)blockIdx.x * (4 / WAVES) + wave / WAVES;
@@ -1081,11 +982,11 @@ static diopiError_t launchTiled(hipStream_t stream, const TaPrefixArgs& x, int64
   return diopiSuccess;
 }
 
-template <typename T, int D, int NC>
-static diopiError_t launchPrefix(hipStream_t stream, const TaPrefixArgs& x, int64_t wgs, float* partial) {
-  const int lds = kPxWaves / 2 * NC * PxShape<T, D>::RUN * 64 * (int)sizeof(f32x4);
-  AMD_HIP(allowDynamicLds(reinterpret_cast<const void*>(decodePrefixKernel<T, D, NC>), lds));
-  hipLaunchKernelGGL((decodePrefixKernel<T, D, NC>), dim3((unsigned)wgs), dim3(kPxWaves * 64), lds, stream, x, partial);
+template <int D, int NC>
+static diopiError_t launchFloat(hipStream_t stream, const TaPrefixArgs& x, int64_t wgs, float* partial) {
+  const int lds = kPxWaves / 2 * NC * PxShape<D>::RUN * 64 * (int)sizeof(f32x4);
+  AMD_HIP(allowDynamicLds(reinterpret_cast<const void*>(decodePrefixFloatKernel<D, NC>), lds));
+  hipLaunchKernelGGL((decodePrefixFloatKernel<D, NC>), dim3((unsigned)wgs), dim3(kPxWaves * 64), lds, stream, x, partial);
   AMD_LAUNCH_CHECK();
   return diopiSuccess;
 }
@@ -1095,38 +996,33 @@ static diopiError_t decodeSharedPrefix(diopiContextHandle_t ctx, hipStream_t str
   const int64_t perKv = a.heads / a.kvHeads, columns = a.batch * perKv, cus = computeUnits(), itemsize = dtypeSize(dtype);
   const int D = a.d <= 64 ? 64 : a.d <= 128 ? 128 : 256;
   x.kStride = (unsigned)(a.kSlotStride * itemsize), x.vStride = (unsigned)(a.vSlotStride * itemsize);
-  const int64_t rowBytes = D * itemsize;
-  const bool tiled = itemsize == 2 && columns > 32;
-  const int64_t tiles = ceilDiv(columns, 16), columnWaves = D == 256 ? PtShape<half_t, 256>::COLUMN_WAVES : PtShape<half_t, 128>::COLUMN_WAVES;
-  const int ncMost = tiled ? (D == 256 ? 1 : D == 128 ? 2 : 3) : columns <= 32 || rowBytes > 256 ? 1 : 2;  // (more spill registers)
+  const bool tiled = itemsize == 2;
+  const int64_t pairs = (int64_t)a.batch * a.heads, tiles = ceilDiv(columns, 16);
+  const int64_t columnWaves = !tiled ? 1 : D == 256 ? PtShape<half_t, 256>::COLUMN_WAVES : PtShape<half_t, 128>::COLUMN_WAVES;
+  const int ncMost = tiled ? (D == 256 ? 1 : D == 128 ? 2 : 3) : columns > 16 && D == 64 ? 2 : 1;  // (more spill registers)
+  // The shortest chunk. Short ones keep more compute units busy, but every pair (sequence, head) has a partial result for each of
+  // them, so it is 64 tokens while that leaves 32 of them for up to 128 pairs and fewer for more, 4 from 1024 on, and longer then,
+  // up to 256. Heads of 128, us with this rule and with 256: 250 tokens, 32 heads, 16 sequences 14.2, 16.2, 500 14.6, 16.6; 8 on 1, 4
+  // sequences, 2000 tokens 15.6, 17.9; 32 on 8, 48 sequences, 250 tokens 17.5, 20.8, 500 18.6, 20.6. With 64 for any number of pairs the
+  // last of these would take 23.3 and 2000 tokens 30.8 instead of 21.6.
+  const int64_t most = std::min<int64_t>(32, std::max<int64_t>(4, 4096 / pairs));
+  const int64_t shortest = std::min<int64_t>(256, std::max<int64_t>(64, ceilDiv(x.len, most)));
   // Few groups of columns read a row least often, but where they and chunks as short as pays leave compute units without work, more
   // take it (8 K/V heads of 64, 192 columns each: 700 tokens 17.0 us, with the fewest groups 22.5; 4096 tokens 24 and 28 us).
-  const int64_t shortest = tiled ? 256 : 128, fewest = ceilDiv(tiles, tiled ? columnWaves * ncMost : ncMost);
-  const int64_t groups = tiled ? std::max(fewest, std::min(ceilDiv(tiles, columnWaves), cus / (a.kvHeads * ceilDiv(x.len, shortest)))) : fewest;
-  const int nc = tiled ? (int)ceilDiv(ceilDiv(tiles, groups), columnWaves) : ncMost;
+  const int64_t fewest = ceilDiv(tiles, columnWaves * ncMost);
+  const int64_t groups = std::max(fewest, std::min(ceilDiv(tiles, columnWaves), cus / (a.kvHeads * ceilDiv(x.len, shortest))));
+  const int nc = (int)ceilDiv(ceilDiv(tiles, groups), columnWaves);
   x.groups = (int)groups;
-  const int64_t step = tiled ? (D == 256 ? 32 : 64) : kPxWaves * (itemsize == 4 ? 16 : 32);
-  // Chunks below the share of a compute unit end where a workgroup's few steps no longer pay for its start and its partial results:
-  // 777 tokens, 8 heads of 64, batch 5 take 17.0 us with 128 and with 64, 18.8 us with 256; 4096 tokens, 8 K/V heads with 64 columns each,
-  // where a step of all waves is 64 tokens, take 22 us with 256, 25 us with 128.
-  const int64_t chunk = std::max<int64_t>(shortest, ceilDiv(x.len * a.kvHeads * groups, cus));
-  x.chunk = (int)(ceilDiv(std::max(chunk, ceilDiv(x.len, kPxMaxSplit)), step) * step);
+  const int64_t step = tiled && D == 256 ? 32 : 64;  // of all waves
+  const int64_t chunk = std::max({shortest, ceilDiv((int64_t)x.len * a.kvHeads * groups, cus), ceilDiv(x.len, kPxMaxSplit)});
+  x.chunk = (int)(ceilDiv(chunk, step) * step);
   x.nsplit = (int)ceilDiv(x.len, x.chunk);
-  const int64_t pairs = (int64_t)a.batch * a.heads, wgs = ceilDiv((int64_t)a.kvHeads * x.nsplit, 8) * 8 * groups;
+  const int64_t wgs = ceilDiv((int64_t)a.kvHeads * x.nsplit, 8) * 8 * groups;
   // (fewer than 2^32 threads to a launch)
   AMD_CHECK(wgs < 1 << 23 && pairs < 1 << 24, "shared prefix attention: %d sequences of %d heads exceed the grid limits", a.batch, a.heads);
   void* ws = nullptr;
   AMD_TRY(requireWorkspace(ctx, pairs * x.nsplit * (2 + a.d) * (int64_t)sizeof(float), &ws));
   float* partial = static_cast<float*>(ws);
-#define PREFIX_CALL(T, SIZE, N) AMD_TRY((launchPrefix<T, SIZE, N>(stream, x, wgs, partial)))
-#define PREFIX_COLUMNS(T, SIZE) \
-  do { if (nc == 1) PREFIX_CALL(T, SIZE, 1); else PREFIX_CALL(T, SIZE, 2); } while (0)
-#define PREFIX_SIZES(T)                       \
-  do {                                        \
-    if (D == 64) PREFIX_CALL(T, 64, 1);       \
-    else if (D == 128) PREFIX_CALL(T, 128, 1); \
-    else PREFIX_CALL(T, 256, 1);              \
-  } while (0)
 #define TILED_CALL(T, SIZE, N) AMD_TRY((launchTiled<T, SIZE, N>(stream, x, wgs, partial)))
 #define TILED_COLUMNS(T, SIZE) \
   do { if (nc == 1) TILED_CALL(T, SIZE, 1); else TILED_CALL(T, SIZE, 2); } while (0)
@@ -1140,24 +1036,21 @@ static diopiError_t decodeSharedPrefix(diopiContextHandle_t ctx, hipStream_t str
   if (tiled) {
     if (dtype == diopi_dtype_bfloat16) TILED_SIZES(bf16_t);
     else TILED_SIZES(half_t);
-  } else if (dtype == diopi_dtype_bfloat16) {
-    PREFIX_SIZES(bf16_t);
-  } else if (dtype == diopi_dtype_float16) {
-    PREFIX_SIZES(half_t);
   } else if (D == 64) {
-    PREFIX_COLUMNS(float, 64);
+    AMD_TRY((nc == 1 ? launchFloat<64, 1> : launchFloat<64, 2>)(stream, x, wgs, partial));
   } else {
-    PREFIX_CALL(float, 128, 1);
+    AMD_TRY((launchFloat<128, 1>(stream, x, wgs, partial)));
   }
 #undef TILED_SIZES
 #undef TILED_COLUMNS
 #undef TILED_CALL
-#undef PREFIX_SIZES
-#undef PREFIX_COLUMNS
-#undef PREFIX_CALL
   TaPartials own{nullptr, 0, 1, 0.f};
   if (a.maxLen > 0) AMD_TRY(decodePartials(ctx, stream, a, dtype, a.maxLen, &own));
-  const bool narrow = x.nsplit + own.nsplit <= 16;
+  // A wave has the elements of nine shares on their way at once. Up to those it needs no help; twice as many are still better left to
+  // one than to four where there are many pairs: 2048 pairs, 10 shares 23.7 us (all three launches) and 27.3; 512 pairs, 18 shares
+  // 18.9 and 17.5.
+  const int shares = x.nsplit + own.nsplit;
+  const bool narrow = shares <= 9 || (shares <= 18 && pairs >= 1024);
 #define PREFIX_MERGE(T)                                                                                                                          \
   do {                                                                                                                                           \
     if (narrow)                                                                                                                                  \
