@@ -494,22 +494,22 @@ static diopiError_t int8Pool(const char* name, const TensorView& q, const Tensor
 // gets one of them where there are few (its step takes 0.5 us, whoever waits for rows does nothing else), and up to 16 where
 // there are many (what a workgroup does before its first step, and its partial results, are then spread over more). With four
 // heads to a workgroup a wave reads 512 adjacent bytes of a token with the other three, and one lane the scales of all four: 64 x
-// (512 .. 4096) tokens, 32 heads of 128, 241 us, with one head 378 (48, 8 heads 61 and 73). Few steps are better dealt over the
-// waves of a head: 1 x 1777 tokens, 8 heads, one step to a wave, 10.2 with one head, 11.5 with four.
-// us at 1, 2, 4, 8, 16 steps to a wave: 1 x 4096, 8 heads 10.7, 11.7, 13.6, 17.6, 24.6; 1 x 8192 14.2, 13.6, 15.2, 17.9, 25.0; 1 x 16384
-// 23.9, 21.4, 18.7, 19.5, 25.2; 8 x 4096 -, -, 23.2, 20.8, 25.7; 16 x (1000 .. 8000) -, -, 52, 44, 47; 48 x (512 .. 4096) -, -, 74, 61, 73;
-// 32 heads, 64 x (512 .. 4096) -, -, 309, 261, 241. Heads of 256: a SIMD holds one wave instead of three, and a step takes twice as long: 16 x (512 ..
-// 4096), 8 heads -, -, 61, 57, 45.
+// (512 .. 4096) tokens, 32 heads of 128, 231 us, with one head 383 (48, 8 heads 59 and 87). Few steps are better dealt over the
+// waves of a head: 1 x 1777 tokens, 8 heads, one step to a wave, 10.3 with one head, 11.4 with four.
+// us at 1, 2, 4, 8, 16 steps to a wave: 1 x 4096, 8 heads 10.6, 11.3, 13.6, 18.0, 25.1; 1 x 8192 14.2, 13.2, 15.2, 18.5, 25.5; 1 x 16384
+// 25.3, 20.0, 18.5, 19.4, 25.7; 8 x 4096 37, 28, 22.7, 20.7, 26.2; 16 x (1000 .. 8000) 84, 58, 48, 47, 47; 48 x (512 .. 4096) 120, 82, 69, 59, 72;
+// 32 heads, 64 x (512 .. 4096) 627, 385, 297, 247, 231. Heads of 256: a SIMD holds one wave instead of three, and a step takes twice as
+// long: 16 x (512 .. 4096), 8 heads 105, 71, 60, 56, 45.
 static void chooseShares(TaInt8Args* x, int64_t len, int D) {
   TaArgs& a = x->a;
   const int64_t steps = (int64_t)a.kvHeads * a.qGroups * a.batch * ceilDiv(len, kI8Tile) * (D == 256 ? 4 : 1);
   const int perWave = steps < 1536 ? 1 : steps < 3072 ? 2 : steps < 6144 ? 4 : steps < 57344 ? 8 : 16;
-  // (heads in twos and fours leave waves without a head: of 5 in fours 3, 70 us where twos take 66)
+  // (heads in twos and fours leave waves without a head: of 5 in fours 3, 74 us where twos take 68)
   const int fits = a.kvHeads % 4 == 0 || a.kvHeads == 3 || a.kvHeads > 8 ? 4 : a.kvHeads >= 2 ? 2 : 1;
   x->headsPerWg = std::min(fits, perWave);
   int64_t tokens = (int64_t)perWave * kI8Tile * kI8Waves / x->headsPerWg;
-  // short sequences in one chunk, without the launch that merges: 16 x (1 .. 300), 8 heads of 64, 9.6 -> 8.0; 64 x (100 .. 500), 32 heads
-  // 41.6 -> 39.8
+  // short sequences in one chunk, without the launch that merges: 16 x (1 .. 300), 8 heads of 64, 9.6 -> 7.6; 64 x (100 .. 500), 32 heads
+  // 42.5 -> 40.4
   if (len <= kI8Block && perWave >= 8) {
     tokens = len;
   } else if (len <= 384 && a.batch >= 8) {
