@@ -110,7 +110,8 @@ constexpr int splitWavesPerSimd(size_t itemsize, int lpt, bool hiw, int mode, in
 // in memory (the two-call modes). QPK: query heads that share this workgroup's K/V head and are all served from one read
 // of its rows (grouped-query layouts; 1 otherwise). With QPK > 1 the grid is one-dimensional and decoded so that the
 // workgroups that share a K/V head's rows run next to each other on one XCD.
-template <typename T, int LPT, bool HIW, int MODE = kTaFused, typename LT = float, int QPK = 1, bool PART = false>
+// BEHIND: the states begin with the partial results a.shared instead of empty (fused, one chunk).
+template <typename T, int LPT, bool HIW, int MODE = kTaFused, typename LT = float, int QPK = 1, bool PART = false, bool BEHIND = false>
 __global__ __launch_bounds__(kTaWaves * 64, splitWavesPerSimd(sizeof(T), LPT, HIW, MODE, QPK, PART)) void decodeSplitKernel(TaArgs a, T* __restrict__ out,
                                                                      float* __restrict__ partial) {
   static_assert(QPK == 1 || !HIW, "several query heads per lane group: the lane groups of a wave take tokens, not heads");
@@ -230,6 +231,17 @@ __global__ __launch_bounds__(kTaWaves * 64, splitWavesPerSimd(sizeof(T), LPT, HI
     m[j] = -INFINITY, l[j] = 0.f;
 #pragma unroll
     for (int e = 0; e < N; ++e) acc[j][e] = 0.f;
+  }
+  if constexpr (BEHIND) {
+    for (int s = HIW ? wave : wave * TPW + grp; s < a.nShared; s += HIW ? kTaWaves : kTaWaves * TPW)
+#pragma unroll
+      for (int j = 0; j < QPK; ++j) {
+        const float* row = a.shared + (((int64_t)b * a.heads + h + headOf(j)) * a.nShared + s) * (2 + a.d);
+        float acc2[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) acc2[e] = live ? row[2 + sub * N + e] : 0.f;
+        mergeState<N>(m[j], l[j], acc[j], row[0], row[1], acc2);
+      }
   }
 
   constexpr int TPI = HIW ? 1 : TPW;  // tokens per wave-wide load
@@ -478,7 +490,8 @@ __device__ __forceinline__ void waitLoadsBut() {  // all but the wave's N younge
 // them for the VALU: second half in bf16 2 - 5 % less. Fused rows of 256 need more than half the registers.)
 // D: head size the rows are laid out for (64, 128, 256); a.d is any multiple of 8 up to it: the pieces past the row's end
 // repeat its first one, meet zeros of q, and give output columns that are not stored.
-template <typename T, int D, int MODE, typename LT>
+// BEHIND: the partial results a.shared are merged with the chunk's at the end (fused, one chunk).
+template <typename T, int D, int MODE, typename LT, bool BEHIND = false>
 __global__ __launch_bounds__(kGqWaves * 64, MODE == kTaFused && D == 256 ? 1 : kGqWgsPerCu) void decodeGroupedKernel(TaArgs a, T* __restrict__ out, float* __restrict__ partial) {
   using M = GqMfma<T>;
   using Frag = typename M::Frag;
@@ -798,6 +811,37 @@ walk:
       const f32x4 v = *reinterpret_cast<const f32x4*>(red + (k * nq + j) * kRedRow + e);
 #pragma unroll
       for (int c = 0; c < 4; ++c) o[c] += v[c] * w[k];
+    }
+    if constexpr (BEHIND) {
+      constexpr int kBatch = 8;  // shares whose numbers are on their way at once
+      const float* const rows = a.shared + ((int64_t)b * a.heads + h + j) * a.nShared * (2 + a.d);
+      mAll -= M::kRaise;
+      for (int s0 = 0; s0 < a.nShared; s0 += kBatch) {
+        float2 ml[kBatch], v[kBatch][2];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+          const float* row = rows + min(s0 + k, a.nShared - 1) * (2 + a.d);
+          ml[k] = *reinterpret_cast<const float2*>(row);
+          v[k][0] = *reinterpret_cast<const float2*>(row + 2 + e), v[k][1] = *reinterpret_cast<const float2*>(row + 4 + e);
+        }
+        float next = mAll;
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+          if (s0 + k >= a.nShared) ml[k].x = -INFINITY;
+          next = fmaxf(next, ml[k].x);
+        }
+        const float keep = mAll == -INFINITY ? 0.f : exp2f(mAll - next);
+        mAll = next, lAll *= keep;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[c] *= keep;
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+          const float wk = exp2f(ml[k].x - next);
+          if (ml[k].x == -INFINITY) continue;
+          lAll += ml[k].y * wk;
+          o[0] += v[k][0].x * wk, o[1] += v[k][0].y * wk, o[2] += v[k][1].x * wk, o[3] += v[k][1].y * wk;
+        }
+      }
     }
     if (a.nsplit == 1) {
       const float inv = lAll > 0.f ? 1.f / lAll : 0.f;
@@ -1322,8 +1366,10 @@ static bool lanesPay(int64_t perKv, int64_t kvHeads, bool wholeLoads, bool partR
   return wide && perKv > 6 && (many(256, 0, 32) || many(512, 16, 64));
 }
 
-// staticScratch: partial results go to the library's own device array instead of workspace from the context. keep: the partial
-// results are not merged but left to the caller.
+constexpr int kTaMostShared = 32;
+
+// staticScratch: partial results go to the library's own device array instead of workspace from the context. keep: more than one
+// chunk's partial results are not merged but left to the caller, and one chunk begins with those in a.shared (then *keep is empty).
 // Launches decodeSplitKernel or decodeGroupedKernel in one mode over (head groups, chunks, sequences) and, for the modes that produce
 // the attention output, merges the chunks. scoresF32: the stored scores of the two-call modes are float32 (else T).
 template <int MODE>
@@ -1348,7 +1394,10 @@ static diopiError_t streamChunks(diopiContextHandle_t ctx, hipStream_t stream, T
   const int groupsPerSeq = qpk > 1 ? a.kvHeads * a.qGroups : (hiw ? a.heads / tpw : a.heads);
   chooseChunk(&a, groupsPerSeq, batch, maxInputLen, grouped, MODE == kTaFused && bytes == 256, MODE != kTaLogitsOut);
   a.nsplit = (int)std::max<int64_t>(1, ceilDiv(maxInputLen, a.chunk));
-  if (keep) a.nsplit = std::max(a.nsplit, 2);  // (one share is written as the result: a second one, without tokens, makes it a partial result)
+  // (one chunk and up to 32 shares of other tokens, us: 4 x (1 .. 20) own tokens of 8 heads of 64, 13, 31 and 32 shares 13.8 -> 10.6, 13.9 -> 12.0,
+  // 17.0 -> 15.6; 48 x (10 .. 300), 32 heads of 128 on 8, 16 shares 36.5 -> 31.1)
+  const bool behind = keep && a.nsplit == 1 && a.nShared <= kTaMostShared;
+  if (keep && !behind) a.nsplit = std::max(a.nsplit, 2);  // (one share is written as the result: a second one, without tokens, makes it a partial result)
   AMD_CHECK(batch <= 65535 && a.nsplit <= 65535, "token attention: batch %ld / splits %d exceed the grid limits", (long)batch,
             a.nsplit);
   float* partial = nullptr;
@@ -1377,17 +1426,19 @@ static diopiError_t streamChunks(diopiContextHandle_t ctx, hipStream_t stream, T
   if (grouped) {
     const int mats = MODE == kTaFused ? 2 : 1, d = (int)(bytes / 2);
     const int lds = gqRingBytes(d, mats) + (MODE == kTaFused ? 0 : kGqWaves * std::min(perKv, kGqHeads) * kGqScoreRow * (int)sizeof(float));
-#define GROUPED_CALL_AS(T, D, LT)                                                                                               \
-  do {                                                                                                                          \
-    AMD_HIP(allowDynamicLds(reinterpret_cast<const void*>(decodeGroupedKernel<T, D, MODE, LT>), lds));                           \
-    hipLaunchKernelGGL((decodeGroupedKernel<T, D, MODE, LT>), grid, dim3(kGqWaves * 64), lds, stream, a, static_cast<T*>(outPtr), \
-                       partial);                                                                                                \
+#define GROUPED_CALL_AS(T, D, LT, BEHIND)                                                                                                \
+  do {                                                                                                                                   \
+    AMD_HIP(allowDynamicLds(reinterpret_cast<const void*>(decodeGroupedKernel<T, D, MODE, LT, BEHIND>), lds));                            \
+    hipLaunchKernelGGL((decodeGroupedKernel<T, D, MODE, LT, BEHIND>), grid, dim3(kGqWaves * 64), lds, stream, a, static_cast<T*>(outPtr), \
+                       partial);                                                                                                         \
   } while (0)
 #define GROUPED_CALL(T, D)                          \
-  if (MODE == kTaFused || scoresF32) {              \
-    GROUPED_CALL_AS(T, D, float);                   \
+  if (behind) {                                     \
+    if constexpr (MODE == kTaFused) GROUPED_CALL_AS(T, D, float, true); \
+  } else if (MODE == kTaFused || scoresF32) {       \
+    GROUPED_CALL_AS(T, D, float, false);            \
   } else {                                          \
-    GROUPED_CALL_AS(T, D, T);                       \
+    GROUPED_CALL_AS(T, D, T, false);                \
   }
 #define GROUPED_SIZES(T) \
   if (d == 64) { GROUPED_CALL(T, 64) } else if (d == 128) { GROUPED_CALL(T, 128) } else { GROUPED_CALL(T, 256) }
@@ -1396,22 +1447,24 @@ static diopiError_t streamChunks(diopiContextHandle_t ctx, hipStream_t stream, T
 #undef GROUPED_CALL
 #undef GROUPED_CALL_AS
   } else {
-#define STREAM_CALL_PART(T, LPT, LT, PART)                                                                                           \
-  if (qpk == 4) hipLaunchKernelGGL((decodeSplitKernel<T, LPT, false, MODE, LT, 4, PART>), grid, block, 0, stream, a, static_cast<T*>(outPtr), partial); \
-  else if (qpk == 2) hipLaunchKernelGGL((decodeSplitKernel<T, LPT, false, MODE, LT, 2, PART>), grid, block, 0, stream, a, static_cast<T*>(outPtr), partial); \
-  else if (hiw) hipLaunchKernelGGL((decodeSplitKernel<T, LPT, true, kTaFused, float, 1, PART>), grid, block, 0, stream, a, static_cast<T*>(outPtr), partial); \
-  else hipLaunchKernelGGL((decodeSplitKernel<T, LPT, false, MODE, LT, 1, PART>), grid, block, 0, stream, a, static_cast<T*>(outPtr), partial)
-#define STREAM_CALL_AS(T, LPT, LT)            \
+#define STREAM_CALL_PART(T, LPT, LT, PART, BEHIND)                                                                                           \
+  if (qpk == 4) hipLaunchKernelGGL((decodeSplitKernel<T, LPT, false, MODE, LT, 4, PART, BEHIND>), grid, block, 0, stream, a, static_cast<T*>(outPtr), partial); \
+  else if (qpk == 2) hipLaunchKernelGGL((decodeSplitKernel<T, LPT, false, MODE, LT, 2, PART, BEHIND>), grid, block, 0, stream, a, static_cast<T*>(outPtr), partial); \
+  else if (hiw) hipLaunchKernelGGL((decodeSplitKernel<T, LPT, true, kTaFused, float, 1, PART, BEHIND>), grid, block, 0, stream, a, static_cast<T*>(outPtr), partial); \
+  else hipLaunchKernelGGL((decodeSplitKernel<T, LPT, false, MODE, LT, 1, PART, BEHIND>), grid, block, 0, stream, a, static_cast<T*>(outPtr), partial)
+#define STREAM_CALL_AS(T, LPT, LT, BEHIND)    \
   if (partRows) {                             \
-    STREAM_CALL_PART(T, LPT, LT, true);       \
+    STREAM_CALL_PART(T, LPT, LT, true, BEHIND);  \
   } else {                                    \
-    STREAM_CALL_PART(T, LPT, LT, false);      \
+    STREAM_CALL_PART(T, LPT, LT, false, BEHIND); \
   }
 #define STREAM_CALL(T, LPT)                                                  \
-  if (MODE == kTaFused || scoresF32) {                                       \
-    STREAM_CALL_AS(T, LPT, float);                                           \
+  if (behind) {                                                              \
+    if constexpr (MODE == kTaFused) { STREAM_CALL_AS(T, LPT, float, true); } \
+  } else if (MODE == kTaFused || scoresF32) {                                \
+    STREAM_CALL_AS(T, LPT, float, false);                                    \
   } else if constexpr (sizeof(T) == 2) { /* (of fp32 rows they are fp32) */  \
-    STREAM_CALL_AS(T, LPT, T);                                               \
+    STREAM_CALL_AS(T, LPT, T, false);                                        \
   }
     TA_DISPATCH(dtype, bytes, STREAM_CALL);
 #undef STREAM_CALL
@@ -1421,14 +1474,14 @@ static diopiError_t streamChunks(diopiContextHandle_t ctx, hipStream_t stream, T
   AMD_LAUNCH_CHECK();
   if (MODE == kTaLogitsOut) return diopiSuccess;
   if (keep) {
-    *keep = TaPartials{partial, a.nsplit, a.chunk, grouped && dtype == diopi_dtype_float16 ? GqMfma<half_t>::kRaise : 0.f};
+    *keep = TaPartials{partial, behind ? 0 : a.nsplit, a.chunk, grouped && dtype == diopi_dtype_float16 ? GqMfma<half_t>::kRaise : 0.f};
     return diopiSuccess;
   }
   return a.nsplit > 1 ? mergeChunks(stream, dtype, outPtr, partial, a, batch) : diopiSuccess;
 }
 
-diopiError_t amd::decodePartials(diopiContextHandle_t ctx, hipStream_t stream, const TaArgs& a, diopiDtype_t dtype, int maxInputLen, TaPartials* keep) {
-  return streamChunks<kTaFused>(ctx, stream, a, dtype, a.d * dtypeSize(dtype), a.batch, maxInputLen, nullptr, true, false, nullptr, keep);
+diopiError_t amd::decodePartials(diopiContextHandle_t ctx, hipStream_t stream, const TaArgs& a, diopiDtype_t dtype, int maxInputLen, void* out, TaPartials* keep) {
+  return streamChunks<kTaFused>(ctx, stream, a, dtype, a.d * dtypeSize(dtype), a.batch, maxInputLen, out, true, false, nullptr, keep);
 }
 
 static diopiError_t decodeAttention(diopiContextHandle_t ctx, diopiTensorHandle_t outH, diopiConstTensorHandle_t qH,

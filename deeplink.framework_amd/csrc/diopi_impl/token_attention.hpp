@@ -33,6 +33,8 @@ struct TaArgs {
   int64_t logitsHeadStride;
   int qGroups;  // grouped-query layouts: workgroups that share the query heads of one K/V head between them
   int batch;    // sequences (the grouped-query kernels decode a one-dimensional grid)
+  const float* shared;  // decodePartials: partial results [batch, heads, nShared, 2 + d] of other tokens of the sequences, as in mergeChunks
+  int nShared;
 };
 
 // max / sum of one value per thread over the workgroup of 256 (red: 4 floats of LDS; two barriers)
@@ -67,13 +69,14 @@ diopiError_t fillArgs(const TaViews& t, bool needK, bool needV, int maxLen, TaAr
 // units of log2), sum and weighted sum of V, chunk i written where i = 0 or a sequence has more than i * chunk tokens.
 diopiError_t mergeChunks(hipStream_t stream, diopiDtype_t dtype, void* out, const float* partial, const TaArgs& a, int64_t batch);
 
-// The partial results that mergeChunks merges, of diopiTokenDecodeAttentionInference's kernels (not of generic arguments), in
-// workspace of the context: at least two chunks.
+// diopiTokenDecodeAttentionInference's kernels (not for generic arguments) behind other tokens, whose partial results are in a.shared.
+// Sequences of one chunk: the result, in `out` (*keep is empty). Longer ones, or where a.shared has too many shares for that: partial results
+// of at least two chunks, which mergeChunks could merge, in workspace of the context.
 struct TaPartials {
   const float* partial;
   int nsplit, chunk;
   float raise;  // sums are against the maximum less this (in units of log2)
 };
-diopiError_t decodePartials(diopiContextHandle_t ctx, hipStream_t stream, const TaArgs& a, diopiDtype_t dtype, int maxInputLen, TaPartials* keep);
+diopiError_t decodePartials(diopiContextHandle_t ctx, hipStream_t stream, const TaArgs& a, diopiDtype_t dtype, int maxInputLen, void* out, TaPartials* keep);
 
 }  // namespace amd

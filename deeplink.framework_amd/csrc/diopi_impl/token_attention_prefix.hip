@@ -1045,7 +1045,9 @@ static diopiError_t decodeSharedPrefix(diopiContextHandle_t ctx, hipStream_t str
 #undef TILED_COLUMNS
 #undef TILED_CALL
   TaPartials own{nullptr, 0, 1, 0.f};
-  if (a.maxLen > 0) AMD_TRY(decodePartials(ctx, stream, a, dtype, a.maxLen, &own));
+  a.shared = partial, a.nShared = x.nsplit;
+  AMD_TRY(decodePartials(ctx, stream, a, dtype, a.maxLen, out, &own));
+  if (own.nsplit == 0) return diopiSuccess;
   // A wave has the elements of nine shares on their way at once. Up to those it needs no help; twice as many are still better left to
   // one than to four where there are many pairs: 2048 pairs, 10 shares 23.7 us (all three launches) and 27.3; 512 pairs, 18 shares
   // 18.9 and 17.5.

@@ -64,6 +64,26 @@ def test_any_number_of_columns(ops, dev, dtype, d):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,d", [(2, 2, 64), (1, 1, 128), (4, 4, 80), (6, 2, 128), (5, 1, 256), (7, 1, 72), (18, 1, 64), (3, 3, 96)])
+def test_one_to_many_shares_of_the_prefix(ops, dev, dtype, heads, kv_heads, d):
+    for prefix in (1, 65, 129, 500, 577, 1000, 2048, 2049, 2113, 4500):   # in shares of 64 or so: up to 32 begin the walk over the own tokens, more are merged
+        check(ops, dev, *batch_of(prefix, [3, 0, 20], heads, kv_heads, d, dtype, 300 + prefix))
+    check(ops, dev, *batch_of(700, [0, 0], heads, kv_heads, d, dtype, 299, spare=0)[:-1], 0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv_heads", [(2, 2), (4, 1)])
+def test_shares_without_a_token_that_counts(ops, dev, dtype, heads, kv_heads):
+    q, k, v, prefix, b_loc, lens, max_len = batch_of(640, [3, 0, 20], heads, kv_heads, 64, dtype, 310)
+    for begin, end in ((0, 64), (64, 200), (0, 640)):                # the first share, one between others, all of them
+        some = prefix.clone()
+        some[begin:end] = -1
+        got = run(ops, dev, q, k, v, some, b_loc, lens, max_len)
+        want, bound = oracle.attend(q, k, v, own_and_shared(some[some >= 0], b_loc, lens, max_len), PART[q.dtype])
+        oracle.assert_within(got, want, bound)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_a_long_prefix_and_long_sequences(ops, dev, dtype):
     check(ops, dev, *batch_of(6001, [1, 700, 30], 4, 2, 128, dtype, 30))
     check(ops, dev, *batch_of(2049, [2600, 1], 2, 2, 64, dtype, 31))
