@@ -83,10 +83,11 @@ __global__ __launch_bounds__(256) void decodePrefixAnyKernel(TaPrefixArgs x, T* 
 // The shared tokens see the same K and V from every sequence, so a K/V head's columns are the query heads that share it of ALL
 // sequences: S^T = K . Q^T and O^T += V^T . P^T with many columns for one read of a row. Partial results (maximum, sum, weighted
 // sum of V) of each chunk of the prefix go to workspace; those of the sequences' own tokens come from the kernels of
-// diopiTokenDecodeAttentionInference, and a last launch merges both.
+// diopiTokenDecodeAttentionInference, which end on the shared tokens' where the own ones are one chunk; a last launch merges the partial
+// results of both where they are more.
 //
 // Long prefixes are bound by memory, every shared row read once (for each group of columns), and, with many columns, by the matrix
-// pipe and the exponentials; short ones by the three launches and the latency of slots, then rows.
+// pipe and the exponentials; short ones by the launches and the latency of slots, then rows.
 //
 // ------------------------------------------------ fp32 --
 // Rows go from the pool into the registers that the products (16x16x4) read, whole 128-byte lines of 8 rows in a load: K as in
@@ -96,7 +97,7 @@ __global__ __launch_bounds__(256) void decodePrefixAnyKernel(TaPrefixArgs x, T* 
 //     probabilities that are zero leave sums that are not finite, and the wave then walks again with care: rows that do not count
 //     are zeros, what is not finite meets a one for each probability that is not zero.
 // Four waves share a chunk's tokens and meet in LDS, a lane always adding to what is its own. 16 000 tokens, 32 heads of 128, 24
-// sequences: 136 us, 3.9 TB/s; two tiles of columns share a read with heads of 64 (with 128 that takes more registers than there are).
+// sequences: 132 us, 4.0 TB/s; two tiles of columns share a read with heads of 64 (with 128 that takes more registers than there are).
 constexpr int kPxWaves = 4;
 constexpr int kPxBlock = 2048;    // tokens whose slots a workgroup holds in LDS at once
 constexpr int kPxMaxSplit = 256;  // chunks of the prefix
@@ -395,7 +396,7 @@ __global__ __launch_bounds__(kPxWaves * 64, 1) void decodePrefixFloatKernel(TaPr
 // to a lane, pieces XOR-swizzled by row), K is read as it lies, V through the transposing read; one barrier per stage. Against
 // rows that each wave loads into its own registers, where V has to be turned round by lane permutations and a wave has a SIMD
 // to itself (us, 16 000 tokens, bf16): 8 K/V heads of 128 with 192 columns each 99 -> 45, with 32 30.5 -> 27.9; 32 with 32 81.6 -> 65.7, with
-// 12 66.5 -> 64.9. Of the 36 us that 192 columns take, the matrix pipe is busy for 7.5 and the vector ALUs issue for 11; the rest is the
+// 12 66.5 -> 64.9 (5 us of each for a launch that merged them, which these no longer need). Of the 36 us that 192 columns take, the matrix pipe is busy for 7.5 and the vector ALUs issue for 11; the rest is the
 // start (slots, then rows) and the end (12.8 MB of partial results), and the waits at the barriers. Half the waves a
 // phase behind the other half, so that one multiplies while the other takes exponentials, was no faster (45 us).
 // The maximum is followed when a score exceeds it by more than 2^8. bf16 probabilities are cut into two bf16 parts (off by at most
@@ -1001,14 +1002,14 @@ static diopiError_t decodeSharedPrefix(diopiContextHandle_t ctx, hipStream_t str
   const int64_t columnWaves = !tiled ? 1 : D == 256 ? PtShape<half_t, 256>::COLUMN_WAVES : PtShape<half_t, 128>::COLUMN_WAVES;
   const int ncMost = tiled ? (D == 256 ? 1 : D == 128 ? 2 : 3) : columns > 16 && D == 64 ? 2 : 1;  // (more spill registers)
   // The shortest chunk. Short ones keep more compute units busy, but every pair (sequence, head) has a partial result for each of
-  // them, so it is 64 tokens while that leaves 32 of them for up to 128 pairs and fewer for more, 4 from 1024 on, and longer then,
-  // up to 256. Heads of 128, us with this rule and with 256: 250 tokens, 32 heads, 16 sequences 14.2, 16.2, 500 14.6, 16.6; 8 on 1, 4
-  // sequences, 2000 tokens 15.6, 17.9; 32 on 8, 48 sequences, 250 tokens 17.5, 20.8, 500 18.6, 20.6. With 64 for any number of pairs the
-  // last of these would take 23.3 and 2000 tokens 30.8 instead of 21.6.
-  const int64_t most = std::min<int64_t>(32, std::max<int64_t>(4, 4096 / pairs));
+  // them, so it is 64 tokens while that leaves 16 of them for up to 256 pairs and fewer for more, 4 from 1024 on, and longer then,
+  // up to 256. Heads of 128, us with this rule and with 256: 250 tokens, 32 heads, 16 sequences 10.0, 12.0, 500 11.1, 12.2; 32 on 8,
+  // 48 sequences, 250 tokens 12.8, 15.9, 500 13.9, 15.8; with 64 for any number of pairs 2000 tokens would take the last 19.6, so 17.1. 32
+  // chunks for few pairs: 4 sequences, 2000 tokens, 8 heads on 1 15.4, so 13.9; 32 on 8 14.1, so 13.1.
+  const int64_t most = std::min<int64_t>(16, std::max<int64_t>(4, 4096 / pairs));
   const int64_t shortest = std::min<int64_t>(256, std::max<int64_t>(64, ceilDiv(x.len, most)));
   // Few groups of columns read a row least often, but where they and chunks as short as pays leave compute units without work, more
-  // take it (8 K/V heads of 64, 192 columns each: 700 tokens 17.0 us, with the fewest groups 22.5; 4096 tokens 24 and 28 us).
+  // take it (8 K/V heads of 64, 192 columns each: 700 tokens 12.0 us, with the fewest groups 16.6; 4096 tokens 16.7 and 20.9 us).
   const int64_t fewest = ceilDiv(tiles, columnWaves * ncMost);
   const int64_t groups = std::max(fewest, std::min(ceilDiv(tiles, columnWaves), cus / (a.kvHeads * ceilDiv(x.len, shortest))));
   const int nc = (int)ceilDiv(ceilDiv(tiles, groups), columnWaves);
@@ -1049,7 +1050,7 @@ static diopiError_t decodeSharedPrefix(diopiContextHandle_t ctx, hipStream_t str
   AMD_TRY(decodePartials(ctx, stream, a, dtype, a.maxLen, out, &own));
   if (own.nsplit == 0) return diopiSuccess;
   // A wave has the elements of nine shares on their way at once. Up to those it needs no help; twice as many are still better left to
-  // one than to four where there are many pairs: 2048 pairs, 10 shares 23.7 us (all three launches) and 27.3; 512 pairs, 18 shares
+  // one than to four where there are many pairs: 2048 pairs, 10 shares 23.7 us (all launches) and 27.3; 512 pairs, 18 shares
   // 18.9 and 17.5.
   const int shares = x.nsplit + own.nsplit;
   const bool narrow = shares <= 9 || (shares <= 18 && pairs >= 1024);
