@@ -505,7 +505,7 @@ def dest_index_copy_kv_pair(k, v, dest_loc, out_k, out_v):
 
 
 def dest_index_copy_kv_pair_int8(k, v, dest_loc, out_k, out_k_scale, out_v, out_v_scale):
-    """k[i] and v[i] quantised to int8 with a scale per token and head, into slot dest_loc[i] of two pools, in one launch
+    """k[i] and v[i] quantised to int8 with a scale per token and head, into slot dest_loc[i] of two pools
     (backend extension, functions_ext.h). Pools [slots, kv_heads, d] int8, scales [slots, kv_heads] float32."""
     _host.diopiDestIndexCopyKVPairInt8(_ctx, out_k, out_k_scale, k, out_v, out_v_scale, v, dest_loc)
     return out_k, out_k_scale, out_v, out_v_scale
@@ -517,9 +517,10 @@ def index_select_kv_pair_int8(k, k_scale, v, v_scale, index, *, dtype=None, out_
     if out_k is None or out_v is None:
         if dtype is None:
             dtype = next((o.dtype for o in (out_k, out_v) if o is not None), torch.get_default_dtype())
-        shape = (index.shape[0], *k.shape[1:])
-        out_k = torch.empty(shape, dtype=dtype, device=k.device) if out_k is None else out_k
-        out_v = torch.empty(shape, dtype=dtype, device=k.device) if out_v is None else out_v
+        new = k.new_empty((index.numel(), *k.shape[1:]), dtype=dtype)
+        if out_k is None:
+            out_k, new = new, _host.like(new) if out_v is None else None
+        out_v = new if out_v is None else out_v
     _host.diopiIndexSelectKVPairInt8(_ctx, out_k, out_v, k, k_scale, v, v_scale, index)
     return out_k, out_v
 

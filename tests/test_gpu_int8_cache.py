@@ -383,3 +383,19 @@ def test_on_another_stream_with_calls_in_flight_on_the_first(ops, dev):
     for i, outs in enumerate(got):
         for o in outs:
             assert_exact(o, want[i])
+
+
+def test_the_results_that_are_not_given_are_made(ops, dev):
+    (kp, ks), (vp, vs) = empty_pools(9, 3, 16)
+    index = torch.tensor([2, 8, 0, 5])
+    args = kp.to(dev), ks.to(dev), vp.to(dev), vs.to(dev), index.to(dev)
+    want = {dtype: (oracle.read(kp, ks, index, dtype), oracle.read(vp, vs, index, dtype)) for dtype in TYPES}
+    for dtype in TYPES:
+        mine = torch.empty(4, 3, 16, dtype=dtype, device=dev)
+        for given in (dict(dtype=dtype), dict(out_k=mine), dict(out_v=mine), dict(dtype=dtype, out_v=mine), dict(out_k=mine, out_v=torch.empty_like(mine))):
+            got = ops.index_select_kv_pair_int8(*args, **given)
+            assert got[0].data_ptr() != got[1].data_ptr()
+            assert all(got[i] is given[key] for i, key in enumerate(("out_k", "out_v")) if key in given)
+            for have, expected in zip(got, want[dtype]):
+                assert_exact(have, expected)
+    assert ops.index_select_kv_pair_int8(*args)[0].dtype == torch.get_default_dtype()
