@@ -10,14 +10,14 @@
 // how the division is done. Rows of zeros have s = 0. A row that holds an infinity or NaN has s = NaN and q = 0: all of it reads
 // back as NaN, none of it as a plausible number. Read back: q * s rounded to fp32, and once more to a 16-bit type.
 //
-// Both are bound by memory: a 16-bit row of 128 moves 256 + 132 bytes. Reading 15001 rows of 8 heads back takes 87 us, 5.3 TB/s.
-// Writing 8192 takes 43 us, 4.7 TB/s, and 6 us more to find repeated slots; its arithmetic, 10 instructions an element, is nearly as long.
+// Both are bound by memory: a 16-bit row of 128 moves 256 + 132 bytes. Reading 15001 rows of 40 heads back takes 84 us, 5.6 TB/s.
+// Writing 8192 of 32 takes 45 us, 4.5 TB/s, about 6 of them to find repeated slots; its arithmetic, 9 instructions an element, is nearly as long.
 //   * a row is spread over LPR lanes of 8 elements each (16 bytes of a 16-bit type in, 8 bytes out), so that the largest
 //     magnitude is a few lane permutations; a lane asks for kKvRows rows before it works on the first;
 //   * quotients go through the reciprocal and are rounded by an addition; only where a remainder could decide otherwise is it
-//     computed (see below). Two divisions to a row and a check of each element's remainder took 95 us where this takes 43;
+//     computed (see below). Two divisions to a row and a check of each element's remainder took 95 us where this takes 45;
 //   * K and V are halves of the grid: the choice by an index per lane kept their addresses out of scalar registers (105 us
-//     became 189 us for the read above).
+//     became 189 us for the read above, as it was then).
 // The last of several tokens with one destination is what the slot holds, as a loop over the tokens would leave it (a row and its
 // scale must not come from two tokens). A workgroup looks through the destinations behind its own while its rows are on their
 // way; above kKvScanTokens tokens two launches of their own find the last of each first.
@@ -30,8 +30,8 @@ namespace amd {
 constexpr int kKvThreads = 256;
 constexpr int kKvRows = 4;               // rows that a lane group has in flight
 constexpr int kKvTokensPerWg = 8;        // most tokens of a workgroup that writes
-// Workgroups look for later tokens with the same slot themselves up to this many tokens: 1777 tokens are written in 8.5 us so and
-// in 11.3 us with the two launches before, 8192 in 60 and 49 us.
+// Workgroups look for later tokens with the same slot themselves up to this many tokens: 4096 tokens of 8 heads are written in 11.1 us so,
+// 4097 in 14.2 with the two launches before; of 32 heads in 27.7 and 26.6.
 constexpr int64_t kKvScanTokens = 4096;
 
 struct KvInt8Pool {
@@ -49,7 +49,7 @@ struct KvInt8Args {
   int heads, d;
   float perHeads;    // 1 / heads
   int tokensPerWg;
-  const int* last;   // the last token of each slot (null: the workgroups look for themselves)
+  const int* last;   // the last token of each slot (null: the workgroups that write look for themselves)
 };
 
 __device__ __forceinline__ int64_t kvSlot(const KvInt8Args& a, int64_t t) {
@@ -143,10 +143,37 @@ struct KvSlot {  // where a token's rows and scales begin in the pools: looked u
   __device__ __forceinline__ KvSlot(const KvInt8Pool& o, int slot) : pool(max(slot, 0) * o.poolSlot), scale(max(slot, 0) * o.scaleSlot), slot(slot) {}
 };
 
+// The slots that a workgroup which writes asks for first: those of its own tokens (in lane i of every wave that of token i) and, where
+// it looks for repeated ones itself (SCAN), of the kKvBatch * kKvThreads tokens behind them. As two words, the second for 32-bit slots
+// the first again: a branch on the type would wait for one load before it asks for the next.
+constexpr int kKvBatch = 8;
+template <bool SCAN>
+struct KvAsked {
+  int2 own, behind[SCAN ? kKvBatch : 1];
+};
+__device__ __forceinline__ int2 kvAsk(const KvInt8Args& a, int64_t t) {
+  const int* p = static_cast<const int*>(a.loc) + (t << (a.loc64 ? 1 : 0));
+  return int2{p[0], p[a.loc64 ? 1 : 0]};
+}
+__device__ __forceinline__ int kvDestination(const KvInt8Args& a, int2 slot) {
+  return kvDestination(a, a.loc64 ? (int64_t)((uint64_t)(uint32_t)slot.y << 32 | (uint32_t)slot.x) : (int64_t)slot.x);
+}
+template <bool SCAN>
+__device__ __forceinline__ KvAsked<SCAN> kvAskFirst(const KvInt8Args& a, int64_t t0, int n) {
+  KvAsked<SCAN> asked;
+  asked.own = kvAsk(a, t0 + min((int)(threadIdx.x & 63), n - 1));
+  if constexpr (SCAN) {
+#pragma unroll
+    for (int k = 0; k < kKvBatch; ++k) asked.behind[k] = kvAsk(a, min(t0 + n + threadIdx.x + k * kKvThreads, a.tokens - 1));
+  }
+  __builtin_amdgcn_sched_barrier(0);  // (ahead of the rows: loads return in order, and the search goes on while those are on their way)
+  return asked;
+}
+
 // Whether a later token has the slot of one of the MOST tokens [t0, t0 + n) of the workgroup, as bits. `mine`: in lane i of every
 // wave the slot of token t0 + i, -1 where there is none.
 template <int MOST>
-__device__ __forceinline__ unsigned kvLater(const KvInt8Args& a, int64_t t0, int n, int mine) {
+__device__ __forceinline__ unsigned kvLater(const KvInt8Args& a, int64_t t0, int n, int mine, const int2 (&first)[kKvBatch]) {
   int slot[MOST];
   uint64_t same[MOST];
   unsigned later = 0;
@@ -155,17 +182,24 @@ __device__ __forceinline__ unsigned kvLater(const KvInt8Args& a, int64_t t0, int
     slot[i] = __builtin_amdgcn_readlane(mine, i);  // (in a scalar register: a comparison each, and nothing else)
     same[i] = __builtin_amdgcn_ballot_w64(mine == slot[i]) >> (i + 1);  // among the workgroup's own
   }
-  constexpr int kBatch = 8;  // asked for at once: their answers are what this takes its time for
-  for (int64_t j0 = t0 + n + threadIdx.x; j0 < a.tokens; j0 += kKvThreads * kBatch) {
-    int64_t at[kBatch];
+  auto compare = [&](int2 asked) {
+    const int s = kvDestination(a, asked);
 #pragma unroll
-    for (int k = 0; k < kBatch; ++k) at[k] = kvSlot(a, min(j0 + k * kKvThreads, a.tokens - 1));
+    for (int i = 0; i < MOST; ++i) same[i] |= __builtin_amdgcn_ballot_w64(s == slot[i]);
+  };
+  const int64_t begin = t0 + n;
 #pragma unroll
-    for (int k = 0; k < kBatch; ++k) {
-      const int s = kvDestination(a, at[k]);
+  for (int k = 0; k < kKvBatch; ++k) {
+    if (begin + k * kKvThreads >= a.tokens) break;
+    compare(first[k]);  // (past the last token: that again)
+  }
+  for (int64_t j0 = begin + kKvThreads * kKvBatch; j0 < a.tokens; j0 += kKvThreads * kKvBatch) {
+    int2 at[kKvBatch];
 #pragma unroll
-      for (int i = 0; i < MOST; ++i) same[i] |= __builtin_amdgcn_ballot_w64(s == slot[i]);
-    }
+    for (int k = 0; k < kKvBatch; ++k) at[k] = kvAsk(a, min(j0 + threadIdx.x + k * kKvThreads, a.tokens - 1));
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int k = 0; k < kKvBatch; ++k) compare(at[k]);
   }
 #pragma unroll
   for (int i = 0; i < MOST; ++i) later |= same[i] != 0 ? 1u << i : 0u;
@@ -174,21 +208,24 @@ __device__ __forceinline__ unsigned kvLater(const KvInt8Args& a, int64_t t0, int
 
 // The slots of the workgroup's tokens [t0, t0 + n), -1 for those that are not written: no destination, or a later token has the
 // same. (One barrier; every thread of the workgroup takes part.)
-__device__ __forceinline__ void kvDestinations(const KvInt8Args& a, int64_t t0, int n, KvSlot (&slots)[kKvTokensPerWg], unsigned (&later)[kKvThreads / 64]) {
+template <bool SCAN>
+__device__ __forceinline__ void kvDestinations(const KvInt8Args& a, int64_t t0, int n, const KvAsked<SCAN>& asked, KvSlot (&slots)[kKvTokensPerWg],
+                                               unsigned (&later)[kKvThreads / 64]) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int mine = -1;
-  if (lane < n) {
-    mine = kvDestination(a, kvSlot(a, t0 + lane));
-    if (a.last != nullptr && mine >= 0 && a.last[mine] != (int)(t0 + lane)) mine = -1;
+  int mine = lane < n ? kvDestination(a, asked.own) : -1;
+  unsigned found = 0;
+  if constexpr (SCAN) {
+    found = n <= 2 ? kvLater<2>(a, t0, n, mine, asked.behind) : kvLater<kKvTokensPerWg>(a, t0, n, mine, asked.behind);
+  } else {
+    if (mine >= 0 && a.last[mine] != (int)(t0 + lane)) mine = -1;
   }
-  const unsigned found = a.last != nullptr ? 0u : n <= 2 ? kvLater<2>(a, t0, n, mine) : kvLater<kKvTokensPerWg>(a, t0, n, mine);
   if (lane == 0) later[wave] = found;
   if (wave == 0 && lane < kKvTokensPerWg) slots[lane] = KvSlot(a.pool[blockIdx.y], mine);
   __syncthreads();
 }
 
 // grid: (workgroups of tokensPerWg tokens, K or V). Rows of a workgroup: (token, head), head fastest.
-template <typename T, int LPR>
+template <typename T, int LPR, bool SCAN>
 __global__ __launch_bounds__(kKvThreads) void kvInt8WriteKernel(KvInt8Args a) {
   constexpr int kGroups = kKvThreads / LPR;
   __shared__ unsigned later[kKvThreads / 64];
@@ -212,8 +249,9 @@ __global__ __launch_bounds__(kKvThreads) void kvInt8WriteKernel(KvInt8Args a) {
       for (int c = 0; c < 8 / Vec16<T>::N; ++c) x[u].v[c] = __builtin_nontemporal_load(reinterpret_cast<const typename Vec16<T>::type*>(src) + c);
     }
   };
+  const KvAsked<SCAN> asked = kvAskFirst<SCAN>(a, t0, n);
   load(group);
-  kvDestinations(a, t0, n, slots, later);
+  kvDestinations<SCAN>(a, t0, n, asked, slots, later);
   const unsigned dead = later[0] | later[1] | later[2] | later[3];
   for (int r0 = group; r0 < rows; r0 += kKvRows * kGroups) {
     if (r0 != group) load(r0);
@@ -251,13 +289,13 @@ __global__ __launch_bounds__(kKvThreads) void kvInt8WriteKernel(KvInt8Args a) {
 }
 
 // Any head size and alignment: a wave per row.
-template <typename T>
+template <typename T, bool SCAN>
 __global__ __launch_bounds__(kKvThreads) void kvInt8WriteAnyKernel(KvInt8Args a) {
   __shared__ unsigned later[kKvThreads / 64];
   __shared__ KvSlot slots[kKvTokensPerWg];
   const int64_t t0 = (int64_t)blockIdx.x * a.tokensPerWg;
   const int n = (int)min((int64_t)a.tokensPerWg, a.tokens - t0);
-  kvDestinations(a, t0, n, slots, later);
+  kvDestinations<SCAN>(a, t0, n, kvAskFirst<SCAN>(a, t0, n), slots, later);
   const unsigned dead = later[0] | later[1] | later[2] | later[3];
   const int lane = threadIdx.x & 63, rows = n * a.heads;
   const KvInt8Pool& o = a.pool[blockIdx.y];
@@ -406,12 +444,11 @@ static bool kvInt8Vector(const KvInt8Args& a, int64_t itemsize) {
   return (bits16 & 15) == 0 && (bits8 & 7) == 0;
 }
 
-// 32 to 128 rows to a workgroup: as many as leave 256 workgroups (one per compute unit) for K and as many for V. Between those
-// the slots are looked up, and looked through, more often than needed: 1777 tokens of 8 heads are written in 8.5 us so and in
-// 9.9 us with 1024 workgroups each; 8192 of 8 take 49 us with 128 rows, 53 us with 256, 51 us with 64, and are read back in 36.5, 39
-// and 38 us.
+// 32 or 64 rows to a workgroup: 64 where that leaves 256 workgroups (one per compute unit) for K and as many for V. us with 64, 128
+// and 256: 8192 tokens of 32 heads written 45.3, 46.7, 45.4, read back 35.8, 36.6, 38.9; 15001 of 40 read back 83.8, 87.1, 91.8. 1777 tokens
+// of 8 with 32 rows, from which the slots are looked up and looked through twice as often: 9.0, with 64 8.0.
 static diopiError_t kvInt8Grid(const char* what, KvInt8Args* a, dim3* grid) {
-  const int64_t rows = std::min<int64_t>(128, std::max<int64_t>(32, a->tokens * a->heads / 256));
+  const int64_t rows = std::min<int64_t>(64, std::max<int64_t>(32, a->tokens * a->heads / 256));
   a->tokensPerWg = (int)std::min<int64_t>(kKvTokensPerWg, ceilDiv(rows, a->heads));
   const int64_t wgs = ceilDiv(a->tokens, a->tokensPerWg);
   AMD_CHECK(wgs < 1 << 24, "%s: %ld rows of %d heads exceed the launch limits", what, (long)a->tokens, a->heads);  // (2^32 threads)
@@ -419,18 +456,19 @@ static diopiError_t kvInt8Grid(const char* what, KvInt8Args* a, dim3* grid) {
   return diopiSuccess;
 }
 
-#define KV_INT8_LAUNCH_TYPE(T, NAME, VEC)                                                                            \
-  do {                                                                                                               \
-    if (!(VEC)) hipLaunchKernelGGL((NAME##AnyKernel<T>), grid, dim3(kKvThreads), 0, stream, a);                       \
-    else if (a.d <= 64) hipLaunchKernelGGL((NAME##Kernel<T, 8>), grid, dim3(kKvThreads), 0, stream, a);               \
-    else if (a.d <= 128) hipLaunchKernelGGL((NAME##Kernel<T, 16>), grid, dim3(kKvThreads), 0, stream, a);             \
-    else hipLaunchKernelGGL((NAME##Kernel<T, 32>), grid, dim3(kKvThreads), 0, stream, a);                             \
+// NAME: kernels of one row width, of any, and their arguments behind the type and the width
+#define KV_INT8_LAUNCH_TYPE(T, NAME, VEC, ...)                                                                                     \
+  do {                                                                                                                             \
+    if (!(VEC)) hipLaunchKernelGGL((NAME##AnyKernel<T __VA_OPT__(, ) __VA_ARGS__>), grid, dim3(kKvThreads), 0, stream, a);             \
+    else if (a.d <= 64) hipLaunchKernelGGL((NAME##Kernel<T, 8 __VA_OPT__(, ) __VA_ARGS__>), grid, dim3(kKvThreads), 0, stream, a);     \
+    else if (a.d <= 128) hipLaunchKernelGGL((NAME##Kernel<T, 16 __VA_OPT__(, ) __VA_ARGS__>), grid, dim3(kKvThreads), 0, stream, a);   \
+    else hipLaunchKernelGGL((NAME##Kernel<T, 32 __VA_OPT__(, ) __VA_ARGS__>), grid, dim3(kKvThreads), 0, stream, a);                   \
   } while (0)
-#define KV_INT8_LAUNCH(DTYPE, NAME, VEC)                                          \
-  do {                                                                            \
-    if (DTYPE == diopi_dtype_bfloat16) KV_INT8_LAUNCH_TYPE(bf16_t, NAME, VEC);    \
-    else if (DTYPE == diopi_dtype_float16) KV_INT8_LAUNCH_TYPE(half_t, NAME, VEC); \
-    else KV_INT8_LAUNCH_TYPE(float, NAME, VEC);                                   \
+#define KV_INT8_LAUNCH(DTYPE, NAME, VEC, ...)                                                              \
+  do {                                                                                                     \
+    if (DTYPE == diopi_dtype_bfloat16) KV_INT8_LAUNCH_TYPE(bf16_t, NAME, VEC __VA_OPT__(, ) __VA_ARGS__);    \
+    else if (DTYPE == diopi_dtype_float16) KV_INT8_LAUNCH_TYPE(half_t, NAME, VEC __VA_OPT__(, ) __VA_ARGS__); \
+    else KV_INT8_LAUNCH_TYPE(float, NAME, VEC __VA_OPT__(, ) __VA_ARGS__);                                   \
   } while (0)
 
 }  // namespace amd
@@ -467,7 +505,9 @@ extern "C" __attribute__((visibility("default"))) diopiError_t diopiDestIndexCop
     AMD_LAUNCH_CHECK();
     a.last = static_cast<const int*>(last);
   }
-  KV_INT8_LAUNCH(x[0].dtype, kvInt8Write, kvInt8Vector(a, x[0].itemsize));
+  const bool vector = kvInt8Vector(a, x[0].itemsize);
+  if (a.last == nullptr) KV_INT8_LAUNCH(x[0].dtype, kvInt8Write, vector, true);
+  else KV_INT8_LAUNCH(x[0].dtype, kvInt8Write, vector, false);
   AMD_LAUNCH_CHECK();
   return diopiSuccess;
 }
