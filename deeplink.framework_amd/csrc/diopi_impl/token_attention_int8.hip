@@ -80,9 +80,9 @@ __global__ __launch_bounds__(256) void decodeInt8AnyKernel(TaInt8Args x, T* __re
 }
 
 // ------------------------------------------------ head sizes of whole 16-byte pieces up to 256: the matrix pipe --
-// Bound by memory: a row is d + 4 bytes, K and V alike. Both products of 32 tokens are matrix products (16x16x32, bf16 operands,
-// fp32 sums) with up to 16 query heads of a K/V head as columns; whole numbers up to 127 are exact in bf16, so the only things
-// rounded are q (not at all: bf16 is one operand, the 11 bits of fp16 two, the 24 of fp32 three) and the probabilities.
+// Bound by memory: a row is d + 4 bytes, K and V alike. Both products of 32 tokens are matrix products (16x16x32, fp32 sums) with up
+// to 16 query heads of a K/V head as columns; whole numbers up to 127 are exact in bf16 and in fp16, so the only things rounded
+// are q (not at all: a 16-bit q is one operand and meets K in its own type, the 24 bits of fp32 are three of bf16) and the probabilities.
 //   * S^T = K . Q^T: lane (token l % 16, group l / 16) needs 8 elements of its token's row for every product: it loads 16
 //     adjacent bytes, which serve two of them (the order of the head's places along k is free as long as q has the same).
 //   * a lane then holds eight tokens' scores of ONE head, so the softmax runs in the lane, and its probabilities are, as they lie,
@@ -100,8 +100,8 @@ constexpr int kI8Block = 512;  // tokens whose slots and scales a workgroup hold
 constexpr int kI8Heads = 16;  // query heads a wave serves
 
 template <typename T>
-struct I8Parts {  // 8-bit parts that hold q, and those that a probability is cut into
-  static constexpr int kQ = std::is_same<T, bf16_t>::value ? 1 : std::is_same<T, half_t>::value ? 2 : 3;
+struct I8Parts {  // operands that hold q, and those that a probability is cut into
+  static constexpr int kQ = std::is_same<T, float>::value ? 3 : 1;
   static constexpr int kP = std::is_same<T, float>::value ? 3 : 2;
 };
 
@@ -111,6 +111,18 @@ __device__ __forceinline__ uint32_t int8PairToBf16(uint32_t w0, uint32_t w1) {
   const float f0 = static_cast<float>(static_cast<int>(static_cast<int8_t>(w0 >> (8 * B0))));
   const float f1 = static_cast<float>(static_cast<int>(static_cast<int8_t>(w1 >> (8 * B1))));
   return __builtin_amdgcn_perm(__float_as_uint(f1), __float_as_uint(f0), 0x07060302u);
+}
+
+// The same as two operands of the product with q: fp16 q meets K in fp16 (exact too), anything else bf16.
+template <typename T, int B0, int B1>
+__device__ __forceinline__ uint32_t int8PairForQ(uint32_t w) {
+  if constexpr (std::is_same<T, half_t>::value) {
+    const float f0 = static_cast<float>(static_cast<int>(static_cast<int8_t>(w >> (8 * B0))));
+    const float f1 = static_cast<float>(static_cast<int>(static_cast<int8_t>(w >> (8 * B1))));
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(f0, f1));
+  } else {
+    return int8PairToBf16<B0, B1>(w, w);
+  }
 }
 
 template <int N>
@@ -129,6 +141,7 @@ __device__ __forceinline__ bf16x8 nextPart(float (&x)[8]) {
   return part;
 }
 
+// (The second launch bound: with three waves to a SIMD five registers of D = 128 go to scratch, and 48 x (512 .. 4096), 8 K/V heads, takes 62 us, so 58.)
 // D: head size the rows are laid out for; a.d is any multiple of 16 up to it: the pieces past the row's end repeat its first
 // one, meet zeros of q, and give output places that are not stored. A workgroup's waves take x.headsPerWg K/V heads of the
 // same tokens and share these out among the waves of a head.
@@ -172,7 +185,7 @@ __global__ __launch_bounds__(kI8Waves * 64, D == 256 ? 1 : 2) void decodeInt8Ker
 
   // q: product (p, s) of a row multiplies 8 places from placeOf(p) + 8 s on
   auto placeOf = [&](int p) { return PIECES == 1 ? 16 * quad : 128 * (p >> 1) + 32 * quad + 16 * (p & 1); };
-  bf16x8 qf[2 * PIECES][PQ];
+  u32x4 qf[2 * PIECES][PQ];
 #pragma unroll
   for (int p = 0; p < PIECES; ++p)
 #pragma unroll
@@ -194,8 +207,15 @@ __global__ __launch_bounds__(kI8Waves * 64, D == 256 ? 1 : 2) void decodeInt8Ker
       }
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = have ? v[j] : 0.f;
+      if constexpr (std::is_same<T, half_t>::value) {
+        f16x8 whole;
 #pragma unroll
-      for (int k = 0; k < PQ; ++k) qf[2 * p + s][k] = nextPart(v);
+        for (int j = 0; j < 8; ++j) whole[j] = static_cast<half_t>(v[j]);
+        qf[2 * p + s][0] = __builtin_bit_cast(u32x4, whole);
+      } else {
+#pragma unroll
+        for (int k = 0; k < PQ; ++k) qf[2 * p + s][k] = __builtin_bit_cast(u32x4, nextPart(v));
+      }
     }
 
   // Loads take whole 128-byte lines of 8 rows (or what of a row there is): K of two tiles of 8 tokens, in lanes 0 .. 7 and 8 .. 15
@@ -260,10 +280,14 @@ __global__ __launch_bounds__(kI8Waves * 64, D == 256 ? 1 : 2) void decodeInt8Ker
             return p & 1 ? swapped(s.k[t][p][c], s.k[t][p - 1][c], kLower) : swapped(s.k[t][p][c], s.k[t][p + 1 < PIECES ? p + 1 : p][c], kUpper);
           };
           const uint32_t w0 = word(2 * half), w1 = word(2 * half + 1);
-          const bf16x8 kf = __builtin_bit_cast(bf16x8, u32x4{int8PairToBf16<0, 1>(w0, w0), int8PairToBf16<2, 3>(w0, w0),
-                                                             int8PairToBf16<0, 1>(w1, w1), int8PairToBf16<2, 3>(w1, w1)});
+          const u32x4 kf = {int8PairForQ<T, 0, 1>(w0), int8PairForQ<T, 2, 3>(w0), int8PairForQ<T, 0, 1>(w1), int8PairForQ<T, 2, 3>(w1)};
+          if constexpr (std::is_same<T, half_t>::value) {
+            s4[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, kf), __builtin_bit_cast(f16x8, qf[2 * p + half][0]), s4[t], 0, 0, 0);
+          } else {
 #pragma unroll
-          for (int k = 0; k < PQ; ++k) s4[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[2 * p + half][k], s4[t], 0, 0, 0);
+            for (int k = 0; k < PQ; ++k)
+              s4[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kf), __builtin_bit_cast(bf16x8, qf[2 * p + half][k]), s4[t], 0, 0, 0);
+          }
         }
     }
     float sc[8], w[8];
@@ -498,7 +522,7 @@ static diopiError_t int8Pool(const char* name, const TensorView& q, const Tensor
 // waves of a head: 1 x 1777 tokens, 8 heads, one step to a wave, 10.3 with one head, 11.4 with four.
 // us at 1, 2, 4, 8, 16 steps to a wave: 1 x 4096, 8 heads 10.6, 11.3, 13.6, 18.0, 25.1; 1 x 8192 14.2, 13.2, 15.2, 18.5, 25.5; 1 x 16384
 // 25.3, 20.0, 18.5, 19.4, 25.7; 8 x 4096 37, 28, 22.7, 20.7, 26.2; 16 x (1000 .. 8000) 84, 58, 48, 47, 47; 48 x (512 .. 4096) 120, 82, 69, 59, 72;
-// 32 heads, 64 x (512 .. 4096) 627, 385, 297, 247, 231. Heads of 256: a SIMD holds one wave instead of three, and a step takes twice as
+// 32 heads, 64 x (512 .. 4096) 627, 385, 297, 247, 231. Heads of 256: a SIMD holds one wave instead of two, and a step takes twice as
 // long: 16 x (512 .. 4096), 8 heads 105, 71, 60, 56, 45.
 static void chooseShares(TaInt8Args* x, int64_t len, int D) {
   TaArgs& a = x->a;
