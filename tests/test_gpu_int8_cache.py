@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from tests import cache_oracle as oracle
+from tests.cache_graph import recorded
 from tests.parity import assert_exact
 
 pytestmark = pytest.mark.gpu
@@ -252,6 +253,15 @@ def test_one_key_far_above_the_rest_and_values_only_below_it(ops, dev, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [64, 128, 256, 20])
+def test_q_below_the_smallest_normal_number_of_fp16(ops, dev, dtype, d):
+    q, pools, b_loc, lens, max_len = batch_of([70, 3, 150], 4, 2, d, dtype, 65)
+    (kp, ks), (vp, vs) = pools
+    q, ks = (q.float() * 2.0 ** -20).to(dtype), ks * 2.0 ** 20      # scores as they were
+    check_attention(ops, dev, q, [(kp, ks), (vp, vs)], b_loc, lens, max_len)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("d", [64, 128, 20])
 def test_scales_that_are_nan_infinite_huge_and_zero(ops, dev, dtype, d):
     q, pools, b_loc, lens, max_len = batch_of([70, 70, 70, 70, 90], 2, 1, d, dtype, 60, torch.int64)
@@ -366,6 +376,31 @@ def test_recorded_into_a_graph_and_replayed_next_to_eager_calls(ops, dev, pkg):
             assert_exact(have, w)
     del graph
     scope.close()
+
+
+@pytest.mark.parametrize("tokens", [1500, 5000])                 # repeated slots found by the workgroups, and in workspace beforehand
+def test_repeated_slots_recorded_into_two_graphs(ops, dev, pkg, tokens):
+    slots = tokens // 2
+    pools = [[t.to(dev) for pool in empty_pools(slots, 2, 64, seed=i) for t in pool] for i in range(2)]
+    x = [rows(tokens, 2, 64, torch.bfloat16, 120 + i).to(dev) for i in range(2)]
+    dest = [torch.randint(0, slots, (tokens,), generator=g(130 + i)).to(dev) for i in range(2)]
+    calls = [lambda i=i: ops.dest_index_copy_kv_pair_int8(x[i], x[i], dest[i], *pools[i]) for i in range(2)]
+    with recorded(ops, pkg, calls[0]) as (first, _), recorded(ops, pkg, calls[1]) as (second, _):
+        for r in range(4):
+            for i in range(2):
+                dest[i].copy_(torch.randint(0, slots, (tokens,), generator=g(140 + 2 * r + i)))
+            before = [t.clone() for t in pools[0] + pools[1]]
+            first.replay()
+            second.replay()
+            torch.cuda.synchronize()
+            kept = [t.clone() for t in pools[0] + pools[1]]
+            for t, old in zip(pools[0] + pools[1], before):
+                t.copy_(old)
+            for call in calls:
+                call()
+            torch.cuda.synchronize()
+            for have, want in zip(kept, pools[0] + pools[1]):
+                assert_exact(have, want)
 
 
 def test_on_another_stream_with_calls_in_flight_on_the_first(ops, dev):

@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from tests import cache_oracle as oracle
+from tests.cache_graph import recorded
 from tests.parity import assert_exact
 
 pytestmark = pytest.mark.gpu
@@ -157,6 +158,14 @@ def test_scores_of_the_largest_size(ops, dev, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_numbers_below_the_smallest_normal_one_of_fp16(ops, dev, dtype, d):
+    q, k, v, prefix, b_loc, lens, max_len = batch_of(300, [70, 3, 0], 8, 2, d, torch.float32, 65)
+    for a, b, c in ((2.0 ** -20, 2.0 ** 13, 1), (2.0 ** 13, 2.0 ** -20, 1), (1, 1, 2.0 ** -18)):
+        check(ops, dev, (q * a).to(dtype), (k * b).to(dtype), (v * c).to(dtype), prefix, b_loc, lens, max_len)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_q_and_pools_at_other_strides_and_alignments(ops, dev, dtype):
     for d, shift in [(128, 0), (128, 1), (64, 8), (80, 4)]:
         q, k, v, prefix, b_loc, lens, max_len = batch_of(150, [33, 0, 200], 6, 2, d, dtype, 70)
@@ -266,6 +275,28 @@ def test_recorded_into_a_graph_and_replayed_next_to_eager_calls(ops, dev, pkg, d
         assert_exact(kept, want)
     del graph
     scope.close()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv_heads", [(2, 2), (8, 1)])
+def test_short_sequences_recorded_into_two_graphs(ops, dev, pkg, dtype, heads, kv_heads):
+    """The shared tokens' partial results are read by the launch behind, in each graph's own workspace."""
+    cases = [[t.to(dev) if hasattr(t, "to") else t for t in batch_of(700 + 300 * i, [20, 3, 11], heads, kv_heads, 64, dtype, 400 + i)] for i in range(2)]
+    calls = [lambda c=c: ops.token_decode_attention_shared_prefix(c[0], c[1], c[2], c[3], c[4], c[5], c[5], c[6]) for c in cases]
+    with recorded(ops, pkg, calls[0]) as (first, a), recorded(ops, pkg, calls[1]) as (second, b):
+        for i in range(4):
+            for c in cases:
+                c[0].mul_(0.75)
+                c[5].copy_(torch.tensor([20 - 5 * i, 3, 0 if i else 11]))
+            first.replay()
+            second.replay()
+            first.replay()
+            torch.cuda.synchronize()
+            kept = a.clone(), b.clone()
+            want = calls[0](), calls[1]()
+            torch.cuda.synchronize()
+            assert_exact(kept[0], want[0])
+            assert_exact(kept[1], want[1])
 
 
 def test_on_another_stream_with_calls_in_flight_on_the_first(ops, dev):
