@@ -73,6 +73,18 @@ def test_one_to_many_shares_of_the_prefix(ops, dev, dtype, heads, kv_heads, d):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,d", [(2, 1, 20), (3, 3, 1), (4, 2, 300), (2, 2, 1024), (1, 1, 513), (8, 2, 256), (2, 1, 132), (2, 1, 250)])
+def test_head_sizes_of_any_kind_in_many_chunks(ops, dev, dtype, heads, kv_heads, d):
+    for prefix, lens in ((1, [0]), (255, [1, 0]), (256, [0, 700]), (3000, [20, 0, 300]), (5001, [1] * 9)):
+        check(ops, dev, *batch_of(prefix, lens, heads, kv_heads, d, dtype, 500 + prefix))
+    q, k, v, prefix, b_loc, lens, max_len = batch_of(1500, [500, 3], heads, kv_heads, d, dtype, 499)
+    prefix[::3], prefix[512:1024] = -1, k.shape[0] + 5                # some slots, and whole chunks, outside the pool
+    got = run(ops, dev, q, k, v, prefix, b_loc, lens, max_len)
+    want, bound = oracle.attend(q, k, v, own_and_shared(prefix[(prefix >= 0) & (prefix < k.shape[0])], b_loc, lens, max_len), PART[q.dtype])
+    oracle.assert_within(got, want, bound)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("heads,kv_heads", [(2, 2), (4, 1)])
 def test_shares_without_a_token_that_counts(ops, dev, dtype, heads, kv_heads):
     q, k, v, prefix, b_loc, lens, max_len = batch_of(640, [3, 0, 20], heads, kv_heads, 64, dtype, 310)
