@@ -79,4 +79,22 @@ struct TaPartials {
 };
 diopiError_t decodePartials(diopiContextHandle_t ctx, hipStream_t stream, const TaArgs& a, diopiDtype_t dtype, int maxInputLen, void* out, TaPartials* keep);
 
+// As decodePartials, for rows of any kind and for int8 pools: partial results of the first `walked` tokens in `loc` and the own ones behind
+// them, of at least one chunk; if nothing else is to be merged (alone) and there is one chunk, the result (own->nsplit is 0 then).
+struct TaAnyArgs {
+  TaArgs a;
+  const void* loc;  // slots of shared tokens
+  bool locIs64;
+  int walked;
+  const float* kScale;  // null: the pool is of q's type
+  const float* vScale;
+  int64_t kScaleSlot, kScaleHead, vScaleSlot, vScaleHead;
+  int chunk, split;  // (set by walkAny)
+};
+diopiError_t walkAny(diopiContextHandle_t ctx, hipStream_t stream, TaAnyArgs x, diopiDtype_t dtype, void* out, bool alone, TaPartials* own);
+
+// out from the partial results of nShared chunks of tokens that all sequences have and `own` of what comes behind (with `walked` of the
+// shared tokens in front).
+diopiError_t mergeShares(hipStream_t stream, const TaArgs& a, diopiDtype_t dtype, void* out, const float* shared, int nShared, const TaPartials& own, int walked);
+
 }  // namespace amd

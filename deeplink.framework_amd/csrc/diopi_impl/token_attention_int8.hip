@@ -21,64 +21,6 @@ struct TaInt8Args {
   unsigned kStride, vStride;  // slot strides of the pools in bytes, as decodeInt8Kernel takes them
 };
 
-// Any head size up to 1024: one workgroup per (sequence, head), 256 tokens at a time, one token's dot product per thread and
-// P.V with the threads over d. A correctness path.
-template <typename T>
-__global__ __launch_bounds__(256) void decodeInt8AnyKernel(TaInt8Args x, T* __restrict__ out) {
-  __shared__ float prob[256];
-  __shared__ int64_t slotOf[256];
-  __shared__ float red[4];
-  const TaArgs& a = x.a;
-  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
-  const int len = (int)min(max(ldIndex(a.bLen, b, a.len64), (int64_t)0), (int64_t)a.maxLen);
-  const int kvh = h / (a.heads / a.kvHeads);
-  const int64_t locBase = (int64_t)b * a.locRowStride + (a.maxLen - len);
-  const T* q = reinterpret_cast<const T*>(a.q) + b * a.qBatchStride + h * a.qHeadStride;
-  const int8_t* kHead = reinterpret_cast<const int8_t*>(a.k) + kvh * a.kHeadStride;
-  const int8_t* vHead = reinterpret_cast<const int8_t*>(a.v) + kvh * a.vHeadStride;
-  float m = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};  // acc[j]: element tid + 256 j of the output row
-  for (int t0 = 0; t0 < len; t0 += 256) {
-    const int t = t0 + tid;
-    int64_t slot = t < len ? ldIndex(a.bLoc, locBase + t, a.loc64) : -1;
-    if (slot >= a.slots) slot = -1;
-    float sc = -INFINITY, vs = 0.f;  // the score in units of log2; the scale of V
-    if (slot >= 0) {
-      const int8_t* k = kHead + slot * a.kSlotStride;
-      float d = 0.f;
-      for (int e = 0; e < a.d; ++e) d += static_cast<float>(q[e]) * static_cast<float>(k[e]);
-      sc = d * (x.kScale[slot * x.kScaleSlot + kvh * x.kScaleHead] * a.scaleLog2e);
-      vs = x.vScale[slot * x.vScaleSlot + kvh * x.vScaleHead];
-    }
-    const float mn = fmaxf(m, blockMax256(sc, red));
-    const float ref = mn == -INFINITY ? 0.f : mn;  // (scores that are NaN leave no maximum, and make all of the row NaN)
-    const float pr = slot < 0 ? 0.f : exp2f(sc - ref);
-    prob[tid] = pr * vs;
-    slotOf[tid] = slot;
-    const float bs = blockSum256(pr, red);  // its barriers also publish prob / slotOf
-    const float corr = m == -INFINITY ? 1.f : exp2f(m - ref);  // (no maximum yet: the sums are 0, or NaN)
-    l = l * corr + bs;
-    const int cnt = min(256, len - t0);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int e = tid + 256 * j;
-      if (e < a.d) {
-        float o = acc[j] * corr;
-        for (int i = 0; i < cnt; ++i)
-          if (slotOf[i] >= 0) o += prob[i] * static_cast<float>(vHead[slotOf[i] * a.vSlotStride + e]);
-        acc[j] = o;
-      }
-    }
-    m = mn;
-    __syncthreads();  // prob / slotOf are rewritten by the next block of tokens
-  }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int e = tid + 256 * j;
-    if (e < a.d) out[((int64_t)b * a.heads + h) * a.d + e] = static_cast<T>(acc[j] * inv);
-  }
-}
-
 // ------------------------------------------------ head sizes of whole 16-byte pieces up to 256: the matrix pipe --
 // Bound by memory: a row is d + 4 bytes, K and V alike. Both products of 32 tokens are matrix products (16x16x32, fp32 sums) with up
 // to 16 query heads of a K/V head as columns; whole numbers up to 127 are exact in bf16 and in fp16, so the only things rounded
@@ -623,10 +565,10 @@ extern "C" __attribute__((visibility("default"))) diopiError_t diopiTokenDecodeA
                        a.vHeadStride | a.d;
   const int64_t widest = std::max({a.kSlotStride, a.vSlotStride, x.kScaleSlot, x.vScaleSlot});
   if ((bits & 15) == 0 && a.d <= 256 && a.slots <= 0x7fffffff && widest <= 0xffffffffll) return decodeInt8(ctx, stream, x, t.q, out.data);
-  const dim3 grid(a.heads, a.batch);
-  if (t.q.dtype == diopi_dtype_bfloat16) hipLaunchKernelGGL((decodeInt8AnyKernel<bf16_t>), grid, dim3(256), 0, stream, x, out.ptr<bf16_t>());
-  else if (t.q.dtype == diopi_dtype_float16) hipLaunchKernelGGL((decodeInt8AnyKernel<half_t>), grid, dim3(256), 0, stream, x, out.ptr<half_t>());
-  else hipLaunchKernelGGL((decodeInt8AnyKernel<float>), grid, dim3(256), 0, stream, x, out.ptr<float>());
-  AMD_LAUNCH_CHECK();
-  return diopiSuccess;
+  TaAnyArgs any{};
+  any.a = a, any.kScale = x.kScale, any.vScale = x.vScale;
+  any.kScaleSlot = x.kScaleSlot, any.kScaleHead = x.kScaleHead, any.vScaleSlot = x.vScaleSlot, any.vScaleHead = x.vScaleHead;
+  TaPartials own;
+  AMD_TRY(walkAny(ctx, stream, any, t.q.dtype, out.data, true, &own));
+  return own.nsplit == 0 ? diopiSuccess : mergeShares(stream, a, t.q.dtype, out.data, nullptr, 0, own, 0);
 }

@@ -19,109 +19,15 @@ struct TaPrefixArgs {
   int len;
   int chunk, nsplit;          // of the shared tokens
   int groups;                 // of columns
-  int walked;                 // decodePrefixAnyKernel: shared tokens that it walks itself
-  int anyChunk, anySplit;     // of those and the longest sequence's own
   unsigned kStride, vStride;  // slot strides of the pools in bytes
 };
 
-// Any head size up to 64 J, any strides: a workgroup per (sequence, head, chunk) walks the first x.walked of the shared tokens and the
-// sequence's own, a wave a token at a time with the row spread over its lanes (K and V in whole lines), UNR of them asked for
-// at once; slots are looked up 64 at a time. The one of several chunks that is not the first and has no tokens writes nothing.
-constexpr int kPaWaves = 4;
-template <typename T, int J, int UNR>
-__global__ __launch_bounds__(kPaWaves * 64) void decodePrefixAnyKernel(TaPrefixArgs x, T* __restrict__ out, float* __restrict__ partial) {
-  __shared__ float red[kPaWaves][64 * J], state[kPaWaves][2];
-  const TaArgs& a = x.a;
-  const int h = blockIdx.x, b = blockIdx.y, split = blockIdx.z, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int len = (int)min(max(ldIndex(a.bLen, b, a.len64), (int64_t)0), (int64_t)a.maxLen), all = x.walked + len;
-  const int begin = split * x.anyChunk, end = min(all, begin + x.anyChunk);
-  if (begin >= all && split != 0) return;
-  const int kvh = h / (a.heads / a.kvHeads);
-  const int64_t locBase = (int64_t)b * a.locRowStride + (a.maxLen - len);
-  const T* q = reinterpret_cast<const T*>(a.q) + b * a.qBatchStride + h * a.qHeadStride;
-  const T* kHead = reinterpret_cast<const T*>(a.k) + kvh * a.kHeadStride;
-  const T* vHead = reinterpret_cast<const T*>(a.v) + kvh * a.vHeadStride;
-  int at[J];  // the lane's elements of a row; past its end the first one, which q's zero leaves out
-  float qf[J], acc[J], m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int j = 0; j < J; ++j) {
-    const int e = lane + 64 * j;
-    at[j] = e < a.d ? e : 0;
-    qf[j] = e < a.d ? static_cast<float>(q[e]) * a.scaleLog2e : 0.f;
-    acc[j] = 0.f;
-  }
-  for (int t0 = begin + wave * 64; t0 < end; t0 += kPaWaves * 64) {
-    const int t = min(t0 + lane, end - 1), cnt = min(64, end - t0);
-    int64_t mine = t < x.walked ? ldIndex(x.loc, t, x.loc64) : ldIndex(a.bLoc, locBase + (t - x.walked), a.loc64);
-    if (mine < 0 || mine >= a.slots) mine = -1;  // slots outside the pool are skipped, never dereferenced
-    for (int i = 0; i < cnt; i += UNR) {
-      float k[UNR][J], v[UNR][J], sc[UNR], mt = m;
-      bool counts[UNR];
-#pragma unroll
-      for (int u = 0; u < UNR; ++u) {
-        const int from = min(i + u, cnt - 1);
-        const int64_t slot = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(mine >> 32), from) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)mine, from));
-        counts[u] = i + u < cnt && slot >= 0;
-        const T* kRow = kHead + max(slot, (int64_t)0) * a.kSlotStride;
-        const T* vRow = vHead + max(slot, (int64_t)0) * a.vSlotStride;
-#pragma unroll
-        for (int j = 0; j < J; ++j) k[u][j] = static_cast<float>(kRow[at[j]]), v[u][j] = static_cast<float>(vRow[at[j]]);
-      }
-#pragma unroll
-      for (int u = 0; u < UNR; ++u) {
-        float d = 0.f;
-#pragma unroll
-        for (int j = 0; j < J; ++j) d += lane + 64 * j < a.d ? qf[j] * k[u][j] : 0.f;
-        sc[u] = waveSum(d);
-        if (!counts[u]) sc[u] = -INFINITY;
-        mt = fmaxf(mt, sc[u]);
-      }
-      const float ref = mt == -INFINITY ? 0.f : mt, corr = m == -INFINITY ? 1.f : exp2f(m - ref);  // (no maximum yet: the sums are 0, or NaN)
-      m = mt, l *= corr;
-#pragma unroll
-      for (int j = 0; j < J; ++j) acc[j] *= corr;
-#pragma unroll
-      for (int u = 0; u < UNR; ++u) {
-        if (!counts[u]) continue;
-        const float p = exp2f(sc[u] - ref);
-        l += p;
-#pragma unroll
-        for (int j = 0; j < J; ++j) acc[j] += p * v[u][j];
-      }
-    }
-  }
-  if (l != l && m == -INFINITY) m = 0.f;  // scores that are not numbers alone: as a maximum of minus infinity they would be left out
-  if (lane == 0) state[wave][0] = m, state[wave][1] = l;
-#pragma unroll
-  for (int j = 0; j < J; ++j) red[wave][lane + 64 * j] = acc[j];
-  __syncthreads();
-  float mAll = -INFINITY, lAll = 0.f, w[kPaWaves];
-#pragma unroll
-  for (int i = 0; i < kPaWaves; ++i) mAll = fmaxf(mAll, state[i][0]);
-#pragma unroll
-  for (int i = 0; i < kPaWaves; ++i) {
-    w[i] = state[i][0] == -INFINITY ? 0.f : exp2f(state[i][0] - mAll);
-    lAll += state[i][1] * w[i];
-  }
-  const int64_t pair = (int64_t)b * a.heads + h;
-  float* const dst = partial + (pair * x.anySplit + split) * (2 + a.d);
-  if (partial != nullptr && threadIdx.x == 0) dst[0] = mAll, dst[1] = lAll;
-  const float inv = lAll == 0.f ? 0.f : 1.f / lAll;
-  for (int e = threadIdx.x; e < a.d; e += kPaWaves * 64) {
-    float o = 0.f;
-#pragma unroll
-    for (int i = 0; i < kPaWaves; ++i) o += red[i][e] * w[i];
-    if (partial != nullptr) dst[2 + e] = o;
-    else out[pair * a.d + e] = static_cast<T>(o * inv);
-  }
-}
-
-// ------------------------------------------------ head rows of whole 16-byte pieces up to 512 bytes: the matrix pipe --
+// ------------------------------------------------ head rows of whole 16-byte pieces up to 256 elements: the matrix pipe --
 // The shared tokens see the same K and V from every sequence, so a K/V head's columns are the query heads that share it of ALL
 // sequences: S^T = K . Q^T and O^T += V^T . P^T with many columns for one read of a row. Partial results (maximum, sum, weighted
 // sum of V) of each chunk of the prefix go to workspace; those of the sequences' own tokens come from the kernels of
 // diopiTokenDecodeAttentionInference, which end on the shared tokens' where the own ones are one chunk; a last launch merges the partial
-// results of both where they are more.
+// results of both where they are more. (fp32 rows of more than 512 bytes, which those do not take: token_attention_any.hip.)
 //
 // Long prefixes are bound by memory, every shared row read once (for each group of columns), and, with many columns, by the matrix
 // pipe and the exponentials; short ones by the launches and the latency of slots, then rows.
@@ -1031,64 +937,28 @@ static diopiError_t launchFloat(hipStream_t stream, const TaPrefixArgs& x, int64
   return diopiSuccess;
 }
 
-// out from the partial results of x.nsplit chunks of the shared tokens and `own` of what comes behind (with the shared tokens in front
-// that x.walked counts).
-static diopiError_t mergeShares(hipStream_t stream, const TaPrefixArgs& x, diopiDtype_t dtype, void* out, const float* partial, const TaPartials& own) {
-  const TaArgs& a = x.a;
+diopiError_t mergeShares(hipStream_t stream, const TaArgs& a, diopiDtype_t dtype, void* out, const float* shared, int nShared, const TaPartials& own, int walked) {
   const int64_t pairs = (int64_t)a.batch * a.heads;
   // A wave has the elements of nine shares on their way at once. Up to those it needs no help; twice as many are still better left to
   // one than to four where there are many pairs: 2048 pairs, 10 shares 23.7 us (all launches) and 27.3; 512 pairs, 18 shares
   // 18.9 and 17.5.
-  const int shares = x.nsplit + own.nsplit;
+  const int shares = nShared + own.nsplit;
   const bool narrow = shares <= 9 || (shares <= 18 && pairs >= 1024);
   const unsigned blocks = (unsigned)ceilDiv(a.d, 256);
 #define PREFIX_MERGE(T)                                                                                                                               \
   do {                                                                                                                                                \
     if (narrow)                                                                                                                                       \
-      hipLaunchKernelGGL((decodePrefixMergeKernel<T, 1>), dim3((unsigned)ceilDiv(pairs, 4), blocks), dim3(256), 0, stream, static_cast<T*>(out), partial, \
-                         x.nsplit, own.partial, own.nsplit, own.chunk, own.raise, a.bLen, a.len64, a.maxLen, x.walked, pairs, a.heads, a.d);            \
+      hipLaunchKernelGGL((decodePrefixMergeKernel<T, 1>), dim3((unsigned)ceilDiv(pairs, 4), blocks), dim3(256), 0, stream, static_cast<T*>(out), shared, \
+                         nShared, own.partial, own.nsplit, own.chunk, own.raise, a.bLen, a.len64, a.maxLen, walked, pairs, a.heads, a.d);            \
     else                                                                                                                                              \
-      hipLaunchKernelGGL((decodePrefixMergeKernel<T, 4>), dim3((unsigned)pairs, blocks), dim3(256), 0, stream, static_cast<T*>(out), partial, x.nsplit, \
-                         own.partial, own.nsplit, own.chunk, own.raise, a.bLen, a.len64, a.maxLen, x.walked, pairs, a.heads, a.d);                      \
+      hipLaunchKernelGGL((decodePrefixMergeKernel<T, 4>), dim3((unsigned)pairs, blocks), dim3(256), 0, stream, static_cast<T*>(out), shared, nShared, \
+                         own.partial, own.nsplit, own.chunk, own.raise, a.bLen, a.len64, a.maxLen, walked, pairs, a.heads, a.d);                      \
   } while (0)
   if (dtype == diopi_dtype_bfloat16) PREFIX_MERGE(bf16_t);
   else if (dtype == diopi_dtype_float16) PREFIX_MERGE(half_t);
   else PREFIX_MERGE(float);
 #undef PREFIX_MERGE
   AMD_LAUNCH_CHECK();
-  return diopiSuccess;
-}
-
-// Partial results of x.walked shared tokens and the own ones behind them, of at least one chunk; of one alone, if nothing is to be
-// merged with it, the result (own->nsplit is 0 then). Four workgroups to a compute unit, chunks of whole rounds of the waves.
-static diopiError_t walkAny(diopiContextHandle_t ctx, hipStream_t stream, TaPrefixArgs x, diopiDtype_t dtype, void* out, bool alone, TaPartials* own) {
-  const TaArgs& a = x.a;
-  const int64_t pairs = (int64_t)a.batch * a.heads, total = std::max<int64_t>(1, (int64_t)x.walked + a.maxLen);
-  const int64_t most = std::min<int64_t>(kPxMaxSplit, std::max<int64_t>(1, 4 * computeUnits() / pairs));
-  x.anyChunk = (int)(ceilDiv(ceilDiv(total, most), kPaWaves * 64) * kPaWaves * 64);
-  x.anySplit = (int)ceilDiv(total, x.anyChunk);
-  float* partial = nullptr;
-  if (!alone || x.anySplit > 1) {
-    void* ws = nullptr;
-    AMD_TRY(requireWorkspace(ctx, pairs * x.anySplit * (2 + a.d) * (int64_t)sizeof(float), &ws));
-    partial = static_cast<float*>(ws);
-  }
-  const dim3 grid(a.heads, a.batch, x.anySplit);
-#define ANY_CALL_SIZE(T, J, UNR) hipLaunchKernelGGL((decodePrefixAnyKernel<T, J, UNR>), grid, dim3(kPaWaves * 64), 0, stream, x, static_cast<T*>(out), partial)
-#define ANY_CALL(T)                                       \
-  do {                                                    \
-    if (a.d <= 64) ANY_CALL_SIZE(T, 1, 8);                \
-    else if (a.d <= 128) ANY_CALL_SIZE(T, 2, 8);          \
-    else if (a.d <= 256) ANY_CALL_SIZE(T, 4, 4);          \
-    else ANY_CALL_SIZE(T, kTaGenericMaxD / 64, 1);        \
-  } while (0)
-  if (dtype == diopi_dtype_bfloat16) ANY_CALL(bf16_t);
-  else if (dtype == diopi_dtype_float16) ANY_CALL(half_t);
-  else ANY_CALL(float);
-#undef ANY_CALL
-#undef ANY_CALL_SIZE
-  AMD_LAUNCH_CHECK();
-  *own = TaPartials{partial, partial ? x.anySplit : 0, x.anyChunk, 0.f};
   return diopiSuccess;
 }
 
@@ -1147,13 +1017,15 @@ static diopiError_t decodeSharedPrefix(diopiContextHandle_t ctx, hipStream_t str
 #undef TILED_CALL
   TaPartials own{nullptr, 0, 1, 0.f};
   if (a.generic) {  // (rows of more than 512 bytes)
-    AMD_TRY(walkAny(ctx, stream, x, dtype, out, false, &own));
+    TaAnyArgs any{};
+    any.a = a;
+    AMD_TRY(walkAny(ctx, stream, any, dtype, out, false, &own));
   } else {
     a.shared = partial, a.nShared = x.nsplit;
     AMD_TRY(decodePartials(ctx, stream, a, dtype, a.maxLen, out, &own));
     if (own.nsplit == 0) return diopiSuccess;
   }
-  return mergeShares(stream, x, dtype, out, partial, own);
+  return mergeShares(stream, a, dtype, out, partial, x.nsplit, own, 0);
 }
 
 }  // namespace amd
@@ -1192,15 +1064,14 @@ extern "C" __attribute__((visibility("default"))) diopiError_t diopiTokenDecodeA
   if (prefix.shape[0] == 0) return diopiTokenDecodeAttentionInference(ctx, outH, qH, kH, vH, locH, startH, lenH, maxInputLen);  // nothing is shared
   AMD_TRY(makeContiguous(ctx, stream, prefix, &densePrefix));
   x.loc = densePrefix.data, x.loc64 = prefix.dtype == diopi_dtype_int64, x.len = (int)prefix.shape[0];
-  x.nsplit = 0, x.walked = 0;
   // head rows of whole 16-byte pieces up to 256 elements, slot numbers in 31 bits: the matrix pipe
   const int64_t bits = (int64_t)reinterpret_cast<uintptr_t>(a.q) | (int64_t)reinterpret_cast<uintptr_t>(a.k) | (int64_t)reinterpret_cast<uintptr_t>(a.v) |
                        (a.kSlotStride | a.kHeadStride | a.vSlotStride | a.vHeadStride | a.qBatchStride | a.qHeadStride | a.d) * t.q.itemsize;
   if ((bits & 15) == 0 && a.d <= 256 && a.slots <= 0x7fffffff && std::max(a.kSlotStride, a.vSlotStride) * t.q.itemsize <= 0xffffffffll)
     return decodeSharedPrefix(ctx, stream, x, t.q.dtype, out.data);
-  x.walked = x.len;
-  AMD_CHECK((int64_t)a.batch * a.heads < 1 << 24, "shared prefix attention: %d sequences of %d heads exceed the grid limits", a.batch, a.heads);
+  TaAnyArgs any{};
+  any.a = a, any.loc = x.loc, any.locIs64 = x.loc64, any.walked = x.len;
   TaPartials own;
-  AMD_TRY(walkAny(ctx, stream, x, t.q.dtype, out.data, true, &own));
-  return own.nsplit == 0 ? diopiSuccess : mergeShares(stream, x, t.q.dtype, out.data, nullptr, own);
+  AMD_TRY(walkAny(ctx, stream, any, t.q.dtype, out.data, true, &own));
+  return own.nsplit == 0 ? diopiSuccess : mergeShares(stream, a, t.q.dtype, out.data, nullptr, 0, own, any.walked);
 }

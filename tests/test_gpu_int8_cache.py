@@ -239,6 +239,13 @@ def test_slots_outside_the_pool_and_lengths_outside_the_table(ops, dev, dtype, d
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,d", [(2, 1, 20), (3, 3, 1), (4, 2, 300), (2, 2, 1024), (8, 2, 100), (2, 1, 250)])
+def test_head_sizes_of_any_kind_in_many_chunks(ops, dev, dtype, heads, kv_heads, d):
+    for seed, lens in enumerate(([0], [1, 0, 255], [256, 257], [20, 0, 3300], [64] * 9)):
+        check_attention(ops, dev, *batch_of(lens, heads, kv_heads, d, dtype, 200 + seed, torch.int64 if seed % 2 else torch.int32))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_one_key_far_above_the_rest_and_values_only_below_it(ops, dev, dtype):
     """The key with almost all of the weight has V = 0: what is left of each of the others counts."""
     heads, d, n = 2, 128, 400
