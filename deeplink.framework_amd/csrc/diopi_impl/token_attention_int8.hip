@@ -469,7 +469,8 @@ static diopiError_t int8Pool(const char* name, const TensorView& q, const Tensor
 static void chooseShares(TaInt8Args* x, int64_t len, int D) {
   TaArgs& a = x->a;
   const int64_t steps = (int64_t)a.kvHeads * a.qGroups * a.batch * ceilDiv(len, kI8Tile) * (D == 256 ? 4 : 1);
-  const int perWave = steps < 1536 ? 1 : steps < 3072 ? 2 : steps < 6144 ? 4 : steps < 57344 ? 8 : 16;
+  const int64_t perUnit = steps / computeUnits();
+  const int perWave = perUnit < 6 ? 1 : perUnit < 12 ? 2 : perUnit < 24 ? 4 : perUnit < 224 ? 8 : 16;
   // (heads in twos and fours leave waves without a head: of 5 in fours 3, 74 us where twos take 68)
   const int fits = a.kvHeads % 4 == 0 || a.kvHeads == 3 || a.kvHeads > 8 ? 4 : a.kvHeads >= 2 ? 2 : 1;
   x->headsPerWg = std::min(fits, perWave);
