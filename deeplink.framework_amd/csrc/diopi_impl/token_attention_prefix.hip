@@ -392,7 +392,9 @@ __device__ __forceinline__ typename PtMfma<T>::Frag ptPart(float (&x)[8]) {
       const Cut cut = __builtin_amdgcn_cvt_pkrtz(x[i], x[i + 1]);
       const Pair pair = __builtin_bit_cast(Pair, cut);
       part[i] = pair[0], part[i + 1] = pair[1];
-      x[i] = fmaf(static_cast<float>(pair[0]), -1.f, x[i]), x[i + 1] = fmaf(static_cast<float>(pair[1]), -1.f, x[i + 1]);
+      float minus = -1.f;
+      asm("" : "+s"(minus));  // (a constant here becomes a conversion and a subtraction)
+      x[i] = fmaf(static_cast<float>(pair[0]), minus, x[i]), x[i + 1] = fmaf(static_cast<float>(pair[1]), minus, x[i + 1]);
     } else {
       part[i] = static_cast<T>(x[i]), part[i + 1] = static_cast<T>(x[i + 1]);
       x[i] -= static_cast<float>(part[i]), x[i + 1] -= static_cast<float>(part[i + 1]);
