@@ -16,7 +16,6 @@ struct TaInt8Args {
   const float* vScale;
   int64_t kScaleSlot, kScaleHead, vScaleSlot, vScaleHead;  // strides in elements
   int headsPerWg;  // K/V heads of a workgroup: 1, 2 or 4
-  bool qVector;    // q can be read in 16-byte pieces
   bool scaleVector;  // the scales of a workgroup's four heads can be read at once
   unsigned kStride, vStride;  // slot strides of the pools in bytes, as decodeInt8Kernel takes them
 };
@@ -125,40 +124,51 @@ __global__ __launch_bounds__(kI8Waves * 64, D == 256 ? 1 : 2) void decodeInt8Ker
   const int end = min(len, begin + a.chunk);
   const int64_t locBase = (int64_t)b * a.locRowStride + (a.maxLen - len);
 
-  // q: product (p, s) of a row multiplies 8 places from placeOf(p) + 8 s on
+  // q: product (p, s) of a row multiplies 8 places from placeOf(p) + 8 s on. All of it is asked for at once, and worked on when the
+  // block's slots have been asked for too.
   auto placeOf = [&](int p) { return PIECES == 1 ? 16 * quad : 128 * (p >> 1) + 32 * quad + 16 * (p & 1); };
-  u32x4 qf[2 * PIECES][PQ];
+  constexpr int QLOADS = 8 / Vec16<T>::N;
+  typename Vec16<T>::type qr[2 * PIECES][QLOADS];
 #pragma unroll
   for (int p = 0; p < PIECES; ++p)
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       const int e = placeOf(p) + 8 * s;
-      const bool have = col < nq && e < a.d;
-      const T* src = reinterpret_cast<const T*>(a.q) + b * a.qBatchStride + (h + (have ? col : 0)) * a.qHeadStride + (have ? e : 0);
-      float v[8];
-      if (x.qVector) {
+      const T* src = reinterpret_cast<const T*>(a.q) + b * a.qBatchStride + (h + min(col, nq - 1)) * a.qHeadStride + (e < a.d ? e : 0);
 #pragma unroll
-        for (int c = 0; c < 8 / Vec16<T>::N; ++c) {
-          const auto r = *(reinterpret_cast<const typename Vec16<T>::type*>(src) + c);
-#pragma unroll
-          for (int j = 0; j < Vec16<T>::N; ++j) v[c * Vec16<T>::N + j] = static_cast<float>(r[j]);
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = static_cast<float>(src[j]);
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = have ? v[j] : 0.f;
-      if constexpr (std::is_same<T, half_t>::value) {
-        f16x8 whole;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) whole[j] = static_cast<half_t>(v[j]);
-        qf[2 * p + s][0] = __builtin_bit_cast(u32x4, whole);
-      } else {
-#pragma unroll
-        for (int k = 0; k < PQ; ++k) qf[2 * p + s][k] = __builtin_bit_cast(u32x4, nextPart(v));
-      }
+      for (int c = 0; c < QLOADS; ++c) qr[2 * p + s][c] = *(reinterpret_cast<const typename Vec16<T>::type*>(src) + c);
     }
+  // Slots of the block's tokens: a thread looks up two (past the last: that token again) as two words, the second zero, or for 32-bit
+  // indices the first again (a branch, or a conversion in one, would wait for the first load before it asks for the second). Without a
+  // token: what q begins with, for nothing.
+  int low[2], high[2];
+  auto askSlots = [&](int block, int n) {
+    const char* const locBytes = n > 0 ? static_cast<const char*>(a.bLoc) + ((locBase + block) << (a.loc64 ? 3 : 2)) : static_cast<const char*>(a.q);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const char* at = locBytes + ((int64_t)max(min((int)threadIdx.x + 256 * i, n - 1), 0) << (a.loc64 ? 3 : 2));
+      low[i] = *reinterpret_cast<const int*>(at), high[i] = *reinterpret_cast<const int*>(at + (a.loc64 ? 4 : 0));
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  askSlots(begin, min(kI8Block, end - begin));
+  u32x4 qf[2 * PIECES][PQ];
+#pragma unroll
+  for (int p = 0; p < 2 * PIECES; ++p) {
+    const bool have = col < nq && placeOf(p / 2) + 8 * (p % 2) < a.d;
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = have ? static_cast<float>(qr[p][j / Vec16<T>::N][j % Vec16<T>::N]) : 0.f;
+    if constexpr (std::is_same<T, half_t>::value) {
+      f16x8 whole;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) whole[j] = static_cast<half_t>(v[j]);
+      qf[p][0] = __builtin_bit_cast(u32x4, whole);
+    } else {
+#pragma unroll
+      for (int k = 0; k < PQ; ++k) qf[p][k] = __builtin_bit_cast(u32x4, nextPart(v));
+    }
+  }
 
   // Loads take whole 128-byte lines of 8 rows (or what of a row there is): K of two tiles of 8 tokens, in lanes 0 .. 7 and 8 .. 15
   // of each 16 the pieces 2 quad and 2 quad + 1, of which the lanes then swap one with the lane 8 aside; V of two tokens, one for each
@@ -303,17 +313,9 @@ __global__ __launch_bounds__(kI8Waves * 64, D == 256 ? 1 : 2) void decodeInt8Ker
   for (int block = begin; block < end; block += kI8Block) {
     const int n = min(kI8Block, end - block);
     if (block != begin) __syncthreads();  // every wave is done with the block before
-    // slots: a thread looks up two tokens (past the last: that token again) as two words, the second zero, or for 32-bit indices
-    // the first again (a branch, or a conversion in one, would wait for the first load before it asks for the second)
-    const char* const locBytes = static_cast<const char*>(a.bLoc) + ((locBase + block) << (a.loc64 ? 3 : 2));
-    int low[2], high[2];
+    if (block != begin) askSlots(block, n);
     unsigned slot[2];
     bool bad = false;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const char* at = locBytes + ((int64_t)min((int)threadIdx.x + 256 * i, n - 1) << (a.loc64 ? 3 : 2));
-      low[i] = *reinterpret_cast<const int*>(at), high[i] = *reinterpret_cast<const int*>(at + (a.loc64 ? 4 : 0));
-    }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       // slots outside the pool are skipped, never dereferenced
@@ -492,7 +494,13 @@ static diopiError_t decodeInt8(diopiContextHandle_t ctx, hipStream_t stream, TaI
   TaArgs& a = x.a;
   const int64_t perKv = a.heads / a.kvHeads, len = std::max(a.maxLen, 1);
   a.qGroups = (int)ceilDiv(perKv, kI8Heads);
-  x.qVector = q.aligned16() && ((q.stride[0] | q.stride[1]) * q.itemsize) % 16 == 0;
+  if (!q.aligned16() || ((q.stride[0] | q.stride[1]) * q.itemsize) % 16 != 0) {  // the kernel reads whole 16 bytes: a dense copy of q
+    diopiTensorHandle_t th = nullptr;
+    TensorView dense;
+    AMD_TRY(requireTensor(ctx, q.shape, q.ndim, q.dtype, &th, &dense));
+    AMD_TRY(stridedCopy(stream, q, dense));
+    a.q = dense.data, a.qBatchStride = dense.stride[0], a.qHeadStride = dense.stride[1];
+  }
   const int D = a.d <= 64 ? 64 : a.d <= 128 ? 128 : 256;
   chooseShares(&x, len, D);
   x.scaleVector = x.headsPerWg == 4 && a.kvHeads % 4 == 0 && x.kScaleHead == 1 && x.vScaleHead == 1 && (x.kScaleSlot | x.vScaleSlot) % 4 == 0 &&

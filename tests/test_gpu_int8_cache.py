@@ -307,6 +307,17 @@ def test_q_and_pools_at_other_strides_and_alignments(ops, dev, dtype):
             assert_exact(out, want)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_q_off_any_alignment(ops, dev, dtype):
+    q, pools, b_loc, lens, max_len = batch_of([150, 33, 0, 1], 6, 2, 64, dtype, 75)
+    want = run_attention(ops, dev, q, pools, b_loc, lens, max_len)
+    for view in (lambda x: x[1:1 + q.numel()].view(q.shape), lambda x: x[:4 * 6 * 65].view(4, 6, 65)[..., 1:], lambda x: x[3:3 + 4 * 67 * 6].view(6, 4, 67).transpose(0, 1)[..., :64]):
+        moved = view(torch.full((4 * 6 * 70,), 7.0, dtype=dtype, device=dev))
+        moved.copy_(q)
+        got = ops.token_decode_attention_int8(moved, *[t.to(dev) for pool in pools for t in pool], b_loc.to(dev), lens.to(dev), lens.to(dev), max_len)
+        assert_exact(got, want)
+
+
 def test_no_sequences_and_no_tokens(ops, dev):
     kp, ks = torch.ones(4, 2, 64, dtype=torch.int8, device=dev), torch.ones(4, 2, device=dev)
     none = torch.zeros(0, dtype=torch.int32, device=dev)
