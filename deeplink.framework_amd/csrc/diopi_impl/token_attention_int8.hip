@@ -463,7 +463,7 @@ static diopiError_t int8Pool(const char* name, const TensorView& q, const Tensor
 // there are many (what a workgroup does before its first step, and its partial results, are then spread over more). With four
 // heads to a workgroup a wave reads 512 adjacent bytes of a token with the other three, and one lane the scales of all four: 64 x
 // (512 .. 4096) tokens, 32 heads of 128, 231 us, with one head 383 (48, 8 heads 59 and 87). Few steps are better dealt over the
-// waves of a head: 1 x 1777 tokens, 8 heads, one step to a wave, 10.3 with one head, 11.4 with four.
+// waves of a head: 1 x 1777 tokens, 8 heads, one step to a wave, 10.3 with one head, 11.4 with four (each before q and the first slots were asked for at once: 9.9).
 // us at 1, 2, 4, 8, 16 steps to a wave: 1 x 4096, 8 heads 10.6, 11.3, 13.6, 18.0, 25.1; 1 x 8192 14.2, 13.2, 15.2, 18.5, 25.5; 1 x 16384
 // 25.3, 20.0, 18.5, 19.4, 25.7; 8 x 4096 37, 28, 22.7, 20.7, 26.2; 16 x (1000 .. 8000) 84, 58, 48, 47, 47; 48 x (512 .. 4096) 120, 82, 69, 59, 72;
 // 32 heads, 64 x (512 .. 4096) 627, 385, 297, 247, 231. Heads of 256: a SIMD holds one wave instead of two, and a step takes twice as
