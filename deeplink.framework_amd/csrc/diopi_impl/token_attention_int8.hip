@@ -30,9 +30,10 @@ struct TaInt8Args {
 //     the operand P^T of O^T += V^T . P^T. That operand wants eight tokens of V at one place of the head per lane: the lane loads
 //     D / 16 adjacent bytes of each of its eight tokens, and the conversion to bf16 (one instruction per byte, whichever byte)
 //     picks one byte out of each: V is turned round by the conversion that it needs anyway. So no row passes through LDS.
-//   * the scale of K multiplies the score, that of V the probability, both in fp32; the product is cut into parts of 8 bits, each
-//     the rounding of what the ones before it leave: two for 16-bit results (off by at most 2^-16 relative, a hundredth of the
-//     rounding of the result), three for fp32 (all 24 bits). bf16 parts have the range of fp32, so small weights keep theirs.
+//   * the scale of K multiplies the score, that of V the probability, both in fp32; the product is cut into three parts of 8 bits,
+//     each the rounding of what the ones before it leave: all 24 bits, for 16-bit results too (a sum that cancels shows what two
+//     would lose; the third costs 1 %: 64 x (512 .. 4096), 32 heads, 230.7 -> 233.2 us). bf16 parts have the range of fp32, so
+//     small weights keep theirs.
 //   * the running maximum is followed at once (probabilities are at most one: a value near the type's largest does not
 //     overflow); lanes exchange it only when one of them sees a larger one.
 constexpr int kI8Waves = 4;
@@ -43,7 +44,7 @@ constexpr int kI8Heads = 16;  // query heads a wave serves
 template <typename T>
 struct I8Parts {  // operands that hold q, and those that a probability is cut into
   static constexpr int kQ = std::is_same<T, float>::value ? 3 : 1;
-  static constexpr int kP = std::is_same<T, float>::value ? 3 : 2;
+  static constexpr int kP = 3;
 };
 
 // Bytes B0 of w0 and B1 of w1, signed, as two bf16 (exact: the upper half of the fp32 number).
