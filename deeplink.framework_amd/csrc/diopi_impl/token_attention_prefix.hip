@@ -344,9 +344,11 @@ __global__ __launch_bounds__(kPxWaves * 64, 1) void decodePrefixFloatKernel(TaPr
 // multiply at the same time and then both take exponentials (matrix pipe busy for 7.5 us, vector ALUs for 11, LDS between them). Half the
 // waves a phase behind the other half was no faster (45 us).
 //
-// The maximum is followed when a score exceeds it by more than 2^8. bf16 probabilities are cut into two bf16 parts (off by at most
-// 2^-16 relative). fp16 ones, times 2^7 (so at most 2^15), into two fp16 parts: 22 bits of those down to 2^-10 of the largest, 16 down
-// to 2^-16; a step that has smaller ones multiplies what is left of them times 2^24, 2^48 ... too, until nothing is left.
+// The maximum is followed when a score exceeds it by more than 2^8. bf16 probabilities are cut into three bf16 parts, all 24 bits of
+// them (as the own tokens' kernels cut theirs; the third costs 1 to 9 %: 16001 tokens, 48 sequences of 4 columns each, all launches, 47.8 -> 51.8 us, 3 of them 28.6 ->
+// 28.8). fp16 ones, times 2^7 (so at most 2^15), into two fp16 parts: 22 bits of those down to 2^-10 of the largest, 16 down
+// to 2^-16, less than 2^-32 of the largest in any case (an argument of -10 is rounded to 2^-21 of its exponential before that); a
+// step that has smaller ones multiplies what is left of them times 2^24, 2^48 ... too, until nothing is left.
 constexpr int kPtWaves = 8;
 constexpr float kPtRescaleStep = 8.f;  // log2 domain
 constexpr float kPtTwoParts = 16.f;    // two fp16 parts hold 16 bits of what is at least 2^-this
@@ -677,7 +679,7 @@ __global__ __launch_bounds__(kPtWaves * 64, 2) void decodePrefixTiledKernel(TaPr
     for (int s = 0; s < stages; ++s) {
       const bool all = !CAREFUL && clean && (s + 1) * TOKENS <= n;
       const int next = stage + 1 == STAGES ? 0 : stage + 1;
-      Frag hi[NC], lo[NC], some[CAREFUL ? NC : 1];
+      Frag hi[NC], lo[NC], last[HALF ? 1 : NC], some[CAREFUL ? NC : 1];
       u32x4 v[kAhead], keep = {~0u, ~0u, ~0u, ~0u};
       bool small = false;  // of a probability some bits may be left
       if (active) {
@@ -704,7 +706,9 @@ __global__ __launch_bounds__(kPtWaves * 64, 2) void decodePrefixTiledKernel(TaPr
 #pragma unroll
             for (int i = 0; i < 8; ++i) some[c][i] = static_cast<T>(w[i] > 0.f ? 1.f : w[i]);
           }
-          hi[c] = ptPart<T>(w), lo[c] = ptLast<T>(w);
+          hi[c] = ptPart<T>(w);
+          if constexpr (HALF) lo[c] = ptLast<T>(w);
+          else lo[c] = ptPart<T>(w), last[c] = ptLast<T>(w);
         }
       }
       if (s + 1 < stages) {
@@ -730,6 +734,10 @@ __global__ __launch_bounds__(kPtWaves * 64, 2) void decodePrefixTiledKernel(TaPr
           for (int c = 0; c < N; ++c) acc[c][d] = M::run(now, hi[c], acc[c][d]);
 #pragma unroll
           for (int c = 0; c < N; ++c) acc[c][d] = M::run(now, lo[c], acc[c][d]);
+          if constexpr (!HALF) {
+#pragma unroll
+            for (int c = 0; c < N; ++c) acc[c][d] = M::run(now, last[c], acc[c][d]);
+          }
         }
         if constexpr (HALF) {
           if (__builtin_amdgcn_ballot_w64(small) != 0) addRest(stage, s * TOKENS, all, columnTiles, withCare);

@@ -41,3 +41,39 @@ def test_int8_sums_that_cancel(ops, dev, dtype, d):
     bound = 10 * U * sizes
     bound += (want.abs() + bound) * HALF_STEP[dtype] + U * (dtype == torch.float16)
     oracle.assert_within(got, want[..., None].expand(-1, -1, d), bound[..., None].expand(-1, -1, d))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("where", ["shared", "own"])
+def test_sums_that_cancel_behind_a_prefix(ops, dev, dtype, d, where):
+    """Three tokens: one with a weight p < 1 and values v, two of the largest score with values that add up to -p v but for its
+    last bits. Scores are one product of few bits, so only its scaling and the exponential round: p is off by (2 + 3) u |score| + 4 u
+    and u where it is cut, with |score| < 1 by 10 u; sums over three tokens by (3 + 8) u of the magnitudes."""
+    heads, n = 8, 64                                               # a head of a token triple for each of n pools' places
+    score = -torch.rand(n, heads, generator=g(11)).bfloat16().double()
+    p = torch.exp(score)
+    v = (1 + torch.rand(n, heads, generator=g(12))).bfloat16().double()
+    first = (-p * v).to(dtype).double()
+    second = (-p * v - first).to(dtype).double()
+    outs, wants, bounds = [], [], []
+    q = torch.zeros(1, heads, d, dtype=dtype)
+    q[..., 0] = 1
+    for i in range(n):
+        kk, vv = torch.zeros(4, heads, d, dtype=dtype), torch.zeros(4, heads, d, dtype=dtype)
+        kk[0, :, 0] = (score[i] * math.sqrt(d)).to(dtype)
+        for t, x in enumerate((v, first, second)):
+            vv[t] = x[i][:, None].to(dtype)
+        have = kk[0, :, 0].double() / math.sqrt(d)                 # (sqrt(128) does not end: the score that the key stands for)
+        p_i = torch.exp(have)
+        prefix, loc = (torch.arange(3), torch.tensor([[3]])) if where == "shared" else (torch.tensor([3]), torch.arange(3)[None])
+        kk[3, :, 0] = -30000.0 if dtype == torch.float16 else -3e4   # the other side has no weight
+        lens = torch.tensor([loc.shape[1]])
+        outs.append(shared.run(ops, dev, q, kk, vv, prefix, loc, lens, loc.shape[1]).cpu()[0])
+        total = p_i + 2
+        want = (p_i * v[i] + first[i] + second[i]) / total
+        sizes = (p_i * v[i] + first[i].abs() + second[i].abs()) / total
+        bound = (10 * p_i * v[i] / total + 11 * sizes) * U
+        wants.append(want), bounds.append(bound + (want.abs() + bound) * HALF_STEP[dtype] + U * (dtype == torch.float16))
+    spread = lambda rows: torch.stack(rows)[..., None].expand(-1, -1, d)
+    oracle.assert_within(torch.stack(outs), spread(wants), spread(bounds))
