@@ -154,7 +154,7 @@ __global__ __launch_bounds__(kTaWaves * 64, splitWavesPerSimd(sizeof(T), LPT, HI
     nq = base + (g < rem ? 1 : 0);
   }
   auto headOf = [&](int j) { return QPK == 1 ? 0 : min(j, nq - 1); };  // offset of place j's head from h
-  const int len = min(max((int)ldIndex(a.bLen, b, a.len64), 0), a.maxLen);  // a length beyond the table's width is cut to it
+  const int len = cutLength(a.bLen, b, a.len64, a.maxLen);
   const int begin = split * a.chunk;
   if (begin >= len && !(split == 0 && MODE != kTaLogitsOut)) return;  // nothing to do; split 0 still writes zeros for len == 0
   const int end = min(len, begin + a.chunk);
@@ -516,7 +516,7 @@ __global__ __launch_bounds__(kGqWaves * 64, MODE == kTaFused && D == 256 ? 1 : k
   const int b = rest % a.batch, split = a.nsplit - 1 - rest / a.batch;
   const int perKv = a.heads / a.kvHeads, base = perKv / a.qGroups, rem = perKv % a.qGroups;
   const int h = kvh * perKv + g * base + min(g, rem), nq = base + (g < rem ? 1 : 0);  // the sharers are dealt evenly
-  const int len = min(max((int)ldIndex(a.bLen, b, a.len64), 0), a.maxLen);
+  const int len = cutLength(a.bLen, b, a.len64, a.maxLen);
   const int begin = split * a.chunk;
   if (begin >= len && !(split == 0 && MODE != kTaLogitsOut)) return;  // split 0 still writes zeros for len == 0
   const int end = min(len, begin + a.chunk);
@@ -865,7 +865,7 @@ walk:
 // discarded by a select, never multiplied).
 template <typename T, int SPLITS>
 __global__ __launch_bounds__(256) void decodeMergeKernel(T* __restrict__ out, const float* __restrict__ partial,
-                                                          const void* bLen, bool len64, int64_t pairs, int heads,
+                                                          const void* bLen, bool len64, int maxLen, int64_t pairs, int heads,
                                                           int d, int nsplit, int chunk) {
   constexpr int kMaxPerLane = 4;  // d <= 256
   const int lane = threadIdx.x & 63;
@@ -879,7 +879,7 @@ __global__ __launch_bounds__(256) void decodeMergeKernel(T* __restrict__ out, co
     ms = src[lane * row];
     ls = src[lane * row + 1];
   }
-  const int len = (int)ldIndex(bLen, b, len64);
+  const int len = cutLength(bLen, b, len64, maxLen);
   float v[SPLITS][kMaxPerLane];
 #pragma unroll
   for (int u = 0; u < SPLITS; ++u) {
@@ -890,7 +890,7 @@ __global__ __launch_bounds__(256) void decodeMergeKernel(T* __restrict__ out, co
       v[u][k] = e < d ? r[e] : 0.f;
     }
   }
-  const int used = len <= 0 ? 1 : min(nsplit, (len + chunk - 1) / chunk);
+  const int used = min(nsplit, chunksWritten(len, chunk));
   if (lane >= used) ms = -INFINITY, ls = 0.f;
   const float m = waveMax(ms);
   float wgt = (ms == -INFINITY) ? 0.f : exp2f(ms - m);
@@ -915,7 +915,7 @@ __global__ __launch_bounds__(256) void decodeMergeKernel(T* __restrict__ out, co
 // combines splits w, w + 4, ... and the four sums meet in LDS.
 template <typename T>
 __global__ __launch_bounds__(256) void decodeMergeWideKernel(T* __restrict__ out, const float* __restrict__ partial,
-                                                              const void* bLen, bool len64, int heads, int d, int nsplit,
+                                                              const void* bLen, bool len64, int maxLen, int heads, int d, int nsplit,
                                                               int chunk) {
   constexpr int kBatch = 8, kMaxPerLane = 4, kPerLane = kTaMaxSplit / 64;  // d <= 256
   __shared__ float red[4][64 * kMaxPerLane];
@@ -945,8 +945,8 @@ __global__ __launch_bounds__(256) void decodeMergeWideKernel(T* __restrict__ out
     }
   };
   loadBatch(wave);
-  const int len = (int)ldIndex(bLen, b, len64);
-  const int used = len <= 0 ? 1 : min(nsplit, (len + chunk - 1) / chunk);
+  const int len = cutLength(bLen, b, len64, maxLen);
+  const int used = min(nsplit, chunksWritten(len, chunk));
   float m = -INFINITY;
 #pragma unroll
   for (int k = 0; k < kPerLane; ++k) {
@@ -997,7 +997,7 @@ __global__ __launch_bounds__(256) void decodeGenericKernel(TaArgs a, T* __restri
   __shared__ int64_t slotOf[256];
   __shared__ float red[4];
   const int h = blockIdx.x, b = blockIdx.z, tid = threadIdx.x;
-  const int len = min(max((int)ldIndex(a.bLen, b, a.len64), 0), a.maxLen);
+  const int len = cutLength(a.bLen, b, a.len64, a.maxLen);
   const int kvh = h / (a.heads / a.kvHeads);
   const int64_t locBase = (int64_t)b * a.locRowStride + (a.maxLen - len);
   const T* q = reinterpret_cast<const T*>(a.q) + b * a.qBatchStride + h * a.qHeadStride;
@@ -1048,7 +1048,7 @@ __global__ __launch_bounds__(256) void decodeGenericKernel(TaArgs a, T* __restri
 template <typename T, typename OT>
 __global__ __launch_bounds__(256) void tokenLogitsGenericKernel(TaArgs a, OT* __restrict__ att, int64_t attHeadStride) {
   const int h = blockIdx.x, b = blockIdx.z;
-  const int len = min(max((int)ldIndex(a.bLen, b, a.len64), 0), a.maxLen);
+  const int len = cutLength(a.bLen, b, a.len64, a.maxLen);
   const int64_t start = ldIndex(a.bStart, b, a.start64);
   const int begin = blockIdx.y * a.chunk, end = min(len, begin + a.chunk);
   const int kvh = h / (a.heads / a.kvHeads);
@@ -1077,7 +1077,7 @@ __global__ __launch_bounds__(256) void softmaxReduceVGenericKernel(TaArgs a, T* 
   __shared__ int64_t slotOf[256];
   __shared__ float red[4];
   const int h = blockIdx.x, b = blockIdx.z, tid = threadIdx.x;
-  const int len = min(max((int)ldIndex(a.bLen, b, a.len64), 0), a.maxLen);
+  const int len = cutLength(a.bLen, b, a.len64, a.maxLen);
   const int64_t start = ldIndex(a.bStart, b, a.start64);
   const int kvh = h / (a.heads / a.kvHeads);
   const int64_t locBase = (int64_t)b * a.locRowStride + (a.maxLen - len);
@@ -1264,7 +1264,7 @@ diopiError_t mergeChunks(hipStream_t stream, diopiDtype_t dtype, void* out, cons
     AMD_CHECK(a.nsplit <= kTaMaxSplit && a.d <= 256, "token attention: %d splits of head size %d cannot be merged", a.nsplit, a.d);
 #define MERGE_WIDE_CALL(T)                                                                                                       \
   hipLaunchKernelGGL((decodeMergeWideKernel<T>), dim3((unsigned)pairs), dim3(256), 0, stream, static_cast<T*>(out), partial, a.bLen, \
-                     a.len64, a.heads, a.d, a.nsplit, a.chunk)
+                     a.len64, a.maxLen, a.heads, a.d, a.nsplit, a.chunk)
     TA_GENERIC_DISPATCH(dtype, MERGE_WIDE_CALL);
 #undef MERGE_WIDE_CALL
   } else {
@@ -1272,10 +1272,10 @@ diopiError_t mergeChunks(hipStream_t stream, diopiDtype_t dtype, void* out, cons
 #define MERGE_CALL(T)                                                                                                               \
   if (a.nsplit <= kTaNarrowSplits)                                                                                                  \
     hipLaunchKernelGGL((decodeMergeKernel<T, kTaNarrowSplits>), mgrid, mblock, 0, stream, static_cast<T*>(out), partial, a.bLen,     \
-                       a.len64, pairs, a.heads, a.d, a.nsplit, a.chunk);                                                            \
+                       a.len64, a.maxLen, pairs, a.heads, a.d, a.nsplit, a.chunk);                                                            \
   else                                                                                                                              \
     hipLaunchKernelGGL((decodeMergeKernel<T, kTaNarrowSplitsMany>), mgrid, mblock, 0, stream, static_cast<T*>(out), partial, a.bLen, \
-                       a.len64, pairs, a.heads, a.d, a.nsplit, a.chunk)
+                       a.len64, a.maxLen, pairs, a.heads, a.d, a.nsplit, a.chunk)
     TA_GENERIC_DISPATCH(dtype, MERGE_CALL);
 #undef MERGE_CALL
   }

@@ -14,6 +14,17 @@ __device__ __forceinline__ int64_t ldIndex(const void* p, int64_t i, bool is64) 
   return is64 ? reinterpret_cast<const int64_t*>(p)[i] : static_cast<int64_t>(reinterpret_cast<const int32_t*>(p)[i]);
 }
 
+// Tokens of sequence b: a length outside [0, maxLen], what the table's row holds, is cut to that. All launches of a call take it from
+// here: partial results are merged where they were written, and nowhere else. As two words, the second for 32-bit lengths the first
+// again: a conversion in a branch on the type would wait for the length before anything else is asked for (0.3 us of the small merges).
+__device__ __forceinline__ int cutLength(const void* bLen, int64_t b, bool is64, int maxLen) {
+  const int* const p = static_cast<const int*>(bLen) + (b << (is64 ? 1 : 0));
+  const int low = p[0], high = p[is64 ? 1 : 0];
+  return high < 0 ? 0 : is64 && high != 0 ? maxLen : (int)min((unsigned)low, (unsigned)maxLen);
+}
+// Chunks of a sequence whose partial results are written: those that hold tokens, and the first.
+__device__ __forceinline__ int chunksWritten(int len, int chunk) { return len <= 0 ? 1 : (len - 1) / chunk + 1; }
+
 struct TaArgs {
   const void* q;
   const void* k;

@@ -21,7 +21,7 @@ __global__ __launch_bounds__(kPaWaves * 64) void decodeAnyKernel(TaAnyArgs x, T*
   __shared__ float red[kPaWaves][64 * J], state[kPaWaves][2];
   const TaArgs& a = x.a;
   const int h = blockIdx.x, b = blockIdx.y, split = blockIdx.z, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int len = (int)min(max(ldIndex(a.bLen, b, a.len64), (int64_t)0), (int64_t)a.maxLen), all = x.walked + len;
+  const int len = cutLength(a.bLen, b, a.len64, a.maxLen), all = x.walked + len;
   const int begin = split * x.chunk, end = min(all, begin + x.chunk);
   if (begin >= all && split != 0) return;
   const int kvh = h / (a.heads / a.kvHeads);

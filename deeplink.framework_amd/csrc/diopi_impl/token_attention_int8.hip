@@ -119,7 +119,7 @@ __global__ __launch_bounds__(kI8Waves * 64, D == 256 ? 1 : 2) void decodeInt8Ker
   const float* const scales = scaleBuf + wave % hw * kI8Block;
   const int perKv = a.heads / a.kvHeads, base = perKv / a.qGroups, rem = perKv % a.qGroups;
   const int h = kvh * perKv + g * base + min(g, rem), nq = base + (g < rem ? 1 : 0);  // the sharers are dealt evenly
-  const int len = (int)min(max(ldIndex(a.bLen, b, a.len64), (int64_t)0), (int64_t)a.maxLen);
+  const int len = cutLength(a.bLen, b, a.len64, a.maxLen);
   const int begin = split * a.chunk;
   if (begin >= len && split != 0) return;  // split 0 still writes zeros for len == 0
   const int end = min(len, begin + a.chunk);

@@ -872,8 +872,7 @@ __global__ __launch_bounds__(256) void decodePrefixMergeKernel(T* __restrict__ o
     }
   };
   loadBatch(part);
-  const int64_t len = walked + min(max(ldIndex(bLen, pair / heads, len64), (int64_t)0), (int64_t)maxLen);
-  const int used = nShared + (nOwn == 0 ? 0 : len <= 0 ? 1 : (int)((len + chunk - 1) / chunk));
+  const int used = nShared + (nOwn == 0 ? 0 : chunksWritten(walked + cutLength(bLen, pair / heads, len64, maxLen), chunk));
   float m = -INFINITY;
 #pragma unroll
   for (int k = 0; k < kPerLane; ++k) {

@@ -77,3 +77,39 @@ def test_sums_that_cancel_behind_a_prefix(ops, dev, dtype, d, where):
         wants.append(want), bounds.append(bound + (want.abs() + bound) * HALF_STEP[dtype] + U * (dtype == torch.float16))
     spread = lambda rows: torch.stack(rows)[..., None].expand(-1, -1, d)
     oracle.assert_within(torch.stack(outs), spread(wants), spread(bounds))
+
+
+# ------------------------------------------------------------------ lengths
+LENGTHS = [(torch.int64, [2 ** 31, 2 ** 32 + 5, 2 ** 40, 2 ** 31 - 1, -2 ** 32 + 7, -2 ** 63, 2 ** 63 - 1, 3]),
+           (torch.int32, [2 ** 31 - 1, -2 ** 31, 2 ** 31 - 64, 2 ** 31 - 500, 3])]
+
+
+def cut(lens, max_len):
+    return torch.tensor(lens).clamp(0, max_len)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("index,lens", LENGTHS)
+@pytest.mark.parametrize("max_len", [40, 600, 4096])
+@pytest.mark.parametrize("heads,kv_heads,d", [(2, 2, 64), (8, 1, 128), (4, 4, 128), (2, 1, 18)])
+def test_any_length_is_cut_to_the_table(ops, dev, dtype, index, lens, max_len, heads, kv_heads, d):
+    """Every launch of a call has to cut a length to the same: one chunk, several, and more than the small merge takes."""
+    batch, slots = len(lens), max_len + 200
+    q = torch.randn(batch, heads, d, generator=g(21)).to(dtype).to(dev)
+    k, v = [torch.randn(slots, kv_heads, d, generator=g(22 + i)).to(dtype).to(dev) for i in range(2)]
+    (kp, ks), (vp, vs) = [[t.to(dev) for t in pool] for pool in int8.empty_pools(slots, kv_heads, d)]
+    loc = torch.randint(0, slots, (batch, max_len + 3), generator=g(24)).to(index).to(dev)
+    prefix = torch.randperm(slots, generator=g(25))[:130].to(index).to(dev)
+    start = (torch.arange(batch) * max_len).to(index).to(dev)
+    given, within = torch.tensor(lens).to(index).to(dev), cut(lens, max_len).to(index).to(dev)
+
+    def halves(n):
+        scores = torch.zeros(heads, batch * max_len, dtype=torch.float32, device=dev)
+        ops.token_attention(q, k, scores, loc, start, n, max_len)
+        return torch.cat([scores.flatten(), ops.token_softmax_reducev(scores, v, torch.empty_like(q), loc, start, n, max_len).float().flatten()])
+
+    for call in (lambda n: ops.token_decode_attention(q, k, v, loc, start, n, max_len),
+                 lambda n: ops.token_decode_attention_int8(q, kp, ks, vp, vs, loc, start, n, max_len),
+                 lambda n: ops.token_decode_attention_shared_prefix(q, k, v, prefix, loc, start, n, max_len),
+                 halves):
+        assert_exact(call(given), call(within))
