@@ -330,12 +330,14 @@ __global__ __launch_bounds__(kTaWaves * 64, splitWavesPerSimd(sizeof(T), LPT, HI
             else if (j < nq) scores[j * a.logitsHeadStride + t] = static_cast<LT>(sc[u]);
           }
         }
-      } else if (mn != -INFINITY) {
-        float corr = __builtin_amdgcn_exp2f(m[j] - mn);  // m == -inf gives 0, acc and l are 0 then anyway
+      } else {
+        // (no maximum yet: tokens that do not count weigh nothing, and scores that are not numbers, which no maximum shows, are not left out)
+        const float ref = mn == -INFINITY ? 0.f : mn;
+        float corr = __builtin_amdgcn_exp2f(m[j] - ref);  // m == -inf gives 0: acc and l are 0 then, or NaN
         float p[UNR], ps = 0.f;
 #pragma unroll
         for (int u = 0; u < UNR; ++u) {
-          p[u] = __builtin_amdgcn_exp2f(sc[u] - mn);
+          p[u] = __builtin_amdgcn_exp2f(sc[u] - ref);
           ps += p[u];
         }
         l[j] = l[j] * corr + ps;

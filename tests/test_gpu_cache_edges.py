@@ -113,3 +113,36 @@ def test_any_length_is_cut_to_the_table(ops, dev, dtype, index, lens, max_len, h
                  lambda n: ops.token_decode_attention_shared_prefix(q, k, v, prefix, loc, start, n, max_len),
                  halves):
         assert_exact(call(given), call(within))
+
+
+# ------------------------------------------------------------------ scores that are not numbers, or far from zero
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,d", [(2, 2, 64), (8, 8, 64), (8, 1, 128), (12, 4, 80), (2, 1, 18)])
+@pytest.mark.parametrize("prefix_len", [0, 1, 40, 250, 9500])      # no, one, several shares, and more than the own tokens end on
+def test_a_key_that_is_not_a_number_is_never_left_out(ops, dev, dtype, heads, kv_heads, d, prefix_len):
+    lens = [1, 2, 3, 0, 17]
+    q, k, v, prefix, loc, n, max_len = shared.batch_of(prefix_len, lens, heads, kv_heads, d, dtype, 60)
+    for b, t in ((0, 0), (1, 0), (1, 1), (2, 1), (4, 0), (4, 16)):     # token t of sequence b
+        slot = loc[b, max_len - lens[b] + t]
+        kept = k[slot, kv_heads - 1].clone()
+        k[slot, kv_heads - 1, 3] = math.nan
+        got = shared.run(ops, dev, q, k, v, prefix, loc, n, max_len).cpu()
+        hit = torch.zeros(len(lens), heads, d, dtype=torch.bool)
+        hit[b, heads - heads // kv_heads:] = True
+        assert torch.equal(got.isnan(), hit)
+        k[slot, kv_heads - 1] = kept
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,d", [(2, 2, 64), (8, 8, 64), (8, 1, 128), (2, 1, 18)])
+def test_stored_scores_that_are_not_numbers(ops, dev, dtype, heads, kv_heads, d):
+    lens, max_len = torch.tensor([1, 2, 40, 5]), 40
+    v = torch.randn(90, kv_heads, d, generator=g(65)).to(dtype).to(dev)
+    loc, start = torch.randint(0, 90, (4, max_len), generator=g(66)).to(dev), torch.arange(4) * max_len
+    for b, t in ((0, 0), (1, 0), (1, 1), (2, 39), (3, 2)):
+        scores = torch.randn(heads, 4 * max_len, generator=g(67))
+        scores[heads - 1, b * max_len + t] = math.nan
+        out = ops.token_softmax_reducev(scores.to(dev), v, torch.empty(4, heads, d, dtype=dtype, device=dev), loc, start.to(dev), lens.to(dev), max_len).cpu()
+        hit = torch.zeros(4, heads, d, dtype=torch.bool)
+        hit[b, heads - 1] = True
+        assert torch.equal(out.isnan(), hit)
