@@ -35,7 +35,9 @@ struct TaInt8Args {
 //     would lose; the third costs 1 %: 64 x (512 .. 4096), 32 heads, 230.7 -> 233.2 us). bf16 parts have the range of fp32, so
 //     small weights keep theirs.
 //   * the running maximum is followed at once (probabilities are at most one: a value near the type's largest does not
-//     overflow); lanes exchange it only when one of them sees a larger one.
+//     overflow); lanes exchange it only when one of them sees a larger one. Scores are rounded in units of log2 before it is taken
+//     from them (K's scales in LDS hold 1 / (sqrt(d) ln 2) too): a multiply-add would leave the rounding of the maximum in the
+//     exponent, which from 2^31 on is more than a number holds.
 constexpr int kI8Waves = 4;
 constexpr int kI8Tile = 32;   // tokens of a wave's step
 constexpr int kI8Block = 512;  // tokens whose slots and scales a workgroup holds in LDS at once
@@ -215,8 +217,8 @@ __global__ __launch_bounds__(kI8Waves * 64, D == 256 ? 1 : 2) void decodeInt8Ker
   f32x4 acc[RUN];
 #pragma unroll
   for (int t = 0; t < RUN; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-  // this lane's head: the largest score, the same in units of log2, and what scores are taken against (that, or 0 while there is none)
-  float most = -INFINITY, m = -INFINITY, mRef = 0.f, l = 0.f;
+  // this lane's head: the largest score (in units of log2), and what scores are taken against (that, or 0 while there is none)
+  float m = -INFINITY, mRef = 0.f, l = 0.f;
   auto multiply = [&](Step& s, int at, bool all) {  // all: every one of the tokens counts
     f32x4 ks[2], vs[2], s4[2];
 #pragma unroll
@@ -262,16 +264,14 @@ __global__ __launch_bounds__(kI8Waves * 64, D == 256 ? 1 : 2) void decodeInt8Ker
     float mt = sc[0];
 #pragma unroll
     for (int i = 1; i < 8; ++i) mt = fmaxf(mt, sc[i]);
-    if (__builtin_amdgcn_ballot_w64(mt > most) != 0) {
+    if (__builtin_amdgcn_ballot_w64(mt > m) != 0) {
       auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mt), __float_as_uint(mt), false, false);
       mt = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
       sw = __builtin_amdgcn_permlane16_swap(__float_as_uint(mt), __float_as_uint(mt), false, false);
       mt = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
-      if (mt > most) {
-        most = mt;
-        const float mNew = mt * a.scaleLog2e;
-        const float corr = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mNew);  // (no maximum yet: the sums are 0, or NaN)
-        m = mRef = mNew;
+      if (mt > m) {
+        const float corr = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mt);  // (no maximum yet: the sums are 0, or NaN)
+        m = mRef = mt;
         l *= corr;
 #pragma unroll
         for (int t = 0; t < RUN; ++t)
@@ -281,7 +281,7 @@ __global__ __launch_bounds__(kI8Waves * 64, D == 256 ? 1 : 2) void decodeInt8Ker
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float e = __builtin_amdgcn_exp2f(fmaf(sc[i], a.scaleLog2e, -mRef));
+      const float e = __builtin_amdgcn_exp2f(sc[i] - mRef);
       l += e;
       w[i] *= e;
     }
@@ -356,7 +356,7 @@ __global__ __launch_bounds__(kI8Waves * 64, D == 256 ? 1 : 2) void decodeInt8Ker
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int w = 0; w < kI8Waves; ++w) {
-        scaleBuf[w * kI8Block + threadIdx.x + 256 * i] = ksv[i][w];
+        scaleBuf[w * kI8Block + threadIdx.x + 256 * i] = ksv[i][w] * a.scaleLog2e;
         scaleBuf[(kI8Waves + w) * kI8Block + threadIdx.x + 256 * i] = vsv[i][w];
       }
     __syncthreads();

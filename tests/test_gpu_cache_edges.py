@@ -146,3 +146,25 @@ def test_stored_scores_that_are_not_numbers(ops, dev, dtype, heads, kv_heads, d)
         hit = torch.zeros(4, heads, d, dtype=torch.bool)
         hit[b, heads - 1] = True
         assert torch.equal(out.isnan(), hit)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [64, 128, 256, 20])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_int8_scores_far_from_zero(ops, dev, dtype, d, sign):
+    """Scores of up to 2^60 with either sign, no two within 2^20 of each other: all of the weight is one key's."""
+    batch, heads, n = 24, 3, 100
+    q = torch.zeros(batch, heads, d)
+    q[..., 5] = sign * (1 + torch.rand(batch, heads, generator=g(71))) * 2.0 ** 14
+    q = q.to(dtype)
+    slots = batch * n
+    kp, vp = torch.zeros(slots, heads, d, dtype=torch.int8), torch.randint(-127, 128, (slots, heads, d), generator=g(72), dtype=torch.int8)
+    keys = torch.stack([torch.randperm(120, generator=g(73 + i))[:n] + 7 for i in range(batch)])   # 7 ... 126, each once
+    kp[..., 5] = keys.view(-1, 1).to(torch.int8)
+    ks = ((1 + torch.rand(batch, 1, heads, generator=g(74))) * 2.0 ** torch.linspace(12, 38, batch)[:, None, None]).expand(batch, n, heads).reshape(slots, heads)
+    vs = 0.5 + torch.rand(slots, heads, generator=g(75))
+    loc = torch.arange(slots).view(batch, n)
+    got = int8.run_attention(ops, dev, q, [(kp, ks.contiguous()), (vp, vs)], loc, torch.full((batch,), n), n)
+    winner = loc.gather(1, (keys * sign).argmax(1, keepdim=True))[:, 0]
+    want = vp[winner].double() * vs[winner].double()[..., None]
+    oracle.assert_within(got, want, want.abs() * (HALF_STEP[dtype] + 8 * U))
