@@ -66,6 +66,13 @@ __device__ __forceinline__ float blockSum256(float v, float* red) {
   return v;
 }
 
+// x - ref where x is a product that is rounded before: a multiply-add (which the compiler makes of the two by itself) keeps in the
+// difference what ref, another such product, lost in rounding.
+__device__ __forceinline__ float behindRounded(float x, float ref) {
+#pragma clang fp contract(off)
+  return x - ref;
+}
+
 // ---------------------------------------------------------------- host side --
 struct TaViews {
   TensorView q, k, v, loc, start, len;

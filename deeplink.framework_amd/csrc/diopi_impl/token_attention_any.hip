@@ -73,7 +73,7 @@ __global__ __launch_bounds__(kPaWaves * 64) void decodeAnyKernel(TaAnyArgs x, T*
 #pragma unroll
       for (int u = 0; u < UNR; ++u) {
         if (!counts[u]) continue;
-        const float p = exp2f(sc[u] - ref);
+        const float p = exp2f(behindRounded(sc[u], ref));
         l += p;
         const float w = p * vs[u];
 #pragma unroll

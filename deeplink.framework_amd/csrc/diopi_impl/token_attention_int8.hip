@@ -281,7 +281,7 @@ __global__ __launch_bounds__(kI8Waves * 64, D == 256 ? 1 : 2) void decodeInt8Ker
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float e = __builtin_amdgcn_exp2f(sc[i] - mRef);
+      const float e = __builtin_amdgcn_exp2f(behindRounded(sc[i], mRef));
       l += e;
       w[i] *= e;
     }

@@ -38,12 +38,17 @@ struct TaPrefixArgs {
 //   * the running maximum is followed at once, so a probability is at most one.
 //   * the first walk multiplies V as it is: infinities and NaN in it, or in slot 0 for a slot outside the pool, against
 //     probabilities that are zero leave sums that are not finite, and the wave then walks again with care: rows that do not count
-//     are zeros, what is not finite meets a one for each probability that is not zero.
+//     are zeros, what is not finite meets a one for each probability that is not zero. So it does where the maximum is far from
+//     zero (kPxFar): the first walk's exponents are multiply-adds, which keep what the maximum lost in rounding.
 // Four waves share a chunk's tokens and meet in LDS, a lane always adding to what is its own. 16 000 tokens, 32 heads of 128, 24
 // sequences: 132 us, 4.0 TB/s; two tiles of columns share a read with heads of 64 (with 128 that takes more registers than there are).
 constexpr int kPxWaves = 4;
 constexpr int kPxBlock = 2048;    // tokens whose slots a workgroup holds in LDS at once
 constexpr int kPxMaxSplit = 256;  // chunks of the prefix
+// Maxima up to this size (in units of log2) are off by at most 1/8, so are then the exponents of a walk without care, which does
+// not matter: all of a sum's are, and fp16 probabilities, at most 2^15, have room for it. From 2^31 on nothing would be left of them.
+constexpr float kPxFar = 0x1p22f;
+__device__ __forceinline__ bool pxFar(float m) { return fabsf(m) > kPxFar && m != -INFINITY; }
 
 template <int D>
 struct PxShape {
@@ -193,7 +198,7 @@ __global__ __launch_bounds__(kPxWaves * 64, 1) void decodePrefixFloatKernel(TaPr
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        w[i] = __builtin_amdgcn_exp2f(fmaf(w[i], a.scaleLog2e, -mRef[c]));
+        w[i] = __builtin_amdgcn_exp2f(CAREFUL ? behindRounded(w[i] * a.scaleLog2e, mRef[c]) : fmaf(w[i], a.scaleLog2e, -mRef[c]));
         l[c] += w[i];
       }
 #pragma unroll
@@ -266,13 +271,16 @@ __global__ __launch_bounds__(kPxWaves * 64, 1) void decodePrefixFloatKernel(TaPr
     walk(n, clean, std::false_type{});
   }
   uint32_t largest = 0;
+  bool far = false;
 #pragma unroll
-  for (int c = 0; c < NC; ++c)
+  for (int c = 0; c < NC; ++c) {
+    far |= pairOf[c] >= 0 && (pxFar(m[c]) || !(l[c] < INFINITY));  // (of scores far below the maximum l alone may have become too large)
 #pragma unroll
     for (int t = 0; t < RUN; ++t)
 #pragma unroll
       for (int i = 0; i < 4; ++i) largest = max(largest, pairOf[c] >= 0 ? __float_as_uint(acc[c][t][i]) & 0x7fffffffu : 0u);
-  if (__syncthreads_or(largest >= 0x7f800000u)) {
+  }
+  if (__syncthreads_or(far || largest >= 0x7f800000u)) {
     clear();
     for (int block = begin; block < end; block += kPxBlock) {
       const int n = min(kPxBlock, end - block);
@@ -543,7 +551,7 @@ __global__ __launch_bounds__(kPtWaves * 64, 2) void decodePrefixTiledKernel(TaPr
     return n;
   };
   // the scores of column tile c: its maximum followed (and all that was summed against the old one), as powers of two
-  auto powersOf = [&](int c, const f32x4 (&s4)[2], const Counts& n, bool all, float (&arg)[8], bool follow, float step) {
+  auto powersOf = [&](int c, const f32x4 (&s4)[2], const Counts& n, bool all, float (&arg)[8], bool follow, float step, auto withCare) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) arg[i] = s4[i >> 2][i & 3];
     if (!all) {
@@ -574,7 +582,7 @@ __global__ __launch_bounds__(kPtWaves * 64, 2) void decodePrefixTiledKernel(TaPr
     }
     const float ref = mRef[c] - M::kRaise;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) arg[i] = fmaf(arg[i], a.scaleLog2e, -ref);
+    for (int i = 0; i < 8; ++i) arg[i] = decltype(withCare)::value ? behindRounded(arg[i] * a.scaleLog2e, ref) : fmaf(arg[i], a.scaleLog2e, -ref);
   };
   auto readV = [&](int d, int stage) {  // eight tokens at the lane's place of the head
     const unsigned at = ring + (unsigned)(stage * S::STAGEB + (TOKENS + half * 32) * ROWB);
@@ -616,7 +624,7 @@ __global__ __launch_bounds__(kPtWaves * 64, 2) void decodePrefixTiledKernel(TaPr
 #pragma unroll
     for (int c = 0; c < N; ++c) {
       float w[8];
-      powersOf(c, s4[c], n, all, w, false, 0.f);
+      powersOf(c, s4[c], n, all, w, false, 0.f, withCare);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         w[i] = __builtin_amdgcn_exp2f(w[i]);
@@ -694,7 +702,7 @@ __global__ __launch_bounds__(kPtWaves * 64, 2) void decodePrefixTiledKernel(TaPr
 #pragma unroll
         for (int c = 0; c < N; ++c) {
           float w[8], lowest = 0.f;
-          powersOf(c, s4[c], counts, all, w, true, CAREFUL ? 0.f : kPtRescaleStep);
+          powersOf(c, s4[c], counts, all, w, true, CAREFUL ? 0.f : kPtRescaleStep, withCare);
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             if (HALF) lowest = fminf(lowest, w[i]);
@@ -773,13 +781,16 @@ __global__ __launch_bounds__(kPtWaves * 64, 2) void decodePrefixTiledKernel(TaPr
     else walk(n, clean, std::integral_constant<int, NC == 1 ? 1 : NC - 1>{}, std::false_type{});
   }
   uint32_t largest = 0;
+  bool far = false;
 #pragma unroll
-  for (int c = 0; c < NC; ++c)
+  for (int c = 0; c < NC; ++c) {
+    far |= pairOf[c] >= 0 && (pxFar(m[c]) || !(l[c] < INFINITY));  // (as in decodePrefixFloatKernel)
 #pragma unroll
     for (int t = 0; t < DT; ++t)
 #pragma unroll
       for (int i = 0; i < 4; ++i) largest = max(largest, pairOf[c] >= 0 ? __float_as_uint(acc[c][t][i]) & 0x7fffffffu : 0u);
-  if (__syncthreads_or(largest >= 0x7f800000u)) {
+  }
+  if (__syncthreads_or(far || largest >= 0x7f800000u)) {
     clear();
     for (int block = begin; block < end; block += kPxBlock) {
       const int n = min(kPxBlock, end - block);

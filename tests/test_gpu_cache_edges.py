@@ -168,3 +168,31 @@ def test_int8_scores_far_from_zero(ops, dev, dtype, d, sign):
     winner = loc.gather(1, (keys * sign).argmax(1, keepdim=True))[:, 0]
     want = vp[winner].double() * vs[winner].double()[..., None]
     oracle.assert_within(got, want, want.abs() * (HALF_STEP[dtype] + 8 * U))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,d", [(2, 2, 64), (8, 2, 128), (20, 1, 64), (2, 2, 256), (2, 1, 18)])
+@pytest.mark.parametrize("where", ["shared", "own"])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_scores_far_from_zero_behind_a_prefix(ops, dev, dtype, heads, kv_heads, d, where, sign):
+    """All elements of a key alike, so scores are 2^28 and more (2^50 where the type holds that) and either equal or far
+    apart: the result is the mean of the values with the best key, on the side that has it."""
+    lens = [30, 1, 0, 70] * 4
+    _, k, v, prefix, loc, n, max_len = shared.batch_of(300, lens, heads, kv_heads, d, torch.float32, 80)
+    top = 2.0 ** 13 if dtype == torch.float16 else 2.0 ** 22
+    q = (sign * (1 + torch.rand(len(lens), heads, 1, generator=g(81))).expand(-1, -1, d) * top).to(dtype)
+    slots = k.shape[0]
+    step = torch.randperm(slots, generator=g(82)) % 100            # a few keys alike, some of them among the best
+    key = 1 + step / 128
+    better = torch.zeros(slots, dtype=torch.bool)
+    better[prefix.long() if where == "shared" else torch.cat([oracle.slots_of(loc, n, max_len, b) for b in range(len(lens))])] = True
+    key = torch.where(better, key * 2 if sign > 0 else key / 2, key)
+    k = (key[:, None, None] * top).expand(slots, kv_heads, d).to(dtype)
+    v = (v.sign() * (0.5 + torch.rand(slots, kv_heads, 1, generator=g(83)))).to(dtype)
+    got = shared.run(ops, dev, q, k.contiguous(), v, prefix, loc, n, max_len)
+    want = torch.zeros(len(lens), heads, d).double()
+    for b, seen in enumerate(shared.own_and_shared(prefix, loc, n, max_len)):
+        best = (key[seen] * sign) == (key[seen] * sign).max()
+        want[b] = v[seen[best]].double().mean(0).repeat_interleave(heads // kv_heads, 0)
+    # (ten weights of one at most: (10 + 8) u of values below 1.5, and the rounding)
+    oracle.assert_within(got, want, (want.abs() + 27 * U) * HALF_STEP[dtype] + 27 * U + U * (dtype == torch.float16))
