@@ -407,7 +407,7 @@ __global__ __launch_bounds__(kTaWaves * 64, splitWavesPerSimd(sizeof(T), LPT, HI
         V o;
 #pragma unroll
         for (int e = 0; e < N; ++e) o[e] = static_cast<T>(acc[j][e] * inv);
-        if (live) *reinterpret_cast<V*>(out + ((int64_t)b * a.heads + h + j) * a.d + sub * N) = o;
+        if (live) storeElements(out + ((int64_t)b * a.heads + h + j) * a.d + sub * N, o);
       } else {
         float* dst = partial + (((int64_t)b * a.heads + h + j) * a.nsplit + split) * (2 + a.d);
         if (sub == 0) dst[0] = m[j], dst[1] = l[j];
@@ -850,7 +850,7 @@ walk:
       typename M::Quad r;
 #pragma unroll
       for (int c = 0; c < 4; ++c) r[c] = static_cast<T>(o[c] * inv);
-      *reinterpret_cast<typename M::Quad*>(out + ((int64_t)b * a.heads + h + j) * a.d + e) = r;
+      storeElements(out + ((int64_t)b * a.heads + h + j) * a.d + e, r);
     } else {
       float* dst = partial + (((int64_t)b * a.heads + h + j) * a.nsplit + split) * (2 + a.d);
       if (e == 0) dst[0] = mAll, dst[1] = lAll;

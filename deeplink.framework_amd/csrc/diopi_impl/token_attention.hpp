@@ -66,6 +66,12 @@ __device__ __forceinline__ float blockSum256(float v, float* red) {
   return v;
 }
 
+// Adjacent elements of a result, which may begin at any of them: one store, but of no more alignment than an element has.
+template <typename V, typename T>
+__device__ __forceinline__ void storeElements(T* at, const V& v) {
+  __builtin_memcpy(at, &v, sizeof(V));
+}
+
 // x - ref where x is a product that is rounded before: a multiply-add (which the compiler makes of the two by itself) keeps in the
 // difference what ref, another such product, lost in rounding.
 __device__ __forceinline__ float behindRounded(float x, float ref) {

@@ -393,7 +393,7 @@ __global__ __launch_bounds__(kI8Waves * 64, D == 256 ? 1 : 2) void decodeInt8Ker
       Quad r;
 #pragma unroll
       for (int c = 0; c < 4; ++c) r[c] = static_cast<T>(o[c] * inv);
-      *reinterpret_cast<Quad*>(out + ((int64_t)b * a.heads + h + j) * a.d + e) = r;
+      storeElements(out + ((int64_t)b * a.heads + h + j) * a.d + e, r);
     } else {
       float* dst = partial + (((int64_t)b * a.heads + h + j) * a.nsplit + split) * (2 + a.d);
       if (e == 0) dst[0] = mAll, dst[1] = lAll;

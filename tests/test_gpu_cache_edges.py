@@ -196,3 +196,21 @@ def test_scores_far_from_zero_behind_a_prefix(ops, dev, dtype, heads, kv_heads, 
         want[b] = v[seen[best]].double().mean(0).repeat_interleave(heads // kv_heads, 0)
     # (ten weights of one at most: (10 + 8) u of values below 1.5, and the rounding)
     oracle.assert_within(got, want, (want.abs() + 27 * U) * HALF_STEP[dtype] + 27 * U + U * (dtype == torch.float16))
+
+
+# ------------------------------------------------------------------ alignment
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,d", [(2, 2, 64), (8, 8, 128), (8, 1, 128), (4, 2, 80), (2, 2, 256), (2, 1, 18)])
+@pytest.mark.parametrize("max_len", [30, 900])
+def test_results_off_any_alignment(ops, dev, dtype, heads, kv_heads, d, max_len):
+    batch = 3
+    q, k, v, prefix, loc, n, _ = [t.to(dev) if hasattr(t, "to") else t for t in shared.batch_of(100, [max_len, 1, 7], heads, kv_heads, d, dtype, 90, spare=0)]
+    pools = [t.to(dev) for pool in int8.empty_pools(k.shape[0], kv_heads, d) for t in pool]
+    for call in (lambda out: ops.token_decode_attention(q, k, v, loc, n, n, max_len, out=out),
+                 lambda out: ops.token_decode_attention_int8(q, *pools, loc, n, n, max_len, out=out),
+                 lambda out: ops.token_decode_attention_shared_prefix(q, k, v, prefix, loc, n, n, max_len, out=out)):
+        want = call(torch.empty_like(q))
+        around = torch.full((q.numel() + 9,), 7.0, dtype=dtype, device=dev)
+        call(around[1:1 + q.numel()].view(q.shape))
+        assert_exact(around[1:1 + q.numel()].view(q.shape), want)
+        assert bool((around[1 + q.numel():] == 7).all()) and float(around[0]) == 7
