@@ -1085,10 +1085,19 @@ extern "C" __attribute__((visibility("default"))) diopiError_t diopiTokenDecodeA
   AMD_TRY(makeContiguous(ctx, stream, prefix, &densePrefix));
   x.loc = densePrefix.data, x.loc64 = prefix.dtype == diopi_dtype_int64, x.len = (int)prefix.shape[0];
   // head rows of whole 16-byte pieces up to 256 elements, slot numbers in 31 bits: the matrix pipe
-  const int64_t bits = (int64_t)reinterpret_cast<uintptr_t>(a.q) | (int64_t)reinterpret_cast<uintptr_t>(a.k) | (int64_t)reinterpret_cast<uintptr_t>(a.v) |
-                       (a.kSlotStride | a.kHeadStride | a.vSlotStride | a.vHeadStride | a.qBatchStride | a.qHeadStride | a.d) * t.q.itemsize;
-  if ((bits & 15) == 0 && a.d <= 256 && a.slots <= 0x7fffffff && std::max(a.kSlotStride, a.vSlotStride) * t.q.itemsize <= 0xffffffffll)
+  const int64_t bits = (int64_t)reinterpret_cast<uintptr_t>(a.k) | (int64_t)reinterpret_cast<uintptr_t>(a.v) |
+                       (a.kSlotStride | a.kHeadStride | a.vSlotStride | a.vHeadStride | a.d) * t.q.itemsize;
+  if ((bits & 15) == 0 && a.d <= 256 && a.slots <= 0x7fffffff && std::max(a.kSlotStride, a.vSlotStride) * t.q.itemsize <= 0xffffffffll) {
+    if (!t.q.aligned16() || ((a.qBatchStride | a.qHeadStride) * t.q.itemsize) % 16 != 0) {  // a dense copy of q
+      diopiTensorHandle_t th = nullptr;
+      TensorView dense;
+      AMD_TRY(requireTensor(ctx, t.q.shape, t.q.ndim, t.q.dtype, &th, &dense));
+      AMD_TRY(stridedCopy(stream, t.q, dense));
+      t.q = dense;
+      AMD_TRY(fillArgs(t, true, true, maxInputLen, &a));
+    }
     return decodeSharedPrefix(ctx, stream, x, t.q.dtype, out.data);
+  }
   TaAnyArgs any{};
   any.a = a, any.loc = x.loc, any.locIs64 = x.loc64, any.walked = x.len;
   TaPartials own;

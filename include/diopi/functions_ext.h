@@ -150,8 +150,9 @@ DIOPI_API diopiError_t diopiTokenDecodeAttentionInt8Inference(diopiContextHandle
 /* diopiTokenDecodeAttentionInference for a batch whose sequences all begin with the same tokens, which the pool holds once:
  * sequence b attends to the tokens in slots prefix_loc[0 .. n) (int32 or int64, every one of them for every sequence) and to
  * its own b_seq_len[b] tokens behind them, which b_loc, b_seq_len and max_input_len describe as they do there (none of them
- * count the prefix). The shared rows are read for many sequences at a time. Slots outside the pool are skipped; a sequence
- * without any token gives zeros. The same types and head sizes; n + max_input_len is at most 2^30. */
+ * count the prefix). Shared head rows of whole 16-byte pieces up to 256 elements, in pools aligned likewise, are read
+ * for many sequences at a time (others for each). Slots outside the pool are skipped; a sequence without any token gives
+ * zeros. The same types and head sizes; n + max_input_len is at most 2^30. */
 DIOPI_API diopiError_t diopiTokenDecodeAttentionSharedPrefixInference(diopiContextHandle_t ctx, diopiTensorHandle_t out,
                                                                       diopiConstTensorHandle_t q,
                                                                       diopiConstTensorHandle_t k,

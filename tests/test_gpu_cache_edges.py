@@ -214,3 +214,16 @@ def test_results_off_any_alignment(ops, dev, dtype, heads, kv_heads, d, max_len)
         call(around[1:1 + q.numel()].view(q.shape))
         assert_exact(around[1:1 + q.numel()].view(q.shape), want)
         assert bool((around[1 + q.numel():] == 7).all()) and float(around[0]) == 7
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,d", [(6, 2, 64), (8, 8, 128), (4, 2, 256)])
+def test_q_off_any_alignment_behind_a_prefix(ops, dev, dtype, heads, kv_heads, d):
+    """Bit for bit what an aligned q gives: the shared rows are read for many sequences at a time all the same."""
+    q, k, v, prefix, loc, n, max_len = [t.to(dev) if hasattr(t, "to") else t for t in shared.batch_of(700, [33, 0, 200, 1], heads, kv_heads, d, dtype, 95)]
+    want = ops.token_decode_attention_shared_prefix(q, k, v, prefix, loc, n, n, max_len)
+    for view in (lambda x: x[1:1 + q.numel()].view(q.shape), lambda x: x[:4 * heads * (d + 1)].view(4, heads, d + 1)[..., 1:],
+                 lambda x: x[3:3 + 4 * heads * (d + 3)].view(heads, 4, d + 3).transpose(0, 1)[..., :d]):
+        moved = view(torch.full((4 * heads * (d + 6),), 7.0, dtype=dtype, device=dev))
+        moved.copy_(q)
+        assert_exact(ops.token_decode_attention_shared_prefix(moved, k, v, prefix, loc, n, n, max_len), want)
