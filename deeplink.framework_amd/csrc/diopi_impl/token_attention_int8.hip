@@ -85,7 +85,7 @@ __device__ __forceinline__ bf16x8 nextPart(float (&x)[8]) {
   return part;
 }
 
-// (The second launch bound: with three waves to a SIMD five registers of D = 128 go to scratch, and 48 x (512 .. 4096), 8 K/V heads, takes 62 us, so 58.)
+// (The second launch bound: with three waves to a SIMD ten registers of D = 128 go to scratch, and 48 x (512 .. 4096), 8 K/V heads, takes 64 us, so 59.)
 // D: head size the rows are laid out for; a.d is any multiple of 16 up to it: the pieces past the row's end repeat its first
 // one, meet zeros of q, and give output places that are not stored. A workgroup's waves take x.headsPerWg K/V heads of the
 // same tokens and share these out among the waves of a head.
@@ -463,12 +463,16 @@ static diopiError_t int8Pool(const char* name, const TensorView& q, const Tensor
 // gets one of them where there are few (its step takes 0.5 us, whoever waits for rows does nothing else), and up to 16 where
 // there are many (what a workgroup does before its first step, and its partial results, are then spread over more). With four
 // heads to a workgroup a wave reads 512 adjacent bytes of a token with the other three, and one lane the scales of all four: 64 x
-// (512 .. 4096) tokens, 32 heads of 128, 231 us, with one head 383 (48, 8 heads 59 and 87). Few steps are better dealt over the
-// waves of a head: 1 x 1777 tokens, 8 heads, one step to a wave, 10.3 with one head, 11.4 with four (each before q and the first slots were asked for at once: 9.9).
-// us at 1, 2, 4, 8, 16 steps to a wave: 1 x 4096, 8 heads 10.6, 11.3, 13.6, 18.0, 25.1; 1 x 8192 14.2, 13.2, 15.2, 18.5, 25.5; 1 x 16384
-// 25.3, 20.0, 18.5, 19.4, 25.7; 8 x 4096 37, 28, 22.7, 20.7, 26.2; 16 x (1000 .. 8000) 84, 58, 48, 47, 47; 48 x (512 .. 4096) 120, 82, 69, 59, 72;
-// 32 heads, 64 x (512 .. 4096) 627, 385, 297, 247, 231. Heads of 256: a SIMD holds one wave instead of two, and a step takes twice as
-// long: 16 x (512 .. 4096), 8 heads 105, 71, 60, 56, 45.
+// (512 .. 4096) tokens, 32 heads of 128, 234 us, with one head 365 (48, 8 heads 59 and 82). Few steps are better dealt over the
+// waves of a head: 1 x 1777 tokens, 8 heads, one step to a wave, 10.0 with one head, 11.1 with four.
+// us at 1, 2, 4, 8, 16 steps to a wave: 1 x 4096, 8 heads 10.3, 11.1, 13.4, 17.5, 24.8; 1 x 8192 13.9, 12.9, 15.0, 17.9, 25.4; 1 x 16384
+// 23.9, 19.7, 18.3, 19.5, 25.6; 8 x 4096 34, 27, 22.7, 20.8, 26.0; 16 x (1000 .. 8000) 76, 55, 47, 47, 47; 48 x (512 .. 4096) 109, 75, 66, 59, 68;
+// 32 heads, 64 x (512 .. 4096) 550, 357, 283, 247, 232. Heads of 256: a SIMD holds one wave instead of two, and a step takes twice as
+// long: 16 x (512 .. 4096), 8 heads 92, 65, 58, 55, 46. Next to the line between 8 and 16 (steps for a compute unit in brackets), 8 heads of
+// 128, two sets of lengths of 512 .. 4096: 40 sequences [160] 54 and 49, 52 and 49; 48 [192] 59 and 67, 60 and 58; 52 [208] 62 and 67, 68 and 69;
+// 56 [224] 67 and 74, 70 and 75; 64 [256] 78 and 77, 80 and 79; 96 [384] 118 and 113, 114 and 106; all of 4096: 48 88 and 81, 56 102 and 99, 64 116 and
+// 105. 32 heads, 14 [224] 64 and 71, 16 [256] 69 and 74, 32 [512] 130 and 133, 64 [1024] 247 and 232; of 64, 32 [512] 101 and 108. Which one a set of
+// lengths likes turns on how its last round of workgroups comes out; from 256 on even lengths and the large batches are better in 16.
 static void chooseShares(TaInt8Args* x, int64_t len, int D) {
   TaArgs& a = x->a;
   const int64_t steps = (int64_t)a.kvHeads * a.qGroups * a.batch * ceilDiv(len, kI8Tile) * (D == 256 ? 4 : 1);
@@ -478,8 +482,8 @@ static void chooseShares(TaInt8Args* x, int64_t len, int D) {
   const int fits = a.kvHeads % 4 == 0 || a.kvHeads == 3 || a.kvHeads > 8 ? 4 : a.kvHeads >= 2 ? 2 : 1;
   x->headsPerWg = std::min(fits, perWave);
   int64_t tokens = (int64_t)perWave * kI8Tile * kI8Waves / x->headsPerWg;
-  // short sequences in one chunk, without the launch that merges: 16 x (1 .. 300), 8 heads of 64, 9.6 -> 7.6; 64 x (100 .. 500), 32 heads
-  // 42.5 -> 40.4
+  // short sequences in one chunk, without the launch that merges: 16 x (1 .. 300), 8 heads of 64, 9.4 -> 7.6; 64 x (100 .. 500), 32 heads
+  // 41.1 -> 38.6
   if (len <= kI8Block && perWave >= 8) {
     tokens = len;
   } else if (len <= 384 && a.batch >= 8) {

@@ -347,7 +347,8 @@ __global__ __launch_bounds__(kPxWaves * 64, 1) void decodePrefixFloatKernel(TaPr
 // to a lane, pieces XOR-swizzled by row), K is read as it lies, V through the transposing read; one barrier per stage. Against
 // rows that each wave loads into its own registers, where V has to be turned round by lane permutations and a wave has a SIMD
 // to itself (us, 16 000 tokens, bf16): 8 K/V heads of 128 with 192 columns each 99 -> 45, with 32 30.5 -> 27.9; 32 with 32 81.6 -> 65.7, with
-// 12 66.5 -> 64.9 (5 us of each for a launch that merged them, which these no longer need). Of the 36 us that 192 columns take,
+// 12 66.5 -> 64.9 (5 us of each for a launch that merged them, which these no longer need; now, with one to four own tokens, 44.4, 27.0, 61.7
+// and 60.6). Of the 36 us that 192 columns take in fp16,
 // 11 do not grow with the prefix (slots, then rows; at the end 12.8 MB of partial results); in the others the two waves of a SIMD
 // multiply at the same time and then both take exponentials (matrix pipe busy for 7.5 us, vector ALUs for 11, LDS between them). Half the
 // waves a phase behind the other half was no faster (45 us).
