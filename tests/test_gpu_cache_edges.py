@@ -148,6 +148,25 @@ def test_stored_scores_that_are_not_numbers(ops, dev, dtype, heads, kv_heads, d)
         assert torch.equal(out.isnan(), hit)
 
 
+@pytest.mark.parametrize("heads,kv_heads,d", [(2, 2, 64), (8, 8, 64), (8, 1, 128)])
+def test_stored_scores_of_minus_infinity(ops, dev, heads, kv_heads, d):
+    """Steps of the walk over fp32 rows in which a caller has masked every token, ahead of any that counts, are passed over,
+    whatever the values are."""
+    dtype = torch.float32
+    max_len, masked = 100, 64
+    v = torch.randn(200, kv_heads, d, generator=g(68)).to(dtype)
+    loc = torch.randperm(200, generator=g(69))[:max_len].repeat(2, 1)
+    scores = torch.randn(heads, 2 * max_len, generator=g(70))
+    scores[:, :masked] = -math.inf
+    poisoned = v.clone()
+    poisoned[loc[0, :masked]] = math.nan
+    start, lens = torch.tensor([0, max_len]), torch.tensor([max_len, max_len])
+    halves = lambda vv: ops.token_softmax_reducev(scores.to(dev), vv.to(dev), torch.empty(2, heads, d, dtype=dtype, device=dev), loc.to(dev), start.to(dev), lens.to(dev), max_len)[0].cpu()
+    got, want = halves(poisoned), halves(v)
+    assert bool(want.isfinite().all())
+    assert_exact(got, want)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("d", [64, 128, 256, 20])
 @pytest.mark.parametrize("sign", [1, -1])
