@@ -344,7 +344,7 @@ __global__ __launch_bounds__(kTaWaves * 64, splitWavesPerSimd(sizeof(T), LPT, HI
         float p[UNR], ps = 0.f;
 #pragma unroll
         for (int u = 0; u < UNR; ++u) {
-          p[u] = __builtin_amdgcn_exp2f(sc[u] - ref);
+          p[u] = __builtin_amdgcn_exp2f(behindRounded(sc[u], ref));
           ps += p[u];
         }
         l[j] = l[j] * corr + ps;
@@ -684,7 +684,7 @@ walk:
         const float mRaised = mRef - M::kRaise;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float e = __builtin_amdgcn_exp2f(sc[i] - mRaised);
+          const float e = __builtin_amdgcn_exp2f(behindRounded(sc[i], mRaised));
           ps += whole[i] = e;
           const T hi = static_cast<T>(e);
           const float left = e - static_cast<float>(hi);
