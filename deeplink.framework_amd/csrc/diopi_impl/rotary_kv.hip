@@ -10,6 +10,8 @@
 //
 // DestIndexCopyKV: out[dest_loc[i], :, :] = k[i, :, :], a pure byte move done with the
 // widest vector the row size and pointers allow; one workgroup per token row.
+#include <algorithm>
+
 #include "gemm.hpp"
 
 namespace amd {
@@ -225,6 +227,73 @@ static diopiError_t launchDestCopy(hipStream_t stream, KvScatterArgs a, int pool
   else if ((bits & 1) == 0) KV_LAUNCH(uint16_t);
   else KV_LAUNCH(uint8_t);
 #undef KV_LAUNCH
+  AMD_LAUNCH_CHECK();
+  return diopiSuccess;
+}
+
+// ------------------------------------------------- rotation on the way into the cache --
+// out_q = q rotated, pool_k[dest] = k rotated, pool_v[dest] = v for the rows of new tokens (see diopiRotaryDestIndexCopyKVPair).
+struct RotaryAppendArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* outQ;
+  void* poolK;
+  void* poolV;
+  const void* cosT;
+  const void* sinT;
+  const void* positions;  // null: token i takes table row i % tableRows
+  const void* destLoc;
+  bool pos64, loc64, interleaved;
+  int64_t tokens, slots, tableRows;
+  int heads, kvHeads, d, tableCols;
+  int64_t qTok, qHead, oTok, oHead, kTok, kHead, vTok, vHead, pkSlot, pkHead, pvSlot, pvHead;  // elements
+};
+
+__device__ __forceinline__ int64_t indexAt(const void* p, int64_t i, bool is64) {
+  return is64 ? static_cast<const int64_t*>(p)[i] : static_cast<int64_t>(static_cast<const int32_t*>(p)[i]);
+}
+
+// Any strides and alignment: a workgroup per token, a pair per lane.
+template <typename T, typename CT>
+__global__ __launch_bounds__(256) void rotaryAppendAnyKernel(RotaryAppendArgs a) {
+  const int half = a.d / 2, items = (a.heads + 2 * a.kvHeads) * half;
+  for (int64_t t = blockIdx.x; t < a.tokens; t += gridDim.x) {
+    int64_t slot = indexAt(a.destLoc, t, a.loc64);
+    if (slot < 0) slot += a.slots;
+    const bool kept = slot >= 0 && slot < a.slots;  // an out-of-range slot is dropped, never written
+    const int64_t trow = a.positions != nullptr ? indexAt(a.positions, t, a.pos64) : t % a.tableRows;
+    const bool inside = trow >= 0 && trow < a.tableRows;
+    for (int w = threadIdx.x; w < items; w += 256) {
+      const int h = w / half, p = w - h * half;
+      const int i0 = a.interleaved ? 2 * p : p, i1 = a.interleaved ? 2 * p + 1 : p + half;
+      if (h >= a.heads + a.kvHeads) {
+        if (!kept) continue;
+        const int hv = h - a.heads - a.kvHeads;
+        const T* x = static_cast<const T*>(a.v) + t * a.vTok + hv * a.vHead;
+        T* o = static_cast<T*>(a.poolV) + slot * a.pvSlot + hv * a.pvHead;
+        o[i0] = x[i0], o[i1] = x[i1];
+        continue;
+      }
+      const bool isQ = h < a.heads;
+      if (!isQ && !kept) continue;
+      const int hk = h - a.heads;
+      const T* x = isQ ? static_cast<const T*>(a.q) + t * a.qTok + h * a.qHead : static_cast<const T*>(a.k) + t * a.kTok + hk * a.kHead;
+      T* o = isQ ? static_cast<T*>(a.outQ) + t * a.oTok + h * a.oHead : static_cast<T*>(a.poolK) + slot * a.pkSlot + hk * a.pkHead;
+      const int64_t at = (inside ? trow : 0) * a.tableCols + (a.interleaved && a.tableCols == a.d ? 2 * p : p);
+      const float c = inside ? static_cast<float>(static_cast<const CT*>(a.cosT)[at]) : 0.f;
+      const float s = inside ? static_cast<float>(static_cast<const CT*>(a.sinT)[at]) : 0.f;
+      const float x0 = static_cast<float>(x[i0]), x1 = static_cast<float>(x[i1]);
+      o[i0] = static_cast<T>(x0 * c - x1 * s);
+      o[i1] = static_cast<T>(x0 * s + x1 * c);
+    }
+  }
+}
+
+template <typename T, typename CT>
+static diopiError_t launchRotaryAppend(hipStream_t stream, const RotaryAppendArgs& a) {
+  const unsigned blocks = (unsigned)std::min<int64_t>(a.tokens, 1 << 23);  // (fewer than 2^32 threads)
+  hipLaunchKernelGGL((rotaryAppendAnyKernel<T, CT>), dim3(blocks), dim3(256), 0, stream, a);
   AMD_LAUNCH_CHECK();
   return diopiSuccess;
 }
@@ -465,6 +534,78 @@ extern "C" __attribute__((visibility("default"))) diopiError_t diopiDestIndexCop
     return diopiSuccess;
   }
   return i32 ? launchDestCopy<int32_t>(stream, a, 2, rowBytesK) : launchDestCopy<int64_t>(stream, a, 2, rowBytesK);
+}
+
+extern "C" __attribute__((visibility("default"))) diopiError_t diopiRotaryDestIndexCopyKVPair(
+    diopiContextHandle_t ctx, diopiTensorHandle_t outQH, diopiConstTensorHandle_t qH, diopiTensorHandle_t outKH, diopiConstTensorHandle_t kH,
+    diopiTensorHandle_t outVH, diopiConstTensorHandle_t vH, diopiConstTensorHandle_t cosH, diopiConstTensorHandle_t sinH,
+    diopiConstTensorHandle_t posH, diopiConstTensorHandle_t locH, bool interleaved) {
+  hipStream_t stream;
+  AMD_TRY(getStream(ctx, &stream));
+  TensorView outQ, q, outK, k, outV, v, c, s, pos, loc;
+  AMD_TRY(getView(outQH, &outQ, "out_q"));
+  AMD_TRY(getView(qH, &q, "q"));
+  AMD_TRY(getView(outKH, &outK, "out_k"));
+  AMD_TRY(getView(kH, &k, "k"));
+  AMD_TRY(getView(outVH, &outV, "out_v"));
+  AMD_TRY(getView(vH, &v, "v"));
+  AMD_TRY(getView(cosH, &c, "cos"));
+  AMD_TRY(getView(sinH, &s, "sin"));
+  AMD_TRY(getView(posH, &pos, "positions"));
+  AMD_TRY(getView(locH, &loc, "dest_loc"));
+  const char* const what = "diopiRotaryDestIndexCopyKVPair";
+  AMD_CHECK(outK.defined() && k.defined() && outV.defined() && v.defined() && c.defined() && s.defined() && loc.defined(), "%s: null tensor", what);
+  AMD_CHECK(q.defined() == outQ.defined(), "%s: q and out_q are both given or both null", what);
+  const TensorView* const rows[] = {&k, &v, &outK, &outV, &q, &outQ};
+  const char* const names[] = {"k", "v", "out_k", "out_v", "q", "out_q"};
+  for (int i = 0; i < (q.defined() ? 6 : 4); ++i) {
+    AMD_CHECK(rows[i]->ndim == 3, "%s: %s must have three dims (tokens or slots, heads, head_dim)", what, names[i]);
+    AMD_CHECK(rows[i]->dtype == k.dtype, "%s: %s is %s, k is %s", what, names[i], dtypeName(rows[i]->dtype), dtypeName(k.dtype));
+    AMD_CHECK(rows[i]->shape[2] == k.shape[2], "%s: %s has a head_dim of %ld, k of %ld", what, names[i], (long)rows[i]->shape[2], (long)k.shape[2]);
+    AMD_CHECK(rows[i]->stride[2] == 1 || rows[i]->shape[2] == 1, "%s: head_dim of %s must be contiguous", what, names[i]);
+  }
+  AMD_CHECK(k.dtype == diopi_dtype_bfloat16 || k.dtype == diopi_dtype_float16 || k.dtype == diopi_dtype_float32, "%s: unsupported dtype %s", what, dtypeName(k.dtype));
+  for (int i = 0; i < 2; ++i) {
+    AMD_CHECK(v.shape[i] == k.shape[i], "%s: k and v differ at dim %d", what, i);
+    AMD_CHECK(outV.shape[i] == outK.shape[i], "%s: out_k and out_v differ at dim %d", what, i);
+    if (q.defined()) AMD_CHECK(outQ.shape[i] == q.shape[i], "%s: q and out_q differ at dim %d", what, i);
+  }
+  AMD_CHECK(outK.shape[1] == k.shape[1], "%s: k has %ld heads, the pools %ld", what, (long)k.shape[1], (long)outK.shape[1]);
+  const int64_t tokens = k.shape[0], d = k.shape[2];
+  AMD_CHECK(!q.defined() || q.shape[0] == tokens, "%s: q has %ld tokens, k %ld", what, (long)q.shape[0], (long)tokens);
+  AMD_CHECK(loc.dtype == diopi_dtype_int32 || loc.dtype == diopi_dtype_int64, "%s: dest_loc must be int32 or int64, got %s", what, dtypeName(loc.dtype));
+  AMD_CHECK(loc.ndim == 1 && loc.numel == tokens, "%s: dest_loc must have one dim and an entry for each of %ld tokens", what, (long)tokens);
+  AMD_CHECK(!pos.defined() || ((pos.dtype == diopi_dtype_int32 || pos.dtype == diopi_dtype_int64) && pos.ndim == 1 && pos.numel == tokens),
+            "%s: positions must be int32 or int64, of one dim and with an entry for each of %ld tokens", what, (long)tokens);
+  AMD_CHECK(d % 2 == 0, "%s: head_dim %ld is odd", what, (long)d);
+  AMD_CHECK(c.dtype == s.dtype && c.ndim == 2 && s.ndim == 2 && c.shape[0] == s.shape[0] && c.shape[1] == s.shape[1], "%s: cos and sin must be alike, [rows, n]", what);
+  AMD_CHECK(c.dtype == k.dtype || c.dtype == diopi_dtype_float32, "%s: cos is %s, k is %s", what, dtypeName(c.dtype), dtypeName(k.dtype));
+  AMD_CHECK(c.shape[1] == d || c.shape[1] == d / 2, "%s: cos last dim %ld is neither %ld nor %ld", what, (long)c.shape[1], (long)d, (long)d / 2);
+  const int64_t heads = q.defined() ? q.shape[1] : 0;
+  AMD_CHECK((heads + 2 * k.shape[1]) * d < (int64_t)1 << 31, "%s: rows of %ld and %ld heads of %ld", what, (long)heads, (long)k.shape[1], (long)d);
+  if (tokens == 0 || d == 0 || (heads == 0 && k.shape[1] == 0)) return diopiSuccess;
+  AMD_CHECK(outK.shape[0] > 0, "%s: the KV pool has no slots", what);
+  AMD_CHECK(c.shape[0] > 0 && (pos.defined() || tokens % c.shape[0] == 0), "%s: %ld table rows do not divide %ld tokens", what, (long)c.shape[0], (long)tokens);
+  TensorView cc, cs, cpos, cloc;
+  AMD_TRY(makeContiguous(ctx, stream, c, &cc));
+  AMD_TRY(makeContiguous(ctx, stream, s, &cs));
+  if (pos.defined()) AMD_TRY(makeContiguous(ctx, stream, pos, &cpos));
+  AMD_TRY(makeContiguous(ctx, stream, loc, &cloc));
+  RotaryAppendArgs a{};
+  a.q = q.data, a.k = k.data, a.v = v.data, a.outQ = outQ.data, a.poolK = outK.data, a.poolV = outV.data;
+  a.cosT = cc.data, a.sinT = cs.data, a.positions = cpos.data, a.destLoc = cloc.data;
+  a.pos64 = cpos.dtype == diopi_dtype_int64, a.loc64 = cloc.dtype == diopi_dtype_int64, a.interleaved = interleaved;
+  a.tokens = tokens, a.slots = outK.shape[0], a.tableRows = c.shape[0];
+  a.heads = (int)heads, a.kvHeads = (int)k.shape[1], a.d = (int)d, a.tableCols = (int)c.shape[1];
+  a.qTok = q.stride[0], a.qHead = q.stride[1], a.oTok = outQ.stride[0], a.oHead = outQ.stride[1];
+  a.kTok = k.stride[0], a.kHead = k.stride[1], a.vTok = v.stride[0], a.vHead = v.stride[1];
+  a.pkSlot = outK.stride[0], a.pkHead = outK.stride[1], a.pvSlot = outV.stride[0], a.pvHead = outV.stride[1];
+  const bool wide = c.dtype == diopi_dtype_float32;
+  switch (k.dtype) {
+    case diopi_dtype_bfloat16: return wide ? launchRotaryAppend<bf16_t, float>(stream, a) : launchRotaryAppend<bf16_t, bf16_t>(stream, a);
+    case diopi_dtype_float16: return wide ? launchRotaryAppend<half_t, float>(stream, a) : launchRotaryAppend<half_t, half_t>(stream, a);
+    default: return launchRotaryAppend<float, float>(stream, a);
+  }
 }
 
 extern "C" __attribute__((visibility("default"))) diopiError_t diopiIndexPutInp(

@@ -290,7 +290,8 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
   X(diopiDestIndexCopyKVPair) X(diopiTokenAttentionInference) X(diopiTokenSoftmaxReduceVInference)                            \
   X(diopiContextAttentionInference) X(diopiTokenDecodeAttentionInference) X(diopiTokenDecodeAttentionInferenceNoAlloc)        \
   X(diopiWeightOnlyInt8Linear) X(diopiSiluMul) X(diopiLinearSiluMul) X(diopiLinearRotary) X(diopiDestIndexCopyKVPairInt8)      \
-  X(diopiIndexSelectKVPairInt8) X(diopiTokenDecodeAttentionInt8Inference) X(diopiTokenDecodeAttentionSharedPrefixInference)
+  X(diopiIndexSelectKVPairInt8) X(diopiTokenDecodeAttentionInt8Inference) X(diopiTokenDecodeAttentionSharedPrefixInference) \
+  X(diopiPagedContextAttentionInference) X(diopiTokenDecodeAttentionWindowInference) X(diopiRotaryDestIndexCopyKVPair)
 
 #define X(f)                                        \
   struct Tag_##f {                                  \

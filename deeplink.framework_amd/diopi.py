@@ -290,6 +290,9 @@ SIGNATURES = {
     "diopiIndexSelectKVPairInt8": [_T, _T, _T, _T, _T, _T, _T],
     "diopiTokenDecodeAttentionInt8Inference": [_T, _T, _T, _T, _T, _T, _T, _T, _T, c_int],
     "diopiTokenDecodeAttentionSharedPrefixInference": [_T, _T, _T, _T, _T, _T, _T, _T, c_int],
+    "diopiPagedContextAttentionInference": [_T, _T, _T, _T, _T, _T, _T, _T, c_int, c_int, c_int, c_int],
+    "diopiTokenDecodeAttentionWindowInference": [_T, _T, _T, _T, _T, _T, _T, c_int, c_int, c_int],
+    "diopiRotaryDestIndexCopyKVPair": [_T, _T, _T, _T, _T, _T, _T, _T, _T, _T, c_bool],
     "diopiWeightOnlyInt8Linear": [_T, _T, _T, _T, _T],
     "diopiSiluMul": [_T, _T, _T],
     "diopiLinearSiluMul": [_T, _T, _T],

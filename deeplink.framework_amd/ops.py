@@ -511,6 +511,15 @@ def dest_index_copy_kv_pair_int8(k, v, dest_loc, out_k, out_k_scale, out_v, out_
     return out_k, out_k_scale, out_v, out_v_scale
 
 
+def rotary_dest_index_copy_kv_pair(q, k, v, cos, sin, dest_loc, out_k, out_v, *, positions=None, interleaved=False, out_q=None):
+    """q rotated (returned), out_k[dest_loc[i]] = k[i] rotated and out_v[dest_loc[i]] = v[i] in one launch (backend extension,
+    functions_ext.h). cos, sin: rows for the tokens, or for the positions that `positions` names. q may be None."""
+    if out_q is None and q is not None:
+        out_q = _host.like(q)
+    _host.diopiRotaryDestIndexCopyKVPair(_ctx, out_q, q, out_k, k, out_v, v, cos, sin, positions, dest_loc, bool(interleaved))
+    return out_q
+
+
 def index_select_kv_pair_int8(k, k_scale, v, v_scale, index, *, dtype=None, out_k=None, out_v=None):
     """k[index] * k_scale[index] and v[index] * v_scale[index] of an int8 cache in `dtype` (by default that of out_k, or
     torch's default type), in one launch (backend extension, functions_ext.h)."""
@@ -559,6 +568,24 @@ def token_decode_attention_shared_prefix(q, k, v, prefix_loc, b_loc, b_start_loc
     if out is None:
         out = _host.like(q)
     _host.diopiTokenDecodeAttentionSharedPrefixInference(_ctx, out, q, k, v, prefix_loc, b_loc, b_start_loc, b_seq_len, int(max_input_len))
+    return out
+
+
+def token_decode_attention_window(q, k, v, b_loc, b_start_loc, b_seq_len, max_input_len, window, sinks=0, *, out=None):
+    """token_decode_attention over the last `window` tokens of each sequence and its first `sinks` (backend extension,
+    functions_ext.h). window = 0: all."""
+    if out is None:
+        out = _host.like(q)
+    _host.diopiTokenDecodeAttentionWindowInference(_ctx, out, q, k, v, b_loc, b_start_loc, b_seq_len, int(max_input_len), int(window), int(sinks))
+    return out
+
+
+def paged_context_attention(q, k, v, b_loc, b_start_loc, b_new_len, b_seq_len, max_new_len, max_input_len, *, window=0, sinks=0, out=None):
+    """Attention of the new tokens of each sequence (rows b_start_loc[b] ... of q), its last ones, over all that the paged pool holds of
+    it, or the last `window` tokens and the first `sinks` (backend extension, functions_ext.h)."""
+    if out is None:
+        out = _host.like(q)
+    _host.diopiPagedContextAttentionInference(_ctx, out, q, k, v, b_loc, b_start_loc, b_new_len, b_seq_len, int(max_new_len), int(max_input_len), int(window), int(sinks))
     return out
 
 

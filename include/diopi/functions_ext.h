@@ -163,6 +163,51 @@ DIOPI_API diopiError_t diopiTokenDecodeAttentionSharedPrefixInference(diopiConte
                                                                       diopiConstTensorHandle_t b_seq_len,
                                                                       int max_input_len);
 
+/* Attention of several new tokens of each sequence over all that the paged pool holds of it, the new ones (written before) among
+ * them: the next piece of a long prompt, speculated tokens, a batch in which some sequences decode and others bring a prompt.
+ * q [tokens, heads, d]: rows [b_start_loc[b], b_start_loc[b] + b_new_len[b]) are the new tokens of sequence b, the last b_new_len[b] of
+ * its b_seq_len[b] tokens; slots as in the decode entry points: token j of sequence b is in slot b_loc[b, max_input_len - b_seq_len[b] + j].
+ * A token at position p of its sequence sees the tokens j <= p; with window > 0 of these only the last `window` (itself among them)
+ * and the sequence's first `sinks` (j > p - window or j < sinks); window = 0: all. Table entries of tokens that no new
+ * token sees are not used. b_new_len[b] is cut to [0, max_new_len] and b_seq_len[b] to [0, max_input_len]; new tokens before the
+ * sequence's first (more of them than tokens) and those whose visible slots all lie outside the pool give zeros; slots outside the
+ * pool are skipped; rows of q and out outside [0, tokens) are left out, and rows of out of no sequence left as they were.
+ * Sequences do not share rows of q. float32, float16 or bfloat16, grouped K/V heads (heads % kv_heads == 0), any strides with a contiguous head dimension
+ * of up to 1024; out [tokens, heads, d] likewise; max_input_len is at most 2^30. Scores, softmax and sums are in fp32. The reference has
+ * prompts without a cache and single tokens alone (ext_ops.py:52-133). */
+DIOPI_API diopiError_t diopiPagedContextAttentionInference(diopiContextHandle_t ctx, diopiTensorHandle_t out,
+                                                           diopiConstTensorHandle_t q, diopiConstTensorHandle_t k,
+                                                           diopiConstTensorHandle_t v, diopiConstTensorHandle_t b_loc,
+                                                           diopiConstTensorHandle_t b_start_loc,
+                                                           diopiConstTensorHandle_t b_new_len,
+                                                           diopiConstTensorHandle_t b_seq_len, int max_new_len,
+                                                           int max_input_len, int window, int sinks);
+
+/* diopiTokenDecodeAttentionInference where a token sees the last `window` tokens of its sequence (itself among them) and the first
+ * `sinks` alone; window = 0: all. The same arguments and rules; table entries of tokens outside both are not used, so their slots
+ * may have been given to others. max_input_len is at most 2^30. No counterpart in the reference. */
+DIOPI_API diopiError_t diopiTokenDecodeAttentionWindowInference(diopiContextHandle_t ctx, diopiTensorHandle_t out,
+                                                                diopiConstTensorHandle_t q, diopiConstTensorHandle_t k,
+                                                                diopiConstTensorHandle_t v, diopiConstTensorHandle_t b_loc,
+                                                                diopiConstTensorHandle_t b_start_loc,
+                                                                diopiConstTensorHandle_t b_seq_len, int max_input_len,
+                                                                int window, int sinks);
+
+/* What a layer does with the q, k and v rows of new tokens before its attention, in one launch: out_q = q rotated, out_k[dest_loc[i]] =
+ * k[i] rotated, out_v[dest_loc[i]] = v[i]; the rotation is diopiRotaryEmbedding's (head_dim even, interleaved as there, computed in
+ * fp32), the scatter diopiDestIndexCopyKVPair's (negative destinations count from the end, those outside the pool are dropped).
+ * cos, sin [rows, head_dim / 2 or head_dim], of x's type or float32. positions [tokens] (int32 or int64): token i takes table row positions[i],
+ * and zeros stand for a row outside the table; null: row i % rows, rows dividing the tokens. q [tokens, heads, d] and out_q may be the
+ * same tensor, or both null; k, v [tokens, kv_heads, d], pools [slots, kv_heads, d], all of one type (float32, float16, bfloat16), at any strides with a
+ * contiguous head dimension. Destinations differ from each other: of tokens with one and the same, the slot may be left with
+ * elements of any (padding goes to a slot that nobody reads, or outside the pool). The reference runs a rotation of q, one of k and two scatters. */
+DIOPI_API diopiError_t diopiRotaryDestIndexCopyKVPair(diopiContextHandle_t ctx, diopiTensorHandle_t out_q,
+                                                      diopiConstTensorHandle_t q, diopiTensorHandle_t out_k,
+                                                      diopiConstTensorHandle_t k, diopiTensorHandle_t out_v,
+                                                      diopiConstTensorHandle_t v, diopiConstTensorHandle_t cos,
+                                                      diopiConstTensorHandle_t sin, diopiConstTensorHandle_t positions,
+                                                      diopiConstTensorHandle_t dest_loc, bool interleaved);
+
 /* out[M,N] = input[M,K] @ (weight[N,K] (int8) * scale[N])^T + bias[N].
  * input/out bf16 or fp16; scale fp16/bf16/fp32 per output channel; bias nullable.
  * The int8 -> bf16/fp16 conversion happens while the MFMA operand tile is loaded; the
