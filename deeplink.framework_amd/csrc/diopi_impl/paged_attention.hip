@@ -18,8 +18,7 @@
 
 namespace amd {
 
-// Any head size up to 64 J, any strides: a workgroup per (new token, head), a wave a token of the pool at a time with the row spread
-// over its lanes, UNR of them asked for at once; slots are looked up 64 at a time. Only tokens that are seen are walked.
+// Any head size up to 64 J, any strides: a workgroup per (new token, head), whose waves take 64 tokens that it sees in turn (PaColumn).
 // Bound by the vector ALUs, whose sums over the lanes cost more than the products.
 constexpr int kPgWaves = 4;
 template <typename T, int J, int UNR>
@@ -35,64 +34,14 @@ __global__ __launch_bounds__(kPgWaves * 64) void pagedAnyKernel(PaArgs a) {
     const int64_t row = s.start + t;
     const int len = cutLength(a.bLen, at.b, a.len64, a.maxLen);
     const int64_t locBase = (int64_t)at.b * a.locRowStride + (a.maxLen - len);
-    const int low = max(0, p - a.window + 1), head = min(a.sinks, low), n = p < 0 ? 0 : head + p + 1 - low;  // token i of n: i, or behind the gap
-    const T* q = reinterpret_cast<const T*>(a.q) + row * a.qTok + h * a.qHead;
-    const T* kHead = reinterpret_cast<const T*>(a.k) + kvh * a.kHeadStride;
-    const T* vHead = reinterpret_cast<const T*>(a.v) + kvh * a.vHeadStride;
-    int at_[J];  // the lane's elements of a row; past its end the first one, which q's zero leaves out
-    float qf[J], acc[J], m = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int j = 0; j < J; ++j) {
-      const int e = lane + 64 * j;
-      at_[j] = e < a.d ? e : 0;
-      qf[j] = e < a.d ? static_cast<float>(q[e]) * a.scaleLog2e : 0.f;
-      acc[j] = 0.f;
-    }
-    for (int t0 = wave * 64; t0 < n; t0 += kPgWaves * 64) {
-      const int i0 = min(t0 + lane, n - 1), cnt = min(64, n - t0);
-      int64_t mine = ldIndex(a.bLoc, locBase + (i0 < head ? i0 : low + (i0 - head)), a.loc64);
-      if (mine < 0 || mine >= a.slots) mine = -1;  // slots outside the pool are skipped, never dereferenced
-      for (int i = 0; i < cnt; i += UNR) {
-        float k[UNR][J], v[UNR][J], sc[UNR], mt = m;
-        bool counts[UNR];
-#pragma unroll
-        for (int w = 0; w < UNR; ++w) {
-          const int from = min(i + w, cnt - 1);
-          const int64_t slot = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(mine >> 32), from) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)mine, from));
-          counts[w] = i + w < cnt && slot >= 0;
-          const T* kRow = kHead + max(slot, (int64_t)0) * a.kSlotStride;
-          const T* vRow = vHead + max(slot, (int64_t)0) * a.vSlotStride;
-#pragma unroll
-          for (int j = 0; j < J; ++j) k[w][j] = static_cast<float>(kRow[at_[j]]), v[w][j] = static_cast<float>(vRow[at_[j]]);
-        }
-#pragma unroll
-        for (int w = 0; w < UNR; ++w) {
-          float dot = 0.f;
-#pragma unroll
-          for (int j = 0; j < J; ++j) dot += lane + 64 * j < a.d ? qf[j] * k[w][j] : 0.f;
-          sc[w] = waveSum(dot);
-          if (!counts[w]) sc[w] = -INFINITY;
-          mt = fmaxf(mt, sc[w]);
-        }
-        const float ref = mt == -INFINITY ? 0.f : mt, corr = m == -INFINITY ? 1.f : exp2f(m - ref);  // (no maximum yet: the sums are 0, or NaN)
-        m = mt, l *= corr;
-#pragma unroll
-        for (int j = 0; j < J; ++j) acc[j] *= corr;
-#pragma unroll
-        for (int w = 0; w < UNR; ++w) {
-          if (!counts[w]) continue;
-          const float e = exp2f(behindRounded(sc[w], ref));
-          l += e;
-#pragma unroll
-          for (int j = 0; j < J; ++j) acc[j] += e * v[w][j];
-        }
-      }
-    }
-    if (l != l && m == -INFINITY) m = 0.f;  // scores that are not numbers alone: as a maximum of minus infinity they would be left out
+    int head, low;
+    paSeen(a, p, &head, &low);
+    PaColumn<T, J, UNR> c;
+    c.walk(a, reinterpret_cast<const T*>(a.q) + row * a.qTok + h * a.qHead, kvh, locBase, 0, head, low, p + 1, wave * 64, kPgWaves * 64);
     __syncthreads();  // (the sums of the token before have been read)
-    if (lane == 0) state[wave][0] = m, state[wave][1] = l;
+    if (lane == 0) state[wave][0] = c.m, state[wave][1] = c.l;
 #pragma unroll
-    for (int j = 0; j < J; ++j) red[wave][lane + 64 * j] = acc[j];
+    for (int j = 0; j < J; ++j) red[wave][lane + 64 * j] = c.acc[j];
     __syncthreads();
     float mAll = -INFINITY, lAll = 0.f, w[kPgWaves];
 #pragma unroll
@@ -207,6 +156,7 @@ extern "C" __attribute__((visibility("default"))) diopiError_t diopiPagedContext
   a.heads = (int)q.shape[1], a.kvHeads = (int)k.shape[1], a.d = (int)q.shape[2], a.batch = (int)batch;
   a.maxNew = maxNewLen, a.maxLen = maxInputLen;
   a.scaleLog2e = kLog2eTA / sqrtf((float)a.d);
+  if (pagedAttentionTiles(a, q.dtype)) return pagedAttentionMfma(ctx, stream, a, q.dtype);
   return pagedAttentionAny(stream, a, q.dtype);
 }
 

@@ -74,9 +74,83 @@ __device__ __forceinline__ PaPlace paFind(const PaArgs& a, int64_t u, F&& count)
   return p;
 }
 
+// The tokens that one at position p sees: [0, head) and [low, p].
+__device__ __forceinline__ void paSeen(const PaArgs& a, int p, int* head, int* low) {
+  *low = max(0, p - a.window + 1);
+  *head = max(0, min(a.sinks, min(*low, p + 1)));
+}
+
+// A wave's part of the attention of one (new token, head), any layout: the tokens [first0, first1) and [next0, next1) of the sequence,
+// 64 at a time from the `offset`th on and every `step`th 64 of them. A row is spread over the lanes (element lane + 64 j), UNR rows are
+// asked for at once; slots outside the pool are skipped, never dereferenced. m: the largest score in units of log2, l and acc: sums of
+// the weights against it, and of V.
+template <typename T, int J, int UNR>
+struct PaColumn {
+  float m = -INFINITY, l = 0.f, acc[J];
+  __device__ __forceinline__ void walk(const PaArgs& a, const T* q, int kvh, int64_t locBase, int first0, int first1, int next0, int next1, int offset, int step) {
+    const int lane = threadIdx.x & 63, head = max(0, first1 - first0), n = head + max(0, next1 - next0);
+    const T* kHead = reinterpret_cast<const T*>(a.k) + kvh * a.kHeadStride;
+    const T* vHead = reinterpret_cast<const T*>(a.v) + kvh * a.vHeadStride;
+    int at[J];  // the lane's elements of a row; past its end the first one, which q's zero leaves out
+    float qf[J];
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const int e = lane + 64 * j;
+      at[j] = e < a.d ? e : 0;
+      qf[j] = e < a.d ? static_cast<float>(q[e]) * a.scaleLog2e : 0.f;
+      acc[j] = 0.f;
+    }
+    for (int t0 = offset; t0 < n; t0 += step) {
+      const int i0 = min(t0 + lane, n - 1), cnt = min(64, n - t0);
+      int64_t mine = ldIndex(a.bLoc, locBase + (i0 < head ? first0 + i0 : next0 + (i0 - head)), a.loc64);
+      if (mine < 0 || mine >= a.slots) mine = -1;
+      for (int i = 0; i < cnt; i += UNR) {
+        float k[UNR][J], v[UNR][J], sc[UNR], mt = m;
+        bool counts[UNR];
+#pragma unroll
+        for (int w = 0; w < UNR; ++w) {
+          const int from = min(i + w, cnt - 1);
+          const int64_t slot = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(mine >> 32), from) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)mine, from));
+          counts[w] = i + w < cnt && slot >= 0;
+          const T* kRow = kHead + max(slot, (int64_t)0) * a.kSlotStride;
+          const T* vRow = vHead + max(slot, (int64_t)0) * a.vSlotStride;
+#pragma unroll
+          for (int j = 0; j < J; ++j) k[w][j] = static_cast<float>(kRow[at[j]]), v[w][j] = static_cast<float>(vRow[at[j]]);
+        }
+#pragma unroll
+        for (int w = 0; w < UNR; ++w) {
+          float dot = 0.f;
+#pragma unroll
+          for (int j = 0; j < J; ++j) dot += lane + 64 * j < a.d ? qf[j] * k[w][j] : 0.f;
+          sc[w] = waveSum(dot);
+          if (!counts[w]) sc[w] = -INFINITY;
+          mt = fmaxf(mt, sc[w]);
+        }
+        const float ref = mt == -INFINITY ? 0.f : mt, corr = m == -INFINITY ? 1.f : exp2f(m - ref);  // (no maximum yet: the sums are 0, or NaN)
+        m = mt, l *= corr;
+#pragma unroll
+        for (int j = 0; j < J; ++j) acc[j] *= corr;
+#pragma unroll
+        for (int w = 0; w < UNR; ++w) {
+          if (!counts[w]) continue;
+          const float e = exp2f(behindRounded(sc[w], ref));
+          l += e;
+#pragma unroll
+          for (int j = 0; j < J; ++j) acc[j] += e * v[w][j];
+        }
+      }
+    }
+    if (l != l && m == -INFINITY) m = 0.f;  // scores that are not numbers alone: as a maximum of minus infinity they would be left out
+  }
+};
+
 #endif
 
 // Attention over rows of any size and layout, q and pool of one type.
 diopiError_t pagedAttentionAny(hipStream_t stream, const PaArgs& a, diopiDtype_t dtype);
+
+// Attention on the matrix pipe: whether it takes these rows, and its launches.
+bool pagedAttentionTiles(const PaArgs& a, diopiDtype_t dtype);
+diopiError_t pagedAttentionMfma(diopiContextHandle_t ctx, hipStream_t stream, const PaArgs& a, diopiDtype_t dtype);
 
 }  // namespace amd
