@@ -186,6 +186,7 @@ extern "C" __attribute__((visibility("default"))) diopiError_t diopiTokenDecodeA
   if (window == 0 || (int64_t)window + sinks >= maxInputLen) return diopiTokenDecodeAttentionInference(ctx, outH, qH, kH, vH, locH, startH, lenH, maxInputLen);
   if (t.q.numel == 0) return diopiSuccess;
   AMD_CHECK(ta.batch <= 65535, "window attention: batch %d exceeds the grid limits", ta.batch);
+  if (!ta.generic) return decodeWindow(ctx, stream, ta, t.q.dtype, window, sinks, out.data);
   a.q = ta.q, a.k = ta.k, a.v = ta.v, a.out = out.data;
   a.bLoc = ta.bLoc, a.bLen = ta.bLen, a.loc64 = ta.loc64, a.len64 = ta.len64;
   a.locRowStride = ta.locRowStride;

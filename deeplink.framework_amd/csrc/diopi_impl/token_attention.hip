@@ -111,7 +111,8 @@ constexpr int splitWavesPerSimd(size_t itemsize, int lpt, bool hiw, int mode, in
 // of its rows (grouped-query layouts; 1 otherwise). With QPK > 1 the grid is one-dimensional and decoded so that the
 // workgroups that share a K/V head's rows run next to each other on one XCD.
 // BEHIND: the states begin with the partial results a.shared instead of empty (fused, one chunk).
-template <typename T, int LPT, bool HIW, int MODE = kTaFused, typename LT = float, int QPK = 1, bool PART = false, bool BEHIND = false>
+// WINDOW: the first a.sinks tokens of a sequence longer than a.maxLen lie apart (fused; a variant of its own, as every slot is asked).
+template <typename T, int LPT, bool HIW, int MODE = kTaFused, typename LT = float, int QPK = 1, bool PART = false, bool BEHIND = false, bool WINDOW = false>
 __global__ __launch_bounds__(kTaWaves * 64, splitWavesPerSimd(sizeof(T), LPT, HIW, MODE, QPK, PART)) void decodeSplitKernel(TaArgs a, T* __restrict__ out,
                                                                      float* __restrict__ partial) {
   static_assert(QPK == 1 || !HIW, "several query heads per lane group: the lane groups of a wave take tokens, not heads");
@@ -159,6 +160,7 @@ __global__ __launch_bounds__(kTaWaves * 64, splitWavesPerSimd(sizeof(T), LPT, HI
   if (begin >= len && !(split == 0 && MODE != kTaLogitsOut)) return;  // nothing to do; split 0 still writes zeros for len == 0
   const int end = min(len, begin + a.chunk);
   const int64_t locBase = (int64_t)b * a.locRowStride + (a.maxLen - len);
+  const int gap = WINDOW ? cutLength(a.bLen, b, a.len64, a.tableLen) - len : 0;
   // the scores of this lane's (first) head for the tokens of sequence b (two-call modes); head h + j is j rows further
   LT* scores = nullptr;
   if constexpr (MODE != kTaFused)
@@ -259,7 +261,7 @@ __global__ __launch_bounds__(kTaWaves * 64, splitWavesPerSimd(sizeof(T), LPT, HI
     for (int u = 0; u < UNR; ++u) {
       int t = t0 + u * TPI;
       slotTok[u] = t;
-      slot[u] = t >= end ? -1 : (idxInLds ? (int64_t)sidx[t - begin] : ldIndex(a.bLoc, locBase + t, a.loc64));
+      slot[u] = t >= end ? -1 : (idxInLds ? (int64_t)sidx[t - begin] : ldIndex(a.bLoc, locBase + t - (WINDOW && t < a.sinks ? gap : 0), a.loc64));
     }
   };
   auto loadRows = [&](V (&kk)[UNR], V (&vv)[UNR], float (&lg)[QPK][UNR], bool (&okk)[UNR]) {
@@ -499,8 +501,8 @@ __device__ __forceinline__ void waitLoadsBut() {  // all but the wave's N younge
 // them for the VALU: second half in bf16 2 - 5 % less. Fused rows of 256 need more than half the registers.)
 // D: head size the rows are laid out for (64, 128, 256); a.d is any multiple of 8 up to it: the pieces past the row's end
 // repeat its first one, meet zeros of q, and give output columns that are not stored.
-// BEHIND: the partial results a.shared are merged with the chunk's at the end (fused, one chunk).
-template <typename T, int D, int MODE, typename LT, bool BEHIND = false>
+// BEHIND: the partial results a.shared are merged with the chunk's at the end (fused, one chunk). WINDOW: as there (fused).
+template <typename T, int D, int MODE, typename LT, bool BEHIND = false, bool WINDOW = false>
 __global__ __launch_bounds__(kGqWaves * 64, MODE == kTaFused && D == 256 ? 1 : kGqWgsPerCu) void decodeGroupedKernel(TaArgs a, T* __restrict__ out, float* __restrict__ partial) {
   using M = GqMfma<T>;
   using Frag = typename M::Frag;
@@ -530,6 +532,7 @@ __global__ __launch_bounds__(kGqWaves * 64, MODE == kTaFused && D == 256 ? 1 : k
   if (begin >= len && !(split == 0 && MODE != kTaLogitsOut)) return;  // split 0 still writes zeros for len == 0
   const int end = min(len, begin + a.chunk);
   const int64_t locBase = (int64_t)b * a.locRowStride + (a.maxLen - len);
+  const int gap = WINDOW ? cutLength(a.bLen, b, a.len64, a.tableLen) - len : 0;
   LT* scores = nullptr;
   if constexpr (MODE != kTaFused)
     scores = static_cast<LT*>(const_cast<void*>(a.logits)) + h * a.logitsHeadStride + ldIndex(a.bStart, b, a.start64);
@@ -599,7 +602,8 @@ walk:
     for (int i = 0; i < kGqBlock / 64; ++i) {
       const int t = i * 64 + lane;
       if (t < tiles * kGqTile) {  // past the wave's last token: that token again (its score is masked)
-        const int64_t s = ldIndex(a.bLoc, locBase + b0 + min(t, cnt - 1), a.loc64);
+        const int at = b0 + min(t, cnt - 1);
+        const int64_t s = ldIndex(a.bLoc, locBase + at - (WINDOW && at < a.sinks ? gap : 0), a.loc64);
         const bool in = s >= 0 && s < a.slots;  // slots outside the pool are skipped, never dereferenced
         slots[t] = in ? (int)s : -1;
         bad |= !in;
@@ -1137,6 +1141,11 @@ static diopiError_t checkIndex(const TensorView& t, const char* name) {
   return diopiSuccess;
 }
 
+// at most kTaMaxSplit chunks per sequence; chunks stay a multiple of 64 tokens
+static int longestChunk(int maxLen) {
+  return (int64_t)maxLen > (int64_t)kTaChunk * kTaMaxSplit ? (int)(ceilDiv(ceilDiv(maxLen, kTaMaxSplit), 64) * 64) : kTaChunk;
+}
+
 // q, the slot table, the starts and the lengths.
 diopiError_t tableArgs(const TaViews& t, int maxLen, TaArgs* a) {
   const TensorView& q = t.q;
@@ -1210,9 +1219,7 @@ diopiError_t fillArgs(const TaViews& t, bool needK, bool needV, int maxLen, TaAr
   a->vHeadStride = needV ? t.v.stride[1] : 0;
   a->slots = kv.shape[0];
   a->kvHeads = (int)kv.shape[1];
-  // at most kTaMaxSplit chunks per sequence; chunks stay a multiple of 64 tokens
-  a->chunk = kTaChunk;
-  if ((int64_t)maxLen > (int64_t)kTaChunk * kTaMaxSplit) a->chunk = (int)(ceilDiv(ceilDiv(maxLen, kTaMaxSplit), 64) * 64);
+  a->chunk = longestChunk(maxLen);
   return diopiSuccess;
 }
 
@@ -1405,6 +1412,7 @@ static diopiError_t streamChunks(diopiContextHandle_t ctx, hipStream_t stream, T
   a.nsplit = (int)std::max<int64_t>(1, ceilDiv(maxInputLen, a.chunk));
   // (one chunk and up to 32 shares of other tokens, us: 4 x (1 .. 20) own tokens of 8 heads of 64, 13, 31 and 32 shares 13.8 -> 10.6, 13.9 -> 12.0,
   // 17.0 -> 15.6; 48 x (10 .. 300), 32 heads of 128 on 8, 16 shares 36.5 -> 31.1)
+  const bool windowed = a.sinks > 0;
   const bool behind = keep && a.nsplit == 1 && a.nShared <= kTaMostShared;
   if (keep && !behind) a.nsplit = std::max(a.nsplit, 2);  // (one share is written as the result: a second one, without tokens, makes it a partial result)
   AMD_CHECK(batch <= 65535 && a.nsplit <= 65535, "token attention: batch %ld / splits %d exceed the grid limits", (long)batch,
@@ -1435,15 +1443,17 @@ static diopiError_t streamChunks(diopiContextHandle_t ctx, hipStream_t stream, T
   if (grouped) {
     const int mats = MODE == kTaFused ? 2 : 1, d = (int)(bytes / 2);
     const int lds = gqRingBytes(d, mats) + (MODE == kTaFused ? 0 : kGqWaves * std::min(perKv, kGqHeads) * kGqScoreRow * (int)sizeof(float));
-#define GROUPED_CALL_AS(T, D, LT, BEHIND)                                                                                                \
+#define GROUPED_CALL_AS(T, D, LT, ...)                                                                                                   \
   do {                                                                                                                                   \
-    AMD_HIP(allowDynamicLds(reinterpret_cast<const void*>(decodeGroupedKernel<T, D, MODE, LT, BEHIND>), lds));                            \
-    hipLaunchKernelGGL((decodeGroupedKernel<T, D, MODE, LT, BEHIND>), grid, dim3(kGqWaves * 64), lds, stream, a, static_cast<T*>(outPtr), \
+    AMD_HIP(allowDynamicLds(reinterpret_cast<const void*>(decodeGroupedKernel<T, D, MODE, LT, __VA_ARGS__>), lds));                            \
+    hipLaunchKernelGGL((decodeGroupedKernel<T, D, MODE, LT, __VA_ARGS__>), grid, dim3(kGqWaves * 64), lds, stream, a, static_cast<T*>(outPtr), \
                        partial);                                                                                                         \
   } while (0)
 #define GROUPED_CALL(T, D)                          \
   if (behind) {                                     \
     if constexpr (MODE == kTaFused) GROUPED_CALL_AS(T, D, float, true); \
+  } else if (windowed) {                            \
+    if constexpr (MODE == kTaFused) GROUPED_CALL_AS(T, D, float, false, true); \
   } else if (MODE == kTaFused || scoresF32) {       \
     GROUPED_CALL_AS(T, D, float, false);            \
   } else {                                          \
@@ -1456,20 +1466,22 @@ static diopiError_t streamChunks(diopiContextHandle_t ctx, hipStream_t stream, T
 #undef GROUPED_CALL
 #undef GROUPED_CALL_AS
   } else {
-#define STREAM_CALL_PART(T, LPT, LT, PART, BEHIND)                                                                                           \
-  if (qpk == 4) hipLaunchKernelGGL((decodeSplitKernel<T, LPT, false, MODE, LT, 4, PART, BEHIND>), grid, block, 0, stream, a, static_cast<T*>(outPtr), partial); \
-  else if (qpk == 2) hipLaunchKernelGGL((decodeSplitKernel<T, LPT, false, MODE, LT, 2, PART, BEHIND>), grid, block, 0, stream, a, static_cast<T*>(outPtr), partial); \
-  else if (hiw) hipLaunchKernelGGL((decodeSplitKernel<T, LPT, true, kTaFused, float, 1, PART, BEHIND>), grid, block, 0, stream, a, static_cast<T*>(outPtr), partial); \
-  else hipLaunchKernelGGL((decodeSplitKernel<T, LPT, false, MODE, LT, 1, PART, BEHIND>), grid, block, 0, stream, a, static_cast<T*>(outPtr), partial)
-#define STREAM_CALL_AS(T, LPT, LT, BEHIND)    \
-  if (partRows) {                             \
-    STREAM_CALL_PART(T, LPT, LT, true, BEHIND);  \
-  } else {                                    \
-    STREAM_CALL_PART(T, LPT, LT, false, BEHIND); \
+#define STREAM_CALL_PART(T, LPT, LT, PART, ...)                                                                                              \
+  if (qpk == 4) hipLaunchKernelGGL((decodeSplitKernel<T, LPT, false, MODE, LT, 4, PART, __VA_ARGS__>), grid, block, 0, stream, a, static_cast<T*>(outPtr), partial); \
+  else if (qpk == 2) hipLaunchKernelGGL((decodeSplitKernel<T, LPT, false, MODE, LT, 2, PART, __VA_ARGS__>), grid, block, 0, stream, a, static_cast<T*>(outPtr), partial); \
+  else if (hiw) hipLaunchKernelGGL((decodeSplitKernel<T, LPT, true, kTaFused, float, 1, PART, __VA_ARGS__>), grid, block, 0, stream, a, static_cast<T*>(outPtr), partial); \
+  else hipLaunchKernelGGL((decodeSplitKernel<T, LPT, false, MODE, LT, 1, PART, __VA_ARGS__>), grid, block, 0, stream, a, static_cast<T*>(outPtr), partial)
+#define STREAM_CALL_AS(T, LPT, LT, ...)            \
+  if (partRows) {                                  \
+    STREAM_CALL_PART(T, LPT, LT, true, __VA_ARGS__);  \
+  } else {                                         \
+    STREAM_CALL_PART(T, LPT, LT, false, __VA_ARGS__); \
   }
 #define STREAM_CALL(T, LPT)                                                  \
   if (behind) {                                                              \
     if constexpr (MODE == kTaFused) { STREAM_CALL_AS(T, LPT, float, true); } \
+  } else if (windowed) {                                                     \
+    if constexpr (MODE == kTaFused) { STREAM_CALL_AS(T, LPT, float, false, true); } \
   } else if (MODE == kTaFused || scoresF32) {                                \
     STREAM_CALL_AS(T, LPT, float, false);                                    \
   } else if constexpr (sizeof(T) == 2) { /* (of fp32 rows they are fp32) */  \
@@ -1491,6 +1503,13 @@ static diopiError_t streamChunks(diopiContextHandle_t ctx, hipStream_t stream, T
 
 diopiError_t amd::decodePartials(diopiContextHandle_t ctx, hipStream_t stream, const TaArgs& a, diopiDtype_t dtype, int maxInputLen, void* out, TaPartials* keep) {
   return streamChunks<kTaFused>(ctx, stream, a, dtype, a.d * dtypeSize(dtype), a.batch, maxInputLen, out, true, false, nullptr, keep);
+}
+
+diopiError_t amd::decodeWindow(diopiContextHandle_t ctx, hipStream_t stream, TaArgs a, diopiDtype_t dtype, int window, int sinks, void* out) {
+  a.tableLen = a.maxLen, a.sinks = sinks, a.maxLen = window + sinks;
+  a.chunk = longestChunk(a.maxLen);
+  a.bLoc = static_cast<const char*>(a.bLoc) + (int64_t)(a.tableLen - a.maxLen) * (a.loc64 ? 8 : 4);
+  return streamChunks<kTaFused>(ctx, stream, a, dtype, a.d * dtypeSize(dtype), a.batch, a.maxLen, out, true, false, nullptr);
 }
 
 static diopiError_t decodeAttention(diopiContextHandle_t ctx, diopiTensorHandle_t outH, diopiConstTensorHandle_t qH,

@@ -46,6 +46,9 @@ struct TaArgs {
   int batch;    // sequences (the grouped-query kernels decode a one-dimensional grid)
   const float* shared;  // decodePartials: partial results [batch, heads, nShared, 2 + d] of other tokens of the sequences, as in mergeChunks
   int nShared;
+  // With a window: bLoc and maxLen are those of the tokens that are seen, the first `sinks` and the last others, right-aligned where they
+  // are all there are; of a sequence that has more (up to tableLen) the first ones lie as far to the left as it is longer.
+  int sinks, tableLen;
 };
 
 // max / sum of one value per thread over the workgroup of 256 (red: 4 floats of LDS; two barriers)
@@ -102,6 +105,10 @@ struct TaPartials {
   float raise;  // sums are against the maximum less this (in units of log2)
 };
 diopiError_t decodePartials(diopiContextHandle_t ctx, hipStream_t stream, const TaArgs& a, diopiDtype_t dtype, int maxInputLen, void* out, TaPartials* keep);
+
+// diopiTokenDecodeAttentionInference's kernels (not for generic arguments) over the last `window` tokens of each sequence and its first
+// `sinks`, window + sinks < a.maxLen.
+diopiError_t decodeWindow(diopiContextHandle_t ctx, hipStream_t stream, TaArgs a, diopiDtype_t dtype, int window, int sinks, void* out);
 
 // As decodePartials, for rows of any kind and for int8 pools: partial results of the first `walked` tokens in `loc` and the own ones behind
 // them, of at least one chunk; if nothing else is to be merged (alone) and there is one chunk, the result (own->nsplit is 0 then).
