@@ -290,8 +290,108 @@ __global__ __launch_bounds__(256) void rotaryAppendAnyKernel(RotaryAppendArgs a)
   }
 }
 
+// Head rows of whole 16-byte pieces. A thread keeps its place in the head row, and with it the angles, for all of its heads (up to
+// kAppendHeads, whose rows it asks for at once); the heads of q, k and v are one list, cut into grid.y shares of x.share; tokens with few
+// heads share a workgroup.
+constexpr int kAppendHeads = 4;
+struct RotaryAppendShape {
+  int perHead, across, share, tokPerWg;  // work items of a head; heads side by side; heads of a workgroup; tokens of a workgroup
+  bool tabVec;
+};
+template <typename T, typename CT, bool INTERLEAVED>
+__global__ __launch_bounds__(256) void rotaryAppendKernel(RotaryAppendArgs a, RotaryAppendShape x) {
+  using V = typename Vec16<T>::type;
+  constexpr int N = Vec16<T>::N, A = INTERLEAVED ? N / 2 : N;  // elements of a piece, angles of a work item
+  const int perTok = x.perHead * x.across, local = threadIdx.x / perTok, in = threadIdx.x - local * perTok;
+  const int64_t t = (int64_t)blockIdx.x * x.tokPerWg + local;
+  if (local >= x.tokPerWg || t >= a.tokens) return;
+  const int first = in / x.perHead, j = in - first * x.perHead, half = a.d / 2;
+  const int rotated = a.heads + a.kvHeads, h0 = blockIdx.y * x.share + first, end = min((int)(blockIdx.y + 1) * x.share, rotated + a.kvHeads);
+  // slot and position are asked for before anything waits
+  const int64_t dest = indexAt(a.destLoc, t, a.loc64);
+  const int64_t trow = a.positions != nullptr ? indexAt(a.positions, t, a.pos64) : t % a.tableRows;
+  V v0[kAppendHeads], v1[kAppendHeads];
+  const int step = j * N;
+#pragma unroll
+  for (int u = 0; u < kAppendHeads; ++u) {
+    const int h = h0 + u * x.across;
+    if (h >= end) continue;
+    const T* from = h < a.heads ? static_cast<const T*>(a.q) + t * a.qTok + (int64_t)h * a.qHead
+                    : h < rotated ? static_cast<const T*>(a.k) + t * a.kTok + (int64_t)(h - a.heads) * a.kHead
+                                  : static_cast<const T*>(a.v) + t * a.vTok + (int64_t)(h - rotated) * a.vHead;
+    v0[u] = __builtin_nontemporal_load(reinterpret_cast<const V*>(from + step));
+    if constexpr (!INTERLEAVED) v1[u] = __builtin_nontemporal_load(reinterpret_cast<const V*>(from + half + step));
+  }
+  float c[A], s[A];
+  const bool inside = trow >= 0 && trow < a.tableRows;
+  if (h0 < rotated) {
+    const int64_t at = (inside ? trow : 0) * a.tableCols;
+    if (INTERLEAVED && a.tableCols == a.d) {  // full-width tables hold a pair's angle twice
+#pragma unroll
+      for (int e = 0; e < A; ++e) {
+        c[e] = static_cast<float>(static_cast<const CT*>(a.cosT)[at + (j * A + e) * 2]);
+        s[e] = static_cast<float>(static_cast<const CT*>(a.sinT)[at + (j * A + e) * 2]);
+      }
+    } else {
+      loadAngles<CT, A>(static_cast<const CT*>(a.cosT) + at + j * A, x.tabVec, c);
+      loadAngles<CT, A>(static_cast<const CT*>(a.sinT) + at + j * A, x.tabVec, s);
+    }
+    if (!inside) {
+#pragma unroll
+      for (int e = 0; e < A; ++e) c[e] = s[e] = 0.f;
+    }
+  }
+  const int64_t slot = dest < 0 ? dest + a.slots : dest;
+  const bool kept = slot >= 0 && slot < a.slots;  // an out-of-range slot is dropped, never written
+#pragma unroll
+  for (int u = 0; u < kAppendHeads; ++u) {
+    const int h = h0 + u * x.across;
+    if (h >= end || (h >= a.heads && !kept)) continue;
+    T* to = h < a.heads ? static_cast<T*>(a.outQ) + t * a.oTok + (int64_t)h * a.oHead
+            : h < rotated ? static_cast<T*>(a.poolK) + slot * a.pkSlot + (int64_t)(h - a.heads) * a.pkHead
+                          : static_cast<T*>(a.poolV) + slot * a.pvSlot + (int64_t)(h - rotated) * a.pvHead;
+    V r0 = v0[u], r1;
+    if constexpr (!INTERLEAVED) r1 = v1[u];
+    if (h < rotated) {
+#pragma unroll
+      for (int e = 0; e < A; ++e) {
+        const float x0 = static_cast<float>(INTERLEAVED ? v0[u][2 * e] : v0[u][e]), x1 = static_cast<float>(INTERLEAVED ? v0[u][2 * e + 1] : v1[u][e]);
+        const T y0 = static_cast<T>(x0 * c[e] - x1 * s[e]), y1 = static_cast<T>(x0 * s[e] + x1 * c[e]);
+        if constexpr (INTERLEAVED) r0[2 * e] = y0, r0[2 * e + 1] = y1;
+        else r0[e] = y0, r1[e] = y1;
+      }
+    }
+    __builtin_nontemporal_store(r0, reinterpret_cast<V*>(to + step));
+    if constexpr (!INTERLEAVED) __builtin_nontemporal_store(r1, reinterpret_cast<V*>(to + half + step));
+  }
+}
+
 template <typename T, typename CT>
 static diopiError_t launchRotaryAppend(hipStream_t stream, const RotaryAppendArgs& a) {
+  constexpr int N = Vec16<T>::N;
+  uintptr_t bits = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) | reinterpret_cast<uintptr_t>(a.outQ) |
+                   reinterpret_cast<uintptr_t>(a.poolK) | reinterpret_cast<uintptr_t>(a.poolV);
+  bits |= (uintptr_t)(a.qTok | a.qHead | a.oTok | a.oHead | a.kTok | a.kHead | a.vTok | a.vHead | a.pkSlot | a.pkHead | a.pvSlot | a.pvHead) * sizeof(T);
+  const int piece = a.interleaved ? N : 2 * N;  // elements of a work item
+  if ((bits & 15) == 0 && a.d % piece == 0 && a.d / piece <= 256) {
+    RotaryAppendShape x;
+    const int all = a.heads + 2 * a.kvHeads;
+    x.perHead = a.d / piece;
+    x.across = std::min(all, 256 / x.perHead);
+    const int shares = (int)ceilDiv(all, (int64_t)x.across * kAppendHeads);
+    x.share = (int)ceilDiv(all, shares);
+    x.tokPerWg = 256 / (x.perHead * x.across);
+    const int entries = a.interleaved ? N / 2 : N, align = entries * (int)sizeof(CT) >= 16 ? 16 : 8;
+    x.tabVec = ((reinterpret_cast<uintptr_t>(a.cosT) | reinterpret_cast<uintptr_t>(a.sinT) | (uintptr_t)a.tableCols * sizeof(CT)) % align) == 0;
+    const int64_t blocks = ceilDiv(a.tokens, x.tokPerWg);
+    if (shares <= 65535 && blocks * shares < 1 << 24) {  // (fewer than 2^32 threads)
+      const dim3 grid((unsigned)blocks, (unsigned)shares);
+      if (a.interleaved) hipLaunchKernelGGL((rotaryAppendKernel<T, CT, true>), grid, dim3(256), 0, stream, a, x);
+      else hipLaunchKernelGGL((rotaryAppendKernel<T, CT, false>), grid, dim3(256), 0, stream, a, x);
+      AMD_LAUNCH_CHECK();
+      return diopiSuccess;
+    }
+  }
   const unsigned blocks = (unsigned)std::min<int64_t>(a.tokens, 1 << 23);  // (fewer than 2^32 threads)
   hipLaunchKernelGGL((rotaryAppendAnyKernel<T, CT>), dim3(blocks), dim3(256), 0, stream, a);
   AMD_LAUNCH_CHECK();
