@@ -1,6 +1,6 @@
-// Attention of new tokens over a paged pool on the matrix pipe, 16-bit rows (see paged_attention.hip for what it computes).
+// Attention of new tokens over a paged pool on the matrix pipe (see paged_attention.hip for what it computes).
 //
-// A workgroup takes 128 columns of one K/V head of one sequence, a column being a (new token, query head that reads this K/V head),
+// 16-bit rows: a workgroup takes 128 columns of one K/V head of one sequence, a column being a (new token, query head that reads this K/V head),
 // heads fastest: with G query heads to a K/V head a row of the pool is read once for G heads of 128 / G tokens. It walks the
 // tokens that these see in tiles of 64, or a share of them. Its four waves own 32 columns each.
 //   * S^T = K . Q^T (32x32x16): a lane holds 16 scores of ONE column, so the running maximum and sum of the softmax are the lane's and one
@@ -19,6 +19,7 @@
 // keep an infinity or NaN in V out of a sum, and scores beyond 2^22 would be off against their rounded maximum. A column whose sums come
 // out not finite, or whose maximum is beyond that, is walked again by itself on the vector ALUs, the tokens that it sees alone (PaColumn).
 #include <algorithm>
+#include <type_traits>
 
 #include "paged_attention.hpp"
 
@@ -69,11 +70,12 @@ struct PtSpan {
 };
 
 // Blocks of columns of a sequence, and the most shares that one of them has.
+template <int COLS>
 struct PtPieces {
   int blocks, splits;
   __device__ __forceinline__ PtPieces(const PtArgs& x, const PaSequence& s) {
     const int group = x.a.heads / x.a.kvHeads, tokens = s.end - s.first;
-    blocks = (int)(((int64_t)tokens * group + kPtCols - 1) / kPtCols);
+    blocks = (int)(((int64_t)tokens * group + COLS - 1) / COLS);
     const int upTo = (s.origin + s.end + kPtTile - 1) / kPtTile;
     const int64_t windowed = (x.a.sinks + kPtTile - 1) / kPtTile + ((int64_t)x.a.window + kPtCols + kPtTile - 1) / kPtTile;
     splits = max(1, ((int)min((int64_t)upTo, windowed) + x.tilesPerSplit - 1) / x.tilesPerSplit);
@@ -87,6 +89,33 @@ template <int D>
 __device__ __forceinline__ int ptSwizzleK(int key) { return D >= 128 ? (key & 15) : ((key >> 1) & 7); }
 template <int D>
 __device__ __forceinline__ int ptSwizzleV(int key) { return D >= 128 ? 4 * (key & 3) : 4 * ((key >> 1) & 1); }
+
+// Column `col` of a piece of work by itself, on the vector ALUs of one wave.
+template <typename T, int D>
+__device__ __forceinline__ void pagedAgain(const PtArgs& x, const PaSequence& s, int kvh, int64_t locBase, const PtSpan& span, int t0, int t1, int split, bool whole,
+                                           int col) {
+  const PaArgs& a = x.a;
+  const int lane = threadIdx.x & 63, group = a.heads / a.kvHeads, token = s.first + col / group, h = kvh * group + col % group, p = s.origin + token;
+  const int64_t row = s.start + token;
+  int head, low;
+  paSeen(a, p, &head, &low);
+  // of the tiles' tokens those that it sees: of the first ones, and of the others
+  const int from = span.base(max(t0, span.sinkTiles)), to = t1 > span.sinkTiles ? min(span.base(t1), p + 1) : 0;
+  const int first0 = span.sinkTiles > 0 ? min(t0, span.sinkTiles) * kPtTile : from, first1 = span.sinkTiles > 0 ? min(head, min(t1, span.sinkTiles) * kPtTile) : min(head, to);
+  PaColumn<T, D / 64, (D > 128 ? 4 : 8)> one;
+  one.walk(a, reinterpret_cast<const T*>(a.q) + row * a.qTok + (int64_t)h * a.qHead, kvh, locBase, first0, first1, max(from, low), to, 0, 64);
+  float* dst = x.partial + ((row * a.heads + h) * x.splits + split) * (2 + a.d);
+  T* out = reinterpret_cast<T*>(a.out) + row * a.oTok + (int64_t)h * a.oHead;
+  const float inv = one.l == 0.f ? 0.f : 1.f / one.l;
+  if (!whole && lane == 0) dst[0] = one.m, dst[1] = one.l;
+#pragma unroll
+  for (int j = 0; j < D / 64; ++j) {
+    const int e = lane + 64 * j;
+    if (e >= a.d) continue;
+    if (whole) out[e] = static_cast<T>(one.acc[j] * inv);
+    else dst[2 + e] = one.acc[j];
+  }
+}
 
 // One block of columns over tiles [t0, t1), all of them if `whole`.
 // D: the head size that tiles are laid out for; with PART a.d is any multiple of 8 below it, and the places behind it are zeros.
@@ -378,57 +407,225 @@ __device__ __forceinline__ void pagedTileBlock(const PtArgs& x, const PaSequence
             *reinterpret_cast<const Frag*>(sO + r * OS + c * 8);
   }
   }
-  while (again != 0) {  // (uniform)
-    const int c = __builtin_ctz(again), oc = c0 + c, at = s.first + oc / group, hc = kvh * group + oc % group;
-    again &= again - 1;
-    int head, low;
-    paSeen(a, s.origin + at, &head, &low);
-    // of the tiles' tokens those that it sees: of the first ones, and of the others
-    const int from = span.base(max(t0, span.sinkTiles)), to = t1 > span.sinkTiles ? min(span.base(t1), s.origin + at + 1) : 0;
-    const int first0 = span.sinkTiles > 0 ? min(t0, span.sinkTiles) * kPtTile : from, first1 = span.sinkTiles > 0 ? min(head, min(t1, span.sinkTiles) * kPtTile) : min(head, to);
-    PaColumn<T, D / 64, (D > 128 ? 4 : 8)> one;
-    one.walk(a, reinterpret_cast<const T*>(a.q) + (s.start + at) * a.qTok + (int64_t)hc * a.qHead, kvh, locBase, first0, first1, max(from, low), to, 0, 64);
-    float* dst = x.partial + (((s.start + at) * a.heads + hc) * x.splits + split) * (2 + a.d);
-    T* out = reinterpret_cast<T*>(a.out) + (s.start + at) * a.oTok + (int64_t)hc * a.oHead;
-    const float inv = one.l == 0.f ? 0.f : 1.f / one.l;
-    if (!whole && lane == 0) dst[0] = one.m, dst[1] = one.l;
-#pragma unroll
-    for (int j = 0; j < D / 64; ++j) {
-      const int e = lane + 64 * j;
-      if (e >= a.d) continue;
-      if (whole) out[e] = static_cast<T>(one.acc[j] * inv);
-      else dst[2 + e] = one.acc[j];
-    }
-  }
+  for (; again != 0; again &= again - 1) pagedAgain<T, D>(x, s, kvh, locBase, span, t0, t1, split, whole, c0 + __builtin_ctz(again));
 }
 
-
-// grid: K/V heads fastest (the ids go round the XCDs, so a head's pieces stay on one), then the list of pieces: sequence after sequence,
-// shares from the first, blocks from the last, which has the most tiles.
-template <typename T, int D, bool PART>
-__global__ __launch_bounds__(256, D > 128 ? 1 : 2) void pagedTileKernel(PtArgs x) {
+// A workgroup's pieces of work. grid: K/V heads fastest (the ids go round the XCDs, so a head's pieces stay on one), then the list of
+// pieces: sequence after sequence, shares from the first, blocks from the last, which has the most tiles.
+template <int COLS, typename F>
+__device__ __forceinline__ void pagedPieces(const PtArgs& x, F&& walk) {
   const PaArgs& a = x.a;
   const int kvh = blockIdx.x % a.kvHeads, step = gridDim.x / a.kvHeads, group = a.heads / a.kvHeads;
   for (int64_t u = blockIdx.x / a.kvHeads;; u += step) {
-    const PaPlace at = paFind(a, u, [&](const PaSequence& s) { return PtPieces(x, s).all(); });
+    const PaPlace at = paFind(a, u, [&](const PaSequence& s) { return PtPieces<COLS>(x, s).all(); });
     if (at.b < 0) return;
     const PaSequence s = paSequence(a, at.b);
-    const PtPieces pieces(x, s);
+    const PtPieces<COLS> pieces(x, s);
     const int split = at.at / pieces.blocks, block = pieces.blocks - 1 - at.at % pieces.blocks;
     const int cols = (s.end - s.first) * group, origin = s.origin + s.first;
-    const PtSpan span(a, origin + block * kPtCols / group, origin + min(block * kPtCols + kPtCols - 1, cols - 1) / group);
+    const PtSpan span(a, origin + block * COLS / group, origin + min(block * COLS + COLS - 1, cols - 1) / group);
     const bool whole = span.tiles <= x.tilesPerSplit;
-    const int t0 = split * min(x.tilesPerSplit, 1 << 24), t1 = whole ? span.tiles : min(span.tiles, t0 + x.tilesPerSplit);
-    if (split == 0 || t0 < span.tiles)
-      pagedTileBlock<T, D, PART>(x, s, at.b, kvh, block, span, t0, t1, split, whole);
+    const int t0 = split * x.tilesPerSplit, t1 = min(span.tiles, t0 + x.tilesPerSplit);
+    if (split == 0 || t0 < span.tiles) walk(s, at.b, kvh, block, span, t0, t1, split, whole);
     if (u + step >= at.total) return;
     __syncthreads();  // (the next piece's tiles take the place of this one's output)
   }
 }
 
+template <typename T, int D, bool PART>
+__global__ __launch_bounds__(256, D > 128 ? 1 : 2) void pagedTileKernel(PtArgs x) {
+  pagedPieces<kPtCols>(x, [&](const PaSequence& s, int b, int kvh, int block, const PtSpan& span, int t0, int t1, int split, bool whole) {
+    pagedTileBlock<T, D, PART>(x, s, b, kvh, block, span, t0, t1, split, whole);
+  });
+}
+
+// fp32 rows on the fp32 matrix instructions (true fp32 products and sums). A workgroup takes 16 columns; of every tile its four waves take 16
+// tokens each, with a softmax state of their own, and the states meet in LDS at the end: the chains of loads are short, which is what bounds
+// the short sequences of the fp32 configuration.
+// v_mfma_f32_16x16x4_f32: lane (c = l & 15, g = l >> 4) feeds row c, k = g of both operands and receives D[4 g + r][c].
+//   S^T = K Q^T: the contraction order is free as long as both operands agree, so group g takes the D / 4 consecutive elements from g D / 4
+//   on, 16-byte loads straight into operand registers. The lane ends up with tokens 4 g .. 4 g + 3 of column c, which is P^T's operand
+//   layout when step r takes token 4 g + r from group g: no data moves between lanes.
+//   O^T = V^T P^T: row i of output tile t stands for element i (D / 16) + t, so a lane's D / 16 operands of a token are consecutive in memory,
+//   and its results are D / 4 consecutive elements of column c.
+// Rows go from the pool into registers a tile ahead, slots another one.
+constexpr int kPtFloatCols = 16;
+template <int D, bool PART>
+__device__ __forceinline__ void pagedFloatBlock(const PtArgs& x, const PaSequence& s, int b, int kvh, int block, const PtSpan& span, int t0, int t1, int split,
+                                                bool whole) {
+  constexpr int S = D / 4, E = D / 16, PITCH = D + 4;
+  extern __shared__ __attribute__((aligned(16))) char ptSmem[];
+  float* const so = reinterpret_cast<float*>(ptSmem);  // [4][16][PITCH]
+  __shared__ float sm[4][16], sl[4][16];
+  const PaArgs& a = x.a;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
+  const int group = a.heads / a.kvHeads, cols = (s.end - s.first) * group, c0 = block * kPtFloatCols;
+  const int col = min(c0 + c, cols - 1), token = s.first + col / group, h = kvh * group + col % group, p = s.origin + token;
+  const int pFirst = __builtin_amdgcn_readlane(p, 0), pLast = __builtin_amdgcn_readlane(p, 15);
+  const int window = a.window, sinksSeen = max(0, min(a.sinks, p + 1));
+  const int len = cutLength(a.bLen, b, a.len64, a.maxLen);
+  const int64_t locBase = (int64_t)b * a.locRowStride + (a.maxLen - len);
+  const float* const kHead = reinterpret_cast<const float*>(a.k) + kvh * a.kHeadStride;
+  const float* const vHead = reinterpret_cast<const float*>(a.v) + kvh * a.vHeadStride;
+  f32x4 qf[S / 4], kf[2][S / 4], vf[2][4][E / 4], o[E];
+  // (PART: places past the row's end read its first piece, are zeros in q and K, and give elements that are not stored)
+  auto at = [&](int e) { return !PART || e < a.d ? e : 0; };
+  {
+    const float* q = reinterpret_cast<const float*>(a.q) + (s.start + token) * a.qTok + (int64_t)h * a.qHead;
+#pragma unroll
+    for (int i = 0; i < S / 4; ++i) {
+      qf[i] = *reinterpret_cast<const f32x4*>(q + at(g * S + 4 * i));
+      if (PART && g * S + 4 * i >= a.d) qf[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+  }
+  auto askSlot = [&](int t) {
+    if (t >= t1) return (int64_t)0;
+    return ldIndex(a.bLoc, locBase + min(span.base(t) + 16 * wave + c, span.limit(t) - 1), a.loc64);
+  };
+  uint32_t valid[2];
+  auto fetch = [&](int64_t slot, auto buf) {
+    constexpr int B = decltype(buf)::value;
+    const bool in = slot >= 0 && slot < a.slots;
+    valid[B] = (uint32_t)__builtin_amdgcn_ballot_w64(in) & 0xffffu;
+    // (slots outside the pool are skipped, never dereferenced: the first one inside stands in, slot 0 where there is none)
+    const int instead = valid[B] != 0 ? __builtin_amdgcn_readlane((int)slot, __builtin_ctz(valid[B])) : 0, mine = in ? (int)slot : instead;
+    const float* kr = kHead + (int64_t)mine * a.kSlotStride;
+#pragma unroll
+    for (int i = 0; i < S / 4; ++i) {
+      kf[B][i] = *reinterpret_cast<const f32x4*>(kr + at(g * S + 4 * i));
+      if (PART && g * S + 4 * i >= a.d) kf[B][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float* vr = vHead + (int64_t)__shfl(mine, 4 * g + r, 64) * a.vSlotStride;
+#pragma unroll
+      for (int i = 0; i < E / 4; ++i) vf[B][r][i] = *reinterpret_cast<const f32x4*>(vr + at(c * E + 4 * i));
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < E; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;  // m: in units of log2
+  auto tile = [&](int t, auto buf) {
+    constexpr int B = decltype(buf)::value;
+    const int k0 = span.base(t) + 16 * wave;
+    if (k0 > pLast || k0 >= span.limit(t) || (k0 + 15 <= pFirst - window && k0 >= a.sinks)) return;  // (uniform: nobody sees any of it)
+    f32x4 acc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};  // two chains: half the dependent latency
+#pragma unroll
+    for (int i = 0; i < S; ++i) acc[i & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[B][i >> 2][i & 3], qf[i >> 2][i & 3], acc[i & 1], 0, 0, 0);
+    float w[4], mx = m;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int kj = k0 + 4 * g + r;
+      const bool sees = ((unsigned)(p - kj) < (unsigned)window || kj < sinksSeen) && (valid[B] >> (4 * g + r) & 1) != 0;
+      w[r] = sees ? (acc[0][r] + acc[1][r]) * a.scaleLog2e : -INFINITY;
+      mx = fmaxf(mx, w[r]);
+    }
+    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    const float ref = mx == -INFINITY ? 0.f : mx, keep = exp2f(m - ref);
+    m = mx, l *= keep;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      w[r] = exp2f(behindRounded(w[r], ref));
+      l += w[r];
+    }
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) o[i][r] *= keep;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int i = 0; i < E; ++i) o[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[B][r][i >> 2][i & 3], w[r], o[i], 0, 0, 0);
+  };
+  using B0 = std::integral_constant<int, 0>;
+  using B1 = std::integral_constant<int, 1>;
+  if (t0 < t1) {
+    const int64_t first = askSlot(t0);
+    int64_t next = askSlot(t0 + 1);
+    fetch(first, B0{});
+    for (int t = t0; t < t1; t += 2) {
+      if (t + 1 < t1) {
+        const int64_t slot = next;
+        next = askSlot(t + 2);
+        fetch(slot, B1{});
+      }
+      tile(t, B0{});
+      if (t + 1 >= t1) break;
+      if (t + 2 < t1) {
+        const int64_t slot = next;
+        next = askSlot(t + 3);
+        fetch(slot, B0{});
+      }
+      tile(t + 1, B1{});
+    }
+  }
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+  if (l != l && m == -INFINITY) m = 0.f;  // scores that are not numbers alone: as a maximum of minus infinity they would be left out
+  if (g == 0) sm[wave][c] = m, sl[wave][c] = l;
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+#pragma unroll
+    for (int i = 0; i < E / 4; ++i)
+      *reinterpret_cast<f32x4*>(so + (wave * 16 + c) * PITCH + (4 * g + r) * E + 4 * i) = f32x4{o[4 * i][r], o[4 * i + 1][r], o[4 * i + 2][r], o[4 * i + 3][r]};
+  __syncthreads();
+  // a column to 16 lanes
+  const int mine = threadIdx.x >> 4, e0 = c * E, oc = c0 + mine, at0 = s.first + min(oc, cols - 1) / group, hc = kvh * group + min(oc, cols - 1) % group;
+  const int64_t row = s.start + at0;
+  float mAll = -INFINITY, sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) mAll = fmaxf(mAll, sm[w][mine]);
+  f32x4 v[E / 4] = {};
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const float weight = sm[w][mine] == -INFINITY ? 0.f : exp2f(sm[w][mine] - mAll);
+    sum += sl[w][mine] * weight;
+#pragma unroll
+    for (int i = 0; i < E / 4; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[i][k] += so[(w * 16 + mine) * PITCH + e0 + 4 * i + k] * weight;
+  }
+  bool odd = !(fabsf(sum) < INFINITY);
+#pragma unroll
+  for (int i = 0; i < E / 4; ++i)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) odd |= !(fabsf(v[i][k]) < INFINITY);
+  // columns whose sums are not finite: by themselves, with the tokens that they see alone
+  const uint64_t bad = __builtin_amdgcn_ballot_w64(odd && oc < cols);
+  const bool again = (bad >> (lane & 48) & 0xffffu) != 0;
+  if (oc < cols && !again) {
+    if (whole) {
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      float* out = reinterpret_cast<float*>(a.out) + row * a.oTok + (int64_t)hc * a.oHead + e0;
+#pragma unroll
+      for (int i = 0; i < E / 4; ++i)
+        if (!PART || e0 + 4 * i < a.d) *reinterpret_cast<f32x4*>(out + 4 * i) = v[i] * inv;
+    } else {
+      float* dst = x.partial + ((row * a.heads + hc) * x.splits + split) * (2 + a.d);
+      if (c == 0) dst[0] = mAll, dst[1] = sum;
+#pragma unroll
+      for (int i = 0; i < E / 4; ++i) {
+        if (PART && e0 + 4 * i >= a.d) continue;
+        *reinterpret_cast<float2*>(dst + 2 + e0 + 4 * i) = float2{v[i][0], v[i][1]};
+        *reinterpret_cast<float2*>(dst + 4 + e0 + 4 * i) = float2{v[i][2], v[i][3]};
+      }
+    }
+  }
+  for (int i = 0; i < 4; ++i)
+    if ((bad >> (16 * i) & 0xffffu) != 0) pagedAgain<float, D>(x, s, kvh, locBase, span, t0, t1, split, whole, c0 + 4 * wave + i);
+}
+
+template <int D, bool PART>
+__global__ __launch_bounds__(256) void pagedFloatKernel(PtArgs x) {
+  pagedPieces<kPtFloatCols>(x, [&](const PaSequence& s, int b, int kvh, int block, const PtSpan& span, int t0, int t1, int split, bool whole) {
+    pagedFloatBlock<D, PART>(x, s, b, kvh, block, span, t0, t1, split, whole);
+  });
+}
+
 // out of the rows whose block was walked in shares: a wave per (row, head). Lane i takes maximum and sum of share i, then every lane its
 // elements of all of them.
-template <typename T>
+template <typename T, int COLS>
 __global__ __launch_bounds__(256) void pagedMergeKernel(PtArgs x) {
   constexpr int kPerLane = 4, kBatch = 8;  // d <= 256; shares whose elements are asked for at once
   const PaArgs& a = x.a;
@@ -439,8 +636,8 @@ __global__ __launch_bounds__(256) void pagedMergeKernel(PtArgs x) {
     if (at.b < 0) return;
     const PaSequence s = paSequence(a, at.b);
     const int h = (int)(pair % a.heads), cols = (s.end - s.first) * group, origin = s.origin + s.first;
-    const int block = (at.at * group + h % group) / kPtCols;
-    const PtSpan span(a, origin + block * kPtCols / group, origin + min(block * kPtCols + kPtCols - 1, cols - 1) / group);
+    const int block = (at.at * group + h % group) / COLS;
+    const PtSpan span(a, origin + block * COLS / group, origin + min(block * COLS + COLS - 1, cols - 1) / group);
     const int shares = (span.tiles + x.tilesPerSplit - 1) / x.tilesPerSplit;
     if (shares > 1) {
       const int64_t row = s.start + s.first + at.at;
@@ -493,12 +690,22 @@ static diopiError_t launchTile(hipStream_t stream, const PtArgs& x, int64_t wgs)
   return diopiSuccess;
 }
 
+template <int D, bool PART>
+static diopiError_t launchFloat(hipStream_t stream, const PtArgs& x, int64_t wgs) {
+  constexpr int lds = 4 * 16 * (D + 4) * (int)sizeof(float);
+  AMD_HIP(allowDynamicLds(reinterpret_cast<const void*>(&pagedFloatKernel<D, PART>), lds));
+  hipLaunchKernelGGL((pagedFloatKernel<D, PART>), dim3((unsigned)wgs), dim3(256), lds, stream, x);
+  AMD_LAUNCH_CHECK();
+  return diopiSuccess;
+}
+
 bool pagedAttentionTiles(const PaArgs& a, diopiDtype_t dtype) {
-  if (dtype == diopi_dtype_float32 || a.d % 8 != 0 || a.d > 256 || a.slots > 0x7fffffff) return false;
+  const int64_t size = dtypeSize(dtype);
+  if (a.d * size % 16 != 0 || a.d > 256 || a.slots > 0x7fffffff) return false;
   const int64_t bits = (int64_t)reinterpret_cast<uintptr_t>(a.k) | (int64_t)reinterpret_cast<uintptr_t>(a.v) | (int64_t)reinterpret_cast<uintptr_t>(a.q) |
                        (int64_t)reinterpret_cast<uintptr_t>(a.out) |
-                       (a.kSlotStride | a.kHeadStride | a.vSlotStride | a.vHeadStride | a.qTok | a.qHead | a.oTok | a.oHead) * 2;
-  if ((bits & 15) != 0 || a.kSlotStride < 0 || a.vSlotStride < 0 || std::max(a.kSlotStride, a.vSlotStride) * 2 > 0xffffffffll) return false;
+                       (a.kSlotStride | a.kHeadStride | a.vSlotStride | a.vHeadStride | a.qTok | a.qHead | a.oTok | a.oHead) * size;
+  if ((bits & 15) != 0 || a.kSlotStride < 0 || a.vSlotStride < 0 || std::max(a.kSlotStride, a.vSlotStride) * size > 0xffffffffll) return false;
   // 32 bits hold the columns of a sequence
   return std::min<int64_t>(a.maxNew, a.rows) * (a.heads / a.kvHeads) < 1 << 30;
 }
@@ -506,12 +713,13 @@ bool pagedAttentionTiles(const PaArgs& a, diopiDtype_t dtype) {
 diopiError_t pagedAttentionMfma(diopiContextHandle_t ctx, hipStream_t stream, const PaArgs& a, diopiDtype_t dtype) {
   PtArgs x{};
   x.a = a;
-  x.kSlotBytes = (unsigned)(a.kSlotStride * 2), x.vSlotBytes = (unsigned)(a.vSlotStride * 2);
+  const bool wide = dtype == diopi_dtype_float32;
+  if (!wide) x.kSlotBytes = (unsigned)(a.kSlotStride * 2), x.vSlotBytes = (unsigned)(a.vSlotStride * 2);
   const int64_t group = a.heads / a.kvHeads, tokens = std::min<int64_t>(a.rows, (int64_t)a.batch * a.maxNew), cus = computeUnits();
   const int64_t tiles = std::max<int64_t>(1, std::min<int64_t>(ceilDiv(a.maxLen, kPtTile), ceilDiv(a.sinks, kPtTile) + ceilDiv((int64_t)a.window + kPtCols, kPtTile)));
   // Blocks of columns: what the rows of q fill, and one partly filled for each sequence at most. Where they leave compute units without
   // work the sequences are walked in shares.
-  const int64_t blocks = ceilDiv(tokens * group, kPtCols), most = blocks + std::min<int64_t>(a.batch, tokens);
+  const int64_t blocks = ceilDiv(tokens * group, wide ? kPtFloatCols : kPtCols), most = blocks + std::min<int64_t>(a.batch, tokens);
   const int64_t perKv = std::max<int64_t>(blocks, std::min<int64_t>(a.batch, tokens));
   int64_t splits = std::max<int64_t>(1, 2 * cus / (perKv * a.kvHeads));
   splits = std::min<int64_t>({splits, kPtMaxSplit, ceilDiv(tiles, 2)});
@@ -524,21 +732,27 @@ diopiError_t pagedAttentionMfma(diopiContextHandle_t ctx, hipStream_t stream, co
   }
   const int64_t wgs = most * x.splits * a.kvHeads;
   AMD_CHECK(wgs < 1 << 24, "paged attention: %ld rows of %d heads exceed the grid limits", (long)a.rows, a.heads);  // (2^32 threads)
-#define TILE_CALL(T, D) AMD_TRY((a.d == D ? launchTile<T, D, false>(stream, x, wgs) : launchTile<T, D, true>(stream, x, wgs)))
-#define TILE_SIZES(T)                  \
-  do {                                 \
-    if (a.d <= 64) TILE_CALL(T, 64);   \
-    else if (a.d <= 128) TILE_CALL(T, 128); \
-    else TILE_CALL(T, 256);            \
+#define SIZE_CALL(CALL)               \
+  do {                                \
+    if (a.d <= 64) CALL(64);          \
+    else if (a.d <= 128) CALL(128);   \
+    else CALL(256);                   \
   } while (0)
-  if (dtype == diopi_dtype_bfloat16) TILE_SIZES(bf16_t);
-  else TILE_SIZES(half_t);
-#undef TILE_SIZES
-#undef TILE_CALL
+#define BF16_CALL(D) AMD_TRY((a.d == D ? launchTile<bf16_t, D, false>(stream, x, wgs) : launchTile<bf16_t, D, true>(stream, x, wgs)))
+#define FP16_CALL(D) AMD_TRY((a.d == D ? launchTile<half_t, D, false>(stream, x, wgs) : launchTile<half_t, D, true>(stream, x, wgs)))
+#define FP32_CALL(D) AMD_TRY((a.d == D ? launchFloat<D, false>(stream, x, wgs) : launchFloat<D, true>(stream, x, wgs)))
+  if (dtype == diopi_dtype_bfloat16) SIZE_CALL(BF16_CALL);
+  else if (dtype == diopi_dtype_float16) SIZE_CALL(FP16_CALL);
+  else SIZE_CALL(FP32_CALL);
+#undef FP32_CALL
+#undef FP16_CALL
+#undef BF16_CALL
+#undef SIZE_CALL
   if (x.splits > 1) {
-    const unsigned merges = (unsigned)std::min<int64_t>(ceilDiv(tokens * a.heads, 4), 1 << 23);
-    if (dtype == diopi_dtype_bfloat16) hipLaunchKernelGGL(pagedMergeKernel<bf16_t>, dim3(merges), dim3(256), 0, stream, x);
-    else hipLaunchKernelGGL(pagedMergeKernel<half_t>, dim3(merges), dim3(256), 0, stream, x);
+    const dim3 grid((unsigned)std::min<int64_t>(ceilDiv(tokens * a.heads, 4), 1 << 23)), block(256);
+    if (dtype == diopi_dtype_bfloat16) hipLaunchKernelGGL((pagedMergeKernel<bf16_t, kPtCols>), grid, block, 0, stream, x);
+    else if (dtype == diopi_dtype_float16) hipLaunchKernelGGL((pagedMergeKernel<half_t, kPtCols>), grid, block, 0, stream, x);
+    else hipLaunchKernelGGL((pagedMergeKernel<float, kPtFloatCols>), grid, block, 0, stream, x);
     AMD_LAUNCH_CHECK();
   }
   return diopiSuccess;
