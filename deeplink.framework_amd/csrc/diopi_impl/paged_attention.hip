@@ -29,11 +29,10 @@ __global__ __launch_bounds__(kPgWaves * 64) void pagedAnyKernel(PaArgs a) {
   for (int64_t u = blockIdx.x / a.heads;; u += gridDim.x / a.heads) {
     const PaPlace at = paFind(a, u, [](const PaSequence& s) { return s.end - s.first; });
     if (at.b < 0) return;
-    const PaSequence s = paSequence(a, at.b);
+    const PaSequence& s = at.s;
     const int t = s.first + at.at, p = s.origin + t;
     const int64_t row = s.start + t;
-    const int len = cutLength(a.bLen, at.b, a.len64, a.maxLen);
-    const int64_t locBase = (int64_t)at.b * a.locRowStride + (a.maxLen - len);
+    const int64_t locBase = (int64_t)at.b * a.locRowStride + (a.maxLen - s.len);
     int head, low;
     paSeen(a, p, &head, &low);
     PaColumn<T, J, UNR> c;

@@ -30,14 +30,14 @@ struct PaArgs {
 // The new tokens of a sequence that have a row in q, [first, end), and the position of token 0.
 struct PaSequence {
   int64_t start;  // row of token 0
-  int first, end, origin;
+  int first, end, origin, len;
 };
 __device__ __forceinline__ PaSequence paSequence(const PaArgs& a, int b) {
   PaSequence s;
   const int len = cutLength(a.bLen, b, a.len64, a.maxLen);
   const int n = a.bNew == nullptr ? 1 : cutLength(a.bNew, b, a.new64, a.maxNew);
   s.start = a.bNew == nullptr ? b : ldIndex(a.bStart, b, a.start64);
-  s.origin = len - n;
+  s.origin = len - n, s.len = len;
   // rows outside q are left out (bounds first: a start may be any number)
   s.first = s.start >= 0 ? 0 : (int)min((int64_t)n, s.start < -(int64_t)n ? (int64_t)n : -s.start);
   s.end = s.start >= a.rows ? s.first : (int)min((int64_t)n, a.rows - max(s.start, -(int64_t)n));
@@ -45,31 +45,39 @@ __device__ __forceinline__ PaSequence paSequence(const PaArgs& a, int b) {
   return s;
 }
 
-// Where in the list of all sequences' pieces, count(sequence) of each, piece `u` lies: its sequence (-1: behind the last) and its number
-// there. total: all of them. Every lane of the wave takes part, and all get the same.
+// Where in the list of all sequences' pieces, count(sequence) of each, piece `u` lies: its sequence (b = -1: behind the last) and its
+// number there. total: all of them. Every lane of the wave takes part, and all get the same.
 struct PaPlace {
   int b, at;
   int64_t total;
+  PaSequence s;
 };
 template <typename F>
 __device__ __forceinline__ PaPlace paFind(const PaArgs& a, int64_t u, F&& count) {
   const int lane = threadIdx.x & 63;
-  PaPlace p{-1, 0, 0};
+  PaPlace p;
+  p.b = -1, p.at = 0, p.total = 0;
   for (int b0 = 0; b0 < a.batch; b0 += 64) {
-    const int mine = b0 + lane < a.batch ? count(paSequence(a, b0 + lane)) : 0;
+    const PaSequence s = paSequence(a, min(b0 + lane, a.batch - 1));
+    const int mine = b0 + lane < a.batch ? count(s) : 0;
     int upTo = mine;
+    if (a.batch > 1) {
 #pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const int below = __shfl_up(upTo, off, 64);
-      if (lane >= off) upTo += below;
+      for (int off = 1; off < 64; off <<= 1) {
+        const int below = __shfl_up(upTo, off, 64);
+        if (lane >= off) upTo += below;
+      }
     }
-    const uint64_t behind = __builtin_amdgcn_ballot_w64(p.total + upTo > u);
+    const uint64_t behind = __builtin_amdgcn_ballot_w64(b0 + lane < a.batch && p.total + upTo > u);
     if (p.b < 0 && behind != 0) {
       const int l = __builtin_ctzll(behind);
+      auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
       p.b = b0 + l;
-      p.at = (int)(u - p.total) - (__builtin_amdgcn_readlane(upTo, l) - __builtin_amdgcn_readlane(mine, l));
+      p.at = (int)(u - p.total) - (of(upTo) - of(mine));
+      p.s.start = (int64_t)((uint64_t)(uint32_t)of((int)(s.start >> 32)) << 32 | (uint32_t)of((int)s.start));
+      p.s.first = of(s.first), p.s.end = of(s.end), p.s.origin = of(s.origin), p.s.len = of(s.len);
     }
-    p.total += __builtin_amdgcn_readlane(upTo, 63);
+    p.total += __builtin_amdgcn_readlane(upTo, min(63, a.batch - 1 - b0));
   }
   return p;
 }

@@ -139,8 +139,7 @@ __device__ __forceinline__ void pagedTileBlock(const PtArgs& x, const PaSequence
   const int64_t row = s.start + token;
   const int pFirst = __builtin_amdgcn_readlane(p, 0), pLast = __builtin_amdgcn_readlane(p, 31);
   const int window = a.window, sinksSeen = max(0, min(a.sinks, p + 1));
-  const int len = cutLength(a.bLen, b, a.len64, a.maxLen);
-  const int64_t locBase = (int64_t)b * a.locRowStride + (a.maxLen - len);
+  const int64_t locBase = (int64_t)b * a.locRowStride + (a.maxLen - s.len);
 
   Frag qf[KS];
   {
@@ -419,7 +418,7 @@ __device__ __forceinline__ void pagedPieces(const PtArgs& x, F&& walk) {
   for (int64_t u = blockIdx.x / a.kvHeads;; u += step) {
     const PaPlace at = paFind(a, u, [&](const PaSequence& s) { return PtPieces<COLS>(x, s).all(); });
     if (at.b < 0) return;
-    const PaSequence s = paSequence(a, at.b);
+    const PaSequence& s = at.s;
     const PtPieces<COLS> pieces(x, s);
     const int split = at.at / pieces.blocks, block = pieces.blocks - 1 - at.at % pieces.blocks;
     const int cols = (s.end - s.first) * group, origin = s.origin + s.first;
@@ -463,8 +462,7 @@ __device__ __forceinline__ void pagedFloatBlock(const PtArgs& x, const PaSequenc
   const int col = min(c0 + c, cols - 1), token = s.first + col / group, h = kvh * group + col % group, p = s.origin + token;
   const int pFirst = __builtin_amdgcn_readlane(p, 0), pLast = __builtin_amdgcn_readlane(p, 15);
   const int window = a.window, sinksSeen = max(0, min(a.sinks, p + 1));
-  const int len = cutLength(a.bLen, b, a.len64, a.maxLen);
-  const int64_t locBase = (int64_t)b * a.locRowStride + (a.maxLen - len);
+  const int64_t locBase = (int64_t)b * a.locRowStride + (a.maxLen - s.len);
   const float* const kHead = reinterpret_cast<const float*>(a.k) + kvh * a.kHeadStride;
   const float* const vHead = reinterpret_cast<const float*>(a.v) + kvh * a.vHeadStride;
   f32x4 qf[S / 4], kf[2][S / 4], vf[2][4][E / 4], o[E];
@@ -634,7 +632,7 @@ __global__ __launch_bounds__(256) void pagedMergeKernel(PtArgs x) {
   for (int64_t pair = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);; pair += step) {
     const PaPlace at = paFind(a, pair / a.heads, [](const PaSequence& s) { return s.end - s.first; });
     if (at.b < 0) return;
-    const PaSequence s = paSequence(a, at.b);
+    const PaSequence& s = at.s;
     const int h = (int)(pair % a.heads), cols = (s.end - s.first) * group, origin = s.origin + s.first;
     const int block = (at.at * group + h % group) / COLS;
     const PtSpan span(a, origin + block * COLS / group, origin + min(block * COLS + COLS - 1, cols - 1) / group);
