@@ -29,6 +29,7 @@ constexpr int kPtCols = 128, kPtTile = 64;
 constexpr float kPtRescaleStep = 8.0f;            // log2 domain
 constexpr float kPtLargeScore = 4194304.f;        // 2^22: a maximum beyond it has no more than two places below one
 constexpr int kPtMaxSplit = 64;                   // pagedMergeKernel has a lane for each
+constexpr int kPtFewCols = 32;                    // 16-bit rows: sequences of up to so many columns take the other form
 
 template <typename T>
 struct PtMfma;
@@ -52,6 +53,9 @@ struct PtArgs {
   float* partial;    // [rows, heads, splits, 2 + d]
   int splits, tilesPerSplit;
   unsigned kSlotBytes, vSlotBytes;
+  float* fewPartial;  // of sequences with few columns: [batch, kv_heads, kPtFewCols, fewSplits, 2 + d]
+  int fewSplits = 0, fewChunk = 1;
+  int64_t tilePieces;  // workgroups for each K/V head that take blocks of columns
 };
 
 // The tiles that the tokens at positions pMin ... pMax see: sinkTiles of the sequence's first tokens, the others from token `low` on, up
@@ -68,6 +72,24 @@ struct PtSpan {
   __device__ __forceinline__ int base(int tile) const { return tile < sinkTiles ? tile * kPtTile : low + (tile - sinkTiles) * kPtTile; }
   __device__ __forceinline__ int limit(int tile) const { return tile < sinkTiles ? sinks : end; }
 };
+
+// The tokens that some of the new ones of a sequence with few columns see, in order: the first `sinks`, then from `low` on to the last new one.
+struct PtList {
+  int sinks, low, n;
+  __device__ __forceinline__ PtList(const PaArgs& a, const PaSequence& s) {
+    low = max(0, s.origin + s.first - a.window + 1);
+    const int end = max(0, s.origin + s.end);
+    sinks = min(min(a.sinks, low), end);
+    n = sinks + max(0, end - low);
+  }
+  __device__ __forceinline__ int token(int i) const { return i < sinks ? i : low + (i - sinks); }
+};
+__device__ __forceinline__ int ptColumns(const PaArgs& a, const PaSequence& s) {  // (cut where 32 bits end: then there are many)
+  return (int)min((int64_t)(s.end - s.first) * (a.heads / a.kvHeads), (int64_t)1 << 30);
+}
+__device__ __forceinline__ int ptFewShares(const PtArgs& x, const PaSequence& s) {
+  return max(1, (PtList(x.a, s).n + x.fewChunk - 1) / x.fewChunk);
+}
 
 // Blocks of columns of a sequence, and the most shares that one of them has.
 template <int COLS>
@@ -128,7 +150,7 @@ __device__ __forceinline__ void pagedTileBlock(const PtArgs& x, const PaSequence
   constexpr int KS = D / 16, DT = D / 32, CPR = D / 8, RPL = 64 / CPR, NLD = kPtTile / RPL / 4, STAGE = kPtTile * D;
   constexpr int ROWB = D * (int)sizeof(T);
   constexpr unsigned kStageBytes = STAGE * sizeof(T);
-  extern __shared__ __attribute__((aligned(16))) char ptSmem[];
+  extern __shared__ __attribute__((aligned(1024))) char ptSmem[];  // (the fragments' addresses are put together by XOR)
   const PaArgs& a = x.a;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l31 = lane & 31, half = lane >> 5;
@@ -409,14 +431,15 @@ __device__ __forceinline__ void pagedTileBlock(const PtArgs& x, const PaSequence
   for (; again != 0; again &= again - 1) pagedAgain<T, D>(x, s, kvh, locBase, span, t0, t1, split, whole, c0 + __builtin_ctz(again));
 }
 
-// A workgroup's pieces of work. grid: K/V heads fastest (the ids go round the XCDs, so a head's pieces stay on one), then the list of
-// pieces: sequence after sequence, shares from the first, blocks from the last, which has the most tiles.
-template <int COLS, typename F>
-__device__ __forceinline__ void pagedPieces(const PtArgs& x, F&& walk) {
+// A workgroup's pieces of work: K/V heads fastest (the ids go round the XCDs, so a head's pieces stay on one), then the list of pieces:
+// sequence after sequence, shares from the first, blocks from the last, which has the most tiles. `step` workgroups for each K/V head, the
+// number of pieces unless sequences share rows of q; sequences of up to FEW columns are not among them.
+template <int COLS, int FEW, typename F>
+__device__ __forceinline__ void pagedPieces(const PtArgs& x, int64_t step, F&& walk) {
   const PaArgs& a = x.a;
-  const int kvh = blockIdx.x % a.kvHeads, step = gridDim.x / a.kvHeads, group = a.heads / a.kvHeads;
+  const int kvh = blockIdx.x % a.kvHeads, group = a.heads / a.kvHeads;
   for (int64_t u = blockIdx.x / a.kvHeads;; u += step) {
-    const PaPlace at = paFind(a, u, [&](const PaSequence& s) { return PtPieces<COLS>(x, s).all(); });
+    const PaPlace at = paFind(a, u, [&](const PaSequence& s) { return ptColumns(a, s) <= FEW ? 0 : PtPieces<COLS>(x, s).all(); });
     if (at.b < 0) return;
     const PaSequence& s = at.s;
     const PtPieces<COLS> pieces(x, s);
@@ -431,9 +454,356 @@ __device__ __forceinline__ void pagedPieces(const PtArgs& x, F&& walk) {
   }
 }
 
+// ---------------------------------------------------------------- few columns --
+// Sequences with up to 32 columns of a K/V head (a token or a few speculated ones): bound by memory. A workgroup takes a share of the
+// tokens and its waves cut that, each with a two-stage LDS ring of its own: no barriers until their states meet. With WIDE a
+// wave takes all tokens of a K/V head and the workgroup four heads, for sequences so short that a wave's share would be nothing.
+//   * S^T = K . Q^T (16x16x32), 16 tokens x 16 columns at a time: a lane holds four tokens' scores of one column, and its probabilities
+//     are as they lie the operand P^T of O^T += V^T . P^T, whose 32 places hold the 16 tokens twice: with the rounded
+//     probability and with what the rounding left, which makes 16 bits of it in bf16 and 22 in fp16 at no cost.
+//   * the tokens that are seen are a list without gaps (PtList); their slots are looked up 128 at a time.
+//   * the running maximum is replaced only when a score exceeds it by more than 2^8.
+constexpr int kPfWaves = 4, kPfTile = 16, kPfBlock = 128, kPfStages = 2;
+template <typename T>
+struct PfMfma;
+template <>
+struct PfMfma<bf16_t> {
+  static __device__ __forceinline__ f32x4 run(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+template <>
+struct PfMfma<half_t> {
+  static __device__ __forceinline__ f32x4 run(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+// XOR on the 16-byte piece index of row r in LDS: 16 rows' pieces of one index (K), the 8 rows x 32 bytes of half a transposing read (V)
+// fall on different banks.
+template <int D>
+__device__ __forceinline__ int pfSwizzleK(int r) { return D >= 128 ? (r & 15) : ((r >> 1) & 7); }
+template <int D>
+__device__ __forceinline__ int pfSwizzleV(int r) { return D >= 128 ? 2 * (r & 7) : 2 * ((r >> 1) & 3); }
+
+template <int N>
+__device__ __forceinline__ void waitLoadsBut() {  // all but the wave's N youngest vector-memory operations are done
+  asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
+}
+
+// CT: tiles of 16 columns, 1 or 2. (As a variant and not a branch around the second one's products: of products that are branched around
+// the compiler, hipcc 7.2, has read the result before it was there.)
+template <typename T, int D, bool WIDE, int CT>
+__device__ __forceinline__ void pagedFewBlock(const PtArgs& x, const PaSequence& s, int b, int kvh, int split) {
+  using Frag = typename PtMfma<T>::Frag;
+  using Half = typename PtMfma<T>::Half;
+  constexpr int ROWB = D * 2, CPR = D / 8, RPL = 64 / CPR, NLD = kPfTile / RPL, KS = D / 32, DT = D / 16;
+  constexpr unsigned kMatBytes = kPfTile * ROWB, kStageBytes = 2 * kMatBytes;
+  constexpr float kRaise = PtMfma<T>::kRaise;
+  extern __shared__ __attribute__((aligned(1024))) char ptSmem[];  // (the fragments' addresses are put together by XOR)
+  __shared__ int slotBuf[kPfWaves][kPfBlock];
+  __shared__ float stateBuf[kPfWaves][2][kPtFewCols];
+  __shared__ int again[kPtFewCols];
+  const PaArgs& a = x.a;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c16 = lane & 15, quad = lane >> 4;
+  const int group = a.heads / a.kvHeads, cols = (s.end - s.first) * group;
+  const PtList list(a, s);
+  const int64_t locBase = (int64_t)b * a.locRowStride + (a.maxLen - s.len);
+  const int chunkBegin = split * x.fewChunk, chunkEnd = min(list.n, chunkBegin + x.fewChunk);
+  const int share = WIDE ? chunkEnd - chunkBegin : ((chunkEnd - chunkBegin + kPfWaves - 1) / kPfWaves + kPfTile - 1) / kPfTile * kPfTile;
+  const int from = WIDE ? chunkBegin : chunkBegin + wave * share, to = min(chunkEnd, from + share);
+
+  Frag qf[CT][KS];
+  int p[CT], sinksSeen[CT];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    const int col = min(ct * 16 + c16, cols - 1), token = s.first + col / group;
+    p[ct] = s.origin + token, sinksSeen[ct] = max(0, min(a.sinks, p[ct] + 1));
+    const T* q = reinterpret_cast<const T*>(a.q) + (s.start + token) * a.qTok + (int64_t)(kvh * group + col % group) * a.qHead;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      const int e = 32 * k + 8 * quad;
+      qf[ct][k] = *reinterpret_cast<const Frag*>(q + (e < a.d ? e : 0));
+      if (e >= a.d) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) qf[ct][k][j] = static_cast<T>(0.f);
+      }
+    }
+  }
+  const int pMin = s.origin + s.first, pMax = s.origin + s.end - 1, window = a.window;
+  f32x4 acc[CT][DT];
+  float m[CT], l[CT];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    m[ct] = -INFINITY, l[ct] = 0.f;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) acc[ct][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  // ring: load i of a matrix fills rows i * RPL ... of its tile, lane (row lane / CPR of those, piece lane % CPR) with the piece that the swizzle
+  // puts there; behind a row's end the first piece again, which meets zeros of q or gives places that are not stored
+  const unsigned ring = (unsigned)(uintptr_t)ptSmem + (unsigned)wave * (kPfStages * kStageBytes);
+  int kOff[NLD], vOff[NLD];
+#pragma unroll
+  for (int i = 0; i < NLD; ++i) {
+    const int row = i * RPL + lane / CPR, piece = lane % CPR, kc = piece ^ pfSwizzleK<D>(row), vc = piece ^ pfSwizzleV<D>(row);
+    kOff[i] = kc * 8 < a.d ? kc * 16 : 0, vOff[i] = vc * 8 < a.d ? vc * 16 : 0;
+  }
+  const char* const kBase = reinterpret_cast<const char*>(reinterpret_cast<const T*>(a.k) + kvh * a.kHeadStride);
+  const char* const vBase = reinterpret_cast<const char*>(reinterpret_cast<const T*>(a.v) + kvh * a.vHeadStride);
+  int* const slots = slotBuf[wave];
+  auto issue = [&](int tile, int stage) {
+    const unsigned at = ring + (unsigned)stage * kStageBytes;
+    unsigned slot[NLD];
+#pragma unroll
+    for (int i = 0; i < NLD; ++i) slot[i] = (unsigned)slots[tile * kPfTile + i * RPL + lane / CPR] & 0x7fffffffu;
+#pragma unroll
+    for (int i = 0; i < NLD; ++i) globalLoadToLds16Stream(kBase + ((uint64_t)slot[i] * x.kSlotBytes + (unsigned)kOff[i]), at + i * 1024u);
+#pragma unroll
+    for (int i = 0; i < NLD; ++i) globalLoadToLds16Stream(vBase + ((uint64_t)slot[i] * x.vSlotBytes + (unsigned)vOff[i]), at + kMatBytes + i * 1024u);
+  };
+
+  for (int b0 = from; b0 < to; b0 += kPfBlock) {
+    const int cnt = min(kPfBlock, to - b0), tiles = (cnt + kPfTile - 1) / kPfTile;
+    // slots of the block; past the last token that again; one outside the pool is skipped, never dereferenced: it is marked by its top bit,
+    // and another of the block stands in (slot 0 where there is none)
+    int64_t raw[kPfBlock / 64];
+    uint64_t in[kPfBlock / 64];
+#pragma unroll
+    for (int i = 0; i < kPfBlock / 64; ++i) raw[i] = ldIndex(a.bLoc, locBase + list.token(b0 + min(i * 64 + lane, cnt - 1)), a.loc64);
+    int instead = 0;
+#pragma unroll
+    for (int i = 0; i < kPfBlock / 64; ++i) {
+      in[i] = __builtin_amdgcn_ballot_w64(raw[i] >= 0 && raw[i] < a.slots);
+      if (in[i] != 0) instead = __builtin_amdgcn_readlane((int)raw[i], __builtin_ctzll(in[i]));
+    }
+#pragma unroll
+    for (int i = 0; i < kPfBlock / 64; ++i) slots[i * 64 + lane] = in[i] >> lane & 1 ? (int)raw[i] : (int)(0x80000000u | (unsigned)instead);
+    const bool skips = (in[0] & in[1]) != ~0ull;
+    static_assert(kPfBlock == 128, "two words of 64 slots");
+    exchangeInWave();
+    // (also the reads of the block before: the ring's loads overwrite what they read)
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" : : : "memory");
+    issue(0, 0);
+    for (int t = 0; t < tiles; ++t) {
+      const int stage = t & 1;
+      if (t + 1 < tiles) {
+        // the tile read last in the other stage has been consumed: its reads are done before the loads that overwrite it go out
+        asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+        issue(t + 1, stage ^ 1);
+        waitLoadsBut<2 * NLD>();
+      } else {
+        waitLoadsBut<0>();
+      }
+      const unsigned at = ring + (unsigned)stage * kStageBytes;
+      typedef __attribute__((address_space(3))) const Frag* LdsFrag;
+      typedef __attribute__((address_space(3))) s16x4* LdsTr;
+      const int v0 = b0 + t * kPfTile, last = v0 + kPfTile - 1;
+      // whether every column sees all of the tile (uniform)
+      const bool all = !skips && last < to && list.token(last) <= pMin && (list.token(v0) > pMax - window || last < list.sinks);
+      f32x4 sc[CT][2];
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) sc[ct][0] = sc[ct][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        const Frag kf = *(LdsFrag)(uintptr_t)(at + (unsigned)(c16 * ROWB + (((4 * k + quad) ^ pfSwizzleK<D>(c16)) << 4)));
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) sc[ct][k & 1] = PfMfma<T>::run(kf, qf[ct][k], sc[ct][k & 1]);
+      }
+      Frag pr[CT];
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        float w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = (sc[ct][0][i] + sc[ct][1][i]) * a.scaleLog2e;
+        if (!all) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int v = v0 + 4 * quad + i, kj = list.token(v);
+            const bool sees = v < to && ((unsigned)(p[ct] - kj) < (unsigned)window || kj < sinksSeen[ct]) && slots[t * kPfTile + 4 * quad + i] >= 0;
+            if (!sees) w[i] = -INFINITY;
+          }
+        }
+        float mt = fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3]));
+        if (__builtin_amdgcn_ballot_w64(mt > m[ct] + kPtRescaleStep || (m[ct] == -INFINITY && mt != -INFINITY)) != 0) {
+          auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mt), __float_as_uint(mt), false, false);
+          mt = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+          sw = __builtin_amdgcn_permlane16_swap(__float_as_uint(mt), __float_as_uint(mt), false, false);
+          mt = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+          if (mt > m[ct]) {
+            const float corr = __builtin_amdgcn_exp2f(m[ct] - mt);  // no maximum yet: 0, and the sums are 0
+            m[ct] = mt, l[ct] *= corr;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) acc[ct][d][i] *= corr;
+          }
+        }
+        const float ref = m[ct] == -INFINITY ? 0.f : m[ct];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float e = __builtin_amdgcn_exp2f(behindRounded(w[i], ref) + kRaise);
+          l[ct] += e;
+          const T hi = static_cast<T>(e);
+          pr[ct][i] = hi, pr[ct][4 + i] = static_cast<T>(e - static_cast<float>(hi));
+        }
+      }
+      const int row = 4 * quad + (c16 >> 2);
+      const unsigned vRow = at + kMatBytes + (unsigned)(row * ROWB + (lane & 1) * 8);
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        const unsigned piece = (unsigned)((2 * d + ((lane & 3) >> 1)) ^ pfSwizzleV<D>(row)) << 4;
+        const u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsTr)(uintptr_t)(vRow + piece)));
+        const Frag vf = __builtin_bit_cast(Frag, u32x4{v[0], v[1], v[0], v[1]});
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) acc[ct][d] = PfMfma<T>::run(vf, pr[ct], acc[ct][d]);
+      }
+    }
+  }
+
+  // ---- the states: every lane group holds its own share of l
+  float lowered = 1.f;  // (what raised probabilities have to be divided by)
+  if (kRaise != 0.f) lowered = 1.f / (1 << (int)kRaise);
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(l[ct]), __float_as_uint(l[ct]), false, false);
+    l[ct] = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
+    sw = __builtin_amdgcn_permlane16_swap(__float_as_uint(l[ct]), __float_as_uint(l[ct]), false, false);
+    l[ct] = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
+    l[ct] *= lowered;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[ct][d][i] *= lowered;
+  }
+  const int shares = ptFewShares(x, s);
+  const bool whole = shares == 1;
+  // where column `col` of this K/V head goes, 4 elements from e on, from sums against the maximum
+  auto store = [&](int col, int e, float mCol, float lCol, f32x4 o) {
+    const int token = s.first + col / group;
+    if (whole) {
+      const float inv = lCol > 0.f ? 1.f / lCol : 0.f;
+      Half r;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r[i] = static_cast<T>(o[i] * inv);
+      *reinterpret_cast<Half*>(reinterpret_cast<T*>(a.out) + (s.start + token) * a.oTok + (int64_t)(kvh * group + col % group) * a.oHead + e) = r;
+    } else {
+      float* dst = x.fewPartial + ((((int64_t)b * a.kvHeads + kvh) * kPtFewCols + col) * x.fewSplits + split) * (2 + a.d);
+      if (e == 0) dst[0] = mCol, dst[1] = lCol;
+      *reinterpret_cast<float2*>(dst + 2 + e) = float2{o[0], o[1]};
+      *reinterpret_cast<float2*>(dst + 4 + e) = float2{o[2], o[3]};
+    }
+  };
+  auto finite = [](float v) { return fabsf(v) < INFINITY; };
+  // a column whose sums are not finite: again by itself, the tokens that it sees alone (one wave)
+  auto walkAgain = [&](int col) {
+    const int token = s.first + col / group, h = kvh * group + col % group;
+    int head, low;
+    paSeen(a, s.origin + token, &head, &low);
+    // of the share's tokens those that it sees
+    const int first0 = min(chunkBegin, list.sinks), first1 = min(head, min(chunkEnd, list.sinks));
+    const int next0 = list.low + max(0, chunkBegin - list.sinks), next1 = list.low + max(0, chunkEnd - list.sinks);
+    const int more1 = list.sinks == 0 ? min(head, next1) : 0;  // (without a list of first tokens apart, some may lie in the other part)
+    PaColumn<T, D / 64, (D > 128 ? 4 : 8)> one;
+    const T* q = reinterpret_cast<const T*>(a.q) + (s.start + token) * a.qTok + (int64_t)h * a.qHead;
+    one.walk(a, q, kvh, locBase, list.sinks == 0 ? next0 : first0, list.sinks == 0 ? more1 : first1, max(next0, low), min(next1, s.origin + token + 1), 0, 64);
+    const float inv = one.l == 0.f ? 0.f : 1.f / one.l;
+    T* out = reinterpret_cast<T*>(a.out) + (s.start + token) * a.oTok + (int64_t)h * a.oHead;
+    float* dst = x.fewPartial + ((((int64_t)b * a.kvHeads + kvh) * kPtFewCols + col) * x.fewSplits + split) * (2 + a.d);
+    if (!whole && lane == 0) dst[0] = one.m, dst[1] = one.l;
+#pragma unroll
+    for (int j = 0; j < D / 64; ++j) {
+      const int e = lane + 64 * j;
+      if (e >= a.d) continue;
+      if (whole) out[e] = static_cast<T>(one.acc[j] * inv);
+      else dst[2 + e] = one.acc[j];
+    }
+  };
+  if (WIDE) {
+    uint32_t bad = 0;
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      bool odd = !finite(l[ct]);
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) odd |= !finite(acc[ct][d][i]);
+      const uint64_t lanes = __builtin_amdgcn_ballot_w64(odd && ct * 16 + c16 < cols);
+      const uint32_t sixteen = (uint32_t)((lanes | lanes >> 16 | lanes >> 32 | lanes >> 48) & 0xffffu);
+      bad |= sixteen << (16 * ct);
+      if (ct * 16 + c16 < cols && (sixteen >> c16 & 1) == 0) {
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+          if (16 * d + 4 * quad < a.d) store(ct * 16 + c16, 16 * d + 4 * quad, m[ct], l[ct], acc[ct][d]);
+      }
+    }
+    for (; bad != 0; bad &= bad - 1) walkAgain(__builtin_ctz(bad));
+    return;
+  }
+  // waves meet in LDS, a tile of 16 columns at a time
+  constexpr int kRedRow = D + 4;
+  float* const red = reinterpret_cast<float*>(ptSmem);  // the ring: every load into it has been waited for
+  if (threadIdx.x < kPtFewCols) again[threadIdx.x] = 0;
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct)
+    if (quad == 0) stateBuf[wave][0][ct * 16 + c16] = m[ct], stateBuf[wave][1][ct * 16 + c16] = l[ct];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    __syncthreads();
+#pragma unroll
+    for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(red + (wave * 16 + c16) * kRedRow + 16 * d + 4 * quad) = acc[ct][d];
+    __syncthreads();
+    const int here = min(16, cols - ct * 16);
+    for (int i = threadIdx.x; i < here * (D / 4); i += kPfWaves * 64) {
+      const int j = i / (D / 4), e = (i % (D / 4)) * 4, col = ct * 16 + j;
+      if (e >= a.d) continue;
+      float mAll = -INFINITY, lAll = 0.f;
+#pragma unroll
+      for (int k = 0; k < kPfWaves; ++k) mAll = fmaxf(mAll, stateBuf[k][0][col]);
+      f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < kPfWaves; ++k) {
+        const float mk = stateBuf[k][0][col], w = mk == -INFINITY ? 0.f : exp2f(mk - mAll);
+        lAll += stateBuf[k][1][col] * w;
+        const f32x4 v = *reinterpret_cast<const f32x4*>(red + (k * 16 + j) * kRedRow + e);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[c] += v[c] * w;
+      }
+      bool odd = !finite(lAll);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) odd |= !finite(o[c]);
+      if (odd) again[col] = 1;
+      else store(col, e, mAll, lAll, o);
+    }
+  }
+  __syncthreads();
+  for (int col = wave; col < cols; col += kPfWaves)
+    if (again[col] != 0) walkAgain(col);
+}
+
+// Piece u of the sequences of few columns: sequence after sequence, shares from the first.
+template <typename T, int D, bool WIDE>
+__device__ __forceinline__ void pagedFewPiece(const PtArgs& x, int64_t u, int kvh) {
+  const PaPlace at = paFind(x.a, u, [&](const PaSequence& s) {
+    const int cols = ptColumns(x.a, s);
+    return cols == 0 || cols > kPtFewCols ? 0 : ptFewShares(x, s);
+  });
+  if (at.b < 0) return;
+  if (ptColumns(x.a, at.s) <= 16) pagedFewBlock<T, D, WIDE, 1>(x, at.s, at.b, kvh, at.at);
+  else pagedFewBlock<T, D, WIDE, 2>(x, at.s, at.b, kvh, at.at);
+}
+
+// Sequences of few columns alone. grid: K/V heads (WIDE: groups of four) fastest.
+template <typename T, int D, bool WIDE>
+__global__ __launch_bounds__(kPfWaves * 64, D > 128 ? 1 : 2) void pagedFewKernel(PtArgs x) {
+  const int groups = WIDE ? x.a.kvHeads / kPfWaves : x.a.kvHeads, g = (int)(blockIdx.x % groups);
+  pagedFewPiece<T, D, WIDE>(x, blockIdx.x / groups, WIDE ? g * kPfWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : g);
+}
+
+// Sequences of any number of columns: the first x.tilePieces workgroups for each K/V head take blocks of many, the others few.
 template <typename T, int D, bool PART>
 __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void pagedTileKernel(PtArgs x) {
-  pagedPieces<kPtCols>(x, [&](const PaSequence& s, int b, int kvh, int block, const PtSpan& span, int t0, int t1, int split, bool whole) {
+  const int64_t u = blockIdx.x / x.a.kvHeads;
+  if (u >= x.tilePieces) {
+    pagedFewPiece<T, D, false>(x, u - x.tilePieces, (int)(blockIdx.x % x.a.kvHeads));
+    return;
+  }
+  pagedPieces<kPtCols, kPtFewCols>(x, x.tilePieces, [&](const PaSequence& s, int b, int kvh, int block, const PtSpan& span, int t0, int t1, int split, bool whole) {
     pagedTileBlock<T, D, PART>(x, s, b, kvh, block, span, t0, t1, split, whole);
   });
 }
@@ -453,7 +823,7 @@ template <int D, bool PART>
 __device__ __forceinline__ void pagedFloatBlock(const PtArgs& x, const PaSequence& s, int b, int kvh, int block, const PtSpan& span, int t0, int t1, int split,
                                                 bool whole) {
   constexpr int S = D / 4, E = D / 16, PITCH = D + 4;
-  extern __shared__ __attribute__((aligned(16))) char ptSmem[];
+  extern __shared__ __attribute__((aligned(1024))) char ptSmem[];  // (the fragments' addresses are put together by XOR)
   float* const so = reinterpret_cast<float*>(ptSmem);  // [4][16][PITCH]
   __shared__ float sm[4][16], sl[4][16];
   const PaArgs& a = x.a;
@@ -616,66 +986,85 @@ __device__ __forceinline__ void pagedFloatBlock(const PtArgs& x, const PaSequenc
 
 template <int D, bool PART>
 __global__ __launch_bounds__(256) void pagedFloatKernel(PtArgs x) {
-  pagedPieces<kPtFloatCols>(x, [&](const PaSequence& s, int b, int kvh, int block, const PtSpan& span, int t0, int t1, int split, bool whole) {
+  pagedPieces<kPtFloatCols, 0>(x, x.tilePieces, [&](const PaSequence& s, int b, int kvh, int block, const PtSpan& span, int t0, int t1, int split, bool whole) {
     pagedFloatBlock<D, PART>(x, s, b, kvh, block, span, t0, t1, split, whole);
   });
 }
 
-// out of the rows whose block was walked in shares: a wave per (row, head). Lane i takes maximum and sum of share i, then every lane its
-// elements of all of them.
-template <typename T, int COLS>
-__global__ __launch_bounds__(256) void pagedMergeKernel(PtArgs x) {
+// One row of out from the partial results of `shares` shares, a wave: lane i takes maximum and sum of share i, then every lane its elements of
+// all of them.
+template <typename T>
+__device__ __forceinline__ void pagedJoin(const PaArgs& a, const float* src, int shares, int64_t row, int h) {
   constexpr int kPerLane = 4, kBatch = 8;  // d <= 256; shares whose elements are asked for at once
+  const int lane = threadIdx.x & 63, mine = min(lane, shares - 1);
+  float m = src[mine * (2 + a.d)], l = src[mine * (2 + a.d) + 1], acc[kPerLane] = {0.f, 0.f, 0.f, 0.f}, v[kBatch][kPerLane];
+  auto ask = [&](int i0) {
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i)
+#pragma unroll
+      for (int k = 0; k < kPerLane; ++k) {
+        const int e = lane + 64 * k;
+        v[i][k] = e < a.d ? src[min(i0 + i, shares - 1) * (2 + a.d) + 2 + e] : 0.f;
+      }
+  };
+  ask(0);
+  if (lane >= shares) m = -INFINITY, l = 0.f;
+  const float most = waveMax(m);
+  float w = m == -INFINITY ? 0.f : exp2f(m - most);
+  if (l != l) w = l;  // (scores that are not numbers alone have no maximum)
+  const uint64_t none = __builtin_amdgcn_ballot_w64(w == 0.f && m == -INFINITY);  // shares without a score
+  const float sum = waveSum(l * w);
+  for (int i0 = 0; i0 < shares; i0 += kBatch) {
+    if (i0 > 0) ask(i0);
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      if (i0 + i >= shares) break;
+      const float wi = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), i0 + i));
+      if (none >> (i0 + i) & 1) continue;
+#pragma unroll
+      for (int k = 0; k < kPerLane; ++k) acc[k] += wi * v[i][k];
+    }
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  T* out = reinterpret_cast<T*>(a.out) + row * a.oTok + h * a.oHead;
+#pragma unroll
+  for (int k = 0; k < kPerLane; ++k) {
+    const int e = lane + 64 * k;
+    if (e < a.d) out[e] = static_cast<T>(acc[k] * inv);
+  }
+}
+
+// The rows whose block was walked in shares: a wave per (row, head).
+template <typename T, int COLS, int FEW>
+__global__ __launch_bounds__(256) void pagedMergeKernel(PtArgs x) {
   const PaArgs& a = x.a;
-  const int lane = threadIdx.x & 63, group = a.heads / a.kvHeads;
+  const int group = a.heads / a.kvHeads;
   const int64_t step = (int64_t)gridDim.x * 4;
   for (int64_t pair = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);; pair += step) {
     const PaPlace at = paFind(a, pair / a.heads, [](const PaSequence& s) { return s.end - s.first; });
     if (at.b < 0) return;
     const PaSequence& s = at.s;
-    const int h = (int)(pair % a.heads), cols = (s.end - s.first) * group, origin = s.origin + s.first;
-    const int block = (at.at * group + h % group) / COLS;
+    const int h = (int)(pair % a.heads), cols = ptColumns(a, s), origin = s.origin + s.first, block = (at.at * group + h % group) / COLS;
     const PtSpan span(a, origin + block * COLS / group, origin + min(block * COLS + COLS - 1, cols - 1) / group);
     const int shares = (span.tiles + x.tilesPerSplit - 1) / x.tilesPerSplit;
-    if (shares > 1) {
-      const int64_t row = s.start + s.first + at.at;
-      const float* src = x.partial + (row * a.heads + h) * x.splits * (2 + a.d);
-      const int mine = min(lane, shares - 1);
-      float m = src[mine * (2 + a.d)], l = src[mine * (2 + a.d) + 1], acc[kPerLane] = {0.f, 0.f, 0.f, 0.f};
-      if (lane >= shares) m = -INFINITY, l = 0.f;
-      const float most = waveMax(m);
-      float w = m == -INFINITY ? 0.f : exp2f(m - most);
-      if (l != l) w = l;  // (scores that are not numbers alone have no maximum)
-      const uint64_t none = __builtin_amdgcn_ballot_w64(w == 0.f && m == -INFINITY);  // shares without a score
-      const float sum = waveSum(l * w);
-      for (int i0 = 0; i0 < shares; i0 += kBatch) {
-        float v[kBatch][kPerLane];
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i)
-#pragma unroll
-          for (int k = 0; k < kPerLane; ++k) {
-            const int e = lane + 64 * k;
-            v[i][k] = e < a.d ? src[min(i0 + i, shares - 1) * (2 + a.d) + 2 + e] : 0.f;
-          }
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-          if (i0 + i >= shares) break;
-          const float wi = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), i0 + i));
-          if (none >> (i0 + i) & 1) continue;
-#pragma unroll
-          for (int k = 0; k < kPerLane; ++k) acc[k] += wi * v[i][k];
-        }
-      }
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      T* out = reinterpret_cast<T*>(a.out) + row * a.oTok + h * a.oHead;
-#pragma unroll
-      for (int k = 0; k < kPerLane; ++k) {
-        const int e = lane + 64 * k;
-        if (e < a.d) out[e] = static_cast<T>(acc[k] * inv);
-      }
-    }
+    const int64_t row = s.start + s.first + at.at;
+    if (shares > 1 && cols > FEW) pagedJoin<T>(a, x.partial + (row * a.heads + h) * x.splits * (2 + a.d), shares, row, h);
     if (pair + step >= at.total * a.heads) return;
   }
+}
+
+// The columns of sequences with few of them, `most` for each K/V head: a wave per column.
+template <typename T>
+__global__ __launch_bounds__(256) void pagedFewMergeKernel(PtArgs x, int most) {
+  const PaArgs& a = x.a;
+  const int group = a.heads / a.kvHeads;
+  const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), pair = i / most;
+  const int col = (int)(i % most), kvh = (int)(pair % a.kvHeads);
+  if (pair >= (int64_t)a.batch * a.kvHeads) return;
+  const PaSequence s = paSequence(a, (int)(pair / a.kvHeads));
+  const int cols = ptColumns(a, s), shares = ptFewShares(x, s);
+  if (col >= cols || cols > kPtFewCols || shares == 1) return;
+  pagedJoin<T>(a, x.fewPartial + (pair * kPtFewCols + col) * x.fewSplits * (2 + a.d), shares, s.start + s.first + col / group, kvh * group + col % group);
 }
 
 template <typename T, int D, bool PART>
@@ -684,6 +1073,21 @@ static diopiError_t launchTile(hipStream_t stream, const PtArgs& x, int64_t wgs)
   static_assert(lds >= 4 * 32 * (D + 8) * sizeof(T), "the output has to fit in the stages");
   AMD_HIP(allowDynamicLds(reinterpret_cast<const void*>(&pagedTileKernel<T, D, PART>), (int)lds));
   hipLaunchKernelGGL((pagedTileKernel<T, D, PART>), dim3((unsigned)wgs), dim3(256), lds, stream, x);
+  AMD_LAUNCH_CHECK();
+  return diopiSuccess;
+}
+
+template <typename T, int D>
+static diopiError_t launchFew(hipStream_t stream, const PtArgs& x, int64_t pieces, bool wide) {
+  constexpr int lds = kPfWaves * kPfStages * 2 * kPfTile * D * 2;
+  static_assert(lds >= kPfWaves * 16 * (D + 4) * (int)sizeof(float) && lds <= 4 * kPtTile * D * 2, "the states have to fit in the ring, and the ring in the tiles");
+  if (wide) {
+    AMD_HIP(allowDynamicLds(reinterpret_cast<const void*>(&pagedFewKernel<T, D, true>), lds));
+    hipLaunchKernelGGL((pagedFewKernel<T, D, true>), dim3((unsigned)(pieces * x.a.kvHeads / kPfWaves)), dim3(kPfWaves * 64), lds, stream, x);
+  } else {
+    AMD_HIP(allowDynamicLds(reinterpret_cast<const void*>(&pagedFewKernel<T, D, false>), lds));
+    hipLaunchKernelGGL((pagedFewKernel<T, D, false>), dim3((unsigned)(pieces * x.a.kvHeads)), dim3(kPfWaves * 64), lds, stream, x);
+  }
   AMD_LAUNCH_CHECK();
   return diopiSuccess;
 }
@@ -715,29 +1119,54 @@ diopiError_t pagedAttentionMfma(diopiContextHandle_t ctx, hipStream_t stream, co
   if (!wide) x.kSlotBytes = (unsigned)(a.kSlotStride * 2), x.vSlotBytes = (unsigned)(a.vSlotStride * 2);
   const int64_t group = a.heads / a.kvHeads, tokens = std::min<int64_t>(a.rows, (int64_t)a.batch * a.maxNew), cus = computeUnits();
   const int64_t tiles = std::max<int64_t>(1, std::min<int64_t>(ceilDiv(a.maxLen, kPtTile), ceilDiv(a.sinks, kPtTile) + ceilDiv((int64_t)a.window + kPtCols, kPtTile)));
-  // Blocks of columns: what the rows of q fill, and one partly filled for each sequence at most. Where they leave compute units without
-  // work the sequences are walked in shares.
-  const int64_t blocks = ceilDiv(tokens * group, wide ? kPtFloatCols : kPtCols), most = blocks + std::min<int64_t>(a.batch, tokens);
-  const int64_t perKv = std::max<int64_t>(blocks, std::min<int64_t>(a.batch, tokens));
-  int64_t splits = std::max<int64_t>(1, 2 * cus / (perKv * a.kvHeads));
-  splits = std::min<int64_t>({splits, kPtMaxSplit, ceilDiv(tiles, 2)});
-  x.tilesPerSplit = (int)ceilDiv(tiles, splits);
-  x.splits = (int)ceilDiv(tiles, x.tilesPerSplit);
-  if (x.splits > 1) {
-    void* ws = nullptr;
-    AMD_TRY(requireWorkspace(ctx, a.rows * a.heads * x.splits * (2 + a.d) * (int64_t)sizeof(float), &ws));
-    x.partial = static_cast<float*>(ws);
+  const int64_t limit = 1 << 24;  // workgroups: 2^32 threads
+  const bool onlyFew = !wide && std::min<int64_t>(a.maxNew, a.rows) * group <= kPtFewCols;
+  // Sequences of few columns, 16-bit rows: shares of at least 128 tokens, so many that two workgroups are there for each compute unit.
+  bool wideHeads = false;
+  const int64_t sequences = std::min<int64_t>(a.batch, tokens);
+  if (!wide) {
+    const int64_t seen = std::max<int64_t>(1, std::min<int64_t>(a.maxLen, (int64_t)a.sinks + a.window + kPtFewCols));
+    const int64_t want = std::max<int64_t>(1, 2 * cus / (sequences * a.kvHeads));
+    int64_t chunk = std::max<int64_t>({128, ceilDiv(ceilDiv(seen, want), 64) * 64, ceilDiv(ceilDiv(seen, kPtMaxSplit), 64) * 64});
+    if (seen <= 256) chunk = seen;
+    wideHeads = onlyFew && a.kvHeads % kPfWaves == 0 && seen <= 128;
+    x.fewChunk = (int)chunk, x.fewSplits = (int)ceilDiv(seen, chunk);
+    if (x.fewSplits > 1) {
+      void* ws = nullptr;
+      AMD_TRY(requireWorkspace(ctx, (int64_t)a.batch * a.kvHeads * kPtFewCols * x.fewSplits * (2 + a.d) * (int64_t)sizeof(float), &ws));
+      x.fewPartial = static_cast<float*>(ws);
+    }
   }
-  const int64_t wgs = most * x.splits * a.kvHeads;
-  AMD_CHECK(wgs < 1 << 24, "paged attention: %ld rows of %d heads exceed the grid limits", (long)a.rows, a.heads);  // (2^32 threads)
+  // The others: blocks of columns, what the rows of q fill, and one partly filled for each sequence at most. Where they leave compute units
+  // without work the sequences are walked in shares.
+  const int64_t columns = tokens * group, blockCols = wide ? kPtFloatCols : kPtCols;
+  const int64_t blocks = ceilDiv(columns, blockCols), partly = wide ? sequences : std::min(sequences, columns / (kPtFewCols + 1));
+  x.tilesPerSplit = (int)tiles, x.splits = 1;
+  if (!onlyFew) {
+    const int64_t perKv = std::max<int64_t>(blocks, sequences);
+    int64_t splits = std::max<int64_t>(1, 2 * cus / (perKv * a.kvHeads));
+    splits = std::min<int64_t>({splits, kPtMaxSplit, ceilDiv(tiles, 2)});
+    x.tilesPerSplit = (int)ceilDiv(tiles, splits);
+    x.splits = (int)ceilDiv(tiles, x.tilesPerSplit);
+    if (x.splits > 1) {
+      void* ws = nullptr;
+      AMD_TRY(requireWorkspace(ctx, a.rows * a.heads * x.splits * (2 + a.d) * (int64_t)sizeof(float), &ws));
+      x.partial = static_cast<float*>(ws);
+    }
+  }
+  const int64_t fewPieces = wide ? 0 : (int64_t)a.batch * x.fewSplits;
+  x.tilePieces = onlyFew ? 0 : (blocks + partly) * x.splits;
+  const int64_t wgs = (x.tilePieces + fewPieces) * a.kvHeads;
+  AMD_CHECK(wgs < limit, "paged attention: %ld rows of %d heads exceed the grid limits", (long)a.rows, a.heads);
 #define SIZE_CALL(CALL)               \
   do {                                \
     if (a.d <= 64) CALL(64);          \
     else if (a.d <= 128) CALL(128);   \
     else CALL(256);                   \
   } while (0)
-#define BF16_CALL(D) AMD_TRY((a.d == D ? launchTile<bf16_t, D, false>(stream, x, wgs) : launchTile<bf16_t, D, true>(stream, x, wgs)))
-#define FP16_CALL(D) AMD_TRY((a.d == D ? launchTile<half_t, D, false>(stream, x, wgs) : launchTile<half_t, D, true>(stream, x, wgs)))
+#define HALF_CALL(T, D) AMD_TRY((onlyFew ? launchFew<T, D>(stream, x, fewPieces, wideHeads) : a.d == D ? launchTile<T, D, false>(stream, x, wgs) : launchTile<T, D, true>(stream, x, wgs)))
+#define BF16_CALL(D) HALF_CALL(bf16_t, D)
+#define FP16_CALL(D) HALF_CALL(half_t, D)
 #define FP32_CALL(D) AMD_TRY((a.d == D ? launchFloat<D, false>(stream, x, wgs) : launchFloat<D, true>(stream, x, wgs)))
   if (dtype == diopi_dtype_bfloat16) SIZE_CALL(BF16_CALL);
   else if (dtype == diopi_dtype_float16) SIZE_CALL(FP16_CALL);
@@ -745,12 +1174,21 @@ diopiError_t pagedAttentionMfma(diopiContextHandle_t ctx, hipStream_t stream, co
 #undef FP32_CALL
 #undef FP16_CALL
 #undef BF16_CALL
+#undef HALF_CALL
 #undef SIZE_CALL
+  if (x.fewSplits > 1) {
+    const int mostCols = (int)std::min<int64_t>(kPtFewCols, std::min<int64_t>(a.maxNew, a.rows) * group);
+    const int64_t merges = ceilDiv((int64_t)a.batch * a.kvHeads * mostCols, 4);
+    AMD_CHECK(merges < limit, "paged attention: %d sequences of %d heads exceed the grid limits", a.batch, a.heads);
+    if (dtype == diopi_dtype_bfloat16) hipLaunchKernelGGL(pagedFewMergeKernel<bf16_t>, dim3((unsigned)merges), dim3(256), 0, stream, x, mostCols);
+    else hipLaunchKernelGGL(pagedFewMergeKernel<half_t>, dim3((unsigned)merges), dim3(256), 0, stream, x, mostCols);
+    AMD_LAUNCH_CHECK();
+  }
   if (x.splits > 1) {
     const dim3 grid((unsigned)std::min<int64_t>(ceilDiv(tokens * a.heads, 4), 1 << 23)), block(256);
-    if (dtype == diopi_dtype_bfloat16) hipLaunchKernelGGL((pagedMergeKernel<bf16_t, kPtCols>), grid, block, 0, stream, x);
-    else if (dtype == diopi_dtype_float16) hipLaunchKernelGGL((pagedMergeKernel<half_t, kPtCols>), grid, block, 0, stream, x);
-    else hipLaunchKernelGGL((pagedMergeKernel<float, kPtFloatCols>), grid, block, 0, stream, x);
+    if (dtype == diopi_dtype_bfloat16) hipLaunchKernelGGL((pagedMergeKernel<bf16_t, kPtCols, kPtFewCols>), grid, block, 0, stream, x);
+    else if (dtype == diopi_dtype_float16) hipLaunchKernelGGL((pagedMergeKernel<half_t, kPtCols, kPtFewCols>), grid, block, 0, stream, x);
+    else hipLaunchKernelGGL((pagedMergeKernel<float, kPtFloatCols, 0>), grid, block, 0, stream, x);
     AMD_LAUNCH_CHECK();
   }
   return diopiSuccess;
