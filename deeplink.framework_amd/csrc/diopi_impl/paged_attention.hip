@@ -155,6 +155,7 @@ extern "C" __attribute__((visibility("default"))) diopiError_t diopiPagedContext
   a.heads = (int)q.shape[1], a.kvHeads = (int)k.shape[1], a.d = (int)q.shape[2], a.batch = (int)batch;
   a.maxNew = maxNewLen, a.maxLen = maxInputLen;
   a.scaleLog2e = kLog2eTA / sqrtf((float)a.d);
+  a.group = a.heads / a.kvHeads, a.perGroup = (uint32_t)((((uint64_t)1 << 32) + a.group - 1) / a.group);
   if (pagedAttentionTiles(a, q.dtype)) return pagedAttentionMfma(ctx, stream, a, q.dtype);
   return pagedAttentionAny(stream, a, q.dtype);
 }

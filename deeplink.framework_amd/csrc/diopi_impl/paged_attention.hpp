@@ -23,6 +23,8 @@ struct PaArgs {
   int heads, kvHeads, d, batch, maxNew, maxLen;
   int window, sinks;  // a token at position p sees j <= p with j > p - window or j < sinks (window: maxLen or more where there is none)
   float scaleLog2e;   // log2(e) / sqrt(d)
+  int group;          // query heads to a K/V head
+  uint32_t perGroup;  // ceil(2^32 / group): see paOfGroup
 };
 
 #if defined(__HIPCC__)
@@ -81,6 +83,9 @@ __device__ __forceinline__ PaPlace paFind(const PaArgs& a, int64_t u, F&& count)
   }
   return p;
 }
+
+// n / group, for n * group below 2^32: the product with the rounded-up reciprocal is too large by less than n / 2^32, which is below 1 / group.
+__device__ __forceinline__ int paOfGroup(const PaArgs& a, int n) { return a.group == 1 ? n : (int)__umulhi((uint32_t)n, a.perGroup); }
 
 // The tokens that one at position p sees: [0, head) and [low, p].
 __device__ __forceinline__ void paSeen(const PaArgs& a, int p, int* head, int* low) {

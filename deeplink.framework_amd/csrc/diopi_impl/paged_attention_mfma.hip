@@ -50,7 +50,9 @@ struct PtMfma<half_t> {
 
 struct PtArgs {
   PaArgs a;
-  float* partial;    // [rows, heads, splits, 2 + d]
+  // partial results of blocks of columns: weighted sums of V [rows, heads, splits, d]; maximum and sum [rows, heads, splits]
+  float* partial;
+  float2* partialState;
   int splits, tilesPerSplit;
   unsigned kSlotBytes, vSlotBytes;
   float* fewPartial;  // of sequences with few columns: [batch, kv_heads, kPtFewCols, fewSplits, 2 + d]
@@ -85,7 +87,7 @@ struct PtList {
   __device__ __forceinline__ int token(int i) const { return i < sinks ? i : low + (i - sinks); }
 };
 __device__ __forceinline__ int ptColumns(const PaArgs& a, const PaSequence& s) {  // (cut where 32 bits end: then there are many)
-  return (int)min((int64_t)(s.end - s.first) * (a.heads / a.kvHeads), (int64_t)1 << 30);
+  return (int)min((int64_t)(s.end - s.first) * a.group, (int64_t)1 << 30);
 }
 __device__ __forceinline__ int ptFewShares(const PtArgs& x, const PaSequence& s) {
   return max(1, (PtList(x.a, s).n + x.fewChunk - 1) / x.fewChunk);
@@ -96,7 +98,7 @@ template <int COLS>
 struct PtPieces {
   int blocks, splits;
   __device__ __forceinline__ PtPieces(const PtArgs& x, const PaSequence& s) {
-    const int group = x.a.heads / x.a.kvHeads, tokens = s.end - s.first;
+    const int group = x.a.group, tokens = s.end - s.first;
     blocks = (int)(((int64_t)tokens * group + COLS - 1) / COLS);
     const int upTo = (s.origin + s.end + kPtTile - 1) / kPtTile;
     const int64_t windowed = (x.a.sinks + kPtTile - 1) / kPtTile + ((int64_t)x.a.window + kPtCols + kPtTile - 1) / kPtTile;
@@ -117,7 +119,7 @@ template <typename T, int D>
 __device__ __forceinline__ void pagedAgain(const PtArgs& x, const PaSequence& s, int kvh, int64_t locBase, const PtSpan& span, int t0, int t1, int split, bool whole,
                                            int col) {
   const PaArgs& a = x.a;
-  const int lane = threadIdx.x & 63, group = a.heads / a.kvHeads, token = s.first + col / group, h = kvh * group + col % group, p = s.origin + token;
+  const int lane = threadIdx.x & 63, group = a.group, at = paOfGroup(a, col), token = s.first + at, h = kvh * group + (col - at * group), p = s.origin + token;
   const int64_t row = s.start + token;
   int head, low;
   paSeen(a, p, &head, &low);
@@ -126,16 +128,17 @@ __device__ __forceinline__ void pagedAgain(const PtArgs& x, const PaSequence& s,
   const int first0 = span.sinkTiles > 0 ? min(t0, span.sinkTiles) * kPtTile : from, first1 = span.sinkTiles > 0 ? min(head, min(t1, span.sinkTiles) * kPtTile) : min(head, to);
   PaColumn<T, D / 64, (D > 128 ? 4 : 8)> one;
   one.walk(a, reinterpret_cast<const T*>(a.q) + row * a.qTok + (int64_t)h * a.qHead, kvh, locBase, first0, first1, max(from, low), to, 0, 64);
-  float* dst = x.partial + ((row * a.heads + h) * x.splits + split) * (2 + a.d);
+  const int64_t slice = (row * a.heads + h) * x.splits + split;
+  float* dst = x.partial + slice * a.d;
   T* out = reinterpret_cast<T*>(a.out) + row * a.oTok + (int64_t)h * a.oHead;
   const float inv = one.l == 0.f ? 0.f : 1.f / one.l;
-  if (!whole && lane == 0) dst[0] = one.m, dst[1] = one.l;
+  if (!whole && lane == 0) x.partialState[slice] = float2{one.m, one.l};
 #pragma unroll
   for (int j = 0; j < D / 64; ++j) {
     const int e = lane + 64 * j;
     if (e >= a.d) continue;
     if (whole) out[e] = static_cast<T>(one.acc[j] * inv);
-    else dst[2 + e] = one.acc[j];
+    else dst[e] = one.acc[j];
   }
 }
 
@@ -154,9 +157,9 @@ __device__ __forceinline__ void pagedTileBlock(const PtArgs& x, const PaSequence
   const PaArgs& a = x.a;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l31 = lane & 31, half = lane >> 5;
-  const int group = a.heads / a.kvHeads, cols = (s.end - s.first) * group, c0 = block * kPtCols + wave * 32;
+  const int group = a.group, cols = (s.end - s.first) * group, c0 = block * kPtCols + wave * 32;
   const bool waveLives = c0 < cols;
-  const int col = min(c0 + l31, cols - 1), token = s.first + col / group, h = kvh * group + col % group;
+  const int col = min(c0 + l31, cols - 1), mine = paOfGroup(a, col), token = s.first + mine, h = kvh * group + (col - mine * group);
   const int p = s.origin + token;
   const int64_t row = s.start + token;
   const int pFirst = __builtin_amdgcn_readlane(p, 0), pLast = __builtin_amdgcn_readlane(p, 31);
@@ -391,18 +394,29 @@ __device__ __forceinline__ void pagedTileBlock(const PtArgs& x, const PaSequence
   }
   __syncthreads();  // (the output takes the place of the stages)
   if (!whole) {
-    if (c0 + l31 < cols && (again >> l31 & 1) == 0) {
-      float* dst = x.partial + ((row * a.heads + h) * x.splits + split) * (2 + a.d);
-      if (half == 0) dst[0] = m - M::kRaise, dst[1] = l;
+    if (half == 0 && c0 + l31 < cols && (again >> l31 & 1) == 0) x.partialState[(row * a.heads + h) * x.splits + split] = float2{m - M::kRaise, l};
+    // half of a column's elements at a time through LDS, so that a row of workspace is written in whole pieces
+    constexpr int kHalf = D / 2, OF = kHalf + 4, PER = kHalf / 4;  // floats of a padded row; pieces of 16 bytes
+    float* sO = reinterpret_cast<float*>(ptSmem) + wave * 32 * OF;
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
+    for (int pass = 0; pass < 2; ++pass) {
+      exchangeInWave();
+#pragma unroll
+      for (int dt = 0; dt < DT / 2; ++dt)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          const int e = dt * 32 + g * 8 + half * 4;
-          if (PART && e >= a.d) continue;
-          *reinterpret_cast<float2*>(dst + 2 + e) = float2{o[dt][g * 4], o[dt][g * 4 + 1]};
-          *reinterpret_cast<float2*>(dst + 4 + e) = float2{o[dt][g * 4 + 2], o[dt][g * 4 + 3]};
+          const f32x16& part = o[pass * (DT / 2) + dt];
+          *reinterpret_cast<f32x4*>(sO + l31 * OF + dt * 32 + g * 8 + half * 4) = f32x4{part[g * 4], part[g * 4 + 1], part[g * 4 + 2], part[g * 4 + 3]};
         }
+      exchangeInWave();
+#pragma unroll
+      for (int i = 0; i < 32 * PER / 64; ++i) {
+        const int piece = lane + 64 * i, r = piece / PER, e = (piece % PER) * 4, oc = c0 + r;
+        if (oc >= cols || (again >> r & 1) != 0 || (PART && pass * kHalf + e >= a.d)) continue;
+        const int at = paOfGroup(a, oc);
+        const int64_t to = (s.start + s.first + at) * a.heads + kvh * group + (oc - at * group);
+        *reinterpret_cast<f32x4*>(x.partial + (to * x.splits + split) * a.d + pass * kHalf + e) = *reinterpret_cast<const f32x4*>(sO + r * OF + e);
+      }
     }
   } else {
     // O^T (lane = column) -> LDS [column][d] -> 16-byte stores
@@ -422,9 +436,9 @@ __device__ __forceinline__ void pagedTileBlock(const PtArgs& x, const PaSequence
 #pragma unroll
     for (int i = 0; i < 32 * CPR / 64; ++i) {
       const int chunk = lane + 64 * i, r = chunk / CPR, c = chunk % CPR;
-      const int oc = c0 + r, tok = s.first + oc / group;
+      const int oc = c0 + r, at = paOfGroup(a, oc), tok = s.first + at;
       if (oc < cols && (again >> r & 1) == 0 && (!PART || c * 8 < a.d))
-        *reinterpret_cast<Frag*>(reinterpret_cast<T*>(a.out) + (s.start + tok) * a.oTok + (int64_t)(kvh * group + oc % group) * a.oHead + c * 8) =
+        *reinterpret_cast<Frag*>(reinterpret_cast<T*>(a.out) + (s.start + tok) * a.oTok + (int64_t)(kvh * group + (oc - at * group)) * a.oHead + c * 8) =
             *reinterpret_cast<const Frag*>(sO + r * OS + c * 8);
   }
   }
@@ -437,7 +451,7 @@ __device__ __forceinline__ void pagedTileBlock(const PtArgs& x, const PaSequence
 template <int COLS, int FEW, typename F>
 __device__ __forceinline__ void pagedPieces(const PtArgs& x, int64_t step, F&& walk) {
   const PaArgs& a = x.a;
-  const int kvh = blockIdx.x % a.kvHeads, group = a.heads / a.kvHeads;
+  const int kvh = blockIdx.x % a.kvHeads, group = a.group;
   for (int64_t u = blockIdx.x / a.kvHeads;; u += step) {
     const PaPlace at = paFind(a, u, [&](const PaSequence& s) { return ptColumns(a, s) <= FEW ? 0 : PtPieces<COLS>(x, s).all(); });
     if (at.b < 0) return;
@@ -445,7 +459,7 @@ __device__ __forceinline__ void pagedPieces(const PtArgs& x, int64_t step, F&& w
     const PtPieces<COLS> pieces(x, s);
     const int split = at.at / pieces.blocks, block = pieces.blocks - 1 - at.at % pieces.blocks;
     const int cols = (s.end - s.first) * group, origin = s.origin + s.first;
-    const PtSpan span(a, origin + block * COLS / group, origin + min(block * COLS + COLS - 1, cols - 1) / group);
+    const PtSpan span(a, origin + paOfGroup(a, block * COLS), origin + paOfGroup(a, min(block * COLS + COLS - 1, cols - 1)));
     const bool whole = span.tiles <= x.tilesPerSplit;
     const int t0 = split * x.tilesPerSplit, t1 = min(span.tiles, t0 + x.tilesPerSplit);
     if (split == 0 || t0 < span.tiles) walk(s, at.b, kvh, block, span, t0, t1, split, whole);
@@ -501,7 +515,7 @@ __device__ __forceinline__ void pagedFewBlock(const PtArgs& x, const PaSequence&
   __shared__ int again[kPtFewCols];
   const PaArgs& a = x.a;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c16 = lane & 15, quad = lane >> 4;
-  const int group = a.heads / a.kvHeads, cols = (s.end - s.first) * group;
+  const int group = a.group, cols = (s.end - s.first) * group;
   const PtList list(a, s);
   const int64_t locBase = (int64_t)b * a.locRowStride + (a.maxLen - s.len);
   const int chunkBegin = split * x.fewChunk, chunkEnd = min(list.n, chunkBegin + x.fewChunk);
@@ -512,9 +526,9 @@ __device__ __forceinline__ void pagedFewBlock(const PtArgs& x, const PaSequence&
   int p[CT], sinksSeen[CT];
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
-    const int col = min(ct * 16 + c16, cols - 1), token = s.first + col / group;
+    const int col = min(ct * 16 + c16, cols - 1), at = paOfGroup(a, col), token = s.first + at;
     p[ct] = s.origin + token, sinksSeen[ct] = max(0, min(a.sinks, p[ct] + 1));
-    const T* q = reinterpret_cast<const T*>(a.q) + (s.start + token) * a.qTok + (int64_t)(kvh * group + col % group) * a.qHead;
+    const T* q = reinterpret_cast<const T*>(a.q) + (s.start + token) * a.qTok + (int64_t)(kvh * group + (col - at * group)) * a.qHead;
 #pragma unroll
     for (int k = 0; k < KS; ++k) {
       const int e = 32 * k + 8 * quad;
@@ -675,13 +689,13 @@ __device__ __forceinline__ void pagedFewBlock(const PtArgs& x, const PaSequence&
   const bool whole = shares == 1;
   // where column `col` of this K/V head goes, 4 elements from e on, from sums against the maximum
   auto store = [&](int col, int e, float mCol, float lCol, f32x4 o) {
-    const int token = s.first + col / group;
+    const int at = paOfGroup(a, col), token = s.first + at;
     if (whole) {
       const float inv = lCol > 0.f ? 1.f / lCol : 0.f;
       Half r;
 #pragma unroll
       for (int i = 0; i < 4; ++i) r[i] = static_cast<T>(o[i] * inv);
-      *reinterpret_cast<Half*>(reinterpret_cast<T*>(a.out) + (s.start + token) * a.oTok + (int64_t)(kvh * group + col % group) * a.oHead + e) = r;
+      *reinterpret_cast<Half*>(reinterpret_cast<T*>(a.out) + (s.start + token) * a.oTok + (int64_t)(kvh * group + (col - at * group)) * a.oHead + e) = r;
     } else {
       float* dst = x.fewPartial + ((((int64_t)b * a.kvHeads + kvh) * kPtFewCols + col) * x.fewSplits + split) * (2 + a.d);
       if (e == 0) dst[0] = mCol, dst[1] = lCol;
@@ -692,7 +706,7 @@ __device__ __forceinline__ void pagedFewBlock(const PtArgs& x, const PaSequence&
   auto finite = [](float v) { return fabsf(v) < INFINITY; };
   // a column whose sums are not finite: again by itself, the tokens that it sees alone (one wave)
   auto walkAgain = [&](int col) {
-    const int token = s.first + col / group, h = kvh * group + col % group;
+    const int at = paOfGroup(a, col), token = s.first + at, h = kvh * group + (col - at * group);
     int head, low;
     paSeen(a, s.origin + token, &head, &low);
     // of the share's tokens those that it sees
@@ -818,34 +832,37 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void pagedTileKernel(PtArgs x
 //   O^T = V^T P^T: row i of output tile t stands for element i (D / 16) + t, so a lane's D / 16 operands of a token are consecutive in memory,
 //   and its results are D / 4 consecutive elements of column c.
 // Rows go from the pool into registers a tile ahead, slots another one.
+// NC tiles of 16 columns share the rows in registers.
 constexpr int kPtFloatCols = 16;
-template <int D, bool PART>
+template <int D, bool PART, int NC>
 __device__ __forceinline__ void pagedFloatBlock(const PtArgs& x, const PaSequence& s, int b, int kvh, int block, const PtSpan& span, int t0, int t1, int split,
                                                 bool whole) {
-  constexpr int S = D / 4, E = D / 16, PITCH = D + 4;
-  extern __shared__ __attribute__((aligned(1024))) char ptSmem[];  // (the fragments' addresses are put together by XOR)
-  float* const so = reinterpret_cast<float*>(ptSmem);  // [4][16][PITCH]
-  __shared__ float sm[4][16], sl[4][16];
+  constexpr int S = D / 4, E = D / 16, PITCH = D + 4, COLS = kPtFloatCols * NC;
+  extern __shared__ __attribute__((aligned(1024))) char ptSmem[];
+  float* const so = reinterpret_cast<float*>(ptSmem);  // [4][COLS][PITCH]
+  __shared__ float sm[4][COLS], sl[4][COLS];
   const PaArgs& a = x.a;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
-  const int group = a.heads / a.kvHeads, cols = (s.end - s.first) * group, c0 = block * kPtFloatCols;
-  const int col = min(c0 + c, cols - 1), token = s.first + col / group, h = kvh * group + col % group, p = s.origin + token;
-  const int pFirst = __builtin_amdgcn_readlane(p, 0), pLast = __builtin_amdgcn_readlane(p, 15);
-  const int window = a.window, sinksSeen = max(0, min(a.sinks, p + 1));
+  const int group = a.group, cols = (s.end - s.first) * group, c0 = block * COLS;
   const int64_t locBase = (int64_t)b * a.locRowStride + (a.maxLen - s.len);
   const float* const kHead = reinterpret_cast<const float*>(a.k) + kvh * a.kHeadStride;
   const float* const vHead = reinterpret_cast<const float*>(a.v) + kvh * a.vHeadStride;
-  f32x4 qf[S / 4], kf[2][S / 4], vf[2][4][E / 4], o[E];
+  f32x4 qf[NC][S / 4], kf[2][S / 4], vf[2][4][E / 4], o[NC][E];
+  int p[NC], sinksSeen[NC];
   // (PART: places past the row's end read its first piece, are zeros in q and K, and give elements that are not stored)
   auto at = [&](int e) { return !PART || e < a.d ? e : 0; };
-  {
+#pragma unroll
+  for (int n = 0; n < NC; ++n) {
+    const int col = min(c0 + 16 * n + c, cols - 1), place = paOfGroup(a, col), token = s.first + place, h = kvh * group + (col - place * group);
+    p[n] = s.origin + token, sinksSeen[n] = max(0, min(a.sinks, p[n] + 1));
     const float* q = reinterpret_cast<const float*>(a.q) + (s.start + token) * a.qTok + (int64_t)h * a.qHead;
 #pragma unroll
     for (int i = 0; i < S / 4; ++i) {
-      qf[i] = *reinterpret_cast<const f32x4*>(q + at(g * S + 4 * i));
-      if (PART && g * S + 4 * i >= a.d) qf[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      qf[n][i] = *reinterpret_cast<const f32x4*>(q + at(g * S + 4 * i));
+      if (PART && g * S + 4 * i >= a.d) qf[n][i] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
   }
+  const int pFirst = __builtin_amdgcn_readlane(p[0], 0), pLast = __builtin_amdgcn_readlane(p[NC - 1], 15), window = a.window;
   auto askSlot = [&](int t) {
     if (t >= t1) return (int64_t)0;
     return ldIndex(a.bLoc, locBase + min(span.base(t) + 16 * wave + c, span.limit(t) - 1), a.loc64);
@@ -870,41 +887,55 @@ __device__ __forceinline__ void pagedFloatBlock(const PtArgs& x, const PaSequenc
       for (int i = 0; i < E / 4; ++i) vf[B][r][i] = *reinterpret_cast<const f32x4*>(vr + at(c * E + 4 * i));
     }
   };
+  float m[NC], l[NC];  // m: in units of log2
 #pragma unroll
-  for (int i = 0; i < E; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, l = 0.f;  // m: in units of log2
+  for (int n = 0; n < NC; ++n) {
+    m[n] = -INFINITY, l[n] = 0.f;
+#pragma unroll
+    for (int i = 0; i < E; ++i) o[n][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
   auto tile = [&](int t, auto buf) {
     constexpr int B = decltype(buf)::value;
     const int k0 = span.base(t) + 16 * wave;
     if (k0 > pLast || k0 >= span.limit(t) || (k0 + 15 <= pFirst - window && k0 >= a.sinks)) return;  // (uniform: nobody sees any of it)
-    f32x4 acc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};  // two chains: half the dependent latency
+    f32x4 acc[NC][2];  // two chains each: half the dependent latency
 #pragma unroll
-    for (int i = 0; i < S; ++i) acc[i & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[B][i >> 2][i & 3], qf[i >> 2][i & 3], acc[i & 1], 0, 0, 0);
-    float w[4], mx = m;
+    for (int n = 0; n < NC; ++n) acc[n][0] = acc[n][1] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int kj = k0 + 4 * g + r;
-      const bool sees = ((unsigned)(p - kj) < (unsigned)window || kj < sinksSeen) && (valid[B] >> (4 * g + r) & 1) != 0;
-      w[r] = sees ? (acc[0][r] + acc[1][r]) * a.scaleLog2e : -INFINITY;
-      mx = fmaxf(mx, w[r]);
+    for (int i = 0; i < S; ++i)
+#pragma unroll
+      for (int n = 0; n < NC; ++n) acc[n][i & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[B][i >> 2][i & 3], qf[n][i >> 2][i & 3], acc[n][i & 1], 0, 0, 0);
+    float w[NC][4];
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+      float mx = m[n];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int kj = k0 + 4 * g + r;
+        const bool sees = ((unsigned)(p[n] - kj) < (unsigned)window || kj < sinksSeen[n]) && (valid[B] >> (4 * g + r) & 1) != 0;
+        w[n][r] = sees ? (acc[n][0][r] + acc[n][1][r]) * a.scaleLog2e : -INFINITY;
+        mx = fmaxf(mx, w[n][r]);
+      }
+      mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      const float ref = mx == -INFINITY ? 0.f : mx, keep = exp2f(m[n] - ref);
+      m[n] = mx, l[n] *= keep;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        w[n][r] = exp2f(behindRounded(w[n][r], ref));
+        l[n] += w[n][r];
+      }
+#pragma unroll
+      for (int i = 0; i < E; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[n][i][r] *= keep;
     }
-    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-    const float ref = mx == -INFINITY ? 0.f : mx, keep = exp2f(m - ref);
-    m = mx, l *= keep;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      w[r] = exp2f(behindRounded(w[r], ref));
-      l += w[r];
-    }
-#pragma unroll
-    for (int i = 0; i < E; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) o[i][r] *= keep;
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
-      for (int i = 0; i < E; ++i) o[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[B][r][i >> 2][i & 3], w[r], o[i], 0, 0, 0);
+      for (int i = 0; i < E; ++i)
+#pragma unroll
+        for (int n = 0; n < NC; ++n) o[n][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[B][r][i >> 2][i & 3], w[n][r], o[n][i], 0, 0, 0);
   };
   using B0 = std::integral_constant<int, 0>;
   using B1 = std::integral_constant<int, 1>;
@@ -928,143 +959,217 @@ __device__ __forceinline__ void pagedFloatBlock(const PtArgs& x, const PaSequenc
       tile(t + 1, B1{});
     }
   }
-  l += __shfl_xor(l, 16, 64);
-  l += __shfl_xor(l, 32, 64);
-  if (l != l && m == -INFINITY) m = 0.f;  // scores that are not numbers alone: as a maximum of minus infinity they would be left out
-  if (g == 0) sm[wave][c] = m, sl[wave][c] = l;
 #pragma unroll
-  for (int r = 0; r < 4; ++r)
+  for (int n = 0; n < NC; ++n) {
+    l[n] += __shfl_xor(l[n], 16, 64);
+    l[n] += __shfl_xor(l[n], 32, 64);
+    if (l[n] != l[n] && m[n] == -INFINITY) m[n] = 0.f;  // scores that are not numbers alone: as a maximum of minus infinity they would be left out
+    if (g == 0) sm[wave][16 * n + c] = m[n], sl[wave][16 * n + c] = l[n];
 #pragma unroll
-    for (int i = 0; i < E / 4; ++i)
-      *reinterpret_cast<f32x4*>(so + (wave * 16 + c) * PITCH + (4 * g + r) * E + 4 * i) = f32x4{o[4 * i][r], o[4 * i + 1][r], o[4 * i + 2][r], o[4 * i + 3][r]};
-  __syncthreads();
-  // a column to 16 lanes
-  const int mine = threadIdx.x >> 4, e0 = c * E, oc = c0 + mine, at0 = s.first + min(oc, cols - 1) / group, hc = kvh * group + min(oc, cols - 1) % group;
-  const int64_t row = s.start + at0;
-  float mAll = -INFINITY, sum = 0.f;
-#pragma unroll
-  for (int w = 0; w < 4; ++w) mAll = fmaxf(mAll, sm[w][mine]);
-  f32x4 v[E / 4] = {};
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    const float weight = sm[w][mine] == -INFINITY ? 0.f : exp2f(sm[w][mine] - mAll);
-    sum += sl[w][mine] * weight;
-#pragma unroll
-    for (int i = 0; i < E / 4; ++i)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) v[i][k] += so[(w * 16 + mine) * PITCH + e0 + 4 * i + k] * weight;
-  }
-  bool odd = !(fabsf(sum) < INFINITY);
-#pragma unroll
-  for (int i = 0; i < E / 4; ++i)
-#pragma unroll
-    for (int k = 0; k < 4; ++k) odd |= !(fabsf(v[i][k]) < INFINITY);
-  // columns whose sums are not finite: by themselves, with the tokens that they see alone
-  const uint64_t bad = __builtin_amdgcn_ballot_w64(odd && oc < cols);
-  const bool again = (bad >> (lane & 48) & 0xffffu) != 0;
-  if (oc < cols && !again) {
-    if (whole) {
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      float* out = reinterpret_cast<float*>(a.out) + row * a.oTok + (int64_t)hc * a.oHead + e0;
+    for (int r = 0; r < 4; ++r)
 #pragma unroll
       for (int i = 0; i < E / 4; ++i)
-        if (!PART || e0 + 4 * i < a.d) *reinterpret_cast<f32x4*>(out + 4 * i) = v[i] * inv;
-    } else {
-      float* dst = x.partial + ((row * a.heads + hc) * x.splits + split) * (2 + a.d);
-      if (c == 0) dst[0] = mAll, dst[1] = sum;
+        *reinterpret_cast<f32x4*>(so + (wave * COLS + 16 * n + c) * PITCH + (4 * g + r) * E + 4 * i) =
+            f32x4{o[n][4 * i][r], o[n][4 * i + 1][r], o[n][4 * i + 2][r], o[n][4 * i + 3][r]};
+  }
+  __syncthreads();
+  // a column to 16 lanes
 #pragma unroll
-      for (int i = 0; i < E / 4; ++i) {
-        if (PART && e0 + 4 * i >= a.d) continue;
-        *reinterpret_cast<float2*>(dst + 2 + e0 + 4 * i) = float2{v[i][0], v[i][1]};
-        *reinterpret_cast<float2*>(dst + 4 + e0 + 4 * i) = float2{v[i][2], v[i][3]};
+  for (int n = 0; n < NC; ++n) {
+    const int mine = 16 * n + (threadIdx.x >> 4), e0 = c * E, oc = c0 + mine, place = paOfGroup(a, min(oc, cols - 1)), h = kvh * group + (min(oc, cols - 1) - place * group);
+    const int64_t row = s.start + s.first + place;
+    float mAll = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) mAll = fmaxf(mAll, sm[w][mine]);
+    f32x4 v[E / 4] = {};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float weight = sm[w][mine] == -INFINITY ? 0.f : exp2f(sm[w][mine] - mAll);
+      sum += sl[w][mine] * weight;
+#pragma unroll
+      for (int i = 0; i < E / 4; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[i][k] += so[(w * COLS + mine) * PITCH + e0 + 4 * i + k] * weight;
+    }
+    bool odd = !(fabsf(sum) < INFINITY);
+#pragma unroll
+    for (int i = 0; i < E / 4; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) odd |= !(fabsf(v[i][k]) < INFINITY);
+    // columns whose sums are not finite: by themselves, with the tokens that they see alone
+    const uint64_t bad = __builtin_amdgcn_ballot_w64(odd && oc < cols);
+    if (oc < cols && (bad >> (lane & 48) & 0xffffu) == 0) {
+      if (whole) {
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        float* out = reinterpret_cast<float*>(a.out) + row * a.oTok + (int64_t)h * a.oHead + e0;
+#pragma unroll
+        for (int i = 0; i < E / 4; ++i)
+          if (!PART || e0 + 4 * i < a.d) *reinterpret_cast<f32x4*>(out + 4 * i) = v[i] * inv;
+      } else {
+        const int64_t slice = (row * a.heads + h) * x.splits + split;
+        if (c == 0) x.partialState[slice] = float2{mAll, sum};
+#pragma unroll
+        for (int i = 0; i < E / 4; ++i)
+          if (!PART || e0 + 4 * i < a.d) *reinterpret_cast<f32x4*>(x.partial + slice * a.d + e0 + 4 * i) = v[i];
       }
     }
+    for (int i = 0; i < 4; ++i)
+      if ((bad >> (16 * i) & 0xffffu) != 0) pagedAgain<float, D>(x, s, kvh, locBase, span, t0, t1, split, whole, c0 + 16 * n + 4 * wave + i);
   }
-  for (int i = 0; i < 4; ++i)
-    if ((bad >> (16 * i) & 0xffffu) != 0) pagedAgain<float, D>(x, s, kvh, locBase, span, t0, t1, split, whole, c0 + 4 * wave + i);
 }
 
-template <int D, bool PART>
+template <int D, bool PART, int NC>
 __global__ __launch_bounds__(256) void pagedFloatKernel(PtArgs x) {
-  pagedPieces<kPtFloatCols, 0>(x, x.tilePieces, [&](const PaSequence& s, int b, int kvh, int block, const PtSpan& span, int t0, int t1, int split, bool whole) {
-    pagedFloatBlock<D, PART>(x, s, b, kvh, block, span, t0, t1, split, whole);
+  pagedPieces<kPtFloatCols * NC, 0>(x, x.tilePieces, [&](const PaSequence& s, int b, int kvh, int block, const PtSpan& span, int t0, int t1, int split, bool whole) {
+    pagedFloatBlock<D, PART, NC>(x, s, b, kvh, block, span, t0, t1, split, whole);
   });
 }
 
-// One row of out from the partial results of `shares` shares, a wave: lane i takes maximum and sum of share i, then every lane its elements of
-// all of them.
-template <typename T>
-__device__ __forceinline__ void pagedJoin(const PaArgs& a, const float* src, int shares, int64_t row, int h) {
-  constexpr int kPerLane = 4, kBatch = 8;  // d <= 256; shares whose elements are asked for at once
-  const int lane = threadIdx.x & 63, mine = min(lane, shares - 1);
-  float m = src[mine * (2 + a.d)], l = src[mine * (2 + a.d) + 1], acc[kPerLane] = {0.f, 0.f, 0.f, 0.f}, v[kBatch][kPerLane];
-  auto ask = [&](int i0) {
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i)
-#pragma unroll
-      for (int k = 0; k < kPerLane; ++k) {
-        const int e = lane + 64 * k;
-        v[i][k] = e < a.d ? src[min(i0 + i, shares - 1) * (2 + a.d) + 2 + e] : 0.f;
-      }
-  };
-  ask(0);
-  if (lane >= shares) m = -INFINITY, l = 0.f;
+// Weights of `shares` partial results with (maximum, sum) `state` in lane i for share i: that share's in lane i, divided by the sum of all.
+// *none: shares without a score, as bits. (shares <= 64)
+__device__ __forceinline__ float pagedWeights(float2 state, int shares, uint64_t* none) {
+  const int lane = threadIdx.x & 63;
+  float m = lane < shares ? state.x : -INFINITY, l = lane < shares ? state.y : 0.f;
   const float most = waveMax(m);
   float w = m == -INFINITY ? 0.f : exp2f(m - most);
   if (l != l) w = l;  // (scores that are not numbers alone have no maximum)
-  const uint64_t none = __builtin_amdgcn_ballot_w64(w == 0.f && m == -INFINITY);  // shares without a score
+  *none = __builtin_amdgcn_ballot_w64(w == 0.f && m == -INFINITY);
   const float sum = waveSum(l * w);
-  for (int i0 = 0; i0 < shares; i0 += kBatch) {
-    if (i0 > 0) ask(i0);
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      if (i0 + i >= shares) break;
-      const float wi = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), i0 + i));
-      if (none >> (i0 + i) & 1) continue;
-#pragma unroll
-      for (int k = 0; k < kPerLane; ++k) acc[k] += wi * v[i][k];
-    }
-  }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  T* out = reinterpret_cast<T*>(a.out) + row * a.oTok + h * a.oHead;
-#pragma unroll
-  for (int k = 0; k < kPerLane; ++k) {
-    const int e = lane + 64 * k;
-    if (e < a.d) out[e] = static_cast<T>(acc[k] * inv);
-  }
+  return w * (sum == 0.f ? 0.f : 1.f / sum);
 }
 
-// The rows whose block was walked in shares: a wave per (row, head).
-template <typename T, int COLS, int FEW>
-__global__ __launch_bounds__(256) void pagedMergeKernel(PtArgs x) {
+// The blocks of columns that were walked in shares: a wave joins MANY columns, four of them at a time with four shares of each on their way, or
+// one with eight of them.
+template <typename T, int COLS, int FEW, int PAIRS, int MANY>
+__global__ __launch_bounds__(256) void pagedMergeKernel(PtArgs x, int64_t step) {
+  constexpr int kTogether = MANY == 1 ? 1 : 4, kBatch = MANY == 1 ? 8 : 4, kPtMergeCols = 4 * MANY;
+  // d <= 128 PAIRS: a lane has elements 2 lane, 2 lane + 1 of every 128
   const PaArgs& a = x.a;
-  const int group = a.heads / a.kvHeads;
-  const int64_t step = (int64_t)gridDim.x * 4;
-  for (int64_t pair = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);; pair += step) {
-    const PaPlace at = paFind(a, pair / a.heads, [](const PaSequence& s) { return s.end - s.first; });
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kvh = blockIdx.x % a.kvHeads, group = a.group;
+  for (int64_t u = blockIdx.x / a.kvHeads;; u += step) {
+    const PaPlace at = paFind(a, u, [&](const PaSequence& s) {
+      const int cols = ptColumns(a, s);
+      return cols <= FEW ? 0 : (cols + kPtMergeCols - 1) / kPtMergeCols;
+    });
     if (at.b < 0) return;
     const PaSequence& s = at.s;
-    const int h = (int)(pair % a.heads), cols = ptColumns(a, s), origin = s.origin + s.first, block = (at.at * group + h % group) / COLS;
-    const PtSpan span(a, origin + block * COLS / group, origin + min(block * COLS + COLS - 1, cols - 1) / group);
-    const int shares = (span.tiles + x.tilesPerSplit - 1) / x.tilesPerSplit;
-    const int64_t row = s.start + s.first + at.at;
-    if (shares > 1 && cols > FEW) pagedJoin<T>(a, x.partial + (row * a.heads + h) * x.splits * (2 + a.d), shares, row, h);
-    if (pair + step >= at.total * a.heads) return;
+    const int cols = ptColumns(a, s), origin = s.origin + s.first, first = at.at * kPtMergeCols + wave * (kPtMergeCols / 4);
+#pragma unroll
+    for (int c0 = 0; c0 < kPtMergeCols / 4; c0 += kTogether) {
+      int shares[kTogether], most = 0;
+      int64_t row[kTogether];
+      int head[kTogether];
+      float2 state[kTogether], acc[kTogether][PAIRS], v[kTogether][kBatch][PAIRS];
+      const float* src[kTogether];
+#pragma unroll
+      for (int c = 0; c < kTogether; ++c) {
+        const int col = min(first + c0 + c, cols - 1), place = paOfGroup(a, col), block = col / COLS;
+        const PtSpan span(a, origin + paOfGroup(a, block * COLS), origin + paOfGroup(a, min(block * COLS + COLS - 1, cols - 1)));
+        shares[c] = first + c0 + c < cols ? (span.tiles + x.tilesPerSplit - 1) / x.tilesPerSplit : 0;
+        if (shares[c] <= 1) shares[c] = 0;  // (a block walked whole has its results)
+        most = max(most, shares[c]);
+        row[c] = s.start + s.first + place, head[c] = kvh * group + (col - place * group);
+        const int64_t slice = (row[c] * a.heads + head[c]) * x.splits;
+        state[c] = x.partialState[slice + min(lane, max(shares[c] - 1, 0))];
+        src[c] = x.partial + slice * a.d;
+#pragma unroll
+        for (int k = 0; k < PAIRS; ++k) acc[c][k] = float2{0.f, 0.f};
+      }
+      uint64_t none[kTogether];
+      float w[kTogether];
+      for (int i0 = 0; i0 < most; i0 += kBatch) {
+#pragma unroll
+        for (int c = 0; c < kTogether; ++c)
+#pragma unroll
+          for (int i = 0; i < kBatch; ++i)
+#pragma unroll
+            for (int k = 0; k < PAIRS; ++k) {
+              const int e = 2 * lane + 128 * k;
+              v[c][i][k] = e < a.d && i0 + i < shares[c] ? *reinterpret_cast<const float2*>(src[c] + (i0 + i) * a.d + e) : float2{0.f, 0.f};
+            }
+#pragma unroll
+        for (int c = 0; c < kTogether; ++c) {
+          if (i0 == 0) w[c] = pagedWeights(state[c], shares[c], &none[c]);
+#pragma unroll
+          for (int i = 0; i < kBatch; ++i) {
+            if (i0 + i >= shares[c] || (none[c] >> (i0 + i) & 1) != 0) continue;
+            const float wi = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w[c]), i0 + i));
+#pragma unroll
+            for (int k = 0; k < PAIRS; ++k) acc[c][k].x += wi * v[c][i][k].x, acc[c][k].y += wi * v[c][i][k].y;
+          }
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < kTogether; ++c) {
+        if (shares[c] == 0) continue;
+        T* out = reinterpret_cast<T*>(a.out) + row[c] * a.oTok + (int64_t)head[c] * a.oHead;
+        typedef T Two __attribute__((ext_vector_type(2)));
+#pragma unroll
+        for (int k = 0; k < PAIRS; ++k) {
+          const int e = 2 * lane + 128 * k;
+          if (e < a.d) *reinterpret_cast<Two*>(out + e) = Two{static_cast<T>(acc[c][k].x), static_cast<T>(acc[c][k].y)};
+        }
+      }
+    }
+    if (u + step >= at.total) return;
   }
 }
 
-// The columns of sequences with few of them, `most` for each K/V head: a wave per column.
-template <typename T>
+// The columns of sequences with few of them, `most` for each K/V head: a wave per column, or with WIDE a workgroup, whose waves take every
+// fourth share. What does not depend on the lengths is asked for before they are there (shares without tokens were never written:
+// what is read of them is left out).
+template <typename T, bool WIDE>
 __global__ __launch_bounds__(256) void pagedFewMergeKernel(PtArgs x, int most) {
+  constexpr int kPerLane = 4, kBatch = 8, kStep = WIDE ? 4 : 1;  // d <= 256
+  __shared__ float red[WIDE ? 4 : 1][64 * kPerLane];
   const PaArgs& a = x.a;
-  const int group = a.heads / a.kvHeads;
-  const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), pair = i / most;
-  const int col = (int)(i % most), kvh = (int)(pair % a.kvHeads);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = a.group;
+  const int64_t i = WIDE ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave, pair = i / most;
+  const int col = (int)(i - pair * most), b = (int)(pair / a.kvHeads), kvh = (int)(pair - (int64_t)b * a.kvHeads);
   if (pair >= (int64_t)a.batch * a.kvHeads) return;
-  const PaSequence s = paSequence(a, (int)(pair / a.kvHeads));
+  const float* src = x.fewPartial + (pair * kPtFewCols + col) * x.fewSplits * (2 + a.d);
+  const float2 state = *reinterpret_cast<const float2*>(src + min(lane, x.fewSplits - 1) * (2 + a.d));
+  float v[kBatch][kPerLane], acc[kPerLane] = {0.f, 0.f, 0.f, 0.f};
+  auto ask = [&](int first) {
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k)
+#pragma unroll
+      for (int j = 0; j < kPerLane; ++j) {
+        const int e = lane + 64 * j;
+        v[k][j] = e < a.d ? src[min(first + kStep * k, x.fewSplits - 1) * (2 + a.d) + 2 + e] : 0.f;
+      }
+  };
+  const int first = WIDE ? wave : 0;
+  ask(first);
+  const PaSequence s = paSequence(a, b);
   const int cols = ptColumns(a, s), shares = ptFewShares(x, s);
   if (col >= cols || cols > kPtFewCols || shares == 1) return;
-  pagedJoin<T>(a, x.fewPartial + (pair * kPtFewCols + col) * x.fewSplits * (2 + a.d), shares, s.start + s.first + col / group, kvh * group + col % group);
+  uint64_t none;
+  const float w = pagedWeights(state, shares, &none);
+  for (int i0 = first; i0 < shares; i0 += kStep * kBatch) {
+    if (i0 != first) ask(i0);
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int share = i0 + kStep * k;
+      if (share >= shares || (none >> share & 1) != 0) continue;
+      const float wi = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), share));
+#pragma unroll
+      for (int j = 0; j < kPerLane; ++j) acc[j] += wi * v[k][j];
+    }
+  }
+  const int place = paOfGroup(a, col);
+  T* out = reinterpret_cast<T*>(a.out) + (s.start + s.first + place) * a.oTok + (int64_t)(kvh * group + (col - place * group)) * a.oHead;
+  if (!WIDE) {
+#pragma unroll
+    for (int j = 0; j < kPerLane; ++j)
+      if (lane + 64 * j < a.d) out[lane + 64 * j] = static_cast<T>(acc[j]);
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < kPerLane; ++j) red[wave][lane + 64 * j] = acc[j];
+  __syncthreads();
+  const int e = threadIdx.x;
+  if (e < a.d) out[e] = static_cast<T>((red[0][e] + red[WIDE ? 1 : 0][e]) + (red[WIDE ? 2 : 0][e] + red[WIDE ? 3 : 0][e]));
 }
 
 template <typename T, int D, bool PART>
@@ -1092,11 +1197,11 @@ static diopiError_t launchFew(hipStream_t stream, const PtArgs& x, int64_t piece
   return diopiSuccess;
 }
 
-template <int D, bool PART>
+template <int D, bool PART, int NC>
 static diopiError_t launchFloat(hipStream_t stream, const PtArgs& x, int64_t wgs) {
-  constexpr int lds = 4 * 16 * (D + 4) * (int)sizeof(float);
-  AMD_HIP(allowDynamicLds(reinterpret_cast<const void*>(&pagedFloatKernel<D, PART>), lds));
-  hipLaunchKernelGGL((pagedFloatKernel<D, PART>), dim3((unsigned)wgs), dim3(256), lds, stream, x);
+  constexpr int lds = 4 * kPtFloatCols * NC * (D + 4) * (int)sizeof(float);
+  AMD_HIP(allowDynamicLds(reinterpret_cast<const void*>(&pagedFloatKernel<D, PART, NC>), lds));
+  hipLaunchKernelGGL((pagedFloatKernel<D, PART, NC>), dim3((unsigned)wgs), dim3(256), lds, stream, x);
   AMD_LAUNCH_CHECK();
   return diopiSuccess;
 }
@@ -1108,8 +1213,9 @@ bool pagedAttentionTiles(const PaArgs& a, diopiDtype_t dtype) {
                        (int64_t)reinterpret_cast<uintptr_t>(a.out) |
                        (a.kSlotStride | a.kHeadStride | a.vSlotStride | a.vHeadStride | a.qTok | a.qHead | a.oTok | a.oHead) * size;
   if ((bits & 15) != 0 || a.kSlotStride < 0 || a.vSlotStride < 0 || std::max(a.kSlotStride, a.vSlotStride) * size > 0xffffffffll) return false;
-  // 32 bits hold the columns of a sequence
-  return std::min<int64_t>(a.maxNew, a.rows) * (a.heads / a.kvHeads) < 1 << 30;
+  // columns of a sequence that paOfGroup divides (and 32 bits hold)
+  const int64_t columns = std::min<int64_t>(a.maxNew, a.rows) * a.group + kPtCols;
+  return columns < 1 << 30 && columns * a.group < (int64_t)1 << 32;
 }
 
 diopiError_t pagedAttentionMfma(diopiContextHandle_t ctx, hipStream_t stream, const PaArgs& a, diopiDtype_t dtype) {
@@ -1117,7 +1223,7 @@ diopiError_t pagedAttentionMfma(diopiContextHandle_t ctx, hipStream_t stream, co
   x.a = a;
   const bool wide = dtype == diopi_dtype_float32;
   if (!wide) x.kSlotBytes = (unsigned)(a.kSlotStride * 2), x.vSlotBytes = (unsigned)(a.vSlotStride * 2);
-  const int64_t group = a.heads / a.kvHeads, tokens = std::min<int64_t>(a.rows, (int64_t)a.batch * a.maxNew), cus = computeUnits();
+  const int64_t group = a.group, tokens = std::min<int64_t>(a.rows, (int64_t)a.batch * a.maxNew), cus = computeUnits();
   const int64_t tiles = std::max<int64_t>(1, std::min<int64_t>(ceilDiv(a.maxLen, kPtTile), ceilDiv(a.sinks, kPtTile) + ceilDiv((int64_t)a.window + kPtCols, kPtTile)));
   const int64_t limit = 1 << 24;  // workgroups: 2^32 threads
   const bool onlyFew = !wide && std::min<int64_t>(a.maxNew, a.rows) * group <= kPtFewCols;
@@ -1129,6 +1235,7 @@ diopiError_t pagedAttentionMfma(diopiContextHandle_t ctx, hipStream_t stream, co
     const int64_t want = std::max<int64_t>(1, 2 * cus / (sequences * a.kvHeads));
     int64_t chunk = std::max<int64_t>({128, ceilDiv(ceilDiv(seen, want), 64) * 64, ceilDiv(ceilDiv(seen, kPtMaxSplit), 64) * 64});
     if (seen <= 256) chunk = seen;
+    if (!onlyFew) chunk = std::max<int64_t>(chunk, std::min<int64_t>(seen, 4096));  // (next to blocks of columns, which take longer)
     wideHeads = onlyFew && a.kvHeads % kPfWaves == 0 && seen <= 128;
     x.fewChunk = (int)chunk, x.fewSplits = (int)ceilDiv(seen, chunk);
     if (x.fewSplits > 1) {
@@ -1137,25 +1244,34 @@ diopiError_t pagedAttentionMfma(diopiContextHandle_t ctx, hipStream_t stream, co
       x.fewPartial = static_cast<float*>(ws);
     }
   }
-  // The others: blocks of columns, what the rows of q fill, and one partly filled for each sequence at most. Where they leave compute units
-  // without work the sequences are walked in shares.
-  const int64_t columns = tokens * group, blockCols = wide ? kPtFloatCols : kPtCols;
-  const int64_t blocks = ceilDiv(columns, blockCols), partly = wide ? sequences : std::min(sequences, columns / (kPtFewCols + 1));
+  // The others: blocks of columns, what the rows of q fill, and one partly filled for each sequence but one at most. Where they leave compute
+  // units without work the sequences are walked in shares.
+  const int64_t columns = tokens * group;
+  // fp32: two tiles of columns to a block where sequences have that many and there are blocks for half of the compute units all the same (us, one
+  // tile -> two: 4 x 50 new tokens behind 100 ... 1000, 32 heads of 128 76 -> 61, 2 x 700 behind 300 361 -> 277; 16 x (1 .. 40), 8 heads of 64, 88
+  // blocks, 11.5 -> 16.6). More than 128 elements leave no registers for it.
+  const bool pairs = wide && a.d <= 128 && columns >= kPtFloatCols * sequences && ceilDiv(columns, 2 * kPtFloatCols) * a.kvHeads >= cus / 2;
+  const int64_t blockCols = wide ? (pairs ? 2 : 1) * kPtFloatCols : kPtCols;
+  const int64_t partly = std::max<int64_t>(1, wide ? sequences : std::min(sequences, columns / (kPtFewCols + 1))) - 1;
+  const int64_t blocks = ceilDiv(columns, blockCols) + partly;
   x.tilesPerSplit = (int)tiles, x.splits = 1;
   if (!onlyFew) {
-    const int64_t perKv = std::max<int64_t>(blocks, sequences);
-    int64_t splits = std::max<int64_t>(1, 2 * cus / (perKv * a.kvHeads));
-    splits = std::min<int64_t>({splits, kPtMaxSplit, ceilDiv(tiles, 2)});
-    x.tilesPerSplit = (int)ceilDiv(tiles, splits);
+    // As many shares as make one round of workgroups, of at least 6 tiles (fp32: 2, and three shares or none): partial results and the launch
+    // that joins them cost a share of 6 tiles half as much again. us, whole -> shares: 1 x 512 new tokens behind 8000, 32 heads on 8 218 -> 98, 1 x 300
+    // behind 9000, 40 heads 220 -> 106, 1 x 64 behind 4000, 32 heads 105 -> 29, 4 x (200 .. 333) behind 100 ... 3000, 32 on 8 85 -> 68; against
+    // it with more blocks than half a round: the same four next to 20 single tokens 92 -> 110, 4 x 512, 32 on 8 219 -> 254.
+    const int64_t units = blocks * a.kvHeads, slots = (a.d > 128 ? 1 : 2) * cus, splits = (2 * slots + units) / (2 * units), least = wide ? 2 : 6;
+    if (splits > (wide ? 2 : 1) && tiles >= 2 * least) x.tilesPerSplit = (int)std::max<int64_t>({least, ceilDiv(tiles, splits), ceilDiv(tiles, kPtMaxSplit)});
     x.splits = (int)ceilDiv(tiles, x.tilesPerSplit);
     if (x.splits > 1) {
       void* ws = nullptr;
-      AMD_TRY(requireWorkspace(ctx, a.rows * a.heads * x.splits * (2 + a.d) * (int64_t)sizeof(float), &ws));
-      x.partial = static_cast<float*>(ws);
+      const int64_t slices = a.rows * a.heads * x.splits;
+      AMD_TRY(requireWorkspace(ctx, slices * (2 + a.d) * (int64_t)sizeof(float), &ws));
+      x.partial = static_cast<float*>(ws), x.partialState = reinterpret_cast<float2*>(x.partial + slices * a.d);
     }
   }
   const int64_t fewPieces = wide ? 0 : (int64_t)a.batch * x.fewSplits;
-  x.tilePieces = onlyFew ? 0 : (blocks + partly) * x.splits;
+  x.tilePieces = onlyFew ? 0 : blocks * x.splits;
   const int64_t wgs = (x.tilePieces + fewPieces) * a.kvHeads;
   AMD_CHECK(wgs < limit, "paged attention: %ld rows of %d heads exceed the grid limits", (long)a.rows, a.heads);
 #define SIZE_CALL(CALL)               \
@@ -1167,28 +1283,54 @@ diopiError_t pagedAttentionMfma(diopiContextHandle_t ctx, hipStream_t stream, co
 #define HALF_CALL(T, D) AMD_TRY((onlyFew ? launchFew<T, D>(stream, x, fewPieces, wideHeads) : a.d == D ? launchTile<T, D, false>(stream, x, wgs) : launchTile<T, D, true>(stream, x, wgs)))
 #define BF16_CALL(D) HALF_CALL(bf16_t, D)
 #define FP16_CALL(D) HALF_CALL(half_t, D)
-#define FP32_CALL(D) AMD_TRY((a.d == D ? launchFloat<D, false>(stream, x, wgs) : launchFloat<D, true>(stream, x, wgs)))
+#define FP32_CALL_AS(D, NC) AMD_TRY((a.d == D ? launchFloat<D, false, NC>(stream, x, wgs) : launchFloat<D, true, NC>(stream, x, wgs)))
+#define FP32_CALL(D)                                   \
+  do {                                                 \
+    if (!pairs) FP32_CALL_AS(D, 1);                    \
+    else if constexpr (D <= 128) FP32_CALL_AS(D, 2);   \
+  } while (0)
   if (dtype == diopi_dtype_bfloat16) SIZE_CALL(BF16_CALL);
   else if (dtype == diopi_dtype_float16) SIZE_CALL(FP16_CALL);
   else SIZE_CALL(FP32_CALL);
 #undef FP32_CALL
+#undef FP32_CALL_AS
 #undef FP16_CALL
 #undef BF16_CALL
 #undef HALF_CALL
 #undef SIZE_CALL
   if (x.fewSplits > 1) {
     const int mostCols = (int)std::min<int64_t>(kPtFewCols, std::min<int64_t>(a.maxNew, a.rows) * group);
-    const int64_t merges = ceilDiv((int64_t)a.batch * a.kvHeads * mostCols, 4);
+    const bool wideMerge = x.fewSplits > 8;
+    const int64_t merges = ceilDiv((int64_t)a.batch * a.kvHeads * mostCols, wideMerge ? 1 : 4);
     AMD_CHECK(merges < limit, "paged attention: %d sequences of %d heads exceed the grid limits", a.batch, a.heads);
-    if (dtype == diopi_dtype_bfloat16) hipLaunchKernelGGL(pagedFewMergeKernel<bf16_t>, dim3((unsigned)merges), dim3(256), 0, stream, x, mostCols);
-    else hipLaunchKernelGGL(pagedFewMergeKernel<half_t>, dim3((unsigned)merges), dim3(256), 0, stream, x, mostCols);
+#define FEW_MERGE(T)                                                                                                                                    \
+  do {                                                                                                                                                  \
+    if (wideMerge) hipLaunchKernelGGL((pagedFewMergeKernel<T, true>), dim3((unsigned)merges), dim3(256), 0, stream, x, mostCols);                        \
+    else hipLaunchKernelGGL((pagedFewMergeKernel<T, false>), dim3((unsigned)merges), dim3(256), 0, stream, x, mostCols);                                 \
+  } while (0)
+    if (dtype == diopi_dtype_bfloat16) FEW_MERGE(bf16_t);
+    else FEW_MERGE(half_t);
+#undef FEW_MERGE
     AMD_LAUNCH_CHECK();
   }
   if (x.splits > 1) {
-    const dim3 grid((unsigned)std::min<int64_t>(ceilDiv(tokens * a.heads, 4), 1 << 23)), block(256);
-    if (dtype == diopi_dtype_bfloat16) hipLaunchKernelGGL((pagedMergeKernel<bf16_t, kPtCols, kPtFewCols>), grid, block, 0, stream, x);
-    else if (dtype == diopi_dtype_float16) hipLaunchKernelGGL((pagedMergeKernel<half_t, kPtCols, kPtFewCols>), grid, block, 0, stream, x);
-    else hipLaunchKernelGGL((pagedMergeKernel<float, kPtFloatCols, 0>), grid, block, 0, stream, x);
+    // a wave per column where that is less than four workgroups for a compute unit
+    const bool single = columns * a.kvHeads < 16 * cus;
+    const int64_t pieces = ceilDiv(columns, single ? 4 : 32) + partly;
+    AMD_CHECK(pieces * a.kvHeads < limit, "paged attention: %ld rows of %d heads exceed the grid limits", (long)a.rows, a.heads);
+    const dim3 grid((unsigned)(pieces * a.kvHeads)), block(256);
+#define TILE_MERGE(T, COLS, FEW)                                                                                                        \
+  do {                                                                                                                                  \
+    if (single && a.d <= 128) hipLaunchKernelGGL((pagedMergeKernel<T, COLS, FEW, 1, 1>), grid, block, 0, stream, x, pieces);             \
+    else if (single) hipLaunchKernelGGL((pagedMergeKernel<T, COLS, FEW, 2, 1>), grid, block, 0, stream, x, pieces);                      \
+    else if (a.d <= 128) hipLaunchKernelGGL((pagedMergeKernel<T, COLS, FEW, 1, 8>), grid, block, 0, stream, x, pieces);                  \
+    else hipLaunchKernelGGL((pagedMergeKernel<T, COLS, FEW, 2, 8>), grid, block, 0, stream, x, pieces);                                  \
+  } while (0)
+    if (dtype == diopi_dtype_bfloat16) TILE_MERGE(bf16_t, kPtCols, kPtFewCols);
+    else if (dtype == diopi_dtype_float16) TILE_MERGE(half_t, kPtCols, kPtFewCols);
+    else if (pairs) TILE_MERGE(float, 2 * kPtFloatCols, 0);
+    else TILE_MERGE(float, kPtFloatCols, 0);
+#undef TILE_MERGE
     AMD_LAUNCH_CHECK();
   }
   return diopiSuccess;
