@@ -20,6 +20,7 @@
 // out not finite, or whose maximum is beyond that, is walked again by itself on the vector ALUs, the tokens that it sees alone (PaColumn).
 #include <algorithm>
 #include <type_traits>
+#include <cstdlib>
 
 #include "paged_attention.hpp"
 
@@ -58,6 +59,8 @@ struct PtArgs {
   float* fewPartial;  // of sequences with few columns: [batch, kv_heads, kPtFewCols, fewSplits, 2 + d]
   int fewSplits = 0, fewChunk = 1;
   int64_t tilePieces;  // workgroups for each K/V head that take blocks of columns
+  unsigned tileWgs;    // all of them
+  int64_t turn;
 };
 
 // The tiles that the tokens at positions pMin ... pMax see: sinkTiles of the sequence's first tokens, the others from token `low` on, up
@@ -182,10 +185,13 @@ __device__ __forceinline__ void pagedTileBlock(const PtArgs& x, const PaSequence
 
   // ---- slots: lane l has that of token l of a tile; past the tile's last token that again (whose place has no score)
   auto askSlot = [&](int t) {
-    if (t >= t1) return (int64_t)0;
-    return ldIndex(a.bLoc, locBase + min(span.base(t) + lane, span.limit(t) - 1), a.loc64);
+    if (t >= t1) return int2{0, 0};
+    return paAsk(a.bLoc, locBase + min(span.base(t) + lane, span.limit(t) - 1), a.loc64);
   };
-  auto inPool = [&](int64_t slot) { return slot >= 0 && slot < a.slots; };
+  auto inPool = [&](int2 asked) {
+    const int64_t slot = paIndex(asked, a.loc64);
+    return slot >= 0 && slot < a.slots;
+  };
   // ---- tile copies. Copy instruction i of this wave fills the 1 KiB (i * 4 + wave) of a stage: lane l the place (row l / CPR, piece l % CPR),
   // for which it fetches the piece that the swizzle puts there.
   int kPiece[NLD], vPiece[NLD];
@@ -198,9 +204,9 @@ __device__ __forceinline__ void pagedTileBlock(const PtArgs& x, const PaSequence
   const char* const vBase = reinterpret_cast<const char*>(reinterpret_cast<const T*>(a.v) + kvh * a.vHeadStride);
   const unsigned ldsK0 = (unsigned)(uintptr_t)ptSmem, ldsV0 = ldsK0 + 2 * kStageBytes;
   // (slots outside the pool are skipped, never dereferenced: the tile's first one inside stands in, slot 0 where there is none)
-  auto rowsOf = [&](int64_t slot, uint64_t in, int (&rows)[NLD]) {
-    const int instead = in != 0 ? __builtin_amdgcn_readlane((int)slot, __builtin_ctzll(in)) : 0;
-    const int mine = inPool(slot) ? (int)slot : instead;
+  auto rowsOf = [&](int2 asked, uint64_t in, int (&rows)[NLD]) {
+    const int instead = in != 0 ? __builtin_amdgcn_readlane(asked.x, __builtin_ctzll(in)) : 0;
+    const int mine = inPool(asked) ? asked.x : instead;
 #pragma unroll
     for (int i = 0; i < NLD; ++i) rows[i] = __shfl(mine, (i * 4 + wave) * RPL + lane / CPR, 64);
   };
@@ -245,9 +251,9 @@ __device__ __forceinline__ void pagedTileBlock(const PtArgs& x, const PaSequence
   }
   int rowsNext[NLD], rowsAfter[NLD];      // of tiles t + 1 and t + 2
   uint64_t valid, validNext, validAfter;  // tokens of tiles t, t + 1, t + 2 whose slot is in the pool
-  int64_t asked;                          // slots of tile t + 3
+  int2 asked;                             // slots of tile t + 3
   {
-    const int64_t first = askSlot(t0), second = askSlot(t0 + 1), third = askSlot(t0 + 2);
+    const int2 first = askSlot(t0), second = askSlot(t0 + 1), third = askSlot(t0 + 2);
     int rows[NLD];
     valid = __builtin_amdgcn_ballot_w64(inPool(first));
     validNext = __builtin_amdgcn_ballot_w64(inPool(second)), validAfter = __builtin_amdgcn_ballot_w64(inPool(third));
@@ -445,14 +451,17 @@ __device__ __forceinline__ void pagedTileBlock(const PtArgs& x, const PaSequence
   for (; again != 0; again &= again - 1) pagedAgain<T, D>(x, s, kvh, locBase, span, t0, t1, split, whole, c0 + __builtin_ctz(again));
 }
 
-// A workgroup's pieces of work: K/V heads fastest (the ids go round the XCDs, so a head's pieces stay on one), then the list of pieces:
-// sequence after sequence, shares from the first, blocks from the last, which has the most tiles. `step` workgroups for each K/V head, the
-// number of pieces unless sequences share rows of q; sequences of up to FEW columns are not among them.
+// A workgroup's pieces of work, from a list for each K/V head: sequence after sequence, shares from the first, blocks from the last, which has
+// the most tiles. x.tilePieces workgroups for each K/V head, the number of pieces unless sequences share rows of q; sequences of up to FEW
+// columns are not among them.
+// Where all of them run at once, two to a compute unit, the second round of units (from x.turn pieces on) goes through the rest of the list
+// from its end: a block with many tiles runs next to one with few.
 template <int COLS, int FEW, typename F>
-__device__ __forceinline__ void pagedPieces(const PtArgs& x, int64_t step, F&& walk) {
+__device__ __forceinline__ void pagedPieces(const PtArgs& x, F&& walk) {
   const PaArgs& a = x.a;
   const int kvh = blockIdx.x % a.kvHeads, group = a.group;
-  for (int64_t u = blockIdx.x / a.kvHeads;; u += step) {
+  const int64_t step = x.tilePieces, mine = blockIdx.x / a.kvHeads;
+  for (int64_t u = mine < x.turn ? mine : step - 1 - (mine - x.turn);; u += step) {
     const PaPlace at = paFind(a, u, [&](const PaSequence& s) { return ptColumns(a, s) <= FEW ? 0 : PtPieces<COLS>(x, s).all(); });
     if (at.b < 0) return;
     const PaSequence& s = at.s;
@@ -576,18 +585,19 @@ __device__ __forceinline__ void pagedFewBlock(const PtArgs& x, const PaSequence&
     const int cnt = min(kPfBlock, to - b0), tiles = (cnt + kPfTile - 1) / kPfTile;
     // slots of the block; past the last token that again; one outside the pool is skipped, never dereferenced: it is marked by its top bit,
     // and another of the block stands in (slot 0 where there is none)
-    int64_t raw[kPfBlock / 64];
+    int2 raw[kPfBlock / 64];
     uint64_t in[kPfBlock / 64];
 #pragma unroll
-    for (int i = 0; i < kPfBlock / 64; ++i) raw[i] = ldIndex(a.bLoc, locBase + list.token(b0 + min(i * 64 + lane, cnt - 1)), a.loc64);
+    for (int i = 0; i < kPfBlock / 64; ++i) raw[i] = paAsk(a.bLoc, locBase + list.token(b0 + min(i * 64 + lane, cnt - 1)), a.loc64);
     int instead = 0;
 #pragma unroll
     for (int i = 0; i < kPfBlock / 64; ++i) {
-      in[i] = __builtin_amdgcn_ballot_w64(raw[i] >= 0 && raw[i] < a.slots);
-      if (in[i] != 0) instead = __builtin_amdgcn_readlane((int)raw[i], __builtin_ctzll(in[i]));
+      const int64_t slot = paIndex(raw[i], a.loc64);
+      in[i] = __builtin_amdgcn_ballot_w64(slot >= 0 && slot < a.slots);
+      if (in[i] != 0) instead = __builtin_amdgcn_readlane(raw[i].x, __builtin_ctzll(in[i]));
     }
 #pragma unroll
-    for (int i = 0; i < kPfBlock / 64; ++i) slots[i * 64 + lane] = in[i] >> lane & 1 ? (int)raw[i] : (int)(0x80000000u | (unsigned)instead);
+    for (int i = 0; i < kPfBlock / 64; ++i) slots[i * 64 + lane] = in[i] >> lane & 1 ? raw[i].x : (int)(0x80000000u | (unsigned)instead);
     const bool skips = (in[0] & in[1]) != ~0ull;
     static_assert(kPfBlock == 128, "two words of 64 slots");
     exchangeInWave();
@@ -809,15 +819,15 @@ __global__ __launch_bounds__(kPfWaves * 64, D > 128 ? 1 : 2) void pagedFewKernel
   pagedFewPiece<T, D, WIDE>(x, blockIdx.x / groups, WIDE ? g * kPfWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : g);
 }
 
-// Sequences of any number of columns: the first x.tilePieces workgroups for each K/V head take blocks of many, the others few.
+// Sequences of any number of columns: the first x.tileWgs workgroups take blocks of many, the others few.
 template <typename T, int D, bool PART>
 __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void pagedTileKernel(PtArgs x) {
-  const int64_t u = blockIdx.x / x.a.kvHeads;
-  if (u >= x.tilePieces) {
-    pagedFewPiece<T, D, false>(x, u - x.tilePieces, (int)(blockIdx.x % x.a.kvHeads));
+  if (blockIdx.x >= x.tileWgs) {
+    const unsigned i = blockIdx.x - x.tileWgs;
+    pagedFewPiece<T, D, false>(x, i / x.a.kvHeads, (int)(i % x.a.kvHeads));
     return;
   }
-  pagedPieces<kPtCols, kPtFewCols>(x, x.tilePieces, [&](const PaSequence& s, int b, int kvh, int block, const PtSpan& span, int t0, int t1, int split, bool whole) {
+  pagedPieces<kPtCols, kPtFewCols>(x, [&](const PaSequence& s, int b, int kvh, int block, const PtSpan& span, int t0, int t1, int split, bool whole) {
     pagedTileBlock<T, D, PART>(x, s, b, kvh, block, span, t0, t1, split, whole);
   });
 }
@@ -864,12 +874,13 @@ __device__ __forceinline__ void pagedFloatBlock(const PtArgs& x, const PaSequenc
   }
   const int pFirst = __builtin_amdgcn_readlane(p[0], 0), pLast = __builtin_amdgcn_readlane(p[NC - 1], 15), window = a.window;
   auto askSlot = [&](int t) {
-    if (t >= t1) return (int64_t)0;
-    return ldIndex(a.bLoc, locBase + min(span.base(t) + 16 * wave + c, span.limit(t) - 1), a.loc64);
+    if (t >= t1) return int2{0, 0};
+    return paAsk(a.bLoc, locBase + min(span.base(t) + 16 * wave + c, span.limit(t) - 1), a.loc64);
   };
   uint32_t valid[2];
-  auto fetch = [&](int64_t slot, auto buf) {
+  auto fetch = [&](int2 asked, auto buf) {
     constexpr int B = decltype(buf)::value;
+    const int64_t slot = paIndex(asked, a.loc64);
     const bool in = slot >= 0 && slot < a.slots;
     valid[B] = (uint32_t)__builtin_amdgcn_ballot_w64(in) & 0xffffu;
     // (slots outside the pool are skipped, never dereferenced: the first one inside stands in, slot 0 where there is none)
@@ -940,19 +951,19 @@ __device__ __forceinline__ void pagedFloatBlock(const PtArgs& x, const PaSequenc
   using B0 = std::integral_constant<int, 0>;
   using B1 = std::integral_constant<int, 1>;
   if (t0 < t1) {
-    const int64_t first = askSlot(t0);
-    int64_t next = askSlot(t0 + 1);
+    const int2 first = askSlot(t0);
+    int2 next = askSlot(t0 + 1);
     fetch(first, B0{});
     for (int t = t0; t < t1; t += 2) {
       if (t + 1 < t1) {
-        const int64_t slot = next;
+        const int2 slot = next;
         next = askSlot(t + 2);
         fetch(slot, B1{});
       }
       tile(t, B0{});
       if (t + 1 >= t1) break;
       if (t + 2 < t1) {
-        const int64_t slot = next;
+        const int2 slot = next;
         next = askSlot(t + 3);
         fetch(slot, B0{});
       }
@@ -1020,7 +1031,7 @@ __device__ __forceinline__ void pagedFloatBlock(const PtArgs& x, const PaSequenc
 
 template <int D, bool PART, int NC>
 __global__ __launch_bounds__(256) void pagedFloatKernel(PtArgs x) {
-  pagedPieces<kPtFloatCols * NC, 0>(x, x.tilePieces, [&](const PaSequence& s, int b, int kvh, int block, const PtSpan& span, int t0, int t1, int split, bool whole) {
+  pagedPieces<kPtFloatCols * NC, 0>(x, [&](const PaSequence& s, int b, int kvh, int block, const PtSpan& span, int t0, int t1, int split, bool whole) {
     pagedFloatBlock<D, PART, NC>(x, s, b, kvh, block, span, t0, t1, split, whole);
   });
 }
@@ -1272,7 +1283,9 @@ diopiError_t pagedAttentionMfma(diopiContextHandle_t ctx, hipStream_t stream, co
   }
   const int64_t fewPieces = wide ? 0 : (int64_t)a.batch * x.fewSplits;
   x.tilePieces = onlyFew ? 0 : blocks * x.splits;
-  const int64_t wgs = (x.tilePieces + fewPieces) * a.kvHeads;
+  const int64_t tileWgs = x.tilePieces * a.kvHeads, wgs = tileWgs + fewPieces * a.kvHeads;
+  x.tileWgs = (unsigned)std::min(tileWgs, limit);
+  x.turn = tileWgs <= 2 * cus && getenv("PA_PAIR") == nullptr ? ceilDiv(cus, a.kvHeads) : x.tilePieces;
   AMD_CHECK(wgs < limit, "paged attention: %ld rows of %d heads exceed the grid limits", (long)a.rows, a.heads);
 #define SIZE_CALL(CALL)               \
   do {                                \
