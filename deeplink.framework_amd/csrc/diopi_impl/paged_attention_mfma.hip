@@ -20,7 +20,6 @@
 // out not finite, or whose maximum is beyond that, is walked again by itself on the vector ALUs, the tokens that it sees alone (PaColumn).
 #include <algorithm>
 #include <type_traits>
-#include <cstdlib>
 
 #include "paged_attention.hpp"
 
@@ -1267,12 +1266,13 @@ diopiError_t pagedAttentionMfma(diopiContextHandle_t ctx, hipStream_t stream, co
   const int64_t blocks = ceilDiv(columns, blockCols) + partly;
   x.tilesPerSplit = (int)tiles, x.splits = 1;
   if (!onlyFew) {
-    // As many shares as make one round of workgroups, of at least 6 tiles (fp32: 2, and three shares or none): partial results and the launch
-    // that joins them cost a share of 6 tiles half as much again. us, whole -> shares: 1 x 512 new tokens behind 8000, 32 heads on 8 218 -> 98, 1 x 300
+    // As many shares as make one round of workgroups, of at least 6 tiles, or two of 12 (fp32: 2, and three shares or none): partial results and
+    // the launch that joins them cost a share of 6 tiles half as much again, and one workgroup alone on a compute unit takes 1.0 us for a tile
+    // where each of two takes 2.3 (1 x 1024 new tokens, 32 heads, 16 tiles: 43 us in two shares, 33 in one). us, whole -> shares: 1 x 512 new tokens behind 8000, 32 heads on 8 218 -> 98, 1 x 300
     // behind 9000, 40 heads 220 -> 106, 1 x 64 behind 4000, 32 heads 105 -> 29, 4 x (200 .. 333) behind 100 ... 3000, 32 on 8 85 -> 68; against
     // it with more blocks than half a round: the same four next to 20 single tokens 92 -> 110, 4 x 512, 32 on 8 219 -> 254.
     const int64_t units = blocks * a.kvHeads, slots = (a.d > 128 ? 1 : 2) * cus, splits = (2 * slots + units) / (2 * units), least = wide ? 2 : 6;
-    if (splits > (wide ? 2 : 1) && tiles >= 2 * least) x.tilesPerSplit = (int)std::max<int64_t>({least, ceilDiv(tiles, splits), ceilDiv(tiles, kPtMaxSplit)});
+    if (splits > (wide ? 2 : 1) && tiles >= (splits == 2 ? 4 : 2) * least) x.tilesPerSplit = (int)std::max<int64_t>({least, ceilDiv(tiles, splits), ceilDiv(tiles, kPtMaxSplit)});
     x.splits = (int)ceilDiv(tiles, x.tilesPerSplit);
     if (x.splits > 1) {
       void* ws = nullptr;
@@ -1285,7 +1285,7 @@ diopiError_t pagedAttentionMfma(diopiContextHandle_t ctx, hipStream_t stream, co
   x.tilePieces = onlyFew ? 0 : blocks * x.splits;
   const int64_t tileWgs = x.tilePieces * a.kvHeads, wgs = tileWgs + fewPieces * a.kvHeads;
   x.tileWgs = (unsigned)std::min(tileWgs, limit);
-  x.turn = tileWgs <= 2 * cus && getenv("PA_PAIR") == nullptr ? ceilDiv(cus, a.kvHeads) : x.tilePieces;
+  x.turn = tileWgs <= 2 * cus ? ceilDiv(cus, a.kvHeads) : x.tilePieces;
   AMD_CHECK(wgs < limit, "paged attention: %ld rows of %d heads exceed the grid limits", (long)a.rows, a.heads);
 #define SIZE_CALL(CALL)               \
   do {                                \
