@@ -59,7 +59,7 @@ struct PtArgs {
   int fewSplits = 0, fewChunk = 1;
   int64_t tilePieces;  // workgroups for each K/V head that take blocks of columns
   unsigned tileWgs;    // all of them
-  int64_t turn;
+  int64_t turn;        // see pagedPieces
 };
 
 // The tiles that the tokens at positions pMin ... pMax see: sinkTiles of the sequence's first tokens, the others from token `low` on, up
@@ -1246,7 +1246,13 @@ diopiError_t pagedAttentionMfma(diopiContextHandle_t ctx, hipStream_t stream, co
     int64_t chunk = std::max<int64_t>({128, ceilDiv(ceilDiv(seen, want), 64) * 64, ceilDiv(ceilDiv(seen, kPtMaxSplit), 64) * 64});
     if (seen <= 256) chunk = seen;
     if (!onlyFew) chunk = std::max<int64_t>(chunk, std::min<int64_t>(seen, 4096));  // (next to blocks of columns, which take longer)
-    wideHeads = onlyFew && a.kvHeads % kPfWaves == 0 && seen <= 128;
+    // A wave for each K/V head, with no shares, where a workgroup for each would be more than one round of them, of up to 128 tokens for each such
+    // round and 512 (us, a workgroup -> a wave: 16 x 1 new token behind 130, 32 heads of 128, one round, 9.1 -> 15.3; 24 x 1 behind 60 12.8 -> 10.5, behind
+    // 250 21.6 -> 22.1; 64 x 1, four rounds, behind 130 35.6 -> 27.0, behind 500 86.1 -> 83.3; 200 x 5, 32 heads on 8, behind 130 56.7 -> 30.7; 64 x 1
+    // behind 1 ... 1000, lengths that differ much, 95 -> 111).
+    const int64_t units = sequences * a.kvHeads, round = (a.d > 128 ? 1 : 2) * cus;
+    wideHeads = onlyFew && a.kvHeads % kPfWaves == 0 && units > round && seen <= std::min<int64_t>(512, 128 * units / round);
+    if (wideHeads) chunk = seen;
     x.fewChunk = (int)chunk, x.fewSplits = (int)ceilDiv(seen, chunk);
     if (x.fewSplits > 1) {
       void* ws = nullptr;
