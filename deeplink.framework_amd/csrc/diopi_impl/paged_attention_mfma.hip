@@ -1245,7 +1245,10 @@ diopiError_t pagedAttentionMfma(diopiContextHandle_t ctx, hipStream_t stream, co
     const int64_t want = std::max<int64_t>(1, 2 * cus / (sequences * a.kvHeads));
     int64_t chunk = std::max<int64_t>({128, ceilDiv(ceilDiv(seen, want), 64) * 64, ceilDiv(ceilDiv(seen, kPtMaxSplit), 64) * 64});
     if (seen <= 256) chunk = seen;
-    if (!onlyFew) chunk = std::max<int64_t>(chunk, std::min<int64_t>(seen, 4096));  // (next to blocks of columns, which take longer)
+    // next to blocks of columns, which take longer: shares of 4096, and no shares (nor a launch that joins them, 4.5 us) where the rows of q
+    // are so many that no sequence has few, unless rows of none are among them
+    const int64_t mostFew = kPtFewCols / group, others = (int64_t)(a.batch - 1) * a.maxNew;
+    if (!onlyFew) chunk = a.rows - others > mostFew ? seen : std::max<int64_t>(chunk, std::min<int64_t>(seen, 4096));
     // A wave for each K/V head, with no shares, where a workgroup for each would be more than one round of them, of up to 128 tokens for each such
     // round and 512 (us, a workgroup -> a wave: 16 x 1 new token behind 130, 32 heads of 128, one round, 9.1 -> 15.3; 24 x 1 behind 60 12.8 -> 10.5, behind
     // 250 21.6 -> 22.1; 64 x 1, four rounds, behind 130 35.6 -> 27.0, behind 500 86.1 -> 83.3; 200 x 5, 32 heads on 8, behind 130 56.7 -> 30.7; 64 x 1
