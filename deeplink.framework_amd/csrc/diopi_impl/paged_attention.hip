@@ -19,7 +19,8 @@
 namespace amd {
 
 // Any head size up to 64 J, any strides: a workgroup per (new token, head), whose waves take 64 tokens that it sees in turn (PaColumn).
-// Bound by the vector ALUs, whose sums over the lanes cost more than the products.
+// Bound by the vector ALUs, whose sums over the lanes cost more than the products (2 x 2048 new tokens behind 6000, 32 heads of 128 bf16, which
+// pagedTileKernel takes: 72 ms).
 constexpr int kPgWaves = 4;
 template <typename T, int J, int UNR>
 __global__ __launch_bounds__(kPgWaves * 64) void pagedAnyKernel(PaArgs a) {

@@ -15,6 +15,10 @@
 //   * a workgroup finds its piece of work in the lengths on the device: the grid is as large as the rows of q can make it, and sequences
 //     of one new token and of thousands are dealt alike. The pieces of one K/V head's sequence are neighbours on one XCD.
 //   * shares of a sequence leave (maximum, sum, weighted sum of V) in workspace, which pagedMergeKernel joins.
+// Bound by the matrix pipe and the vector ALUs, between which the two waves of a SIMD change places less than they could: bf16, 32 heads of 128, 2 x
+// 2048 new tokens behind 6000 519 us, 0.92 PFLOP/s, the pipe busy 47 % of the time, the ALUs about as long, LDS 24 %. A block spends 8.6 us besides its
+// tiles (search 2.3, slots and first tiles 3.7, output 2.6), of which a second workgroup on the compute unit hides a part: prompts of
+// 2048 with a window of 512, 11 tiles to a block, 128 us.
 // What a column does not see (later tokens, those before the window, slots outside the pool) has no score; but a weight of zero does not
 // keep an infinity or NaN in V out of a sum, and scores beyond 2^22 would be off against their rounded maximum. A column whose sums come
 // out not finite, or whose maximum is beyond that, is walked again by itself on the vector ALUs, the tokens that it sees alone (PaColumn).
@@ -484,6 +488,8 @@ __device__ __forceinline__ void pagedPieces(const PtArgs& x, F&& walk) {
 //     are as they lie the operand P^T of O^T += V^T . P^T, whose 32 places hold the 16 tokens twice: with the rounded
 //     probability and with what the rounding left, which makes 16 bits of it in bf16 and 22 in fp16 at no cost.
 //   * the tokens that are seen are a list without gaps (PtList); their slots are looked up 128 at a time.
+// bf16, heads of 128: 64 x 1 new token behind 2048, 32 heads 340 us, 6.3 TB/s; 1 x 5 behind 1777, 32 heads on 8, a chain of loads, 9.5 us and 4 for
+// the launch that joins the shares.
 //   * the running maximum is replaced only when a score exceeds it by more than 2^8.
 constexpr int kPfWaves = 4, kPfTile = 16, kPfBlock = 128, kPfStages = 2;
 template <typename T>
@@ -841,7 +847,8 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void pagedTileKernel(PtArgs x
 //   O^T = V^T P^T: row i of output tile t stands for element i (D / 16) + t, so a lane's D / 16 operands of a token are consecutive in memory,
 //   and its results are D / 4 consecutive elements of column c.
 // Rows go from the pool into registers a tile ahead, slots another one.
-// NC tiles of 16 columns share the rows in registers.
+// NC tiles of 16 columns share the rows in registers. 16 x (1 .. 40) new tokens behind 0 .. 260, 8 heads of 64 12 us, latency; 2 x 700 behind 300, 32
+// heads of 128 259 us, 58 TFLOP/s: a wave's products wait for its softmax.
 constexpr int kPtFloatCols = 16;
 template <int D, bool PART, int NC>
 __device__ __forceinline__ void pagedFloatBlock(const PtArgs& x, const PaSequence& s, int b, int kvh, int block, const PtSpan& span, int t0, int t1, int split,
@@ -1049,7 +1056,7 @@ __device__ __forceinline__ float pagedWeights(float2 state, int shares, uint64_t
 }
 
 // The blocks of columns that were walked in shares: a wave joins MANY columns, four of them at a time with four shares of each on their way, or
-// one with eight of them.
+// one with eight of them. Latency: 4 to 5 us.
 template <typename T, int COLS, int FEW, int PAIRS, int MANY>
 __global__ __launch_bounds__(256) void pagedMergeKernel(PtArgs x, int64_t step) {
   constexpr int kTogether = MANY == 1 ? 1 : 4, kBatch = MANY == 1 ? 8 : 4, kPtMergeCols = 4 * MANY;

@@ -292,7 +292,8 @@ __global__ __launch_bounds__(256) void rotaryAppendAnyKernel(RotaryAppendArgs a)
 
 // Head rows of whole 16-byte pieces. A thread keeps its place in the head row, and with it the angles, for all of its heads (up to
 // kAppendHeads, whose rows it asks for at once); the heads of q, k and v are one list, cut into grid.y shares of x.share; tokens with few
-// heads share a workgroup.
+// heads share a workgroup. Bound by HBM: 8192 tokens, 32 heads of 128 bf16 for q, k and v, 407 MB in 72 us, 5.7 TB/s (two rotations and a scatter:
+// 90 us, 104 with the gather of the tables' rows).
 constexpr int kAppendHeads = 4;
 struct RotaryAppendShape {
   int perHead, across, share, tokPerWg;  // work items of a head; heads side by side; heads of a workgroup; tokens of a workgroup
