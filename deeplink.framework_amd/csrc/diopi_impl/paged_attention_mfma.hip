@@ -536,6 +536,14 @@ __device__ __forceinline__ void pagedFewBlock(const PtArgs& x, const PaSequence&
   const int share = WIDE ? chunkEnd - chunkBegin : ((chunkEnd - chunkBegin + kPfWaves - 1) / kPfWaves + kPfTile - 1) / kPfTile * kPfTile;
   const int from = WIDE ? chunkBegin : chunkBegin + wave * share, to = min(chunkEnd, from + share);
 
+  // slots of a block of tokens, past the last one that again; the first block's are asked for before the rows of q: loads come back in order
+  int2 raw[kPfBlock / 64];
+  auto askSlots = [&](int b0) {
+    const int cnt = min(kPfBlock, to - b0);
+#pragma unroll
+    for (int i = 0; i < kPfBlock / 64; ++i) raw[i] = paAsk(a.bLoc, locBase + list.token(b0 + min(i * 64 + lane, cnt - 1)), a.loc64);
+  };
+  if (from < to) askSlots(from);
   Frag qf[CT][KS];
   int p[CT], sinksSeen[CT];
 #pragma unroll
@@ -588,12 +596,10 @@ __device__ __forceinline__ void pagedFewBlock(const PtArgs& x, const PaSequence&
 
   for (int b0 = from; b0 < to; b0 += kPfBlock) {
     const int cnt = min(kPfBlock, to - b0), tiles = (cnt + kPfTile - 1) / kPfTile;
-    // slots of the block; past the last token that again; one outside the pool is skipped, never dereferenced: it is marked by its top bit,
-    // and another of the block stands in (slot 0 where there is none)
-    int2 raw[kPfBlock / 64];
+    // a slot outside the pool is skipped, never dereferenced: it is marked by its top bit, and another of the block stands in (slot 0
+    // where there is none)
     uint64_t in[kPfBlock / 64];
-#pragma unroll
-    for (int i = 0; i < kPfBlock / 64; ++i) raw[i] = paAsk(a.bLoc, locBase + list.token(b0 + min(i * 64 + lane, cnt - 1)), a.loc64);
+    if (b0 != from) askSlots(b0);
     int instead = 0;
 #pragma unroll
     for (int i = 0; i < kPfBlock / 64; ++i) {
@@ -764,7 +770,12 @@ __device__ __forceinline__ void pagedFewBlock(const PtArgs& x, const PaSequence&
     for (; bad != 0; bad &= bad - 1) walkAgain(__builtin_ctz(bad));
     return;
   }
-  // waves meet in LDS, a tile of 16 columns at a time
+  // waves meet in LDS, a tile of 16 columns at a time (without a wait for what has been stored: 1 us)
+  auto meet = []() {
+    asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" : : : "memory");
+  };
   constexpr int kRedRow = D + 4;
   float* const red = reinterpret_cast<float*>(ptSmem);  // the ring: every load into it has been waited for
   if (threadIdx.x < kPtFewCols) again[threadIdx.x] = 0;
@@ -773,10 +784,10 @@ __device__ __forceinline__ void pagedFewBlock(const PtArgs& x, const PaSequence&
     if (quad == 0) stateBuf[wave][0][ct * 16 + c16] = m[ct], stateBuf[wave][1][ct * 16 + c16] = l[ct];
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
-    __syncthreads();
+    meet();
 #pragma unroll
     for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(red + (wave * 16 + c16) * kRedRow + 16 * d + 4 * quad) = acc[ct][d];
-    __syncthreads();
+    meet();
     const int here = min(16, cols - ct * 16);
     for (int i = threadIdx.x; i < here * (D / 4); i += kPfWaves * 64) {
       const int j = i / (D / 4), e = (i % (D / 4)) * 4, col = ct * 16 + j;
@@ -800,6 +811,9 @@ __device__ __forceinline__ void pagedFewBlock(const PtArgs& x, const PaSequence&
       else store(col, e, mAll, lAll, o);
     }
   }
+  meet();
+  if (__builtin_amdgcn_ballot_w64(again[lane & (kPtFewCols - 1)] != 0) == 0) return;  // (the same for all waves)
+  asm volatile("s_waitcnt vmcnt(0)" : : : "memory");  // (pieces of such a column may have been stored by other waves)
   __syncthreads();
   for (int col = wave; col < cols; col += kPfWaves)
     if (again[col] != 0) walkAgain(col);
