@@ -861,18 +861,18 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void pagedTileKernel(PtArgs x
 //   O^T = V^T P^T: row i of output tile t stands for element i (D / 16) + t, so a lane's D / 16 operands of a token are consecutive in memory,
 //   and its results are D / 4 consecutive elements of column c.
 // Rows go from the pool into registers a tile ahead, slots another one.
-// NC tiles of 16 columns share the rows in registers. 16 x (1 .. 40) new tokens behind 0 .. 260, 8 heads of 64 12 us, latency; 2 x 700 behind 300, 32
+// NC tiles of 16 columns share the rows in registers. G: groups of four waves, which take tiles by turns. 16 x (1 .. 40) new tokens behind 0 .. 260, 8 heads of 64 11 us, latency; 2 x 700 behind 300, 32
 // heads of 128 259 us, 58 TFLOP/s: a wave's products wait for its softmax.
 constexpr int kPtFloatCols = 16;
-template <int D, bool PART, int NC>
+template <int D, bool PART, int NC, int G>
 __device__ __forceinline__ void pagedFloatBlock(const PtArgs& x, const PaSequence& s, int b, int kvh, int block, const PtSpan& span, int t0, int t1, int split,
                                                 bool whole) {
-  constexpr int S = D / 4, E = D / 16, PITCH = D + 4, COLS = kPtFloatCols * NC;
+  constexpr int S = D / 4, E = D / 16, PITCH = D + 4, COLS = kPtFloatCols * NC, WAVES = 4 * G;
   extern __shared__ __attribute__((aligned(1024))) char ptSmem[];
-  float* const so = reinterpret_cast<float*>(ptSmem);  // [4][COLS][PITCH]
-  __shared__ float sm[4][COLS], sl[4][COLS];
+  float* const so = reinterpret_cast<float*>(ptSmem);  // [WAVES][COLS][PITCH]
+  __shared__ float sm[WAVES][COLS], sl[WAVES][COLS];
   const PaArgs& a = x.a;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = wave & 3, c = lane & 15, g = lane >> 4;
   const int group = a.group, cols = (s.end - s.first) * group, c0 = block * COLS;
   const int64_t locBase = (int64_t)b * a.locRowStride + (a.maxLen - s.len);
   const float* const kHead = reinterpret_cast<const float*>(a.k) + kvh * a.kHeadStride;
@@ -895,7 +895,7 @@ __device__ __forceinline__ void pagedFloatBlock(const PtArgs& x, const PaSequenc
   const int pFirst = __builtin_amdgcn_readlane(p[0], 0), pLast = __builtin_amdgcn_readlane(p[NC - 1], 15), window = a.window;
   auto askSlot = [&](int t) {
     if (t >= t1) return int2{0, 0};
-    return paAsk(a.bLoc, locBase + min(span.base(t) + 16 * wave + c, span.limit(t) - 1), a.loc64);
+    return paAsk(a.bLoc, locBase + min(span.base(t) + 16 * part + c, span.limit(t) - 1), a.loc64);
   };
   uint32_t valid[2];
   auto fetch = [&](int2 asked, auto buf) {
@@ -927,7 +927,7 @@ __device__ __forceinline__ void pagedFloatBlock(const PtArgs& x, const PaSequenc
   }
   auto tile = [&](int t, auto buf) {
     constexpr int B = decltype(buf)::value;
-    const int k0 = span.base(t) + 16 * wave;
+    const int k0 = span.base(t) + 16 * part;
     if (k0 > pLast || k0 >= span.limit(t) || (k0 + 15 <= pFirst - window && k0 >= a.sinks)) return;  // (uniform: nobody sees any of it)
     f32x4 acc[NC][2];  // two chains each: half the dependent latency
 #pragma unroll
@@ -970,24 +970,25 @@ __device__ __forceinline__ void pagedFloatBlock(const PtArgs& x, const PaSequenc
   };
   using B0 = std::integral_constant<int, 0>;
   using B1 = std::integral_constant<int, 1>;
-  if (t0 < t1) {
-    const int2 first = askSlot(t0);
-    int2 next = askSlot(t0 + 1);
+  const int tFirst = t0 + (wave >> 2);
+  if (tFirst < t1) {
+    const int2 first = askSlot(tFirst);
+    int2 next = askSlot(tFirst + G);
     fetch(first, B0{});
-    for (int t = t0; t < t1; t += 2) {
-      if (t + 1 < t1) {
+    for (int t = tFirst; t < t1; t += 2 * G) {
+      if (t + G < t1) {
         const int2 slot = next;
-        next = askSlot(t + 2);
+        next = askSlot(t + 2 * G);
         fetch(slot, B1{});
       }
       tile(t, B0{});
-      if (t + 1 >= t1) break;
-      if (t + 2 < t1) {
+      if (t + G >= t1) break;
+      if (t + 2 * G < t1) {
         const int2 slot = next;
-        next = askSlot(t + 3);
+        next = askSlot(t + 3 * G);
         fetch(slot, B0{});
       }
-      tile(t + 1, B1{});
+      tile(t + G, B1{});
     }
   }
 #pragma unroll
@@ -1005,16 +1006,17 @@ __device__ __forceinline__ void pagedFloatBlock(const PtArgs& x, const PaSequenc
   }
   __syncthreads();
   // a column to 16 lanes
+  if (G > 1 && wave >= 4) return;
 #pragma unroll
   for (int n = 0; n < NC; ++n) {
     const int mine = 16 * n + (threadIdx.x >> 4), e0 = c * E, oc = c0 + mine, place = paOfGroup(a, min(oc, cols - 1)), h = kvh * group + (min(oc, cols - 1) - place * group);
     const int64_t row = s.start + s.first + place;
     float mAll = -INFINITY, sum = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) mAll = fmaxf(mAll, sm[w][mine]);
+    for (int w = 0; w < WAVES; ++w) mAll = fmaxf(mAll, sm[w][mine]);
     f32x4 v[E / 4] = {};
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < WAVES; ++w) {
       const float weight = sm[w][mine] == -INFINITY ? 0.f : exp2f(sm[w][mine] - mAll);
       sum += sl[w][mine] * weight;
 #pragma unroll
@@ -1049,10 +1051,10 @@ __device__ __forceinline__ void pagedFloatBlock(const PtArgs& x, const PaSequenc
   }
 }
 
-template <int D, bool PART, int NC>
-__global__ __launch_bounds__(256) void pagedFloatKernel(PtArgs x) {
+template <int D, bool PART, int NC, int G>
+__global__ __launch_bounds__(256 * G) void pagedFloatKernel(PtArgs x) {
   pagedPieces<kPtFloatCols * NC, 0>(x, [&](const PaSequence& s, int b, int kvh, int block, const PtSpan& span, int t0, int t1, int split, bool whole) {
-    pagedFloatBlock<D, PART, NC>(x, s, b, kvh, block, span, t0, t1, split, whole);
+    pagedFloatBlock<D, PART, NC, G>(x, s, b, kvh, block, span, t0, t1, split, whole);
   });
 }
 
@@ -1228,11 +1230,11 @@ static diopiError_t launchFew(hipStream_t stream, const PtArgs& x, int64_t piece
   return diopiSuccess;
 }
 
-template <int D, bool PART, int NC>
+template <int D, bool PART, int NC, int G>
 static diopiError_t launchFloat(hipStream_t stream, const PtArgs& x, int64_t wgs) {
-  constexpr int lds = 4 * kPtFloatCols * NC * (D + 4) * (int)sizeof(float);
-  AMD_HIP(allowDynamicLds(reinterpret_cast<const void*>(&pagedFloatKernel<D, PART, NC>), lds));
-  hipLaunchKernelGGL((pagedFloatKernel<D, PART, NC>), dim3((unsigned)wgs), dim3(256), lds, stream, x);
+  constexpr int lds = 4 * G * kPtFloatCols * NC * (D + 4) * (int)sizeof(float);
+  AMD_HIP(allowDynamicLds(reinterpret_cast<const void*>(&pagedFloatKernel<D, PART, NC, G>), lds));
+  hipLaunchKernelGGL((pagedFloatKernel<D, PART, NC, G>), dim3((unsigned)wgs), dim3(256 * G), lds, stream, x);
   AMD_LAUNCH_CHECK();
   return diopiSuccess;
 }
@@ -1311,6 +1313,10 @@ diopiError_t pagedAttentionMfma(diopiContextHandle_t ctx, hipStream_t stream, co
       x.partial = static_cast<float*>(ws), x.partialState = reinterpret_cast<float2*>(x.partial + slices * a.d);
     }
   }
+  // fp32, a tile of columns to a block, no shares: eight waves, the tiles by turns to the first and the last four, where there are four tiles or more (us, four
+  // waves -> eight: 16 x (1 .. 40) new tokens behind 0 .. 260, 8 heads of 64 12.2 -> 11.1, 8 x 1 behind 100 ... 1000, 32 heads of 128 46 -> 42; of two
+  // tiles 8.4 -> 8.8, of shares of two 13.9 -> 16.4)
+  const bool eight = wide && !pairs && (a.d == 64 || a.d == 128) && x.splits == 1 && tiles >= 4;  // (parts of a row: registers spill)
   const int64_t fewPieces = wide ? 0 : (int64_t)a.batch * x.fewSplits;
   x.tilePieces = onlyFew ? 0 : blocks * x.splits;
   const int64_t tileWgs = x.tilePieces * a.kvHeads, wgs = tileWgs + fewPieces * a.kvHeads;
@@ -1326,11 +1332,16 @@ diopiError_t pagedAttentionMfma(diopiContextHandle_t ctx, hipStream_t stream, co
 #define HALF_CALL(T, D) AMD_TRY((onlyFew ? launchFew<T, D>(stream, x, fewPieces, wideHeads) : a.d == D ? launchTile<T, D, false>(stream, x, wgs) : launchTile<T, D, true>(stream, x, wgs)))
 #define BF16_CALL(D) HALF_CALL(bf16_t, D)
 #define FP16_CALL(D) HALF_CALL(half_t, D)
-#define FP32_CALL_AS(D, NC) AMD_TRY((a.d == D ? launchFloat<D, false, NC>(stream, x, wgs) : launchFloat<D, true, NC>(stream, x, wgs)))
-#define FP32_CALL(D)                                   \
-  do {                                                 \
-    if (!pairs) FP32_CALL_AS(D, 1);                    \
-    else if constexpr (D <= 128) FP32_CALL_AS(D, 2);   \
+#define FP32_CALL_AS(D, NC) AMD_TRY((a.d == D ? launchFloat<D, false, NC, 1>(stream, x, wgs) : launchFloat<D, true, NC, 1>(stream, x, wgs)))
+#define FP32_CALL(D)                                       \
+  do {                                                     \
+    if constexpr (D <= 128) {                              \
+      if (pairs) FP32_CALL_AS(D, 2);                       \
+      else if (eight) AMD_TRY((launchFloat<D, false, 1, 2>(stream, x, wgs))); \
+      else FP32_CALL_AS(D, 1);                             \
+    } else {                                               \
+      FP32_CALL_AS(D, 1);                                  \
+    }                                                      \
   } while (0)
   if (dtype == diopi_dtype_bfloat16) SIZE_CALL(BF16_CALL);
   else if (dtype == diopi_dtype_float16) SIZE_CALL(FP16_CALL);

@@ -458,3 +458,23 @@ def test_many_short_sequences(ops, dev, dtype, new, heads, kv_heads, d):
     lens = [new + (17 * b) % (130 if b % 7 else 5) for b in range(n)]
     check(ops, dev, Batch([new] * n, lens, heads, kv_heads, d, dtype, 90))
     check(ops, dev, Batch([min(new, b % 3) for b in range(n)], lens, heads, kv_heads, d, dtype, 91, window=40, sinks=3))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [64, 128])
+def test_short_pieces_of_many_sequences(ops, dev, dtype, d):
+    new = [1 + (11 * b) % 40 for b in range(40)]                    # blocks enough for no shares, of up to seven tiles
+    lens = [n + (53 * b) % 400 for b, n in enumerate(new)]
+    b = Batch(new, lens, 8, 8, d, dtype, 95)
+    b.b_loc[3, :b.max_len - 20] = -1                                # slots outside the pool
+    check(ops, dev, b)
+    check(ops, dev, Batch(new, lens, 8, 8, d, dtype, 96, window=70, sinks=66, index=torch.int64))
+    b = Batch(new, lens, 8, 8, d, dtype, 97)
+    b.v[b.b_loc[5, b.max_len - lens[5]].long()] = math.inf          # the first token of one: all of its new ones see it
+    got = b.run(ops, dev).cpu()
+    rows = slice(b.start[5], b.start[5] + new[5])
+    assert bool(torch.isinf(got[rows]).all())
+    b.v[b.b_loc[5, b.max_len - lens[5]].long()] = 0
+    want, bound, owned = attend(b)
+    owned[rows] = False
+    oracle.assert_within(got[owned], want[owned], bound[owned])
