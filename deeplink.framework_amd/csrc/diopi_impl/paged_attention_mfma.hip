@@ -488,7 +488,7 @@ __device__ __forceinline__ void pagedPieces(const PtArgs& x, F&& walk) {
 //     are as they lie the operand P^T of O^T += V^T . P^T, whose 32 places hold the 16 tokens twice: with the rounded
 //     probability and with what the rounding left, which makes 16 bits of it in bf16 and 22 in fp16 at no cost.
 //   * the tokens that are seen are a list without gaps (PtList); their slots are looked up 128 at a time.
-// bf16, heads of 128: 64 x 1 new token behind 2048, 32 heads 340 us, 6.3 TB/s; 1 x 5 behind 1777, 32 heads on 8, a chain of loads, 9.5 us and 4 for
+// bf16, heads of 128: 64 x 1 new token behind 2048, 32 heads 340 us, 6.3 TB/s; 1 x 5 behind 1777, 32 heads on 8, a chain of loads, 8.6 us and 4 for
 // the launch that joins the shares.
 //   * the running maximum is replaced only when a score exceeds it by more than 2^8.
 constexpr int kPfWaves = 4, kPfTile = 16, kPfBlock = 128, kPfStages = 2;
@@ -1269,9 +1269,10 @@ diopiError_t pagedAttentionMfma(diopiContextHandle_t ctx, hipStream_t stream, co
     int64_t chunk = std::max<int64_t>({128, ceilDiv(ceilDiv(seen, want), 64) * 64, ceilDiv(ceilDiv(seen, kPtMaxSplit), 64) * 64});
     if (seen <= 256) chunk = seen;
     // next to blocks of columns, which take longer: shares of 4096, and no shares (nor a launch that joins them, 4.5 us) where the rows of q
-    // are so many that no sequence has few, unless rows of none are among them
+    // are so many that no sequence has few, unless rows of none are among them (as in a recorded call for up to so many tokens: such a
+    // sequence by itself takes 55 us for each 4096 of its cache, so only where new tokens are meant to be many)
     const int64_t mostFew = kPtFewCols / group, others = (int64_t)(a.batch - 1) * a.maxNew;
-    if (!onlyFew) chunk = a.rows - others > mostFew ? seen : std::max<int64_t>(chunk, std::min<int64_t>(seen, 4096));
+    if (!onlyFew) chunk = a.maxNew >= kPtCols && a.rows - others > mostFew ? seen : std::max<int64_t>(chunk, std::min<int64_t>(seen, 4096));
     // A wave for each K/V head, with no shares, where a workgroup for each would be more than one round of them, of up to 128 tokens for each such
     // round and 512 (us, a workgroup -> a wave: 16 x 1 new token behind 130, 32 heads of 128, one round, 9.1 -> 15.3; 24 x 1 behind 60 12.8 -> 10.5, behind
     // 250 21.6 -> 22.1; 64 x 1, four rounds, behind 130 35.6 -> 27.0, behind 500 86.1 -> 83.3; 200 x 5, 32 heads on 8, behind 130 56.7 -> 30.7; 64 x 1
