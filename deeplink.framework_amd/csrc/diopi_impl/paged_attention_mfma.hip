@@ -82,13 +82,14 @@ struct PtSpan {
 };
 
 // The tokens that some of the new ones of a sequence with few columns see, in order: the first `sinks`, then from `low` on to the last new one.
+// Without a gap between the two, from token 0 on (sinks = 0): the later new tokens' first ones do not end where the first one's window begins.
 struct PtList {
   int sinks, low, n;
   __device__ __forceinline__ PtList(const PaArgs& a, const PaSequence& s) {
     low = max(0, s.origin + s.first - a.window + 1);
-    const int end = max(0, s.origin + s.end);
-    sinks = min(min(a.sinks, low), end);
-    n = sinks + max(0, end - low);
+    if (low <= a.sinks) low = 0;
+    sinks = min(a.sinks, low);
+    n = sinks + max(0, s.origin + s.end - low);
   }
   __device__ __forceinline__ int token(int i) const { return i < sinks ? i : low + (i - sinks); }
 };
@@ -630,7 +631,7 @@ __device__ __forceinline__ void pagedFewBlock(const PtArgs& x, const PaSequence&
       typedef __attribute__((address_space(3))) s16x4* LdsTr;
       const int v0 = b0 + t * kPfTile, last = v0 + kPfTile - 1;
       // whether every column sees all of the tile (uniform)
-      const bool all = !skips && last < to && list.token(last) <= pMin && (list.token(v0) > pMax - window || last < list.sinks);
+      const bool all = !skips && last < to && list.token(last) <= pMin && (list.token(v0) > pMax - window || list.token(last) < a.sinks);
       f32x4 sc[CT][2];
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) sc[ct][0] = sc[ct][1] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -733,7 +734,7 @@ __device__ __forceinline__ void pagedFewBlock(const PtArgs& x, const PaSequence&
     // of the share's tokens those that it sees
     const int first0 = min(chunkBegin, list.sinks), first1 = min(head, min(chunkEnd, list.sinks));
     const int next0 = list.low + max(0, chunkBegin - list.sinks), next1 = list.low + max(0, chunkEnd - list.sinks);
-    const int more1 = list.sinks == 0 ? min(head, next1) : 0;  // (without a list of first tokens apart, some may lie in the other part)
+    const int more1 = list.sinks == 0 ? min(head, next1) : 0;  // (without a list of first tokens apart they lie in the other part)
     PaColumn<T, D / 64, (D > 128 ? 4 : 8)> one;
     const T* q = reinterpret_cast<const T*>(a.q) + (s.start + token) * a.qTok + (int64_t)h * a.qHead;
     one.walk(a, q, kvh, locBase, list.sinks == 0 ? next0 : first0, list.sinks == 0 ? more1 : first1, max(next0, low), min(next1, s.origin + token + 1), 0, 64);
