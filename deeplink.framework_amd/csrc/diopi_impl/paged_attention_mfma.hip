@@ -54,9 +54,10 @@ struct PtMfma<half_t> {
 
 struct PtArgs {
   PaArgs a;
-  // partial results of blocks of columns: weighted sums of V [rows, heads, splits, d]; maximum and sum [rows, heads, splits]
+  // partial results of blocks of columns: weighted sums of V [rows, heads, splits, d]; maximum and sum [rows, heads, splits]. Rows: see ptPartialRow
   float* partial;
   float2* partialState;
+  int64_t partialSeq;  // rows of each sequence; 0: the rows of q
   int splits, tilesPerSplit;
   unsigned kSlotBytes, vSlotBytes;
   float* fewPartial;  // of sequences with few columns: [batch, kv_heads, kPtFewCols, fewSplits, 2 + d]
@@ -121,10 +122,16 @@ __device__ __forceinline__ int ptSwizzleK(int key) { return D >= 128 ? (key & 15
 template <int D>
 __device__ __forceinline__ int ptSwizzleV(int key) { return D >= 128 ? 4 * (key & 3) : 4 * ((key >> 1) & 1); }
 
+// Where partial results have the `at`th new token of sequence b that has a row in q. A row of q for each, or, where q has more rows than the
+// sequences can have new tokens (rows of no sequence, as in a recorded call for up to so many tokens), so many for each sequence.
+__device__ __forceinline__ int64_t ptPartialRow(const PtArgs& x, const PaSequence& s, int b, int at) {
+  return x.partialSeq != 0 ? b * x.partialSeq + at : s.start + s.first + at;
+}
+
 // Column `col` of a piece of work by itself, on the vector ALUs of one wave.
 template <typename T, int D>
-__device__ __forceinline__ void pagedAgain(const PtArgs& x, const PaSequence& s, int kvh, int64_t locBase, const PtSpan& span, int t0, int t1, int split, bool whole,
-                                           int col) {
+__device__ __forceinline__ void pagedAgain(const PtArgs& x, const PaSequence& s, int b, int kvh, int64_t locBase, const PtSpan& span, int t0, int t1, int split,
+                                           bool whole, int col) {
   const PaArgs& a = x.a;
   const int lane = threadIdx.x & 63, group = a.group, at = paOfGroup(a, col), token = s.first + at, h = kvh * group + (col - at * group), p = s.origin + token;
   const int64_t row = s.start + token;
@@ -135,7 +142,7 @@ __device__ __forceinline__ void pagedAgain(const PtArgs& x, const PaSequence& s,
   const int first0 = span.sinkTiles > 0 ? min(t0, span.sinkTiles) * kPtTile : from, first1 = span.sinkTiles > 0 ? min(head, min(t1, span.sinkTiles) * kPtTile) : min(head, to);
   PaColumn<T, D / 64, (D > 128 ? 4 : 8)> one;
   one.walk(a, reinterpret_cast<const T*>(a.q) + row * a.qTok + (int64_t)h * a.qHead, kvh, locBase, first0, first1, max(from, low), to, 0, 64);
-  const int64_t slice = (row * a.heads + h) * x.splits + split;
+  const int64_t slice = (ptPartialRow(x, s, b, at) * a.heads + h) * x.splits + split;
   float* dst = x.partial + slice * a.d;
   T* out = reinterpret_cast<T*>(a.out) + row * a.oTok + (int64_t)h * a.oHead;
   const float inv = one.l == 0.f ? 0.f : 1.f / one.l;
@@ -404,7 +411,7 @@ __device__ __forceinline__ void pagedTileBlock(const PtArgs& x, const PaSequence
   }
   __syncthreads();  // (the output takes the place of the stages)
   if (!whole) {
-    if (half == 0 && c0 + l31 < cols && (again >> l31 & 1) == 0) x.partialState[(row * a.heads + h) * x.splits + split] = float2{m - M::kRaise, l};
+    if (half == 0 && c0 + l31 < cols && (again >> l31 & 1) == 0) x.partialState[(ptPartialRow(x, s, b, mine) * a.heads + h) * x.splits + split] = float2{m - M::kRaise, l};
     // half of a column's elements at a time through LDS, so that a row of workspace is written in whole pieces
     constexpr int kHalf = D / 2, OF = kHalf + 4, PER = kHalf / 4;  // floats of a padded row; pieces of 16 bytes
     float* sO = reinterpret_cast<float*>(ptSmem) + wave * 32 * OF;
@@ -424,7 +431,7 @@ __device__ __forceinline__ void pagedTileBlock(const PtArgs& x, const PaSequence
         const int piece = lane + 64 * i, r = piece / PER, e = (piece % PER) * 4, oc = c0 + r;
         if (oc >= cols || (again >> r & 1) != 0 || (PART && pass * kHalf + e >= a.d)) continue;
         const int at = paOfGroup(a, oc);
-        const int64_t to = (s.start + s.first + at) * a.heads + kvh * group + (oc - at * group);
+        const int64_t to = ptPartialRow(x, s, b, at) * a.heads + kvh * group + (oc - at * group);
         *reinterpret_cast<f32x4*>(x.partial + (to * x.splits + split) * a.d + pass * kHalf + e) = *reinterpret_cast<const f32x4*>(sO + r * OF + e);
       }
     }
@@ -452,7 +459,7 @@ __device__ __forceinline__ void pagedTileBlock(const PtArgs& x, const PaSequence
             *reinterpret_cast<const Frag*>(sO + r * OS + c * 8);
   }
   }
-  for (; again != 0; again &= again - 1) pagedAgain<T, D>(x, s, kvh, locBase, span, t0, t1, split, whole, c0 + __builtin_ctz(again));
+  for (; again != 0; again &= again - 1) pagedAgain<T, D>(x, s, b, kvh, locBase, span, t0, t1, split, whole, c0 + __builtin_ctz(again));
 }
 
 // A workgroup's pieces of work, from a list for each K/V head: sequence after sequence, shares from the first, blocks from the last, which has
@@ -1040,7 +1047,7 @@ __device__ __forceinline__ void pagedFloatBlock(const PtArgs& x, const PaSequenc
         for (int i = 0; i < E / 4; ++i)
           if (!PART || e0 + 4 * i < a.d) *reinterpret_cast<f32x4*>(out + 4 * i) = v[i] * inv;
       } else {
-        const int64_t slice = (row * a.heads + h) * x.splits + split;
+        const int64_t slice = (ptPartialRow(x, s, b, place) * a.heads + h) * x.splits + split;
         if (c == 0) x.partialState[slice] = float2{mAll, sum};
 #pragma unroll
         for (int i = 0; i < E / 4; ++i)
@@ -1048,7 +1055,7 @@ __device__ __forceinline__ void pagedFloatBlock(const PtArgs& x, const PaSequenc
       }
     }
     for (int i = 0; i < 4; ++i)
-      if ((bad >> (16 * i) & 0xffffu) != 0) pagedAgain<float, D>(x, s, kvh, locBase, span, t0, t1, split, whole, c0 + 16 * n + 4 * wave + i);
+      if ((bad >> (16 * i) & 0xffffu) != 0) pagedAgain<float, D>(x, s, b, kvh, locBase, span, t0, t1, split, whole, c0 + 16 * n + 4 * wave + i);
   }
 }
 
@@ -1103,7 +1110,7 @@ __global__ __launch_bounds__(256) void pagedMergeKernel(PtArgs x, int64_t step) 
         if (shares[c] <= 1) shares[c] = 0;  // (a block walked whole has its results)
         most = max(most, shares[c]);
         row[c] = s.start + s.first + place, head[c] = kvh * group + (col - place * group);
-        const int64_t slice = (row[c] * a.heads + head[c]) * x.splits;
+        const int64_t slice = (ptPartialRow(x, s, at.b, place) * a.heads + head[c]) * x.splits;
         state[c] = x.partialState[slice + min(lane, max(shares[c] - 1, 0))];
         src[c] = x.partial + slice * a.d;
 #pragma unroll
@@ -1310,7 +1317,9 @@ diopiError_t pagedAttentionMfma(diopiContextHandle_t ctx, hipStream_t stream, co
     x.splits = (int)ceilDiv(tiles, x.tilesPerSplit);
     if (x.splits > 1) {
       void* ws = nullptr;
-      const int64_t slices = a.rows * a.heads * x.splits;
+      const int64_t perSeq = std::min<int64_t>(a.maxNew, a.rows);
+      if (a.batch * perSeq < a.rows) x.partialSeq = perSeq;
+      const int64_t slices = tokens * a.heads * x.splits;
       AMD_TRY(requireWorkspace(ctx, slices * (2 + a.d) * (int64_t)sizeof(float), &ws));
       x.partial = static_cast<float*>(ws), x.partialState = reinterpret_cast<float2*>(x.partial + slices * a.d);
     }

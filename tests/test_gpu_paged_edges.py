@@ -1,4 +1,4 @@
-"""GPU parity of attention of new tokens over a paged pool where sums are not finite, against the definition in 64 bits
+"""GPU parity of attention of new tokens over a paged pool at its edges (sums that are not finite, workspace), against the definition in 64 bits
 (tests/paged_batch.py)."""
 import math
 
@@ -64,3 +64,60 @@ def test_rows_that_are_not_finite_in_many_short_sequences(ops, dev, dtype, heads
     for n in reach[:3]:
         for j, rows, value in ((lens[n] - 1, b.k, math.nan), (lens[n] - 1, b.v, math.inf), (0, b.v, -math.inf)):
             damaged(ops, dev, b, n, rows, j, value)
+
+
+def workspace(ops, pkg, call):
+    """What the call returns, and the bytes of workspace that it takes."""
+    scope = ops.WorkspaceScope()
+    with scope:
+        before = pkg.runtime.cachingStats()["allocated_bytes"]
+        out = call()
+        taken = pkg.runtime.cachingStats()["allocated_bytes"] - before
+    torch.cuda.synchronize()
+    scope.close()
+    return out, taken
+
+
+def wide_table(b, width):
+    """The arguments of the batch with a slot table and a longest sequence of `width` tokens."""
+    x = list(b.to(torch.device("cuda:0")))
+    table = torch.full((len(b.lens), width), -1, dtype=b.b_loc.dtype)
+    table[:, width - b.max_len:] = b.b_loc[:, :b.max_len]
+    x[3], x[8] = table.to(x[0].device), width
+    return x
+
+
+@pytest.mark.parametrize("dtype,heads,kv_heads,d", [(torch.bfloat16, 32, 8, 128), (torch.float16, 8, 8, 64), (torch.float32, 8, 2, 64)])
+def test_partial_results_of_the_new_tokens_that_there_can_be_not_of_all_rows(ops, dev, pkg, dtype, heads, kv_heads, d):
+    b = Batch([64], [500], heads, kv_heads, d, dtype, 20, tail=8100)
+    out, taken = workspace(ops, pkg, lambda: ops.paged_context_attention(*wide_table(b, 131072)))
+    want, bound, owned = b.attend(PART[dtype])
+    oracle.assert_within(out.cpu()[owned], want[owned], bound[owned])
+    assert 0 < taken <= (2 + d) * 4 * 64 * heads * 64 + (4 << 20)   # (64 new tokens, up to 64 shares)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,d", [(4, 2, 64), (2, 2, 128), (6, 1, 80), (2, 1, 256)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (500, 70)])
+def test_shares_of_new_tokens_in_a_q_of_many_more_rows(ops, dev, dtype, heads, kv_heads, d, window, sinks):
+    b = Batch([70, 50, 0, 66, 1, 3], [1500, 900, 40, 70, 1200, 3], heads, kv_heads, d, dtype, 21, window=window, sinks=sinks, tail=700)
+    out = torch.full(b.q.shape, 77.0, dtype=dtype, device=dev)
+    got = b.run(ops, dev, out=out).cpu()
+    want, bound, owned = b.attend(PART[dtype])
+    oracle.assert_within(got[owned], want[owned], bound[owned])
+    assert bool((got[~owned] == 77).all())
+    for n, j, rows, value in ((0, 1499, b.k, math.nan), (0, 1480, b.v, math.inf), (1, 20, b.v, -math.inf), (4, 1199, b.v, math.inf)):
+        damaged(ops, dev, b, n, rows, j, value)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tail", [0, 700])
+def test_shares_of_new_tokens_whose_first_rows_lie_before_q(ops, dev, dtype, tail):
+    b = Batch([70, 50, 7], [1500, 900, 800], 4, 2, 64, dtype, 22, gap=0, tail=tail)
+    want, bound, owned = b.attend(PART[dtype])
+    x = list(b.to(dev))
+    x[0], x[4] = x[0][9:].contiguous(), x[4] - 9
+    out = torch.full(x[0].shape, 77.0, dtype=dtype, device=dev)
+    got = ops.paged_context_attention(*x, out=out).cpu()
+    oracle.assert_within(got[owned[9:]], want[9:][owned[9:]], bound[9:][owned[9:]])
+    assert bool((got[~owned[9:]] == 77).all())
