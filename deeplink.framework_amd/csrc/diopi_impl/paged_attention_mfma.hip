@@ -60,7 +60,8 @@ struct PtArgs {
   int64_t partialSeq;  // rows of each sequence; 0: the rows of q
   int splits, tilesPerSplit;
   unsigned kSlotBytes, vSlotBytes;
-  float* fewPartial;  // of sequences with few columns: [batch, kv_heads, kPtFewCols, fewSplits, 2 + d]
+  float* fewPartial;  // of sequences with few columns: [rows, heads, fewSplits, 2 + d]
+  int64_t fewSeq;     // its rows of each sequence; 0: the rows of q
   int fewSplits = 0, fewChunk = 1;
   int64_t tilePieces;  // workgroups for each K/V head that take blocks of columns
   unsigned tileWgs;    // all of them
@@ -124,8 +125,8 @@ __device__ __forceinline__ int ptSwizzleV(int key) { return D >= 128 ? 4 * (key 
 
 // Where partial results have the `at`th new token of sequence b that has a row in q. A row of q for each, or, where q has more rows than the
 // sequences can have new tokens (rows of no sequence, as in a recorded call for up to so many tokens), so many for each sequence.
-__device__ __forceinline__ int64_t ptPartialRow(const PtArgs& x, const PaSequence& s, int b, int at) {
-  return x.partialSeq != 0 ? b * x.partialSeq + at : s.start + s.first + at;
+__device__ __forceinline__ int64_t ptPartialRow(int64_t perSequence, const PaSequence& s, int b, int at) {
+  return perSequence != 0 ? b * perSequence + at : s.start + s.first + at;
 }
 
 // Column `col` of a piece of work by itself, on the vector ALUs of one wave.
@@ -142,7 +143,7 @@ __device__ __forceinline__ void pagedAgain(const PtArgs& x, const PaSequence& s,
   const int first0 = span.sinkTiles > 0 ? min(t0, span.sinkTiles) * kPtTile : from, first1 = span.sinkTiles > 0 ? min(head, min(t1, span.sinkTiles) * kPtTile) : min(head, to);
   PaColumn<T, D / 64, (D > 128 ? 4 : 8)> one;
   one.walk(a, reinterpret_cast<const T*>(a.q) + row * a.qTok + (int64_t)h * a.qHead, kvh, locBase, first0, first1, max(from, low), to, 0, 64);
-  const int64_t slice = (ptPartialRow(x, s, b, at) * a.heads + h) * x.splits + split;
+  const int64_t slice = (ptPartialRow(x.partialSeq, s, b, at) * a.heads + h) * x.splits + split;
   float* dst = x.partial + slice * a.d;
   T* out = reinterpret_cast<T*>(a.out) + row * a.oTok + (int64_t)h * a.oHead;
   const float inv = one.l == 0.f ? 0.f : 1.f / one.l;
@@ -411,7 +412,7 @@ __device__ __forceinline__ void pagedTileBlock(const PtArgs& x, const PaSequence
   }
   __syncthreads();  // (the output takes the place of the stages)
   if (!whole) {
-    if (half == 0 && c0 + l31 < cols && (again >> l31 & 1) == 0) x.partialState[(ptPartialRow(x, s, b, mine) * a.heads + h) * x.splits + split] = float2{m - M::kRaise, l};
+    if (half == 0 && c0 + l31 < cols && (again >> l31 & 1) == 0) x.partialState[(ptPartialRow(x.partialSeq, s, b, mine) * a.heads + h) * x.splits + split] = float2{m - M::kRaise, l};
     // half of a column's elements at a time through LDS, so that a row of workspace is written in whole pieces
     constexpr int kHalf = D / 2, OF = kHalf + 4, PER = kHalf / 4;  // floats of a padded row; pieces of 16 bytes
     float* sO = reinterpret_cast<float*>(ptSmem) + wave * 32 * OF;
@@ -431,7 +432,7 @@ __device__ __forceinline__ void pagedTileBlock(const PtArgs& x, const PaSequence
         const int piece = lane + 64 * i, r = piece / PER, e = (piece % PER) * 4, oc = c0 + r;
         if (oc >= cols || (again >> r & 1) != 0 || (PART && pass * kHalf + e >= a.d)) continue;
         const int at = paOfGroup(a, oc);
-        const int64_t to = ptPartialRow(x, s, b, at) * a.heads + kvh * group + (oc - at * group);
+        const int64_t to = ptPartialRow(x.partialSeq, s, b, at) * a.heads + kvh * group + (oc - at * group);
         *reinterpret_cast<f32x4*>(x.partial + (to * x.splits + split) * a.d + pass * kHalf + e) = *reinterpret_cast<const f32x4*>(sO + r * OF + e);
       }
     }
@@ -726,7 +727,7 @@ __device__ __forceinline__ void pagedFewBlock(const PtArgs& x, const PaSequence&
       for (int i = 0; i < 4; ++i) r[i] = static_cast<T>(o[i] * inv);
       *reinterpret_cast<Half*>(reinterpret_cast<T*>(a.out) + (s.start + token) * a.oTok + (int64_t)(kvh * group + (col - at * group)) * a.oHead + e) = r;
     } else {
-      float* dst = x.fewPartial + ((((int64_t)b * a.kvHeads + kvh) * kPtFewCols + col) * x.fewSplits + split) * (2 + a.d);
+      float* dst = x.fewPartial + ((ptPartialRow(x.fewSeq, s, b, at) * a.heads + kvh * group + (col - at * group)) * x.fewSplits + split) * (2 + a.d);
       if (e == 0) dst[0] = mCol, dst[1] = lCol;
       *reinterpret_cast<float2*>(dst + 2 + e) = float2{o[0], o[1]};
       *reinterpret_cast<float2*>(dst + 4 + e) = float2{o[2], o[3]};
@@ -747,7 +748,7 @@ __device__ __forceinline__ void pagedFewBlock(const PtArgs& x, const PaSequence&
     one.walk(a, q, kvh, locBase, list.sinks == 0 ? next0 : first0, list.sinks == 0 ? more1 : first1, max(next0, low), min(next1, s.origin + token + 1), 0, 64);
     const float inv = one.l == 0.f ? 0.f : 1.f / one.l;
     T* out = reinterpret_cast<T*>(a.out) + (s.start + token) * a.oTok + (int64_t)h * a.oHead;
-    float* dst = x.fewPartial + ((((int64_t)b * a.kvHeads + kvh) * kPtFewCols + col) * x.fewSplits + split) * (2 + a.d);
+    float* dst = x.fewPartial + ((ptPartialRow(x.fewSeq, s, b, at) * a.heads + h) * x.fewSplits + split) * (2 + a.d);
     if (!whole && lane == 0) dst[0] = one.m, dst[1] = one.l;
 #pragma unroll
     for (int j = 0; j < D / 64; ++j) {
@@ -1047,7 +1048,7 @@ __device__ __forceinline__ void pagedFloatBlock(const PtArgs& x, const PaSequenc
         for (int i = 0; i < E / 4; ++i)
           if (!PART || e0 + 4 * i < a.d) *reinterpret_cast<f32x4*>(out + 4 * i) = v[i] * inv;
       } else {
-        const int64_t slice = (ptPartialRow(x, s, b, place) * a.heads + h) * x.splits + split;
+        const int64_t slice = (ptPartialRow(x.partialSeq, s, b, place) * a.heads + h) * x.splits + split;
         if (c == 0) x.partialState[slice] = float2{mAll, sum};
 #pragma unroll
         for (int i = 0; i < E / 4; ++i)
@@ -1110,7 +1111,7 @@ __global__ __launch_bounds__(256) void pagedMergeKernel(PtArgs x, int64_t step) 
         if (shares[c] <= 1) shares[c] = 0;  // (a block walked whole has its results)
         most = max(most, shares[c]);
         row[c] = s.start + s.first + place, head[c] = kvh * group + (col - place * group);
-        const int64_t slice = (ptPartialRow(x, s, at.b, place) * a.heads + head[c]) * x.splits;
+        const int64_t slice = (ptPartialRow(x.partialSeq, s, at.b, place) * a.heads + head[c]) * x.splits;
         state[c] = x.partialState[slice + min(lane, max(shares[c] - 1, 0))];
         src[c] = x.partial + slice * a.d;
 #pragma unroll
@@ -1168,7 +1169,14 @@ __global__ __launch_bounds__(256) void pagedFewMergeKernel(PtArgs x, int most) {
   const int64_t i = WIDE ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave, pair = i / most;
   const int col = (int)(i - pair * most), b = (int)(pair / a.kvHeads), kvh = (int)(pair - (int64_t)b * a.kvHeads);
   if (pair >= (int64_t)a.batch * a.kvHeads) return;
-  const float* src = x.fewPartial + (pair * kPtFewCols + col) * x.fewSplits * (2 + a.d);
+  const int place = paOfGroup(a, col), head = kvh * group + (col - place * group);
+  int64_t row = b * x.fewSeq + place;
+  if (x.fewSeq == 0) {  // (rows of q: not before the lengths are there)
+    const PaSequence s = paSequence(a, b);
+    if (col >= ptColumns(a, s)) return;
+    row = s.start + s.first + place;
+  }
+  const float* src = x.fewPartial + (row * a.heads + head) * x.fewSplits * (2 + a.d);
   const float2 state = *reinterpret_cast<const float2*>(src + min(lane, x.fewSplits - 1) * (2 + a.d));
   float v[kBatch][kPerLane], acc[kPerLane] = {0.f, 0.f, 0.f, 0.f};
   auto ask = [&](int first) {
@@ -1198,8 +1206,7 @@ __global__ __launch_bounds__(256) void pagedFewMergeKernel(PtArgs x, int most) {
       for (int j = 0; j < kPerLane; ++j) acc[j] += wi * v[k][j];
     }
   }
-  const int place = paOfGroup(a, col);
-  T* out = reinterpret_cast<T*>(a.out) + (s.start + s.first + place) * a.oTok + (int64_t)(kvh * group + (col - place * group)) * a.oHead;
+  T* out = reinterpret_cast<T*>(a.out) + (s.start + s.first + place) * a.oTok + (int64_t)head * a.oHead;
   if (!WIDE) {
 #pragma unroll
     for (int j = 0; j < kPerLane; ++j)
@@ -1271,6 +1278,7 @@ diopiError_t pagedAttentionMfma(diopiContextHandle_t ctx, hipStream_t stream, co
   // Sequences of few columns, 16-bit rows: shares of at least 128 tokens, so many that two workgroups are there for each compute unit.
   bool wideHeads = false;
   const int64_t sequences = std::min<int64_t>(a.batch, tokens);
+  const int64_t mostFew = kPtFewCols / group, fewTokens = std::min<int64_t>({mostFew, a.maxNew, a.rows});  // new tokens of a sequence of few columns
   if (!wide) {
     const int64_t seen = std::max<int64_t>(1, std::min<int64_t>(a.maxLen, (int64_t)a.sinks + a.window + kPtFewCols));
     const int64_t want = std::max<int64_t>(1, 2 * cus / (sequences * a.kvHeads));
@@ -1279,7 +1287,7 @@ diopiError_t pagedAttentionMfma(diopiContextHandle_t ctx, hipStream_t stream, co
     // next to blocks of columns, which take longer: shares of 4096, and no shares (nor a launch that joins them, 4.5 us) where the rows of q
     // are so many that no sequence has few, unless rows of none are among them (as in a recorded call for up to so many tokens: such a
     // sequence by itself takes 55 us for each 4096 of its cache, so only where new tokens are meant to be many)
-    const int64_t mostFew = kPtFewCols / group, others = (int64_t)(a.batch - 1) * a.maxNew;
+    const int64_t others = (int64_t)(a.batch - 1) * a.maxNew;
     if (!onlyFew) chunk = a.maxNew >= kPtCols && a.rows - others > mostFew ? seen : std::max<int64_t>(chunk, std::min<int64_t>(seen, 4096));
     // A wave for each K/V head, with no shares, where a workgroup for each would be more than one round of them, of up to 128 tokens for each such
     // round and 512 (us, a workgroup -> a wave: 16 x 1 new token behind 130, 32 heads of 128, one round, 9.1 -> 15.3; 24 x 1 behind 60 12.8 -> 10.5, behind
@@ -1288,10 +1296,14 @@ diopiError_t pagedAttentionMfma(diopiContextHandle_t ctx, hipStream_t stream, co
     const int64_t units = sequences * a.kvHeads, round = (a.d > 128 ? 1 : 2) * cus;
     wideHeads = onlyFew && a.kvHeads % kPfWaves == 0 && units > round && seen <= std::min<int64_t>(512, 128 * units / round);
     if (wideHeads) chunk = seen;
+    if (fewTokens == 0) chunk = seen;  // (a token has more columns than that)
     x.fewChunk = (int)chunk, x.fewSplits = (int)ceilDiv(seen, chunk);
     if (x.fewSplits > 1) {
       void* ws = nullptr;
-      AMD_TRY(requireWorkspace(ctx, (int64_t)a.batch * a.kvHeads * kPtFewCols * x.fewSplits * (2 + a.d) * (int64_t)sizeof(float), &ws));
+      // Shares go by the sequences that have rows in q: of a batch with more sequences than that, partial results lie at the rows, which the launch that
+      // joins them cannot ask for before it has the lengths.
+      x.fewSeq = a.batch <= tokens ? fewTokens : 0;
+      AMD_TRY(requireWorkspace(ctx, (x.fewSeq != 0 ? a.batch * x.fewSeq : a.rows) * a.heads * x.fewSplits * (2 + a.d) * (int64_t)sizeof(float), &ws));
       x.fewPartial = static_cast<float*>(ws);
     }
   }
@@ -1364,7 +1376,7 @@ diopiError_t pagedAttentionMfma(diopiContextHandle_t ctx, hipStream_t stream, co
 #undef HALF_CALL
 #undef SIZE_CALL
   if (x.fewSplits > 1) {
-    const int mostCols = (int)std::min<int64_t>(kPtFewCols, std::min<int64_t>(a.maxNew, a.rows) * group);
+    const int mostCols = (int)(fewTokens * group);
     const bool wideMerge = x.fewSplits > 8;
     const int64_t merges = ceilDiv((int64_t)a.batch * a.kvHeads * mostCols, wideMerge ? 1 : 4);
     AMD_CHECK(merges < limit, "paged attention: %d sequences of %d heads exceed the grid limits", a.batch, a.heads);

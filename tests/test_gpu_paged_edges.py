@@ -121,3 +121,35 @@ def test_shares_of_new_tokens_whose_first_rows_lie_before_q(ops, dev, dtype, tai
     got = ops.paged_context_attention(*x, out=out).cpu()
     oracle.assert_within(got[owned[9:]], want[9:][owned[9:]], bound[9:][owned[9:]])
     assert bool((got[~owned[9:]] == 77).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("heads,kv_heads,d", [(8, 2, 128), (8, 8, 64), (10, 2, 80), (4, 4, 256)])
+@pytest.mark.parametrize("width", [3100, 16384])
+@pytest.mark.parametrize("several", [[1, 3, 2, 1], [1, 40, 3, 1]])
+def test_a_batch_with_more_sequences_than_new_tokens(ops, dev, pkg, dtype, heads, kv_heads, d, width, several):
+    new, lens = [0] * 300, [5] * 300
+    for n, at, length in zip(several, (0, 63, 64, 299), (3000, 1100, 17, 700)):
+        new[at], lens[at] = n, max(length, n)
+    b = Batch(new, lens, heads, kv_heads, d, dtype, 23, gap=0, tail=2)
+    x = wide_table(b, width)
+    out = torch.full(b.q.shape, 77.0, dtype=dtype, device=dev)
+    got, taken = workspace(ops, pkg, lambda: ops.paged_context_attention(*x, out=out))
+    want, bound, owned = b.attend(PART[dtype])
+    got = got.cpu()
+    oracle.assert_within(got[owned], want[owned], bound[owned])
+    assert bool((got[~owned] == 77).all())
+    assert 0 < taken <= 2 * (2 + d) * 4 * b.rows * heads * 64 + (4 << 20)   # (up to 64 shares of each row, for few columns and for many)
+    for n, j, value in ((0, 2999, math.inf), (0, 1500, math.nan), (299, 3, -math.inf)):
+        damaged(ops, dev, b, n, b.v, j, value)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("heads,kv_heads,d", [(8, 8, 128), (32, 8, 128), (40, 40, 64)])
+def test_workspace_of_few_new_tokens_is_that_of_their_columns(ops, dev, pkg, dtype, heads, kv_heads, d):
+    b = Batch([1, 1], [900, 300], heads, kv_heads, d, dtype, 24, gap=0, tail=0)
+    x = wide_table(b, 32768)
+    got, taken = workspace(ops, pkg, lambda: ops.paged_context_attention(*x))
+    want, bound, owned = b.attend(PART[dtype])
+    oracle.assert_within(got.cpu()[owned], want[owned], bound[owned])
+    assert 0 < taken <= (2 + d) * 4 * 2 * heads * 64 + 4096
