@@ -57,14 +57,15 @@ struct PtArgs {
   // partial results of blocks of columns: weighted sums of V [rows, heads, splits, d]; maximum and sum [rows, heads, splits]. Rows: see ptPartialRow
   float* partial;
   float2* partialState;
-  int64_t partialSeq;  // rows of each sequence; 0: the rows of q
   int splits, tilesPerSplit;
   unsigned kSlotBytes, vSlotBytes;
-  float* fewPartial;  // of sequences with few columns: [rows, heads, fewSplits, 2 + d]
-  int64_t fewSeq;     // its rows of each sequence; 0: the rows of q
-  int fewSplits = 0, fewChunk = 1;
+  float* fewPartial;  // of sequences with few columns: [slices, fewSplits, 2 + d] (see ptFewSlice)
+  int16_t fewSplits = 0;
+  int16_t fewCols;    // slices of each sequence and K/V head; 0: one for each row of q and head
+  int fewChunk = 1;
   int64_t tilePieces;  // workgroups for each K/V head that take blocks of columns
   unsigned tileWgs;    // all of them
+  int partialSeq;      // rows of `partial` of each sequence; 0: the rows of q
   int64_t turn;        // see pagedPieces
 };
 
@@ -125,8 +126,14 @@ __device__ __forceinline__ int ptSwizzleV(int key) { return D >= 128 ? 4 * (key 
 
 // Where partial results have the `at`th new token of sequence b that has a row in q. A row of q for each, or, where q has more rows than the
 // sequences can have new tokens (rows of no sequence, as in a recorded call for up to so many tokens), so many for each sequence.
-__device__ __forceinline__ int64_t ptPartialRow(int64_t perSequence, const PaSequence& s, int b, int at) {
-  return perSequence != 0 ? b * perSequence + at : s.start + s.first + at;
+__device__ __forceinline__ int64_t ptPartialRow(const PtArgs& x, const PaSequence& s, int b, int at) {
+  return x.partialSeq != 0 ? (int64_t)b * x.partialSeq + at : s.start + s.first + at;
+}
+// The same for column `col` of a sequence with few of them.
+__device__ __forceinline__ int64_t ptFewSlice(const PtArgs& x, const PaSequence& s, int b, int kvh, int col) {
+  if (x.fewCols != 0) return ((int64_t)b * x.a.kvHeads + kvh) * x.fewCols + col;
+  const int at = paOfGroup(x.a, col);
+  return (s.start + s.first + at) * x.a.heads + kvh * x.a.group + (col - at * x.a.group);
 }
 
 // Column `col` of a piece of work by itself, on the vector ALUs of one wave.
@@ -143,7 +150,7 @@ __device__ __forceinline__ void pagedAgain(const PtArgs& x, const PaSequence& s,
   const int first0 = span.sinkTiles > 0 ? min(t0, span.sinkTiles) * kPtTile : from, first1 = span.sinkTiles > 0 ? min(head, min(t1, span.sinkTiles) * kPtTile) : min(head, to);
   PaColumn<T, D / 64, (D > 128 ? 4 : 8)> one;
   one.walk(a, reinterpret_cast<const T*>(a.q) + row * a.qTok + (int64_t)h * a.qHead, kvh, locBase, first0, first1, max(from, low), to, 0, 64);
-  const int64_t slice = (ptPartialRow(x.partialSeq, s, b, at) * a.heads + h) * x.splits + split;
+  const int64_t slice = (ptPartialRow(x, s, b, at) * a.heads + h) * x.splits + split;
   float* dst = x.partial + slice * a.d;
   T* out = reinterpret_cast<T*>(a.out) + row * a.oTok + (int64_t)h * a.oHead;
   const float inv = one.l == 0.f ? 0.f : 1.f / one.l;
@@ -412,7 +419,7 @@ __device__ __forceinline__ void pagedTileBlock(const PtArgs& x, const PaSequence
   }
   __syncthreads();  // (the output takes the place of the stages)
   if (!whole) {
-    if (half == 0 && c0 + l31 < cols && (again >> l31 & 1) == 0) x.partialState[(ptPartialRow(x.partialSeq, s, b, mine) * a.heads + h) * x.splits + split] = float2{m - M::kRaise, l};
+    if (half == 0 && c0 + l31 < cols && (again >> l31 & 1) == 0) x.partialState[(ptPartialRow(x, s, b, mine) * a.heads + h) * x.splits + split] = float2{m - M::kRaise, l};
     // half of a column's elements at a time through LDS, so that a row of workspace is written in whole pieces
     constexpr int kHalf = D / 2, OF = kHalf + 4, PER = kHalf / 4;  // floats of a padded row; pieces of 16 bytes
     float* sO = reinterpret_cast<float*>(ptSmem) + wave * 32 * OF;
@@ -432,7 +439,7 @@ __device__ __forceinline__ void pagedTileBlock(const PtArgs& x, const PaSequence
         const int piece = lane + 64 * i, r = piece / PER, e = (piece % PER) * 4, oc = c0 + r;
         if (oc >= cols || (again >> r & 1) != 0 || (PART && pass * kHalf + e >= a.d)) continue;
         const int at = paOfGroup(a, oc);
-        const int64_t to = ptPartialRow(x.partialSeq, s, b, at) * a.heads + kvh * group + (oc - at * group);
+        const int64_t to = ptPartialRow(x, s, b, at) * a.heads + kvh * group + (oc - at * group);
         *reinterpret_cast<f32x4*>(x.partial + (to * x.splits + split) * a.d + pass * kHalf + e) = *reinterpret_cast<const f32x4*>(sO + r * OF + e);
       }
     }
@@ -727,7 +734,7 @@ __device__ __forceinline__ void pagedFewBlock(const PtArgs& x, const PaSequence&
       for (int i = 0; i < 4; ++i) r[i] = static_cast<T>(o[i] * inv);
       *reinterpret_cast<Half*>(reinterpret_cast<T*>(a.out) + (s.start + token) * a.oTok + (int64_t)(kvh * group + (col - at * group)) * a.oHead + e) = r;
     } else {
-      float* dst = x.fewPartial + ((ptPartialRow(x.fewSeq, s, b, at) * a.heads + kvh * group + (col - at * group)) * x.fewSplits + split) * (2 + a.d);
+      float* dst = x.fewPartial + (ptFewSlice(x, s, b, kvh, col) * x.fewSplits + split) * (2 + a.d);
       if (e == 0) dst[0] = mCol, dst[1] = lCol;
       *reinterpret_cast<float2*>(dst + 2 + e) = float2{o[0], o[1]};
       *reinterpret_cast<float2*>(dst + 4 + e) = float2{o[2], o[3]};
@@ -748,7 +755,7 @@ __device__ __forceinline__ void pagedFewBlock(const PtArgs& x, const PaSequence&
     one.walk(a, q, kvh, locBase, list.sinks == 0 ? next0 : first0, list.sinks == 0 ? more1 : first1, max(next0, low), min(next1, s.origin + token + 1), 0, 64);
     const float inv = one.l == 0.f ? 0.f : 1.f / one.l;
     T* out = reinterpret_cast<T*>(a.out) + (s.start + token) * a.oTok + (int64_t)h * a.oHead;
-    float* dst = x.fewPartial + ((ptPartialRow(x.fewSeq, s, b, at) * a.heads + h) * x.fewSplits + split) * (2 + a.d);
+    float* dst = x.fewPartial + (ptFewSlice(x, s, b, kvh, col) * x.fewSplits + split) * (2 + a.d);
     if (!whole && lane == 0) dst[0] = one.m, dst[1] = one.l;
 #pragma unroll
     for (int j = 0; j < D / 64; ++j) {
@@ -1048,7 +1055,7 @@ __device__ __forceinline__ void pagedFloatBlock(const PtArgs& x, const PaSequenc
         for (int i = 0; i < E / 4; ++i)
           if (!PART || e0 + 4 * i < a.d) *reinterpret_cast<f32x4*>(out + 4 * i) = v[i] * inv;
       } else {
-        const int64_t slice = (ptPartialRow(x.partialSeq, s, b, place) * a.heads + h) * x.splits + split;
+        const int64_t slice = (ptPartialRow(x, s, b, place) * a.heads + h) * x.splits + split;
         if (c == 0) x.partialState[slice] = float2{mAll, sum};
 #pragma unroll
         for (int i = 0; i < E / 4; ++i)
@@ -1111,7 +1118,7 @@ __global__ __launch_bounds__(256) void pagedMergeKernel(PtArgs x, int64_t step) 
         if (shares[c] <= 1) shares[c] = 0;  // (a block walked whole has its results)
         most = max(most, shares[c]);
         row[c] = s.start + s.first + place, head[c] = kvh * group + (col - place * group);
-        const int64_t slice = (ptPartialRow(x.partialSeq, s, at.b, place) * a.heads + head[c]) * x.splits;
+        const int64_t slice = (ptPartialRow(x, s, at.b, place) * a.heads + head[c]) * x.splits;
         state[c] = x.partialState[slice + min(lane, max(shares[c] - 1, 0))];
         src[c] = x.partial + slice * a.d;
 #pragma unroll
@@ -1159,8 +1166,9 @@ __global__ __launch_bounds__(256) void pagedMergeKernel(PtArgs x, int64_t step) 
 
 // The columns of sequences with few of them, `most` for each K/V head: a wave per column, or with WIDE a workgroup, whose waves take every
 // fourth share. What does not depend on the lengths is asked for before they are there (shares without tokens were never written:
-// what is read of them is left out).
-template <typename T, bool WIDE>
+// what is read of them is left out). ROWS: partial results at the rows of q, which have to be found first (a variant, as what the others ask for
+// would wait for that branch: 0.4 us).
+template <typename T, bool WIDE, bool ROWS>
 __global__ __launch_bounds__(256) void pagedFewMergeKernel(PtArgs x, int most) {
   constexpr int kPerLane = 4, kBatch = 8, kStep = WIDE ? 4 : 1;  // d <= 256
   __shared__ float red[WIDE ? 4 : 1][64 * kPerLane];
@@ -1169,14 +1177,13 @@ __global__ __launch_bounds__(256) void pagedFewMergeKernel(PtArgs x, int most) {
   const int64_t i = WIDE ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave, pair = i / most;
   const int col = (int)(i - pair * most), b = (int)(pair / a.kvHeads), kvh = (int)(pair - (int64_t)b * a.kvHeads);
   if (pair >= (int64_t)a.batch * a.kvHeads) return;
-  const int place = paOfGroup(a, col), head = kvh * group + (col - place * group);
-  int64_t row = b * x.fewSeq + place;
-  if (x.fewSeq == 0) {  // (rows of q: not before the lengths are there)
+  int64_t slice = i;
+  if constexpr (ROWS) {
     const PaSequence s = paSequence(a, b);
     if (col >= ptColumns(a, s)) return;
-    row = s.start + s.first + place;
+    slice = ptFewSlice(x, s, b, kvh, col);
   }
-  const float* src = x.fewPartial + (row * a.heads + head) * x.fewSplits * (2 + a.d);
+  const float* src = x.fewPartial + slice * x.fewSplits * (2 + a.d);
   const float2 state = *reinterpret_cast<const float2*>(src + min(lane, x.fewSplits - 1) * (2 + a.d));
   float v[kBatch][kPerLane], acc[kPerLane] = {0.f, 0.f, 0.f, 0.f};
   auto ask = [&](int first) {
@@ -1206,7 +1213,8 @@ __global__ __launch_bounds__(256) void pagedFewMergeKernel(PtArgs x, int most) {
       for (int j = 0; j < kPerLane; ++j) acc[j] += wi * v[k][j];
     }
   }
-  T* out = reinterpret_cast<T*>(a.out) + (s.start + s.first + place) * a.oTok + (int64_t)head * a.oHead;
+  const int place = paOfGroup(a, col);
+  T* out = reinterpret_cast<T*>(a.out) + (s.start + s.first + place) * a.oTok + (int64_t)(kvh * group + (col - place * group)) * a.oHead;
   if (!WIDE) {
 #pragma unroll
     for (int j = 0; j < kPerLane; ++j)
@@ -1297,13 +1305,14 @@ diopiError_t pagedAttentionMfma(diopiContextHandle_t ctx, hipStream_t stream, co
     wideHeads = onlyFew && a.kvHeads % kPfWaves == 0 && units > round && seen <= std::min<int64_t>(512, 128 * units / round);
     if (wideHeads) chunk = seen;
     if (fewTokens == 0) chunk = seen;  // (a token has more columns than that)
-    x.fewChunk = (int)chunk, x.fewSplits = (int)ceilDiv(seen, chunk);
+    x.fewChunk = (int)chunk, x.fewSplits = (int16_t)ceilDiv(seen, chunk);
     if (x.fewSplits > 1) {
       void* ws = nullptr;
       // Shares go by the sequences that have rows in q: of a batch with more sequences than that, partial results lie at the rows, which the launch that
-      // joins them cannot ask for before it has the lengths.
-      x.fewSeq = a.batch <= tokens ? fewTokens : 0;
-      AMD_TRY(requireWorkspace(ctx, (x.fewSeq != 0 ? a.batch * x.fewSeq : a.rows) * a.heads * x.fewSplits * (2 + a.d) * (int64_t)sizeof(float), &ws));
+      // joins them cannot find before it has the lengths.
+      x.fewCols = a.batch <= tokens ? (int16_t)(fewTokens * group) : 0;
+      const int64_t slices = x.fewCols != 0 ? (int64_t)a.batch * a.kvHeads * x.fewCols : a.rows * a.heads;
+      AMD_TRY(requireWorkspace(ctx, slices * x.fewSplits * (2 + a.d) * (int64_t)sizeof(float), &ws));
       x.fewPartial = static_cast<float*>(ws);
     }
   }
@@ -1330,7 +1339,7 @@ diopiError_t pagedAttentionMfma(diopiContextHandle_t ctx, hipStream_t stream, co
     if (x.splits > 1) {
       void* ws = nullptr;
       const int64_t perSeq = std::min<int64_t>(a.maxNew, a.rows);
-      if (a.batch * perSeq < a.rows) x.partialSeq = perSeq;
+      if (a.batch * perSeq < a.rows) x.partialSeq = (int)perSeq;
       const int64_t slices = tokens * a.heads * x.splits;
       AMD_TRY(requireWorkspace(ctx, slices * (2 + a.d) * (int64_t)sizeof(float), &ws));
       x.partial = static_cast<float*>(ws), x.partialState = reinterpret_cast<float2*>(x.partial + slices * a.d);
@@ -1380,14 +1389,18 @@ diopiError_t pagedAttentionMfma(diopiContextHandle_t ctx, hipStream_t stream, co
     const bool wideMerge = x.fewSplits > 8;
     const int64_t merges = ceilDiv((int64_t)a.batch * a.kvHeads * mostCols, wideMerge ? 1 : 4);
     AMD_CHECK(merges < limit, "paged attention: %d sequences of %d heads exceed the grid limits", a.batch, a.heads);
-#define FEW_MERGE(T)                                                                                                                                    \
-  do {                                                                                                                                                  \
-    if (wideMerge) hipLaunchKernelGGL((pagedFewMergeKernel<T, true>), dim3((unsigned)merges), dim3(256), 0, stream, x, mostCols);                        \
-    else hipLaunchKernelGGL((pagedFewMergeKernel<T, false>), dim3((unsigned)merges), dim3(256), 0, stream, x, mostCols);                                 \
+#define FEW_MERGE_AS(T, WIDE, ROWS) hipLaunchKernelGGL((pagedFewMergeKernel<T, WIDE, ROWS>), dim3((unsigned)merges), dim3(256), 0, stream, x, mostCols)
+#define FEW_MERGE(T)                                      \
+  do {                                                    \
+    if (wideMerge && x.fewCols == 0) FEW_MERGE_AS(T, true, true); \
+    else if (wideMerge) FEW_MERGE_AS(T, true, false);     \
+    else if (x.fewCols == 0) FEW_MERGE_AS(T, false, true); \
+    else FEW_MERGE_AS(T, false, false);                   \
   } while (0)
     if (dtype == diopi_dtype_bfloat16) FEW_MERGE(bf16_t);
     else FEW_MERGE(half_t);
 #undef FEW_MERGE
+#undef FEW_MERGE_AS
     AMD_LAUNCH_CHECK();
   }
   if (x.splits > 1) {
