@@ -198,8 +198,8 @@ __global__ __launch_bounds__(kTaWaves * 64, splitWavesPerSimd(sizeof(T), LPT, HI
     }
   }
   // PART: a head row shorter than the LPT pieces the lane group spans (head sizes between the powers of two). The lanes
-  // past its end read the row's first piece instead (memory that exists), hold zeros for q, so that they add nothing
-  // to a score, and store nothing. (A variant of its own: with these selects in the kernel for whole rows the launch
+  // past its end read the row's first piece instead (memory that exists), hold zeros for q, add nothing to a score (not
+  // even zero times an infinity), and store nothing. (A variant of its own: with these selects in the kernel for whole rows the launch
   // at batch 64 reads 377 us against 366.)
   const bool live = !PART || sub * N < a.d;
   const int subIn = PART ? (live ? sub : 0) : sub;
@@ -304,10 +304,12 @@ __global__ __launch_bounds__(kTaWaves * 64, splitWavesPerSimd(sizeof(T), LPT, HI
             const u32x4 raw = __builtin_bit_cast(u32x4, kr[u]);
 #pragma unroll
             for (int c = 0; c < 4; ++c) d = dotPair<T>(qp[j][c], raw[c], d);
+            if constexpr (PART) d = live ? d : 0.f;
             d = headRowSum<LPT>(d) * qScale;
           } else {
 #pragma unroll
             for (int e = 0; e < N; ++e) d += qf[j][e] * static_cast<float>(kr[u][e]);
+            if constexpr (PART) d = live ? d : 0.f;
             d = headRowSum<LPT>(d);
           }
           sc[u] = ok[u] ? d : -INFINITY;

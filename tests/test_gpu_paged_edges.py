@@ -153,3 +153,62 @@ def test_workspace_of_few_new_tokens_is_that_of_their_columns(ops, dev, pkg, dty
     want, bound, owned = b.attend(PART[dtype])
     oracle.assert_within(got.cpu()[owned], want[owned], bound[owned])
     assert 0 < taken <= (2 + d) * 4 * 2 * heads * 64 + 4096
+
+
+FORMS = [(8, 2, 64), (4, 4, 128), (6, 1, 80), (2, 1, 256), (2, 1, 20)]
+
+
+def scored(seed, new, lens, heads, kv_heads, d, dtype, **more):
+    """A batch whose q has ones as its element 3: an infinity there in a row of K is that token's score."""
+    b = Batch(new, lens, heads, kv_heads, d, dtype, seed, **more)
+    b.q[..., 3] = 1
+    return b
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,d", FORMS)
+def test_infinite_scores_of_single_tokens_with_a_window(ops, dev, dtype, heads, kv_heads, d):
+    """As in attention of several new tokens, and as in decode attention without a window."""
+    group = heads // kv_heads
+    for window, sinks in ((0, 0), (50, 4)):
+        b = scored(33, [1, 1, 1], [300, 80, 40], heads, kv_heads, d, dtype, window=window, sinks=sinks, gap=0, tail=0)
+        slots = [[int(b.b_loc[n, b.max_len - b.lens[n] + j]) for j in b.wanted(n)] for n in range(3)]
+        b.k[slots[0], -1, 3] = -math.inf
+        b.k[slots[1][::2], -1, 3] = -math.inf
+        b.k[slots[2][3], -1, 3] = math.inf
+        q, k, v, loc, start, _, seq, _, max_len = b.to(dev)
+        got = ops.token_decode_attention_window(q, k, v, loc, start, seq, max_len, window, sinks).cpu()
+        assert bool((got[0, -group:] == 0).all() & got[2, -group:].isnan().all())
+        b.k[slots[0] + slots[2], -1, 3] = 0
+        b.k[slots[1][::2], -1, 3] = 0
+        for j in b.wanted(1)[::2]:
+            b.b_loc[1, b.max_len - 80 + j] = -1
+        want, bound, _ = b.attend(2.0 ** -16 if dtype != torch.float32 else PART[dtype])
+        oracle.assert_within(got[1, -group:], want[1, -group:], bound[1, -group:])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [64, 80, 96, 112, 20, 24, 160, 256])
+@pytest.mark.parametrize("batch,length,kv_heads", [(3, 900, 2), (64, 40, 8), (300, 20, 8)])
+@pytest.mark.parametrize("group", [1, 2, 4])
+def test_scores_of_minus_infinity_in_decode_attention(ops, dev, dtype, d, batch, length, kv_heads, group):
+    """A key with an infinity that makes its score minus infinity weighs nothing, with heads of any size and whichever pipe takes them; alone and behind
+    a shared prefix."""
+    b = scored(34, [1] * batch, [length - n % 7 for n in range(batch)], group * kv_heads, kv_heads, d, dtype, gap=0, tail=0)
+    slots = [[int(b.b_loc[n, b.max_len - b.lens[n] + j]) for j in range(b.lens[n])] for n in range(batch)]
+    table, keys = b.b_loc.clone(), b.k.clone()
+    for n in range(0, batch, 5):
+        at = range(0, b.lens[n], 3)
+        keys[[slots[n][j] for j in at], :, 3] = -math.inf
+        b.b_loc[n, [b.max_len - b.lens[n] + j for j in at]] = -1
+    part = 2.0 ** -16 if dtype != torch.float32 else PART[dtype]
+    want, bound, _ = b.attend(part)
+    rest, b.b_loc = b.b_loc, table
+    q, _, v, loc, start, _, seq, _, max_len = b.to(dev)
+    oracle.assert_within(ops.token_decode_attention(q, keys.to(dev), v, loc, start, seq, max_len), want, bound)
+    prefix = torch.tensor(slots[1], device=dev)
+    got = ops.token_decode_attention_shared_prefix(q, keys.to(dev), v, prefix, loc, start, seq, max_len)
+    seen = [torch.cat([torch.tensor(slots[1]), rest[n, b.max_len - b.lens[n]:b.max_len].long()]) for n in range(batch)]
+    some = [0, 1, 2, 5, batch - 1] if batch > 3 else [0, 1, 2]
+    want, bound = oracle.attend(b.q[some], b.k, b.v, [seen[n] for n in some], part)
+    oracle.assert_within(got[some], want, bound)
