@@ -212,3 +212,79 @@ def test_scores_of_minus_infinity_in_decode_attention(ops, dev, dtype, d, batch,
     some = [0, 1, 2, 5, batch - 1] if batch > 3 else [0, 1, 2]
     want, bound = oracle.attend(b.q[some], b.k, b.v, [seen[n] for n in some], part)
     oracle.assert_within(got[some], want, bound)
+def with_scores(ops, dev, b, low, high=()):
+    """The last K/V head's scores of tokens `low` ((sequence, token) pairs) are minus infinity, those of `high` infinity: the first weigh nothing, as
+    tokens that are skipped; new tokens that see one of the others give NaN, whose weight is infinity / infinity."""
+    slot = lambda n, j: int(b.b_loc[n, b.max_len - b.lens[n] + j])
+    group, kept, table = b.q.shape[1] // b.k.shape[1], b.k.clone(), b.b_loc.clone()
+    want, bound, owned = b.attend(PART[b.dtype])
+    for n, j in low:
+        b.b_loc[n, b.max_len - b.lens[n] + j] = -1
+    last, last_bound, _ = b.attend(PART[b.dtype])
+    b.b_loc = table
+    want[:, -group:], bound[:, -group:] = last[:, -group:], last_bound[:, -group:]
+    for pairs, value in ((low, -math.inf), (high, math.inf)):
+        for n, j in pairs:
+            b.k[slot(n, j), -1, 3] = value
+    got = b.run(ops, dev).cpu()
+    b.k = kept
+    nan = torch.zeros(b.q.shape, dtype=torch.bool)
+    for n, j in high:
+        for t in range(b.new[n]):
+            if j in b.sees(b.lens[n] - b.new[n] + t):
+                nan[b.start[n] + t, -group:] = True
+    assert torch.equal(got[owned].isnan(), nan[owned])
+    ok = owned[:, None, None] & ~nan
+    oracle.assert_within(got[ok], want[ok], bound[ok])
+    return got
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,d", FORMS)
+@pytest.mark.parametrize("window,sinks", [(0, 0), (30, 60), (90, 4)])
+def test_scores_that_are_infinite(ops, dev, dtype, heads, kv_heads, d, window, sinks):
+    for new, lens in (([40, 3, 1], [150, 90, 70]), ([3, 1], [90, 70])):         # blocks and few columns, few columns alone
+        b = scored(30, new, lens, heads, kv_heads, d, dtype, window=window, sinks=sinks)
+        seen = [b.wanted(n) for n in range(len(new))]
+        some = [(n, j) for n in range(len(new)) for j in seen[n][::3]]
+        with_scores(ops, dev, b, some)
+        with_scores(ops, dev, b, [(n, j) for n in range(len(new)) for j in seen[n][:-2]])                      # all that come before the last two
+        with_scores(ops, dev, b, some, [(0, lens[0] - 1), (1, lens[1] - new[1])])
+        with_scores(ops, dev, b, [], [(0, seen[0][0]), (1, seen[1][-1])])
+        got = with_scores(ops, dev, b, [(n, j) for n in range(len(new)) for j in seen[n]])                     # no others: zeros, as without tokens
+        owned = b.slots_of_rows()[1]
+        assert bool((got[owned][:, -(heads // kv_heads):] == 0).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,d", FORMS)
+@pytest.mark.parametrize("new,tail", [(70, 0), (70, 500), (3, 0)])
+def test_scores_that_are_infinite_in_some_of_the_shares(ops, dev, dtype, heads, kv_heads, d, new, tail):
+    b = scored(31, [new], [2600], heads, kv_heads, d, dtype, tail=tail)
+    with_scores(ops, dev, b, [(0, j) for j in range(1300)])                                                    # the first shares altogether
+    with_scores(ops, dev, b, [(0, j) for j in range(700, 2600 - new)])
+    with_scores(ops, dev, b, [(0, j) for j in range(1300)], [(0, 2000)])
+    with_scores(ops, dev, b, [(0, j) for j in range(2600) if j != 5])
+    got = with_scores(ops, dev, b, [(0, j) for j in range(2600)])
+    assert bool((got[b.start[0]:b.start[0] + new, -(heads // kv_heads):] == 0).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,d", FORMS)
+def test_an_infinity_in_q(ops, dev, dtype, heads, kv_heads, d):
+    """Scores of a head of one new token are infinities of K's signs: NaN where one is positive, zeros where all are negative, the other rows as ever."""
+    for new, lens in (([40, 3], [150, 90]), ([3], [2000])):
+        b = scored(32, new, lens, heads, kv_heads, d, dtype)
+        n = len(new) - 1
+        b.k[..., 3] = -b.k[..., 3].abs() - 0.5
+        b.k[int(b.b_loc[n, b.max_len - lens[n] + lens[n] - 2]), -1, 3] = 2       # the last but one of the last sequence
+        want, bound, owned = b.attend(PART[dtype])
+        first, last = b.start[n], b.start[n] + new[n] - 1
+        b.q[first, -1, 3] = b.q[last, -1, 3] = math.inf
+        got = b.run(ops, dev).cpu()
+        assert bool((got[first, -1] == 0).all() & got[last, -1].isnan().all())
+        owned = owned[:, None].repeat(1, heads)
+        owned[first, -1] = owned[last, -1] = False
+        oracle.assert_within(got[owned], want[owned], bound[owned])
+
+
