@@ -19,8 +19,8 @@
 namespace amd {
 
 // Any head size up to 64 J, any strides: a workgroup per (new token, head), whose waves take 64 tokens that it sees in turn (PaColumn).
-// Bound by the vector ALUs, whose sums over the lanes cost more than the products (2 x 2048 new tokens behind 6000, 32 heads of 128 bf16, which
-// pagedTileKernel takes: 72 ms).
+// Bound by the vector ALUs, whose sums over the lanes cost more than the products. Rows one element off 16-byte pieces, against aligned ones on the matrix
+// pipe: 4 x 128 new tokens behind 1000, 32 heads of 128 on 8, bf16 1.5 ms, 39 us; 48 single tokens with a window of 2048, the same heads in fp16 376 us, 72 us.
 constexpr int kPgWaves = 4;
 template <typename T, int J, int UNR>
 __global__ __launch_bounds__(kPgWaves * 64) void pagedAnyKernel(PaArgs a) {

@@ -16,9 +16,11 @@
 //     of one new token and of thousands are dealt alike. The pieces of one K/V head's sequence are neighbours on one XCD.
 //   * shares of a sequence leave (maximum, sum, weighted sum of V) in workspace, which pagedMergeKernel joins.
 // Bound by the matrix pipe and the vector ALUs, between which the two waves of a SIMD change places less than they could: bf16, 32 heads of 128, 2 x
-// 2048 new tokens behind 6000 519 us, 0.92 PFLOP/s, the pipe busy 47 % of the time, the ALUs about as long, LDS 24 %. A block spends 8.6 us besides its
+// 2048 new tokens behind 6000 555 us, 0.85 PFLOP/s (520 to 555 from card to card and with the same inputs again or others each time), the pipe busy 46 % of
+// the time, the ALUs about as long, LDS 24 %. A block spends 8.6 us besides its
 // tiles (search 2.3, slots and first tiles 3.7, output 2.6), of which a second workgroup on the compute unit hides a part: prompts of
-// 2048 with a window of 512, 11 tiles to a block, 128 us.
+// 2048 with a window of 512, 11 tiles to a block, 133 us. Heads of 256 leave one workgroup to a compute unit, with some registers spilled: 2 x 1024
+// behind 3000, 16 heads, 192 us, 0.61 PFLOP/s.
 // What a column does not see (later tokens, those before the window, slots outside the pool) has no score; but a weight of zero does not
 // keep an infinity or NaN in V out of a sum, and scores beyond 2^22 would be off against their rounded maximum. A column whose sums come
 // out not finite, or whose maximum is beyond that, is walked again by itself on the vector ALUs, the tokens that it sees alone (PaColumn).
@@ -878,7 +880,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void pagedTileKernel(PtArgs x
 //   and its results are D / 4 consecutive elements of column c.
 // Rows go from the pool into registers a tile ahead, slots another one.
 // NC tiles of 16 columns share the rows in registers. G: groups of four waves, which take tiles by turns. 16 x (1 .. 40) new tokens behind 0 .. 260, 8 heads of 64 11 us, latency; 2 x 700 behind 300, 32
-// heads of 128 259 us, 58 TFLOP/s: a wave's products wait for its softmax.
+// heads of 128 264 us, 56 TFLOP/s: a wave's products wait for its softmax (16 heads of 256, with spilled registers, 401 us, 37 TFLOP/s).
 constexpr int kPtFloatCols = 16;
 template <int D, bool PART, int NC, int G>
 __device__ __forceinline__ void pagedFloatBlock(const PtArgs& x, const PaSequence& s, int b, int kvh, int block, const PtSpan& span, int t0, int t1, int split,

@@ -107,8 +107,8 @@ struct TaPartials {
 diopiError_t decodePartials(diopiContextHandle_t ctx, hipStream_t stream, const TaArgs& a, diopiDtype_t dtype, int maxInputLen, void* out, TaPartials* keep);
 
 // diopiTokenDecodeAttentionInference's kernels (not for generic arguments) over the last `window` tokens of each sequence and its first
-// `sinks`, window + sinks < a.maxLen. (64 x (512 .. 6000) tokens, window 2048, 32 heads of 128 bf16 311 us, 6.2 TB/s; 48 x (100 .. 12000), window 2048 and 4
-// first ones, 32 heads on 8 fp16 73 us, 5.1 TB/s)
+// `sinks`, window + sinks < a.maxLen. (64 x (512 .. 6000) tokens, window 2048, 32 heads of 128 bf16 317 us, 6.1 TB/s; 48 x (100 .. 12000), window 2048 and 4
+// first ones, 32 heads on 8 fp16 73 us, 5.1 TB/s; the 64 in fp32 610 us, 6.1 TB/s)
 diopiError_t decodeWindow(diopiContextHandle_t ctx, hipStream_t stream, TaArgs a, diopiDtype_t dtype, int window, int sinks, void* out);
 
 // As decodePartials, for rows of any kind and for int8 pools: partial results of the first `walked` tokens in `loc` and the own ones behind

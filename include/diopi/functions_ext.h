@@ -173,7 +173,9 @@ DIOPI_API diopiError_t diopiTokenDecodeAttentionSharedPrefixInference(diopiConte
  * sequence's first (more of them than tokens) and those whose visible slots all lie outside the pool give zeros; slots outside the
  * pool are skipped; rows of q and out outside [0, tokens) are left out, and rows of out of no sequence left as they were.
  * Sequences do not share rows of q. float32, float16 or bfloat16, grouped K/V heads (heads % kv_heads == 0), any strides with a contiguous head dimension
- * of up to 1024; out [tokens, heads, d] likewise; max_input_len is at most 2^30. Scores, softmax and sums are in fp32. The reference has
+ * of up to 1024; out [tokens, heads, d] likewise; max_input_len is at most 2^30. Scores, softmax and sums are in fp32; before it meets V a weight
+ * is rounded to V's type where a sequence brings more than 32 (new token, query head) pairs for each K/V head, as in diopiContextAttentionInference, and
+ * kept in 16 bits or more where it brings fewer. A score of minus infinity weighs nothing; where a token sees no others its result is zeros. The reference has
  * prompts without a cache and single tokens alone (ext_ops.py:52-133). */
 DIOPI_API diopiError_t diopiPagedContextAttentionInference(diopiContextHandle_t ctx, diopiTensorHandle_t out,
                                                            diopiConstTensorHandle_t q, diopiConstTensorHandle_t k,
