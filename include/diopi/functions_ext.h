@@ -172,7 +172,7 @@ DIOPI_API diopiError_t diopiTokenDecodeAttentionSharedPrefixInference(diopiConte
  * token sees are not used. b_new_len[b] is cut to [0, max_new_len] and b_seq_len[b] to [0, max_input_len]; new tokens before the
  * sequence's first (more of them than tokens) and those whose visible slots all lie outside the pool give zeros; slots outside the
  * pool are skipped; rows of q and out outside [0, tokens) are left out, and rows of out of no sequence left as they were.
- * Sequences do not share rows of q. float32, float16 or bfloat16, grouped K/V heads (heads % kv_heads == 0), any strides with a contiguous head dimension
+ * Sequences do not share rows of q, and out shares no memory with q, k or v. float32, float16 or bfloat16, grouped K/V heads (heads % kv_heads == 0), any strides with a contiguous head dimension
  * of up to 1024; out [tokens, heads, d] likewise; max_input_len is at most 2^30. Scores, softmax and sums are in fp32; before it meets V a weight
  * is rounded to V's type where a sequence brings more than 32 (new token, query head) pairs for each K/V head, as in diopiContextAttentionInference, and
  * kept in 16 bits or more where it brings fewer. A score of minus infinity weighs nothing; where a token sees no others its result is zeros. The reference has

@@ -6,7 +6,9 @@ import pytest
 import torch
 
 from tests import cache_oracle as oracle
+from tests.cache_graph import recorded
 from tests.paged_batch import Batch
+from tests.parity import assert_exact
 
 pytestmark = pytest.mark.gpu
 
@@ -288,3 +290,32 @@ def test_an_infinity_in_q(ops, dev, dtype, heads, kv_heads, d):
         oracle.assert_within(got[owned], want[owned], bound[owned])
 
 
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_calls_with_room_for_more_rows_or_sequences_recorded_into_graphs(ops, dev, pkg, dtype):
+    """A q of many more rows than new tokens, and a batch with more sequences than rows, whose tables change between the replays."""
+    padded = Batch([66, 3, 5], [1200, 900, 40], 8, 2, 64, dtype, 40, tail=900)
+    sparse = Batch([0] * 50 + [2, 0, 1], [7] * 50 + [1500, 9, 800], 8, 2, 64, dtype, 41, gap=0, tail=0)
+    on = [b.to(dev) for b in (padded, sparse)]
+    outs = [torch.full(b.q.shape, 77.0, dtype=dtype, device=dev) for b in (padded, sparse)]
+    calls = [lambda x=x, out=out: ops.paged_context_attention(*x, out=out) for x, out in zip(on, outs)]
+    owned = [b.slots_of_rows()[1] for b in (padded, sparse)]
+    with recorded(ops, pkg, calls[0]) as (first, _), recorded(ops, pkg, calls[1]) as (second, _):
+        for i in range(4):
+            for x, b in zip(on, (padded, sparse)):
+                x[0].mul_(0.75)
+                x[6].copy_(torch.tensor([max(b.new[n], length - 60 * i) for n, length in enumerate(b.lens)]))
+            for out in outs:
+                out.fill_(77)
+            first.replay()
+            second.replay()
+            first.replay()
+            torch.cuda.synchronize()
+            kept = [out.cpu() for out in outs]
+            for call in calls:
+                call()
+            torch.cuda.synchronize()
+            for got, out, rows in zip(kept, outs, owned):
+                assert_exact(got[rows], out.cpu()[rows])
+                assert bool((got[~rows] == 77).all())
