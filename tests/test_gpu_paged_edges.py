@@ -1,5 +1,5 @@
-"""GPU parity of attention of new tokens over a paged pool at its edges (sums that are not finite, workspace), against the definition in 64 bits
-(tests/paged_batch.py)."""
+"""GPU parity of attention of new tokens over a paged pool, and of decode attention, at their edges (sums and scores that are not finite, workspace, graphs),
+against the definition in 64 bits (tests/paged_batch.py, tests/cache_oracle.py)."""
 import math
 
 import pytest
